@@ -318,6 +318,7 @@ int spira_hip_fill_i32(int32_t *ptr, int64_t n, int32_t value, hipStream_t strea
 
 #define SPIRA_F16 0 /* feature / weight storage dtype: IEEE half */
 #define SPIRA_F32 1 /* feature / weight storage dtype: float    */
+#define SPIRA_BF16 2 /* (row operators only: experts, routing, norms, dropout) */
 
 #define SPIRA_OUT_STORE 0     /* write the output in the storage dtype */
 #define SPIRA_OUT_STORE_F32 1 /* write an fp32 buffer                  */
@@ -536,6 +537,101 @@ int spira_hip_ws_scatter(int64_t num_targets, int c_out, int num_offsets, int dt
  * and the hybrid final add, torch/cuda_sparse_convolution_forward.cu:336). */
 int spira_hip_finalize(const float *acc, int64_t num_targets, int c_out, int dtype, const float *scale,
                        const float *shift, const void *residual, int relu, void *targets, hipStream_t stream);
+
+/* ------------------------------------------------------------ row operators
+ * A mixture-of-experts block over rows of features, forward and gradients
+ * (none of it has a counterpart in the reference).  dtype: SPIRA_F16,
+ * SPIRA_BF16 or SPIRA_F32, of every tensor given as void; sums are fp32, each
+ * output is rounded once.  Tensors are contiguous and start on a value's own
+ * alignment.  Repeated calls give identical outputs (no floating-point
+ * atomics). */
+
+/* y[r] = act(x[s] @ weights[e] + bias[e]) for offsets[e] <= r < offsets[e + 1]:
+ * weights [groups, c_in, c_out]; bias [groups, c_out] or null; act: relu or
+ * none; s = sources[r], or r without sources (an s outside [0, num_sources)
+ * stands for a row of zeros).  offsets [groups + 1] int32 on the device,
+ * ascending; rows of no group get zeros. */
+int spira_hip_grouped_linear(int64_t rows, int groups, const int32_t *offsets, const int32_t *sources,
+                             int64_t num_sources, const void *x, int c_in, const void *weights, const void *bias,
+                             int c_out, int dtype, int relu, void *y, hipStream_t stream);
+
+/* dx[r] = dz[r] @ transpose(weights[e]); rows of no group get zeros. */
+int spira_hip_grouped_linear_rows_gradient(int64_t rows, int groups, const int32_t *offsets, const void *dz, int c_out,
+                                           const void *weights, int c_in, int dtype, void *dx, hipStream_t stream);
+
+/* dw[e] = sum over the group's rows of transpose(x[s]) dz[r]. */
+int spira_hip_grouped_linear_weights_gradient_workspace(int64_t rows, int groups, int c_in, int c_out, size_t *bytes);
+int spira_hip_grouped_linear_weights_gradient(int64_t rows, int groups, const int32_t *offsets, const int32_t *sources,
+                                              int64_t num_sources, const void *x, int c_in, const void *dz, int c_out,
+                                              int dtype, void *dw, void *workspace, size_t workspace_bytes,
+                                              hipStream_t stream);
+
+/* With y (the outputs of a relu): dz = dy where y > 0, else 0, for the groups'
+ * rows; without, dz is dy and not written.  dbias[e] = sum of the group's dz,
+ * or null. */
+int spira_hip_grouped_linear_activation_gradient_workspace(int64_t rows, int groups, int c_out, size_t *bytes);
+int spira_hip_grouped_linear_activation_gradient(int64_t rows, int groups, const int32_t *offsets, const void *dy,
+                                                 const void *y, int c_out, int dtype, void *dz, void *dbias,
+                                                 void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The k largest of each token's logits [tokens, experts], the lowest index
+ * first among equals: chosen [tokens, k], and their softmax weights over the
+ * chosen (renormalize) or over all.  A logit of -inf masks its expert; a token
+ * with fewer than k others has -1 and weight 0 in the rest; NaN counts as
+ * largest and makes its token's weights NaN.  Then the assignments (token,
+ * choice) ordered by expert, tokens ascending: offsets [experts + 1], rows
+ * [tokens * k] the token of each row, slots [tokens, k] the row of each
+ * assignment; -1 where there is no expert (rows past offsets[experts]).
+ * 1 to 512 experts, 1 to 16 choices. */
+int spira_hip_route_workspace(int64_t tokens, int experts, int k, size_t *bytes);
+int spira_hip_route(const void *logits, int64_t tokens, int experts, int k, int dtype, int renormalize, float *weights,
+                    int32_t *chosen, int32_t *offsets, int32_t *rows, int32_t *slots, void *workspace,
+                    size_t workspace_bytes, hipStream_t stream);
+
+/* dlogits from the gradient of the weights. */
+int spira_hip_route_backward(const void *logits, int64_t tokens, int experts, int k, int dtype, int renormalize,
+                             const float *weights, const int32_t *chosen, const float *dweights, void *dlogits,
+                             hipStream_t stream);
+
+/* y[t] = sum_j weights[t, j] h[slots[t, j]] over the slots in [0, num_rows);
+ * weights null: 1. */
+int spira_hip_combine(const void *h, int64_t num_rows, const int32_t *slots, const float *weights, int64_t tokens,
+                      int k, int c, int dtype, void *y, hipStream_t stream);
+
+/* dh[slots[t, j]] = weights[t, j] dy[t] (each slot at most once; rows with
+ * rows[r] < 0 get zeros) and dweights[t, j] = <dy[t], h[slots[t, j]]>; either
+ * may be null. */
+int spira_hip_combine_backward(const void *h, int64_t num_rows, const int32_t *rows, const int32_t *slots,
+                               const float *weights, const void *dy, int64_t tokens, int k, int c, int dtype, void *dh,
+                               float *dweights, hipStream_t stream);
+
+/* For n rows of c channels (1 to 16384), with m(v) = mean of v^2 over a row:
+ *   z = h / sqrt(m(h) + eps) * weight     (weight null: z = h)
+ *   r = x + scale * g * z                 (h null: r = x, not written)
+ *   next = r / sqrt(m(r) + eps) * next_weight   (null: none)
+ * gate_form: 0 none, 1 gate [c], 2 gate [n], 3 gate [n, c]; g is the gate or its
+ * sigmoid.  inv_h and inv_r [n] (null without a gradient) get the rows' 1 /
+ * sqrt(m + eps). */
+int spira_hip_gated_residual_norm(const void *x, const void *h, int64_t n, int c, int dtype, const void *weight,
+                                  const void *gate, int gate_form, int gate_sigmoid, float scale,
+                                  const void *next_weight, float eps, void *r, void *next, float *inv_h, float *inv_r,
+                                  hipStream_t stream);
+
+/* The gradients from dr and dnext (either may be null: zero); any of the
+ * outputs may be null. */
+int spira_hip_gated_residual_norm_backward_workspace(int64_t n, int c, int dtype, size_t *bytes);
+int spira_hip_gated_residual_norm_backward(const void *x, const void *h, int64_t n, int c, int dtype,
+                                           const void *weight, const void *gate, int gate_form, int gate_sigmoid,
+                                           float scale, const void *next_weight, const float *inv_h,
+                                           const float *inv_r, const void *dr, const void *dnext, void *dx, void *dh,
+                                           void *dweight, void *dgate, void *dnext_weight, void *workspace,
+                                           size_t workspace_bytes, hipStream_t stream);
+
+/* y[i] = (residual[i] or 0) + (kept ? x[i] / (1 - p) : 0) for n values; kept
+ * where word i % 4 of Philox-4x32 with 7 rounds, counter (i / 4, offset), key
+ * seed, is at least floor(p 2^32).  The gradient of x is the same call on dy. */
+int spira_hip_dropout(const void *x, const void *residual, int64_t n, int dtype, double p, uint64_t seed,
+                      uint64_t offset, void *y, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,654 @@
+// Products grouped by expert (gfx950): group e holds rows offsets[e] to
+// offsets[e + 1], any number of them, and has its own weights W[e]
+// [c_in, c_out].
+//
+//   forward   y[r]  = act(x[source(r)] W[e] + b[e])
+//   rows'     dx[r] = dz[r] W[e]^T
+//   weights'  dW[e] = sum_r x[source(r)]^T dz[r],  db[e] = sum_r dz[r]
+//
+// One tile core serves all three.  An operand's tile lies in LDS either with
+// the summed index along its rows of 128 bytes (KC: features; weights of the
+// rows' gradient), or with it across (KO: weights of the forward pass; both
+// operands of the weights' gradient), as it lies in memory: no operand is
+// transposed beforehand, the 16-bit KO fragments are transposed by the LDS read
+// itself (ds_read_b64_tr_b16).
+//
+// Which group a tile belongs to, each wave finds out by itself from the offsets,
+// on the device: nothing is read back, and uneven groups cost whole tiles only
+// at their ends.  Offsets that are no ascending row numbers cannot lead a tile
+// out of the arrays (they are clamped), and rows outside all groups get zeros.
+//
+// A wave multiplies with the weights as the first operand, so that a lane holds
+// four consecutive output channels of one row.
+#include "numeric.hpp"
+
+#include <algorithm>
+
+namespace spira_hip {
+
+namespace grouped {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+typedef __attribute__((address_space(3))) void lds_void;
+
+// ---------------------------------------------------------------------------
+// groups
+// ---------------------------------------------------------------------------
+struct Groups {
+  const int32_t *offsets;  // [count + 1]
+  int count;
+  int64_t rows;
+};
+
+struct Part {
+  int group;  // -1: the index lies past the last part, `begin` parts after it
+  int64_t begin, end;
+};
+
+__device__ __forceinline__ int64_t bound(const Groups &g, int i) {
+  const int64_t v = g.offsets[i];
+  return v < 0 ? 0 : v > g.rows ? g.rows : v;
+}
+
+// Part `index` of the groups cut into parts of `size` rows, in group order; the
+// same on every lane of the wave.  Lanes count the parts of 64 groups at a time.
+__device__ __forceinline__ Part find_part(const Groups &g, int size, int64_t index) {
+  const int lane = lane_id();
+  int64_t before = 0;
+  for (int first = 0; first < g.count; first += 64) {
+    const int e = first + lane;
+    const int64_t lo = e < g.count ? bound(g, e) : 0, hi = e < g.count ? bound(g, e + 1) : 0;
+    const int parts = hi > lo ? static_cast<int>((hi - lo + size - 1) / size) : 0;
+    int upto = parts;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int u = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += u;
+    }
+    const uint64_t past = ballot(before + upto > index);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int64_t nth = index - before - (__shfl(upto, at, 64) - __shfl(parts, at, 64));
+      const int64_t begin = __shfl(lo, at, 64) + nth * size, end = __shfl(hi, at, 64);
+      return {uniform(first + at), uniform(begin), uniform(begin + size < end ? begin + size : end)};
+    }
+    before += __shfl(upto, 63, 64);
+  }
+  return {-1, uniform(index - before), 0};
+}
+
+// the first part of group `group`, and how many it has
+__device__ __forceinline__ void parts_of(const Groups &g, int size, int group, int64_t &first, int64_t &count) {
+  const int lane = lane_id();
+  int64_t sum = 0;
+  for (int e = lane; e < group; e += 64) {
+    const int64_t n = bound(g, e + 1) - bound(g, e);
+    sum += n > 0 ? (n + size - 1) / size : 0;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  const int64_t n = bound(g, group + 1) - bound(g, group);
+  first = sum;
+  count = n > 0 ? (n + size - 1) / size : 0;
+}
+
+// most parts that any offsets of `count` groups over `rows` rows can have
+static int64_t most_parts(int64_t rows, int64_t count, int64_t size) {
+  return (rows + std::min(rows, count) * (size - 1)) / size;
+}
+
+// zeros in the rows outside all groups, by worker `index` of those without a part
+template <class T>
+__device__ void clear_ungrouped(const Groups &g, T *y, int64_t n, int64_t index, int64_t workers, int threads) {
+  const int64_t lo = bound(g, 0), hi = bound(g, g.count) > lo ? bound(g, g.count) : lo;
+  const int64_t chunks = (n + kVec<T> - 1) / kVec<T>, open = lo + g.rows - hi;
+  for (int64_t i = index * threads + threadIdx.x; i < open * chunks; i += workers * threads) {
+    const int64_t k = i / chunks, r = k < lo ? k : hi + k - lo, at = (i - k * chunks) * kVec<T>;
+    store_chunk(y + r * n + at, n - at, Chunk<T>{});
+  }
+}
+
+// ---------------------------------------------------------------------------
+// tiles
+// ---------------------------------------------------------------------------
+constexpr int kStep = 128;  // bytes of the summed index per step
+template <class T> constexpr int kStepK = kStep / static_cast<int>(sizeof(T));
+
+__device__ __forceinline__ uint32_t lds_of(const void *p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)(const_cast<void *>(p))));
+}
+
+// KC: row r's 16-byte chunk c at r * 128 + (c ^ (r / 2 % 8)) * 16, so that the
+// 16 lanes that read one chunk of 16 rows meet all banks once.
+__device__ __forceinline__ int kc_at(int r, int c) { return r * kStep + ((c ^ ((r >> 1) & 7)) << 4); }
+
+// KO: row k of N values.  16 bits: a transposing read takes, at the same 32
+// bytes of a row, rows k..k+3 and k+8..k+11 (and so on) at once: those pairs of
+// chunks are spread over the banks.  32 bits: rows k, k+4, k+8, k+12.
+template <class T, int N> __device__ __forceinline__ int ko_at(int k, int c) {
+  constexpr int ROW = N * static_cast<int>(sizeof(T));
+  if constexpr (sizeof(T) == 4) {
+    c ^= ((k >> 2) & 3) << 2;
+  } else if constexpr (ROW >= 256) {
+    c ^= ((k & 3) | ((k >> 1) & 4)) << 1;
+  } else {
+    c ^= (((k >> 1) & 1) | ((k >> 2) & 2)) << 1;
+  }
+  return k * ROW + (c << 4);
+}
+
+// fragment kk (of 2) of 16 rows from r0: lane l holds row l % 16, chunk l / 16
+__device__ __forceinline__ uintx4_t kc_frag(const char *tile, int r0, int kk) {
+  const int lane = lane_id();
+  return *reinterpret_cast<const uintx4_t *>(tile + kc_at(r0 + (lane & 15), kk * 4 + (lane >> 4)));
+}
+template <class T, int N> __device__ __forceinline__ uintx4_t ko_frag(const char *tile, int n0, int kk) {
+  const int lane = lane_id(), i = lane & 15, q = lane >> 4;
+  if constexpr (sizeof(T) == 2) {
+    const int k = kk * 32 + q * 8 + (i >> 2), c = n0 / 8 + ((i & 3) >> 1), half = (i & 1) * 8;
+    const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_short4 *)static_cast<uintptr_t>(lds_of(tile + ko_at<T, N>(k, c) + half)));
+    const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_short4 *)static_cast<uintptr_t>(lds_of(tile + ko_at<T, N>(k + 4, c) + half)));
+    const uintx2_t a = __builtin_bit_cast(uintx2_t, lo), b = __builtin_bit_cast(uintx2_t, hi);
+    return {a[0], a[1], b[0], b[1]};
+  } else {
+    uintx4_t r;
+    const int c = n0 / 4 + (i >> 2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      r[j] = *reinterpret_cast<const uint32_t *>(tile + ko_at<T, N>(kk * 16 + q * 4 + j, c) + (i & 3) * 4);
+    return r;
+  }
+}
+
+template <class T> __device__ __forceinline__ void mma(floatx4_t &d, uintx4_t a, uintx4_t b) {
+  if constexpr (std::is_same_v<T, _Float16>) {
+    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), d, 0, 0, 0);
+  } else if constexpr (std::is_same_v<T, __bf16>) {
+    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), d, 0, 0, 0);
+  } else {
+    // (element i of every lane's four: the summed index in another order, the
+    // same for both operands)
+    const floatx4_t x = __builtin_bit_cast(floatx4_t, a), y = __builtin_bit_cast(floatx4_t, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], d, 0, 0, 0);
+  }
+}
+
+// A thread's chunks of a tile on their way through registers.
+template <int N> struct Staged {
+  uintx4_t v[N];
+};
+
+// 128 x 128 outputs by four waves, 64 x 64 each
+constexpr int kRows = 128, kCols = 128, kThreads = 256;
+
+template <class T> struct Product {
+  static constexpr int KC_CHUNKS = kRows * 8 / kThreads;                               // chunks a thread and tile
+  static constexpr int CPR = kCols * static_cast<int>(sizeof(T)) / 16;                 // chunks a KO row
+  static constexpr int KO_CHUNKS = kStepK<T> * CPR / kThreads;
+  static constexpr int TILE = kRows * kStep;                                           // bytes of either form
+  static_assert(KC_CHUNKS == 4 && KO_CHUNKS == 4 && TILE == kStepK<T> * kCols * int(sizeof(T)), "tile shape");
+};
+
+// KC tile of rows row(i) (null: none) from column k0 of `width`
+template <class T, class RowPtr>
+__device__ __forceinline__ Staged<4> stage_kc(RowPtr &&row, int64_t k0, int64_t width) {
+  Staged<4> s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int id = threadIdx.x + i * kThreads;
+    const T *p = row(i);
+    const int64_t k = k0 + (id & 7) * kVec<T>;
+    s.v[i] = load_raw(p + k, p ? width - k : 0);
+  }
+  return s;
+}
+__device__ __forceinline__ void place_kc(char *tile, const Staged<4> &s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int id = threadIdx.x + i * kThreads;
+    *reinterpret_cast<uintx4_t *>(tile + kc_at(id >> 3, id & 7)) = s.v[i];
+  }
+}
+// KO tile: rows row(k) (null: none) for k of the step, from column n0 of `width`
+template <class T, class RowPtr>
+__device__ __forceinline__ Staged<4> stage_ko(RowPtr &&row, int64_t n0, int64_t width) {
+  Staged<4> s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int id = threadIdx.x + i * kThreads;
+    const T *p = row(id / Product<T>::CPR);
+    const int64_t n = n0 + (id % Product<T>::CPR) * kVec<T>;
+    s.v[i] = load_raw(p + n, p ? width - n : 0);
+  }
+  return s;
+}
+template <class T> __device__ __forceinline__ void place_ko(char *tile, const Staged<4> &s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int id = threadIdx.x + i * kThreads;
+    *reinterpret_cast<uintx4_t *>(tile + ko_at<T, kCols>(id / Product<T>::CPR, id % Product<T>::CPR)) = s.v[i];
+  }
+}
+
+struct Sums {
+  floatx4_t v[4][4];  // [row tile][channel tile]
+};
+
+// acc[m][n] += rows' fragments x channels' fragments of one step
+template <class T, class MFrag, class NFrag> __device__ __forceinline__ void multiply(Sums &acc, MFrag &&mf, NFrag &&nf) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    uintx4_t m[4], n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = mf(i, kk);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = nf(i, kk);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma<T>(acc.v[i][j], n[j], m[i]);
+  }
+}
+
+// four consecutive values of a row
+template <class T> __device__ __forceinline__ void store4(T *p, int64_t n, floatx4_t v) {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2), aligned(2)));
+    if (n >= 4) {
+      const T r[4] = {from_float<T>(v[0]), from_float<T>(v[1]), from_float<T>(v[2]), from_float<T>(v[3])};
+      u2 w;
+      __builtin_memcpy(&w, r, 8);
+      *reinterpret_cast<u2 *>(p) = w;
+      return;
+    }
+  } else if (n >= 4) {
+    *reinterpret_cast<uintx4_a4_t *>(p) = __builtin_bit_cast(uintx4_t, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) p[i] = from_float<T>(v[i]);
+}
+
+struct RowsArgs {
+  Groups g;
+  const int32_t *source;  // row of x behind each row (or null: itself)
+  int64_t num_sources;
+  const void *x, *w, *bias;
+  int64_t k, n;  // summed width, output width
+  int relu;
+  void *y;
+};
+
+// Forward (KO weights [k, n]) and rows' gradient (KC weights [n, k]).
+template <class T, bool KO> __global__ __launch_bounds__(kThreads) void rows_kernel(const RowsArgs a) {
+  using P = Product<T>;
+  __shared__ __align__(1024) char lds[4 * P::TILE];  // two stages of both tiles
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const Part part = find_part(a.g, kRows, blockIdx.x);
+  if (part.group < 0) {
+    if (blockIdx.y == 0) {
+      const int64_t used = blockIdx.x - part.begin;
+      clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, part.begin, gridDim.x - used, kThreads);
+    }
+    return;
+  }
+  const int64_t n0 = blockIdx.y * static_cast<int64_t>(kCols);
+  const T *w = static_cast<const T *>(a.w) + part.group * a.k * a.n;
+  const T *row[4], *wrow[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int id = threadIdx.x + i * kThreads;
+    const int64_t r = part.begin + (id >> 3);
+    int64_t s = r < part.end ? r : -1;
+    if (s >= 0 && a.source) {
+      s = a.source[r];
+      if (s >= a.num_sources) s = -1;
+    }
+    row[i] = s >= 0 ? static_cast<const T *>(a.x) + s * a.k : nullptr;
+    const int64_t n = n0 + (id >> 3);
+    wrow[i] = n < a.n ? w + n * a.k : nullptr;
+  }
+  auto stage_w = [&](int64_t k0) {
+    if constexpr (KO)
+      return stage_ko<T>([&](int k) -> const T * { return k0 + k < a.k ? w + (k0 + k) * a.n : nullptr; }, n0, a.n);
+    else
+      return stage_kc<T>([&](int i) { return wrow[i]; }, k0, a.k);
+  };
+  auto place = [&](int s, const Staged<4> &x, const Staged<4> &ws) {
+    place_kc(lds + 2 * s * P::TILE, x);
+    if constexpr (KO) place_ko<T>(lds + (2 * s + 1) * P::TILE, ws);
+    else place_kc(lds + (2 * s + 1) * P::TILE, ws);
+  };
+  const int m0 = (wave >> 1) * 64, c0 = (wave & 1) * 64;
+  Sums acc{};
+  Staged<4> xs = stage_kc<T>([&](int i) { return row[i]; }, 0, a.k), ws = stage_w(0);
+  place(0, xs, ws);
+  __syncthreads();
+  int s = 0;
+  for (int64_t k0 = 0; k0 < a.k; k0 += kStepK<T>, s ^= 1) {
+    const bool more = k0 + kStepK<T> < a.k;
+    if (more) {
+      xs = stage_kc<T>([&](int i) { return row[i]; }, k0 + kStepK<T>, a.k);
+      ws = stage_w(k0 + kStepK<T>);
+    }
+    const char *xt = lds + 2 * s * P::TILE, *wt = xt + P::TILE;
+    multiply<T>(
+        acc, [&](int i, int kk) { return kc_frag(xt, m0 + i * 16, kk); },
+        [&](int i, int kk) {
+          if constexpr (KO) return ko_frag<T, kCols>(wt, c0 + i * 16, kk);
+          else return kc_frag(wt, c0 + i * 16, kk);
+        });
+    if (more) place(s ^ 1, xs, ws);
+    __syncthreads();
+  }
+  const T *bias = static_cast<const T *>(a.bias);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t n = n0 + c0 + j * 16 + (lane >> 4) * 4;
+    floatx4_t b = {0, 0, 0, 0};
+    if (bias)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (n + v < a.n) b[v] = to_float(bias[part.group * a.n + n + v]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = part.begin + m0 + i * 16 + (lane & 15);
+      if (r >= part.end || n >= a.n) continue;
+      floatx4_t v = acc.v[i][j] + b;
+      if (a.relu)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
+      store4(static_cast<T *>(a.y) + r * a.n + n, a.n - n, v);
+    }
+  }
+}
+
+struct WeightsArgs {
+  Groups g;
+  const int32_t *source;
+  int64_t num_sources;
+  const void *x, *dz;
+  int64_t ci, co;
+  int part_rows;   // rows per part; 0: whole groups
+  float *partial;  // [parts, ci, co], or null: dw is written
+  void *dw;
+};
+
+// dW[e] or a part's share of it: both operands KO, summed over rows.
+template <class T> __global__ __launch_bounds__(kThreads) void weights_kernel(const WeightsArgs a) {
+  using P = Product<T>;
+  __shared__ __align__(1024) char lds[4 * P::TILE];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  Part part;
+  if (a.partial) {
+    part = find_part(a.g, a.part_rows, blockIdx.z);
+    if (part.group < 0) return;
+  } else {
+    part = {static_cast<int>(blockIdx.z), bound(a.g, blockIdx.z), bound(a.g, blockIdx.z + 1)};
+  }
+  const int64_t n0 = blockIdx.x * static_cast<int64_t>(kCols), m0 = blockIdx.y * static_cast<int64_t>(kRows);
+  auto stage_x = [&](int64_t r0) {
+    return stage_ko<T>(
+        [&](int k) -> const T * {
+          int64_t s = r0 + k < part.end ? r0 + k : -1;
+          if (s >= 0 && a.source) {
+            s = a.source[s];
+            if (s >= a.num_sources) s = -1;
+          }
+          return s >= 0 ? static_cast<const T *>(a.x) + s * a.ci : nullptr;
+        },
+        m0, a.ci);
+  };
+  auto stage_z = [&](int64_t r0) {
+    return stage_ko<T>(
+        [&](int k) -> const T * {
+          return r0 + k < part.end ? static_cast<const T *>(a.dz) + (r0 + k) * a.co : nullptr;
+        },
+        n0, a.co);
+  };
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  Sums acc{};
+  Staged<4> xs = stage_x(part.begin), zs = stage_z(part.begin);
+  place_ko<T>(lds, xs);
+  place_ko<T>(lds + P::TILE, zs);
+  __syncthreads();
+  int s = 0;
+  for (int64_t r0 = part.begin; r0 < part.end; r0 += kStepK<T>, s ^= 1) {
+    const bool more = r0 + kStepK<T> < part.end;
+    if (more) {
+      xs = stage_x(r0 + kStepK<T>);
+      zs = stage_z(r0 + kStepK<T>);
+    }
+    const char *xt = lds + 2 * s * P::TILE, *zt = xt + P::TILE;
+    multiply<T>(
+        acc, [&](int i, int kk) { return ko_frag<T, kRows>(xt, wm + i * 16, kk); },
+        [&](int i, int kk) { return ko_frag<T, kCols>(zt, wn + i * 16, kk); });
+    if (more) {
+      place_ko<T>(lds + 2 * (s ^ 1) * P::TILE, xs);
+      place_ko<T>(lds + (2 * (s ^ 1) + 1) * P::TILE, zs);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t m = m0 + wm + i * 16 + (lane & 15), n = n0 + wn + j * 16 + (lane >> 4) * 4;
+      if (m >= a.ci || n >= a.co) continue;
+      if (a.partial)
+        store4(a.partial + (blockIdx.z * a.ci + m) * a.co + n, a.co - n, acc.v[i][j]);
+      else
+        store4(static_cast<T *>(a.dw) + (part.group * a.ci + m) * a.co + n, a.co - n, acc.v[i][j]);
+    }
+}
+
+// out[e] = sum of the group's parts, in order: `size` values each
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(const Groups g, int part_rows, int64_t parts, const float *partial,
+                                                   int64_t size, T *out) {
+  int64_t first, count;
+  parts_of(g, part_rows, blockIdx.y, first, count);
+  // (overlapping groups count more parts than there are)
+  const int64_t last = std::min(first + count, parts);
+  const int64_t i = (blockIdx.x * static_cast<int64_t>(256) + threadIdx.x) * 4;
+  if (i >= size) return;
+  floatx4_t sum = {0, 0, 0, 0};
+  for (int64_t p = first; p < last; ++p) {
+    const float *v = partial + p * size + i;
+    if (size - i >= 4) {
+      sum += __builtin_bit_cast(floatx4_t, *reinterpret_cast<const uintx4_a4_t *>(v));
+    } else {
+      for (int j = 0; j < size - i; ++j) sum[j] += v[j];
+    }
+  }
+  store4(out + blockIdx.y * size + i, size - i, sum);
+}
+
+// dz = dy where y > 0 (or dy), and the parts' column sums of it: 64 columns by
+// 16 row lanes
+template <class T>
+__global__ __launch_bounds__(256) void activation_kernel(const Groups g, int part_rows, const T *dy, const T *y,
+                                                         int64_t co, T *dz, float *partial) {
+  constexpr int COLS = 16 * kVec<T>;
+  __shared__ float sums[16][COLS + 1];
+  const Part part = find_part(g, part_rows, blockIdx.y);
+  if (part.group < 0) return;
+  const int c = threadIdx.x & 15, rl = threadIdx.x >> 4;
+  const int64_t at = blockIdx.x * static_cast<int64_t>(COLS) + c * kVec<T>;
+  float s[kVec<T>] = {};
+  if (at < co)
+    for (int64_t r = part.begin + rl; r < part.end; r += 16) {
+      Chunk<T> d = load_chunk(dy + r * co + at, co - at);
+      if (y) {
+        const Chunk<T> v = load_chunk(y + r * co + at, co - at);
+#pragma unroll
+        for (int j = 0; j < kVec<T>; ++j) d.v[j] = v.v[j] > 0.f ? d.v[j] : 0.f;
+        store_chunk(dz + r * co + at, co - at, d);
+      }
+#pragma unroll
+      for (int j = 0; j < kVec<T>; ++j) s[j] += d.v[j];
+    }
+  if (!partial) return;
+#pragma unroll
+  for (int j = 0; j < kVec<T>; ++j) sums[rl][c * kVec<T> + j] = s[j];
+  __syncthreads();
+  const int64_t n = blockIdx.x * static_cast<int64_t>(COLS) + threadIdx.x;
+  if (threadIdx.x < COLS && n < co) {
+    float v = 0;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) v += sums[q][threadIdx.x];
+    partial[blockIdx.y * co + n] = v;
+  }
+}
+
+static int check(int64_t rows, int groups, const int32_t *offsets, int64_t ci, int64_t co) {
+  SPIRA_HIP_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) - 256, "grouped_linear: bad number of rows");
+  SPIRA_HIP_REQUIRE(groups > 0 && groups <= 65535, "grouped_linear: needs 1 to 65535 groups");
+  SPIRA_HIP_REQUIRE(ci > 0 && co > 0 && ci <= (1 << 20) && co <= (1 << 20), "grouped_linear: bad widths");
+  SPIRA_HIP_REQUIRE(offsets, "grouped_linear: no offsets");
+  return kOk;
+}
+
+// (grids have 65535 blocks in y and z: larger parts for more rows than that)
+static int64_t launch_limit(int64_t rows, int64_t groups, int64_t size) {
+  while (most_parts(rows, groups, size) > 65535 - 1) size *= 2;
+  return size;
+}
+
+// Rows per part of the weights' gradient; 0: whole groups, no parts.  Parts are
+// cut where the weights' tiles alone would leave the chip idle.
+static int weight_parts(int64_t rows, int64_t groups, int64_t ci, int64_t co) {
+  const int64_t tiles = div_up(ci, kRows) * div_up(co, kCols) * groups;
+  const int64_t want = 4 * 256;
+  if (tiles >= want || rows == 0) return 0;
+  const int64_t size = std::max<int64_t>(round_up(div_up(rows * div_up(ci, kRows) * div_up(co, kCols), want), 64), 256);
+  return static_cast<int>(launch_limit(rows, groups, size));
+}
+
+constexpr int kSumRows = 256;  // rows per part of the column sums
+
+}  // namespace grouped
+
+}  // namespace spira_hip
+
+using namespace spira_hip;
+
+extern "C" {
+
+int spira_hip_grouped_linear(int64_t rows, int groups, const int32_t *offsets, const int32_t *sources,
+                             int64_t num_sources, const void *x, int c_in, const void *weights, const void *bias,
+                             int c_out, int dtype, int relu, void *y, hipStream_t stream) {
+  if (int rc = grouped::check(rows, groups, offsets, c_in, c_out)) return rc;
+  SPIRA_HIP_REQUIRE(weights && (rows == 0 || y) && (x || num_sources == 0) && num_sources >= 0 &&
+                        (sources || num_sources >= rows),
+                    "grouped_linear: null tensor or too few sources");
+  return with_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    if (rows == 0) return kOk;
+    grouped::RowsArgs a{{offsets, groups, rows}, sources, num_sources, x, weights, bias, c_in, c_out, relu, y};
+    const int64_t parts = grouped::most_parts(rows, groups, grouped::kRows) + 1;
+    hipLaunchKernelGGL((grouped::rows_kernel<T, true>), dim3(parts, div_up(c_out, grouped::kCols)),
+                       dim3(grouped::kThreads), 0, stream, a);
+    SPIRA_HIP_LAUNCH_CHECK();
+    return kOk;
+  });
+}
+
+int spira_hip_grouped_linear_rows_gradient(int64_t rows, int groups, const int32_t *offsets, const void *dz, int c_out,
+                                           const void *weights, int c_in, int dtype, void *dx, hipStream_t stream) {
+  if (int rc = grouped::check(rows, groups, offsets, c_in, c_out)) return rc;
+  SPIRA_HIP_REQUIRE(weights && (rows == 0 || (dz && dx)), "grouped_linear_rows_gradient: null tensor");
+  return with_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    if (rows == 0) return kOk;
+    grouped::RowsArgs a{{offsets, groups, rows}, nullptr, rows, dz, weights, nullptr, c_out, c_in, 0, dx};
+    const int64_t parts = grouped::most_parts(rows, groups, grouped::kRows) + 1;
+    hipLaunchKernelGGL((grouped::rows_kernel<T, false>), dim3(parts, div_up(c_in, grouped::kCols)),
+                       dim3(grouped::kThreads), 0, stream, a);
+    SPIRA_HIP_LAUNCH_CHECK();
+    return kOk;
+  });
+}
+
+int spira_hip_grouped_linear_weights_gradient_workspace(int64_t rows, int groups, int c_in, int c_out, size_t *bytes) {
+  const int part = grouped::weight_parts(rows, groups, c_in, c_out);
+  *bytes = part == 0 ? 0 : grouped::most_parts(rows, groups, part) * static_cast<size_t>(c_in) * c_out * sizeof(float);
+  return kOk;
+}
+
+int spira_hip_grouped_linear_weights_gradient(int64_t rows, int groups, const int32_t *offsets, const int32_t *sources,
+                                              int64_t num_sources, const void *x, int c_in, const void *dz, int c_out,
+                                              int dtype, void *dw, void *workspace, size_t workspace_bytes,
+                                              hipStream_t stream) {
+  if (int rc = grouped::check(rows, groups, offsets, c_in, c_out)) return rc;
+  SPIRA_HIP_REQUIRE(dw && (rows == 0 || dz) && (x || num_sources == 0) && num_sources >= 0 &&
+                        (sources || num_sources >= rows),
+                    "grouped_linear_weights_gradient: null tensor or too few sources");
+  size_t need = 0;
+  spira_hip_grouped_linear_weights_gradient_workspace(rows, groups, c_in, c_out, &need);
+  SPIRA_HIP_REQUIRE(workspace_bytes >= need && (workspace || need == 0),
+                    "grouped_linear_weights_gradient: workspace too small");
+  return with_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const int part = grouped::weight_parts(rows, groups, c_in, c_out);
+    grouped::WeightsArgs a{{offsets, groups, rows}, sources, num_sources, x, dz, c_in, c_out, part,
+                           part ? static_cast<float *>(workspace) : nullptr, dw};
+    const int64_t z = part ? grouped::most_parts(rows, groups, part) : groups;
+    hipLaunchKernelGGL(grouped::weights_kernel<T>,
+                       dim3(div_up(c_out, grouped::kCols), div_up(c_in, grouped::kRows), z), dim3(grouped::kThreads), 0,
+                       stream, a);
+    SPIRA_HIP_LAUNCH_CHECK();
+    if (part) {
+      const int64_t size = static_cast<int64_t>(c_in) * c_out;
+      hipLaunchKernelGGL(grouped::join_kernel<T>, dim3(div_up(size, 1024), groups), dim3(256), 0, stream, a.g, part, z,
+                         a.partial, size, static_cast<T *>(dw));
+      SPIRA_HIP_LAUNCH_CHECK();
+    }
+    return kOk;
+  });
+}
+
+int spira_hip_grouped_linear_activation_gradient_workspace(int64_t rows, int groups, int c_out, size_t *bytes) {
+  const int64_t part = grouped::launch_limit(rows, groups, grouped::kSumRows);
+  *bytes = grouped::most_parts(rows, groups, part) * static_cast<size_t>(c_out) * sizeof(float);
+  return kOk;
+}
+
+int spira_hip_grouped_linear_activation_gradient(int64_t rows, int groups, const int32_t *offsets, const void *dy,
+                                                 const void *y, int c_out, int dtype, void *dz, void *dbias,
+                                                 void *workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (int rc = grouped::check(rows, groups, offsets, 1, c_out)) return rc;
+  SPIRA_HIP_REQUIRE((rows == 0 || dy) && (y == nullptr || dz || rows == 0) && (y || dbias),
+                    "grouped_linear_activation_gradient: null tensor");
+  const int64_t part = grouped::launch_limit(rows, groups, grouped::kSumRows);
+  const int64_t parts = grouped::most_parts(rows, groups, part);
+  SPIRA_HIP_REQUIRE(!dbias || workspace_bytes >= static_cast<size_t>(parts) * c_out * sizeof(float),
+                    "grouped_linear_activation_gradient: workspace too small");
+  return with_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const grouped::Groups g{offsets, groups, rows};
+    auto *partial = dbias ? static_cast<float *>(workspace) : nullptr;
+    if (rows > 0) {
+      hipLaunchKernelGGL(grouped::activation_kernel<T>, dim3(div_up(c_out, 16 * kVec<T>), parts), dim3(256), 0, stream,
+                         g, static_cast<int>(part), static_cast<const T *>(dy), static_cast<const T *>(y), c_out,
+                         static_cast<T *>(dz), partial);
+      SPIRA_HIP_LAUNCH_CHECK();
+    }
+    if (dbias) {
+      hipLaunchKernelGGL(grouped::join_kernel<T>, dim3(div_up(c_out, 1024), groups), dim3(256), 0, stream, g,
+                         static_cast<int>(part), parts, partial, static_cast<int64_t>(c_out), static_cast<T *>(dbias));
+      SPIRA_HIP_LAUNCH_CHECK();
+    }
+    return kOk;
+  });
+}
+
+}  // extern "C"

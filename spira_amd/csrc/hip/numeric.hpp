@@ -1,0 +1,85 @@
+// Feature types of the row operators (experts, routing, norms, dropout): fp16,
+// bf16 and fp32 in memory, fp32 in registers, in chunks of 16 bytes.
+#pragma once
+
+#include "common.hpp"
+
+#include <type_traits>
+
+#include "../../../include/spira_hip.h"
+
+namespace spira_hip {
+
+typedef float floatx4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4_t __attribute__((ext_vector_type(4)));
+
+template <class T> constexpr int kVec = 16 / static_cast<int>(sizeof(T));  // values per chunk
+
+template <class T> __device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
+// (to nearest, ties to even)
+template <class T> __device__ __forceinline__ T from_float(float v) { return static_cast<T>(v); }
+
+// Rows of odd widths and views start at any element: the chunk's type claims an
+// element's alignment only, and the hardware takes 16 bytes at any address in
+// one access.
+typedef uint32_t uintx4_a2_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t uintx4_a4_t __attribute__((ext_vector_type(4), aligned(4)));
+template <class T> using Unaligned = std::conditional_t<sizeof(T) == 2, uintx4_a2_t, uintx4_a4_t>;
+template <class T> struct Packed {
+  T v[kVec<T>];
+};
+template <class T> struct Chunk {
+  float v[kVec<T>];
+};
+
+// n: how many of the chunk's values lie inside the row (any number; values
+// past it are zero, or not written)
+template <class T> __device__ __forceinline__ uintx4_t load_raw(const T *p, int64_t n) {
+  if (n >= kVec<T>) return *reinterpret_cast<const Unaligned<T> *>(p);
+  Packed<T> r;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) r.v[i] = i < n ? p[i] : static_cast<T>(0.f);
+  return __builtin_bit_cast(uintx4_t, r);
+}
+template <class T> __device__ __forceinline__ Chunk<T> unpack(uintx4_t raw) {
+  const Packed<T> r = __builtin_bit_cast(Packed<T>, raw);
+  Chunk<T> c;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) c.v[i] = to_float(r.v[i]);
+  return c;
+}
+template <class T> __device__ __forceinline__ Chunk<T> load_chunk(const T *p, int64_t n) {
+  return unpack<T>(load_raw(p, n));
+}
+template <class T> __device__ __forceinline__ void store_chunk(T *p, int64_t n, const Chunk<T> &c) {
+  Packed<T> r;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) r.v[i] = from_float<T>(c.v[i]);
+  if (n >= kVec<T>) {
+    *reinterpret_cast<Unaligned<T> *>(p) = __builtin_bit_cast(uintx4_t, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i)
+      if (i < n) p[i] = r.v[i];
+  }
+}
+
+// sum over groups of G consecutive lanes (a power of two up to 64), the same in
+// every lane of the group
+template <int G> __device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// f(T{}) for the storage type that `dtype` names
+template <class F> int with_type(int dtype, F &&f) {
+  switch (dtype) {
+    case SPIRA_F16: return f(static_cast<_Float16>(0));
+    case SPIRA_BF16: return f(static_cast<__bf16>(0.f));
+    case SPIRA_F32: return f(0.f);
+    default: set_error("dtype must be fp16, bf16 or fp32"); return kInvalidArgument;
+  }
+}
+
+}  // namespace spira_hip

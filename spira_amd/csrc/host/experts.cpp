@@ -1,0 +1,325 @@
+// Row operators of `_C`: products grouped by expert, the router and the sum of
+// its experts' rows, the gated residual norm and dropout, forward and gradients
+// (no counterparts in the reference).  Outputs and workspaces come from the
+// caching allocator on the current stream; nothing is read back on the host.
+#include "host_common.h"
+
+#include <c10/core/DeviceGuard.h>
+
+namespace spira_host {
+
+using Tensor = torch::Tensor;
+using OptTensor = std::optional<torch::Tensor>;
+
+static int row_dtype(const Tensor &t) {
+  switch (t.scalar_type()) {
+    case torch::kHalf: return SPIRA_F16;
+    case torch::kBFloat16: return SPIRA_BF16;
+    case torch::kFloat: return SPIRA_F32;
+    default: fail("Cannot find implementation for feature dtype ", t.scalar_type());
+  }
+}
+
+static const void *ptr(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
+
+// t is a contiguous tensor of this type, on x's device, of these sizes (-1: any)
+static void require(const Tensor &t, const char *name, const Tensor &x, torch::ScalarType type,
+                    std::initializer_list<int64_t> sizes) {
+  require_device(t, name);
+  SPIRA_CHECK_ARG(t.device() == x.device(), name, " must be on ", x.device());
+  SPIRA_CHECK_ARG(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+  bool fits = t.dim() == static_cast<int64_t>(sizes.size());
+  int64_t d = 0;
+  for (int64_t s : sizes) {
+    if (fits && s >= 0 && t.size(d) != s) fits = false;
+    ++d;
+  }
+  if (!fits) {
+    std::ostringstream os;
+    for (int64_t s : sizes) os << (os.tellp() > 0 ? ", " : "") << (s < 0 ? std::string("any") : std::to_string(s));
+    fail(name, " must have the shape [", os.str(), "], got ", t.sizes());
+  }
+}
+static void require(const OptTensor &t, const char *name, const Tensor &x, torch::ScalarType type,
+                    std::initializer_list<int64_t> sizes) {
+  if (t) require(*t, name, x, type, sizes);
+}
+
+static Tensor like(const Tensor &x, torch::IntArrayRef sizes) { return torch::empty(sizes, x.options()); }
+static Tensor floats(const Tensor &x, torch::IntArrayRef sizes) {
+  return torch::empty(sizes, x.options().dtype(torch::kFloat));
+}
+
+struct Linear {
+  int64_t rows, groups, ci, co;
+};
+
+static Linear check_linear(const Tensor &x, const Tensor &w, const Tensor &offsets, const OptTensor &sources) {
+  require(x, "features", x, x.scalar_type(), {-1, -1});
+  (void)row_dtype(x);
+  require(w, "weight", x, x.scalar_type(), {-1, x.size(1), -1});
+  require(offsets, "offsets", x, torch::kInt, {w.size(0) + 1});
+  require(sources, "rows", x, torch::kInt, {-1});
+  Linear l{sources ? sources->size(0) : x.size(0), w.size(0), w.size(1), w.size(2)};
+  SPIRA_CHECK_ARG(l.groups > 0 && l.ci > 0 && l.co > 0, "weight must not be empty");
+  SPIRA_CHECK_ARG(l.ci <= (1 << 20) && l.co <= (1 << 20), "weight is too wide");
+  SPIRA_CHECK_ARG(l.groups <= 65535, "grouped_linear: needs 1 to 65535 groups");
+  return l;
+}
+
+static Tensor grouped_linear(const Tensor &x, const Tensor &w, const Tensor &offsets, const OptTensor &sources,
+                             const OptTensor &bias, bool relu) {
+  const Linear l = check_linear(x, w, offsets, sources);
+  require(bias, "bias", x, x.scalar_type(), {l.groups, l.co});
+  const c10::DeviceGuard guard(x.device());
+  Tensor y = like(x, {l.rows, l.co});
+  check_rc(spira_hip_grouped_linear(l.rows, l.groups, offsets.data_ptr<int32_t>(),
+                                    static_cast<const int32_t *>(ptr(sources)), x.size(0), x.data_ptr(), l.ci,
+                                    w.data_ptr(), ptr(bias), l.co, row_dtype(x), relu, y.data_ptr(), current_stream()),
+           "grouped_linear");
+  return y;
+}
+
+// (dx, dw, dbias) from dy; y: the outputs of a relu.  With slots (the rows of
+// each token), dx is summed per token.
+static std::tuple<OptTensor, OptTensor, OptTensor> grouped_linear_backward(
+    const Tensor &x, const Tensor &w, const Tensor &offsets, const OptTensor &sources, const OptTensor &slots,
+    const OptTensor &y, const Tensor &dy, bool need_dx, bool need_dw, bool need_db) {
+  const Linear l = check_linear(x, w, offsets, sources);
+  const int dtype = row_dtype(x);
+  const auto *off = offsets.data_ptr<int32_t>();
+  require(dy, "gradient", x, x.scalar_type(), {l.rows, l.co});
+  require(y, "output", x, x.scalar_type(), {l.rows, l.co});
+  SPIRA_CHECK_ARG(sources.has_value() == slots.has_value(), "rows and slots come together");
+  require(slots, "slots", x, torch::kInt, {x.size(0), -1});
+  const c10::DeviceGuard guard(x.device());
+  OptTensor dx, dw, db;
+  Tensor dz = dy;
+  if (y || need_db) {
+    if (y) dz = like(x, {l.rows, l.co});
+    if (need_db) db = like(x, {l.groups, l.co});
+    size_t bytes = 0;
+    check_rc(spira_hip_grouped_linear_activation_gradient_workspace(l.rows, l.groups, l.co, &bytes), "grouped_linear");
+    Tensor ws = workspace(bytes, x.device());
+    check_rc(spira_hip_grouped_linear_activation_gradient(l.rows, l.groups, off, dy.data_ptr(), ptr(y), l.co, dtype,
+                                                          dz.data_ptr(), db ? db->data_ptr() : nullptr, ws.data_ptr(),
+                                                          bytes, current_stream()),
+             "grouped_linear");
+  }
+  if (need_dx) {
+    // (with slots, each row's share is rounded to the features' type before the
+    // few of a token are added in fp32: half the bytes of fp32 shares, and at
+    // most 1.41 times the rounding error of one rounding at the end)
+    Tensor d = like(x, {l.rows, l.ci});
+    check_rc(spira_hip_grouped_linear_rows_gradient(l.rows, l.groups, off, dz.data_ptr(), l.co, w.data_ptr(), l.ci,
+                                                    dtype, d.data_ptr(), current_stream()),
+             "grouped_linear");
+    if (slots) {
+      dx = like(x, x.sizes());
+      if (slots->size(1) > 0)
+        check_rc(spira_hip_combine(d.data_ptr(), l.rows, slots->data_ptr<int32_t>(), nullptr, x.size(0),
+                                   slots->size(1), l.ci, dtype, dx->data_ptr(), current_stream()),
+                 "grouped_linear");
+      else
+        dx->zero_();
+    } else {
+      dx = d;
+    }
+  }
+  if (need_dw) {
+    dw = like(w, w.sizes());
+    size_t bytes = 0;
+    check_rc(spira_hip_grouped_linear_weights_gradient_workspace(l.rows, l.groups, l.ci, l.co, &bytes),
+             "grouped_linear");
+    Tensor ws = workspace(bytes, x.device());
+    check_rc(spira_hip_grouped_linear_weights_gradient(l.rows, l.groups, off,
+                                                       static_cast<const int32_t *>(ptr(sources)), x.size(0),
+                                                       x.data_ptr(), l.ci, dz.data_ptr(), l.co, dtype, dw->data_ptr(),
+                                                       ws.data_ptr(), bytes, current_stream()),
+             "grouped_linear");
+  }
+  return {dx, dw, db};
+}
+
+static std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route(const Tensor &logits, int64_t k, bool renormalize) {
+  require(logits, "logits", logits, logits.scalar_type(), {-1, -1});
+  const int dtype = row_dtype(logits);
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  SPIRA_CHECK_ARG(experts > 0 && experts <= 512, "route_experts: needs 1 to 512 experts, got ", experts);
+  SPIRA_CHECK_ARG(k > 0 && k <= 16 && k <= experts, "route_experts: needs 1 to 16 choices of ", experts,
+                  " experts, got ", k);
+  const c10::DeviceGuard guard(logits.device());
+  size_t bytes = 0;
+  check_rc(spira_hip_route_workspace(tokens, experts, k, &bytes), "route_experts");
+  Tensor weights = floats(logits, {tokens, k}), chosen = empty_i32({tokens, k}, logits.device());
+  Tensor offsets = empty_i32({experts + 1}, logits.device()), rows = empty_i32({tokens * k}, logits.device());
+  Tensor slots = empty_i32({tokens, k}, logits.device()), ws = workspace(bytes, logits.device());
+  check_rc(spira_hip_route(logits.data_ptr(), tokens, experts, k, dtype, renormalize, weights.data_ptr<float>(),
+                           chosen.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), rows.data_ptr<int32_t>(),
+                           slots.data_ptr<int32_t>(), ws.data_ptr(), bytes, current_stream()),
+           "route_experts");
+  return {weights, chosen, offsets, rows, slots};
+}
+
+static Tensor route_backward(const Tensor &logits, const Tensor &weights, const Tensor &chosen, const Tensor &dweights,
+                             bool renormalize) {
+  require(logits, "logits", logits, logits.scalar_type(), {-1, -1});
+  const int dtype = row_dtype(logits);
+  require(chosen, "experts", logits, torch::kInt, {logits.size(0), -1});
+  require(weights, "weights", logits, torch::kFloat, {logits.size(0), chosen.size(1)});
+  require(dweights, "gradient", logits, torch::kFloat, {logits.size(0), chosen.size(1)});
+  const c10::DeviceGuard guard(logits.device());
+  Tensor d = like(logits, logits.sizes());
+  check_rc(spira_hip_route_backward(logits.data_ptr(), logits.size(0), logits.size(1), chosen.size(1), dtype,
+                                    renormalize, weights.data_ptr<float>(), chosen.data_ptr<int32_t>(),
+                                    dweights.data_ptr<float>(), d.data_ptr(), current_stream()),
+           "route_experts");
+  return d;
+}
+
+static void check_combine(const Tensor &h, const Tensor &slots, const Tensor &weights) {
+  require(h, "features", h, h.scalar_type(), {-1, -1});
+  (void)row_dtype(h);
+  require(slots, "slots", h, torch::kInt, {-1, -1});
+  require(weights, "weights", h, torch::kFloat, {slots.size(0), slots.size(1)});
+  SPIRA_CHECK_ARG(slots.size(1) > 0 && h.size(1) > 0, "combine_experts: no choices or no channels");
+}
+
+static Tensor combine(const Tensor &h, const Tensor &slots, const Tensor &weights) {
+  check_combine(h, slots, weights);
+  const c10::DeviceGuard guard(h.device());
+  Tensor y = like(h, {slots.size(0), h.size(1)});
+  check_rc(spira_hip_combine(h.data_ptr(), h.size(0), slots.data_ptr<int32_t>(), weights.data_ptr<float>(),
+                             slots.size(0), slots.size(1), h.size(1), row_dtype(h), y.data_ptr(), current_stream()),
+           "combine_experts");
+  return y;
+}
+
+static std::tuple<OptTensor, OptTensor> combine_backward(const Tensor &h, const Tensor &rows, const Tensor &slots,
+                                                         const Tensor &weights, const Tensor &dy, bool need_dh,
+                                                         bool need_dw) {
+  check_combine(h, slots, weights);
+  require(rows, "rows", h, torch::kInt, {h.size(0)});
+  require(dy, "gradient", h, h.scalar_type(), {slots.size(0), h.size(1)});
+  const c10::DeviceGuard guard(h.device());
+  OptTensor dh, dw;
+  if (need_dh) dh = like(h, h.sizes());
+  if (need_dw) dw = floats(h, weights.sizes());
+  check_rc(spira_hip_combine_backward(h.data_ptr(), h.size(0), rows.data_ptr<int32_t>(), slots.data_ptr<int32_t>(),
+                                      weights.data_ptr<float>(), dy.data_ptr(), slots.size(0), slots.size(1),
+                                      h.size(1), row_dtype(h), dh ? dh->data_ptr() : nullptr,
+                                      dw ? dw->data_ptr<float>() : nullptr, current_stream()),
+           "combine_experts");
+  return {dh, dw};
+}
+
+struct NormShape {
+  int64_t n, c;
+  int gate_form;
+};
+
+static NormShape check_norm(const Tensor &x, const OptTensor &h, const OptTensor &weight, const OptTensor &gate,
+                            const OptTensor &next_weight) {
+  const auto type = x.scalar_type();
+  require(x, "residual", x, type, {-1, -1});
+  (void)row_dtype(x);
+  const int64_t n = x.size(0), c = x.size(1);
+  SPIRA_CHECK_ARG(c > 0 && c <= 16384, "gated_residual_norm: needs 1 to 16384 channels, got ", c);
+  require(h, "update", x, type, {n, c});
+  require(weight, "weight", x, type, {c});
+  require(next_weight, "next_weight", x, type, {c});
+  SPIRA_CHECK_ARG(h || next_weight, "gated_residual_norm: neither an update nor a next norm");
+  SPIRA_CHECK_ARG(h || (!weight && !gate), "gated_residual_norm: a weight or gate without an update");
+  int form = 0;
+  if (gate) {
+    form = gate->dim() == 1 ? 1 : gate->dim() == 2 && gate->size(1) == 1 && c > 1 ? 2 : 3;
+    if (form == 1) require(*gate, "gate", x, type, {c});
+    else require(*gate, "gate (of two dimensions)", x, type, {n, form == 2 ? 1 : c});
+  }
+  return {n, c, form};
+}
+
+// (r or None without an update, next or None, 1 / root mean squares of the
+// update and of r, or None unless `train`)
+static std::tuple<OptTensor, OptTensor, OptTensor, OptTensor> gated_residual_norm(
+    const Tensor &x, const OptTensor &h, const OptTensor &weight, const OptTensor &gate, bool gate_sigmoid,
+    double scale, const OptTensor &next_weight, double eps, bool train) {
+  const NormShape s = check_norm(x, h, weight, gate, next_weight);
+  const c10::DeviceGuard guard(x.device());
+  OptTensor r, next, inv_h, inv_r;
+  if (h) r = like(x, x.sizes());
+  if (next_weight) next = like(x, x.sizes());
+  if (train && weight) inv_h = floats(x, {s.n});
+  if (train && next_weight) inv_r = floats(x, {s.n});
+  const auto at = [](OptTensor &t) { return t ? t->data_ptr() : nullptr; };
+  check_rc(spira_hip_gated_residual_norm(x.data_ptr(), ptr(h), s.n, s.c, row_dtype(x), ptr(weight), ptr(gate),
+                                         s.gate_form, gate_sigmoid, scale, ptr(next_weight), eps, at(r), at(next),
+                                         static_cast<float *>(at(inv_h)), static_cast<float *>(at(inv_r)),
+                                         current_stream()),
+           "gated_residual_norm");
+  return {r, next, inv_h, inv_r};
+}
+
+// (dx, dh, dweight, dgate, dnext_weight), each None unless it is in `need`
+static std::vector<OptTensor> gated_residual_norm_backward(
+    const Tensor &x, const OptTensor &h, const OptTensor &weight, const OptTensor &gate, bool gate_sigmoid,
+    double scale, const OptTensor &next_weight, const OptTensor &inv_h, const OptTensor &inv_r, const OptTensor &dr,
+    const OptTensor &dnext, const std::array<bool, 5> &need) {
+  const NormShape s = check_norm(x, h, weight, gate, next_weight);
+  const auto type = x.scalar_type();
+  require(inv_h, "inverse root mean squares", x, torch::kFloat, {s.n});
+  require(inv_r, "inverse root mean squares", x, torch::kFloat, {s.n});
+  require(dr, "gradient", x, type, {s.n, s.c});
+  require(dnext, "gradient", x, type, {s.n, s.c});
+  SPIRA_CHECK_ARG((!weight || inv_h) && (!dnext || (inv_r && next_weight)),
+                  "gated_residual_norm: the forward pass kept nothing for a gradient");
+  const c10::DeviceGuard guard(x.device());
+  std::vector<OptTensor> d(5);
+  if (need[0]) d[0] = like(x, x.sizes());
+  if (need[1] && h) d[1] = like(x, x.sizes());
+  if (need[2] && weight) d[2] = like(x, {s.c});
+  if (need[3] && gate) d[3] = like(x, gate->sizes());
+  if (need[4] && next_weight) d[4] = dnext ? like(x, {s.c}) : torch::zeros({s.c}, x.options());
+  size_t bytes = 0;
+  check_rc(spira_hip_gated_residual_norm_backward_workspace(s.n, s.c, row_dtype(x), &bytes), "gated_residual_norm");
+  Tensor ws = workspace(bytes, x.device());
+  const auto at = [&](int i) { return d[i] ? d[i]->data_ptr() : nullptr; };
+  check_rc(spira_hip_gated_residual_norm_backward(
+               x.data_ptr(), ptr(h), s.n, s.c, row_dtype(x), ptr(weight), ptr(gate), s.gate_form, gate_sigmoid, scale,
+               ptr(next_weight), static_cast<const float *>(ptr(inv_h)), static_cast<const float *>(ptr(inv_r)),
+               ptr(dr), ptr(dnext), at(0), at(1), at(2), at(3), at(4), ws.data_ptr(), bytes, current_stream()),
+           "gated_residual_norm");
+  return d;
+}
+
+static Tensor dropout(const Tensor &x, double p, uint64_t seed, uint64_t offset, const OptTensor &residual) {
+  require_device(x, "features");
+  const int dtype = row_dtype(x);
+  SPIRA_CHECK_ARG(p >= 0.0 && p <= 1.0, "dropout: p must be in [0, 1], got ", p);
+  if (residual) {
+    require_device(*residual, "residual");
+    SPIRA_CHECK_ARG(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type() &&
+                        residual->device() == x.device(),
+                    "residual must have the features' shape, type and device");
+  }
+  const c10::DeviceGuard guard(x.device());
+  Tensor y = like(x, x.sizes());
+  check_rc(spira_hip_dropout(x.data_ptr(), ptr(residual), x.numel(), dtype, p, seed, offset, y.data_ptr(),
+                             current_stream()),
+           "dropout");
+  return y;
+}
+
+void register_experts(pybind11::module_ &m) {
+  m.def("grouped_linear", &grouped_linear);
+  m.def("grouped_linear_backward", &grouped_linear_backward);
+  m.def("route_experts", &route);
+  m.def("route_experts_backward", &route_backward);
+  m.def("combine_experts", &combine);
+  m.def("combine_experts_backward", &combine_backward);
+  m.def("gated_residual_norm", &gated_residual_norm);
+  m.def("gated_residual_norm_backward", &gated_residual_norm_backward);
+  m.def("dropout", &dropout);
+}
+
+}  // namespace spira_host

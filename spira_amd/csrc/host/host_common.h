@@ -129,5 +129,6 @@ std::vector<int32_t> indexes_l1(int kx, int ky, int kz, int dataflow, int *front
 void register_coords(pybind11::module_ &m);
 void register_mapping(pybind11::module_ &m);
 void register_conv(pybind11::module_ &m);
+void register_experts(pybind11::module_ &m);
 
 }  // namespace spira_host

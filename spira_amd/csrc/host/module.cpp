@@ -8,4 +8,5 @@ PYBIND11_MODULE(_C, m) {
   spira_host::register_coords(m);
   spira_host::register_mapping(m);
   spira_host::register_conv(m);
+  spira_host::register_experts(m);
 }
