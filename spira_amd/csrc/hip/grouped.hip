@@ -96,6 +96,13 @@ __device__ __forceinline__ void parts_of(const Groups &g, int size, int group, i
   count = n > 0 ? (n + size - 1) / size : 0;
 }
 
+// parts of all groups
+__device__ __forceinline__ int64_t count_parts(const Groups &g, int size) {
+  int64_t first, count;
+  parts_of(g, size, g.count - 1, first, count);
+  return first + count;
+}
+
 // most parts that any offsets of `count` groups over `rows` rows can have
 static int64_t most_parts(int64_t rows, int64_t count, int64_t size) {
   return (rows + std::min(rows, count) * (size - 1)) / size;
@@ -118,8 +125,10 @@ __device__ void clear_ungrouped(const Groups &g, T *y, int64_t n, int64_t index,
 constexpr int kStep = 128;  // bytes of the summed index per step
 template <class T> constexpr int kStepK = kStep / static_cast<int>(sizeof(T));
 
-__device__ __forceinline__ uint32_t lds_of(const void *p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)(const_cast<void *>(p))));
+// Four 16-bit values of 16 lanes, transposed: lane i of the 16 gets value i % 4
+// of lanes i / 4 + {0, 4, 8, 12}.
+__device__ __forceinline__ short4v read_tr(const char *p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(const_cast<char *>(p)));
 }
 
 // KC: row r's 16-byte chunk c at r * 128 + (c ^ (r / 2 % 8)) * 16, so that the
@@ -150,10 +159,7 @@ template <class T, int N> __device__ __forceinline__ uintx4_t ko_frag(const char
   const int lane = lane_id(), i = lane & 15, q = lane >> 4;
   if constexpr (sizeof(T) == 2) {
     const int k = kk * 32 + q * 8 + (i >> 2), c = n0 / 8 + ((i & 3) >> 1), half = (i & 1) * 8;
-    const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_short4 *)static_cast<uintptr_t>(lds_of(tile + ko_at<T, N>(k, c) + half)));
-    const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_short4 *)static_cast<uintptr_t>(lds_of(tile + ko_at<T, N>(k + 4, c) + half)));
+    const auto lo = read_tr(tile + ko_at<T, N>(k, c) + half), hi = read_tr(tile + ko_at<T, N>(k + 4, c) + half);
     const uintx2_t a = __builtin_bit_cast(uintx2_t, lo), b = __builtin_bit_cast(uintx2_t, hi);
     return {a[0], a[1], b[0], b[1]};
   } else {
@@ -371,6 +377,394 @@ template <class T, bool KO> __global__ __launch_bounds__(kThreads) void rows_ker
   }
 }
 
+// ---------------------------------------------------------------------------
+// Rows streamed past weights that stay in LDS.  Where a group's weights fit
+// there, the operator is bound by its rows' bytes: a block lays the weights out
+// once, one 1 KB block per MFMA fragment in lane order, and its eight waves then
+// walk the rows of its part on their own, without barriers, each holding a
+// tile's rows in registers and fetching the next tile's meanwhile.
+//
+// The 64 channels of four fragments are dealt out so that a lane's sums are 16
+// consecutive channels of its row: whole 128-byte lines are written straight
+// from registers.
+// ---------------------------------------------------------------------------
+constexpr int kStreamWaves = 8, kStreamThreads = 64 * kStreamWaves;
+constexpr int kMostStreamFragments = 144;  // 1 KB each: 16 KB of the LDS left
+
+// the channel (of 64) of operand row i of fragment j
+__device__ __forceinline__ int dealt(int j, int i) { return (i >> 2) * 16 + j * 4 + (i & 3); }
+
+struct StreamArgs {
+  RowsArgs a;
+  int part_rows;
+};
+
+// KF: fragments (64 bytes) of a row; MT: 16-row tiles a wave takes at a time
+template <class T, bool KO, int KF, int MT>
+__global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(KF * MT <= 8 ? 4 : 2))) void stream_kernel(const StreamArgs sa) {
+  constexpr int FK = 64 / static_cast<int>(sizeof(T));  // values of the summed index per fragment
+  constexpr int MOST = kMostStreamFragments / kStreamWaves;
+  extern __shared__ __align__(1024) char wlds[];
+  const RowsArgs &a = sa.a;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, lq = lane >> 4;
+  const Part part = find_part(a.g, sa.part_rows, blockIdx.x);
+  if (part.group < 0) {
+    clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, part.begin, gridDim.x - (blockIdx.x - part.begin), kStreamThreads);
+    return;
+  }
+  const T *w = static_cast<const T *>(a.w) + part.group * a.k * a.n;
+  const int quads = static_cast<int>((a.n + 63) / 64);  // of fragments
+  const int fragments = quads * 4 * KF;
+  // the first tile's rows are on their way while the weights are laid out
+  const T *row[MT];
+  uintx4_t next[MT][KF];
+  auto find_rows = [&](int64_t r0) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int64_t r = r0 + m * 16 + l16;
+      int64_t s = r < part.end ? r : -1;
+      if (s >= 0 && a.source) {
+        s = a.source[r];
+        if (s >= a.num_sources) s = -1;
+      }
+      row[m] = s >= 0 ? static_cast<const T *>(a.x) + s * a.k : nullptr;
+    }
+  };
+  auto fetch = [&] {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int f = 0; f < KF; ++f) {
+        const int64_t k = f * FK + lq * kVec<T>;
+        next[m][f] = load_raw(row[m] + k, row[m] ? a.k - k : 0);
+      }
+  };
+  find_rows(part.begin + wave * 16 * MT);
+  if constexpr (KO) {
+    // as they lie in memory, [KF FK, quads 64], zeros past their ends; then, all
+    // in registers between two barriers, to fragments
+    const int cpr = quads * 64 / kVec<T>;
+    for (int id = threadIdx.x; id < KF * FK * cpr; id += kStreamThreads) {
+      const int k = id / cpr, c = id - k * cpr;
+      const T *p = w + k * a.n + c * kVec<T>;
+      *reinterpret_cast<uintx4_t *>(wlds + id * 16) = load_raw(p, k < a.k ? a.n - c * kVec<T> : 0);
+    }
+    __syncthreads();
+    uintx4_t v[MOST];
+#pragma unroll
+    for (int q = 0; q < MOST; ++q) {
+      const int id = q * kStreamWaves + wave;
+      if (id >= fragments) break;
+      const int j = id / KF % 4, f = id % KF, col = id / (4 * KF) * 64;
+      const int pitch = quads * 64 * static_cast<int>(sizeof(T));
+      if constexpr (sizeof(T) == 2) {
+        const char *at = wlds + (f * 32 + lq * 8 + (l16 >> 2)) * pitch + (col + dealt(j, (l16 & 3) * 4)) * 2;
+        const auto lo = read_tr(at), hi = read_tr(at + 4 * pitch);
+        const uintx2_t x = __builtin_bit_cast(uintx2_t, lo), y = __builtin_bit_cast(uintx2_t, hi);
+        v[q] = uintx4_t{x[0], x[1], y[0], y[1]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[q][i] = *reinterpret_cast<const uint32_t *>(wlds + (f * 16 + lq * 4 + i) * pitch + (col + dealt(j, l16)) * 4);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < MOST; ++q) {
+      const int id = q * kStreamWaves + wave;
+      if (id < fragments) *reinterpret_cast<uintx4_t *>(wlds + id * 1024 + lane * 16) = v[q];
+    }
+  } else {
+    for (int id = wave; id < fragments; id += kStreamWaves) {
+      const int j = id / KF % 4, f = id % KF;
+      const int64_t n = id / (4 * KF) * 64 + dealt(j, l16), k = f * FK + lq * kVec<T>;
+      *reinterpret_cast<uintx4_t *>(wlds + id * 1024 + lane * 16) = load_raw(w + n * a.k + k, n < a.n ? a.k - k : 0);
+    }
+  }
+  fetch();
+  __syncthreads();
+  const T *bias = a.bias ? static_cast<const T *>(a.bias) + part.group * a.n : nullptr;
+  for (int64_t r0 = part.begin + wave * 16 * MT; r0 < part.end; r0 += kStreamWaves * 16 * MT) {
+    uintx4_t x[MT][KF];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int f = 0; f < KF; ++f) x[m][f] = next[m][f];
+    find_rows(r0 + kStreamWaves * 16 * MT);
+    fetch();
+    for (int q = 0; q < quads; ++q) {
+      floatx4_t acc[MT][4] = {};
+      const char *wq = wlds + q * 4 * KF * 1024 + lane * 16;
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uintx4_t b = *reinterpret_cast<const uintx4_t *>(wq + (j * KF + f) * 1024);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) mma<T>(acc[m][j], b, x[m][f]);
+        }
+      const int64_t n = q * 64 + lq * 16;
+      if (n >= a.n) continue;
+#pragma unroll
+      for (int h = 0; h < 16 / kVec<T>; ++h) {
+        Chunk<T> b{};
+        if (bias) b = load_chunk(bias + n + h * kVec<T>, a.n - n - h * kVec<T>);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int64_t r = r0 + m * 16 + l16;
+          if (r >= part.end) continue;
+          Chunk<T> c;
+#pragma unroll
+          for (int v = 0; v < kVec<T>; ++v) {
+            const float s = acc[m][(h * kVec<T> + v) / 4][v % 4] + b.v[v];
+            c.v[v] = a.relu && s < 0.f ? 0.f : s;
+          }
+          store_chunk(static_cast<T *>(a.y) + r * a.n + n + h * kVec<T>, a.n - n - h * kVec<T>, c);
+        }
+      }
+    }
+  }
+}
+
+// Whether the weights fit (their fragments), and the shape that holds a row.
+template <class T> static bool streams(int64_t k, int64_t n) {
+  const int64_t f = div_up(k * static_cast<int64_t>(sizeof(T)), 64);
+  const int64_t kf = f <= 4 ? f : f <= 6 ? 6 : f <= 8 ? 8 : f <= 12 ? 12 : 16;
+  return f <= 16 && kf * 4 * div_up(n, 64) <= kMostStreamFragments;
+}
+
+template <class T, bool KO> static int launch_stream(const RowsArgs &a, hipStream_t stream) {
+  const auto go = [&](auto KF, auto MT) -> int {
+    constexpr int kf = decltype(KF)::value, mt = decltype(MT)::value;
+    const size_t lds = static_cast<size_t>(kf) * 4 * div_up(a.n, 64) * 1024;
+    // a part gives each wave one or two tiles
+    const int rows = kStreamWaves * 16 * mt * (a.g.rows >= 65536 ? 2 : 1);
+    const auto kernel = stream_kernel<T, KO, kf, mt>;
+    SPIRA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, kMostStreamFragments * 1024));
+    hipLaunchKernelGGL(kernel, dim3(most_parts(a.g.rows, a.g.count, rows) + 1), dim3(kStreamThreads), lds, stream,
+                       StreamArgs{a, rows});
+    SPIRA_HIP_LAUNCH_CHECK();
+    return kOk;
+  };
+  using std::integral_constant;
+  const int64_t f = div_up(a.k * static_cast<int64_t>(sizeof(T)), 64);
+  constexpr integral_constant<int, 1> one;
+  constexpr integral_constant<int, 2> two;
+  switch (f) {
+    case 1: return go(integral_constant<int, 1>{}, two);
+    case 2: return go(integral_constant<int, 2>{}, two);
+    case 3: return go(integral_constant<int, 3>{}, two);
+    case 4: return go(integral_constant<int, 4>{}, two);
+    case 5: case 6: return go(integral_constant<int, 6>{}, two);
+    case 7: case 8: return go(integral_constant<int, 8>{}, one);
+    case 9: case 10: case 11: case 12: return go(integral_constant<int, 12>{}, one);
+    default: return go(integral_constant<int, 16>{}, one);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Tiles fed by DMA: rows and widths of whole 16-byte chunks.  The global loads
+// write LDS themselves (no registers, no address arithmetic but one add a
+// load), a step ahead of the products, in two stages.  The LDS swizzle is made
+// by the order in which the lanes fetch a row's chunks.  Chunks past a row's end
+// and rows that are not there are out of the buffer's range: they load zeros.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kOutOfRange = 0x80000000u;
+constexpr int64_t kBufferLimit = int64_t(1) << 31;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *base, int64_t bytes) {
+  const int64_t n = bytes < 0 ? 0 : bytes < kBufferLimit ? bytes : kBufferLimit - 1;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(n), 0x00020000);
+}
+// 1 KB to LDS, 16 bytes from each lane's offset
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, uint32_t offset, char *to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void *)to, 16, offset, 0, 0, 0);
+}
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
+
+// Block w's place among `count` pieces of work so that each of the 8 XCDs (w %
+// 8) takes one range of them; w itself past them.
+__device__ __forceinline__ int64_t xcd_order(int64_t w, int64_t count) {
+  if (w >= count) return w;
+  const int64_t q = count / 8, r = count % 8, x = w % 8;
+  return x * q + (x < r ? x : r) + w / 8;
+}
+
+template <class T, int M, int N, int WM, int WN> struct Tile {
+  static constexpr int NW = (M / WM) * (N / WN), NT = 64 * NW;
+  static constexpr int MI = WM / 16, NI = WN / 16;
+  static constexpr int XL = M / 8 / NW, WL = N / 8 / NW;  // loads (1 KB) a wave and step
+  static constexpr int XBYTES = M * kStep, WBYTES = N * kStep;
+  static_assert(XL >= 1 && WL >= 1 && XL * NW * 8 == M && WL * NW * 8 == N, "tile shape");
+};
+
+// where lane `lane` of a tile's load `i` (1 KB) reads: KC row and chunk; KO row k and chunk
+__device__ __forceinline__ void kc_source(int i, int lane, int &r, int &c) {
+  r = i * 8 + (lane >> 3);
+  c = (lane & 7) ^ ((r >> 1) & 7);
+}
+template <class T, int N> __device__ __forceinline__ void ko_source(int i, int lane, int &k, int &c) {
+  constexpr int CPR = N * static_cast<int>(sizeof(T)) / 16;
+  const int id = i * 64 + lane;
+  k = id / CPR;
+  c = (ko_at<T, N>(k, id % CPR) - k * CPR * 16) >> 4;
+}
+
+template <class T, int MI, int NI> struct TileSums {
+  floatx4_t v[MI][NI];
+};
+
+template <class T, int MI, int NI, class MFrag, class NFrag>
+__device__ __forceinline__ void multiply_tile(TileSums<T, MI, NI> &acc, MFrag &&mf, NFrag &&nf) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    uintx4_t m[MI], n[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) n[i] = nf(i, kk);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) m[i] = mf(i, kk);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) mma<T>(acc.v[i][j], n[j], m[i]);
+  }
+}
+
+template <class T, bool KO, int M, int N, int WM, int WN>
+__global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) void tile_kernel(const RowsArgs a) {
+  using S = Tile<T, M, N, WM, WN>;
+  __shared__ __align__(1024) char x0[S::XBYTES], x1[S::XBYTES], w0[S::WBYTES], w1[S::WBYTES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t cols = (a.n + N - 1) / N, parts = count_parts(a.g, M);
+  const int64_t place = xcd_order(blockIdx.x, parts * cols);
+  const Part part = find_part(a.g, M, place / cols);
+  if (part.group < 0) {
+    clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, place - parts * cols, gridDim.x - parts * cols, S::NT);
+    return;
+  }
+  const int64_t n0 = place % cols * N;
+  const uint32_t kbytes = static_cast<uint32_t>(a.k * static_cast<int64_t>(sizeof(T)));
+  const uint32_t nbytes = static_cast<uint32_t>(a.n * static_cast<int64_t>(sizeof(T)));
+  const __amdgpu_buffer_rsrc_t xr =
+      a.source ? buffer(a.x, a.num_sources * kbytes)
+               : buffer(static_cast<const char *>(a.x) + part.begin * kbytes, (part.end - part.begin) * kbytes);
+  const __amdgpu_buffer_rsrc_t wr =
+      buffer(static_cast<const char *>(a.w) + part.group * a.k * nbytes, a.k * static_cast<int64_t>(nbytes));
+  uint32_t xo[S::XL], xc[S::XL], wo[S::WL], wc[S::WL];
+#pragma unroll
+  for (int i = 0; i < S::XL; ++i) {
+    int r, c;
+    kc_source(wave * S::XL + i, lane, r, c);
+    xc[i] = c * 16;
+    xo[i] = kOutOfRange;
+    if (part.begin + r < part.end) {
+      const int64_t s = a.source ? a.source[part.begin + r] : r;
+      if (s >= 0 && (!a.source || s < a.num_sources)) xo[i] = static_cast<uint32_t>(s) * kbytes + xc[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < S::WL; ++i) {
+    int r, c;
+    if constexpr (KO) {
+      ko_source<T, N>(wave * S::WL + i, lane, r, c);
+      wc[i] = 0;
+      wo[i] = r * nbytes + static_cast<uint32_t>(n0 * sizeof(T)) + c * 16;
+    } else {
+      kc_source(wave * S::WL + i, lane, r, c);
+      wc[i] = c * 16;
+      wo[i] = n0 + r < a.n ? static_cast<uint32_t>(n0 + r) * kbytes + wc[i] : kOutOfRange;
+    }
+  }
+  const int steps = static_cast<int>((kbytes + kStep - 1) / kStep);
+  auto issue = [&](int step, char *xs, char *ws) {
+    const uint32_t kb = step * kStep;
+#pragma unroll
+    for (int i = 0; i < S::XL; ++i)
+      load_lds(xr, kb + xc[i] < kbytes ? xo[i] + kb : kOutOfRange, xs + (wave * S::XL + i) * 1024);
+    // (KO weights past the last row of the group: out of range)
+    const uint32_t wb = KO ? step * static_cast<uint32_t>(kStepK<T>) * nbytes : kb;
+#pragma unroll
+    for (int i = 0; i < S::WL; ++i)
+      load_lds(wr, KO || kb + wc[i] < kbytes ? wo[i] + wb : kOutOfRange, ws + (wave * S::WL + i) * 1024);
+  };
+  const int m0 = wave / (N / WN) * WM, c0 = wave % (N / WN) * WN;
+  TileSums<T, S::MI, S::NI> acc{};
+  auto compute = [&](const char *xs, const char *ws) {
+    multiply_tile<T, S::MI, S::NI>(
+        acc, [&](int i, int kk) { return kc_frag(xs, m0 + i * 16, kk); },
+        [&](int i, int kk) {
+          if constexpr (KO) return ko_frag<T, N>(ws, c0 + i * 16, kk);
+          else return kc_frag(ws, c0 + i * 16, kk);
+        });
+  };
+  issue(0, x0, w0);
+  wait_loads();
+  __syncthreads();
+  for (int step = 0;;) {
+    if (step + 1 < steps) issue(step + 1, x1, w1);
+    compute(x0, w0);
+    if (++step == steps) break;
+    wait_loads();
+    __syncthreads();
+    if (step + 1 < steps) issue(step + 1, x0, w0);
+    compute(x1, w1);
+    if (++step == steps) break;
+    wait_loads();
+    __syncthreads();
+  }
+  const T *bias = a.bias ? static_cast<const T *>(a.bias) + part.group * a.n : nullptr;
+#pragma unroll
+  for (int j = 0; j < S::NI; ++j) {
+    const int64_t n = n0 + c0 + j * 16 + (lane >> 4) * 4;
+    if (n >= a.n) continue;  // (widths are whole chunks, so that four values are inside or not)
+    floatx4_t b = {0, 0, 0, 0};
+    if (bias)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) b[v] = to_float(bias[n + v]);
+#pragma unroll
+    for (int i = 0; i < S::MI; ++i) {
+      const int64_t r = part.begin + m0 + i * 16 + (lane & 15);
+      if (r >= part.end) continue;
+      floatx4_t v = acc.v[i][j] + b;
+      if (a.relu)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
+      store4(static_cast<T *>(a.y) + r * a.n + n, 4, v);
+    }
+  }
+}
+
+static bool aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Whether DMA can feed the tiles.
+template <class T> static bool dma_fits(const RowsArgs &a) {
+  const int64_t size = sizeof(T);
+  return a.k % kVec<T> == 0 && a.n % kVec<T> == 0 && aligned(a.x) && aligned(a.w) && a.k * a.n * size < kBufferLimit &&
+         a.k * size <= (1 << 22) && (!a.source || a.num_sources * a.k * size < kBufferLimit);
+}
+
+template <class T, bool KO, int M, int N, int WM, int WN> static int launch_tile(const RowsArgs &a, hipStream_t stream) {
+  const int64_t blocks = (most_parts(a.g.rows, a.g.count, M)) * div_up(a.n, N) + 1;
+  SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear: too many tiles");
+  hipLaunchKernelGGL((tile_kernel<T, KO, M, N, WM, WN>), dim3(blocks), dim3(Tile<T, M, N, WM, WN>::NT), 0, stream, a);
+  SPIRA_HIP_LAUNCH_CHECK();
+  return kOk;
+}
+
+template <class T, bool KO> static int launch_rows(const RowsArgs &a, hipStream_t stream) {
+  if (streams<T>(a.k, a.n)) return launch_stream<T, KO>(a, stream);
+  if (dma_fits<T>(a)) {
+    if constexpr (sizeof(T) == 2)
+      if (a.g.rows / a.g.count >= 512 && a.n >= 256) return launch_tile<T, KO, 256, 256, 128, 64>(a, stream);
+    return launch_tile<T, KO, 128, 128, 64, 64>(a, stream);
+  }
+  hipLaunchKernelGGL((rows_kernel<T, KO>), dim3(most_parts(a.g.rows, a.g.count, kRows) + 1, div_up(a.n, kCols)),
+                     dim3(kThreads), 0, stream, a);
+  SPIRA_HIP_LAUNCH_CHECK();
+  return kOk;
+}
+
 struct WeightsArgs {
   Groups g;
   const int32_t *source;
@@ -450,18 +844,121 @@ template <class T> __global__ __launch_bounds__(kThreads) void weights_kernel(co
     }
 }
 
-// out[e] = sum of the group's parts, in order: `size` values each
+// The same fed by DMA, as tile_kernel.
+template <class T, int M, int N, int WM, int WN>
+__global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) __attribute__((amdgpu_waves_per_eu(2))) void weights_tile_kernel(const WeightsArgs a) {
+  using S = Tile<T, M, N, WM, WN>;
+  __shared__ __align__(1024) char x0[S::XBYTES], x1[S::XBYTES], z0[S::WBYTES], z1[S::WBYTES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t mt = (a.ci + M - 1) / M, nt = (a.co + N - 1) / N, tiles = mt * nt;
+  const int64_t parts = a.partial ? count_parts(a.g, a.part_rows) : a.g.count;
+  const int64_t place = xcd_order(blockIdx.x, parts * tiles);
+  if (place >= parts * tiles) return;
+  const int64_t nth = place / tiles;
+  Part part;
+  if (a.partial) part = find_part(a.g, a.part_rows, nth);
+  else part = {static_cast<int>(nth), uniform(bound(a.g, nth)), uniform(bound(a.g, nth + 1))};
+  const int64_t m0 = place % tiles / nt * M, n0 = place % nt * N;
+  const uint32_t xbytes = static_cast<uint32_t>(a.ci * static_cast<int64_t>(sizeof(T)));
+  const uint32_t zbytes = static_cast<uint32_t>(a.co * static_cast<int64_t>(sizeof(T)));
+  const __amdgpu_buffer_rsrc_t gathered = buffer(a.x, a.num_sources * xbytes);
+  int xk[S::XL], zk[S::WL];
+  uint32_t xo[S::XL], zo[S::WL];
+#pragma unroll
+  for (int i = 0; i < S::XL; ++i) {
+    int c;
+    ko_source<T, M>(wave * S::XL + i, lane, xk[i], c);
+    xo[i] = static_cast<uint32_t>(m0 * sizeof(T)) + c * 16;
+    if (xo[i] >= xbytes) xo[i] = kOutOfRange;
+  }
+#pragma unroll
+  for (int i = 0; i < S::WL; ++i) {
+    int c;
+    ko_source<T, N>(wave * S::WL + i, lane, zk[i], c);
+    zo[i] = static_cast<uint32_t>(n0 * sizeof(T)) + c * 16;
+    if (zo[i] >= zbytes) zo[i] = kOutOfRange;
+  }
+  // the sources of a step's rows, fetched a step before their loads are issued
+  int32_t src[S::XL];
+  auto look = [&](int64_t r0) {
+#pragma unroll
+    for (int i = 0; i < S::XL; ++i) src[i] = r0 + xk[i] < part.end ? a.source[r0 + xk[i]] : -1;
+  };
+  auto issue = [&](int64_t r0, char *xs, char *zs) {
+    if (a.source) {
+#pragma unroll
+      for (int i = 0; i < S::XL; ++i) {
+        const bool in = src[i] >= 0 && src[i] < a.num_sources && xo[i] != kOutOfRange;
+        load_lds(gathered, in ? static_cast<uint32_t>(src[i]) * xbytes + xo[i] : kOutOfRange, xs + (wave * S::XL + i) * 1024);
+      }
+      look(r0 + kStepK<T>);
+    } else {
+      const __amdgpu_buffer_rsrc_t xr = buffer(static_cast<const char *>(a.x) + r0 * xbytes, (part.end - r0) * xbytes);
+#pragma unroll
+      for (int i = 0; i < S::XL; ++i)
+        load_lds(xr, xo[i] + xk[i] * xbytes, xs + (wave * S::XL + i) * 1024);
+    }
+    const __amdgpu_buffer_rsrc_t zr = buffer(static_cast<const char *>(a.dz) + r0 * zbytes, (part.end - r0) * zbytes);
+#pragma unroll
+    for (int i = 0; i < S::WL; ++i)
+      load_lds(zr, zo[i] + zk[i] * zbytes, zs + (wave * S::WL + i) * 1024);
+  };
+  const int wm = wave / (N / WN) * WM, wn = wave % (N / WN) * WN;
+  TileSums<T, S::MI, S::NI> acc{};
+  auto compute = [&](const char *xs, const char *zs) {
+    multiply_tile<T, S::MI, S::NI>(
+        acc, [&](int i, int kk) { return ko_frag<T, M>(xs, wm + i * 16, kk); },
+        [&](int i, int kk) { return ko_frag<T, N>(zs, wn + i * 16, kk); });
+  };
+  if (part.begin < part.end) {
+    if (a.source) look(part.begin);
+    issue(part.begin, x0, z0);
+    wait_loads();
+    __syncthreads();
+    for (int64_t r0 = part.begin;;) {
+      if (r0 + kStepK<T> < part.end) issue(r0 + kStepK<T>, x1, z1);
+      compute(x0, z0);
+      if ((r0 += kStepK<T>) >= part.end) break;
+      wait_loads();
+      __syncthreads();
+      if (r0 + kStepK<T> < part.end) issue(r0 + kStepK<T>, x0, z0);
+      compute(x1, z1);
+      if ((r0 += kStepK<T>) >= part.end) break;
+      wait_loads();
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < S::NI; ++j) {
+      const int64_t m = m0 + wm + i * 16 + (lane & 15), n = n0 + wn + j * 16 + (lane >> 4) * 4;
+      if (m >= a.ci || n >= a.co) continue;
+      if (a.partial) store4(a.partial + (nth * a.ci + m) * a.co + n, 4, acc.v[i][j]);
+      else store4(static_cast<T *>(a.dw) + (part.group * a.ci + m) * a.co + n, 4, acc.v[i][j]);
+    }
+}
+
+template <class T> static bool dma_fits(const WeightsArgs &a) {
+  const int64_t size = sizeof(T);
+  return a.ci % kVec<T> == 0 && a.co % kVec<T> == 0 && aligned(a.x) && aligned(a.dz) && a.ci * size <= (1 << 22) &&
+         a.co * size <= (1 << 22) && (!a.source || a.num_sources * a.ci * size < kBufferLimit);
+}
+
+// out[e] = sum of the group's parts (`size` values each): 16 lanes of four values
+// by 16 threads, each over every 16th part, joined in a fixed tree
 template <class T>
 __global__ __launch_bounds__(256) void join_kernel(const Groups g, int part_rows, int64_t parts, const float *partial,
                                                    int64_t size, T *out) {
+  __shared__ floatx4_t sums[16][16];
   int64_t first, count;
   parts_of(g, part_rows, blockIdx.y, first, count);
   // (overlapping groups count more parts than there are)
   const int64_t last = std::min(first + count, parts);
-  const int64_t i = (blockIdx.x * static_cast<int64_t>(256) + threadIdx.x) * 4;
-  if (i >= size) return;
+  const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t i = (blockIdx.x * static_cast<int64_t>(16) + c) * 4;
   floatx4_t sum = {0, 0, 0, 0};
-  for (int64_t p = first; p < last; ++p) {
+  for (int64_t p = first + q; p < last; p += 16) {
     const float *v = partial + p * size + i;
     if (size - i >= 4) {
       sum += __builtin_bit_cast(floatx4_t, *reinterpret_cast<const uintx4_a4_t *>(v));
@@ -469,7 +966,12 @@ __global__ __launch_bounds__(256) void join_kernel(const Groups g, int part_rows
       for (int j = 0; j < size - i; ++j) sum[j] += v[j];
     }
   }
-  store4(out + blockIdx.y * size + i, size - i, sum);
+  sums[q][c] = sum;
+  for (int half = 8; half > 0; half /= 2) {
+    __syncthreads();
+    if (q < half) sums[q][c] += sums[q + half][c];
+  }
+  if (q == 0 && i < size) store4(out + blockIdx.y * size + i, size - i, sums[0][c]);
 }
 
 // dz = dy where y > 0 (or dy), and the parts' column sums of it: 64 columns by
@@ -554,11 +1056,7 @@ int spira_hip_grouped_linear(int64_t rows, int groups, const int32_t *offsets, c
     using T = decltype(t);
     if (rows == 0) return kOk;
     grouped::RowsArgs a{{offsets, groups, rows}, sources, num_sources, x, weights, bias, c_in, c_out, relu, y};
-    const int64_t parts = grouped::most_parts(rows, groups, grouped::kRows) + 1;
-    hipLaunchKernelGGL((grouped::rows_kernel<T, true>), dim3(parts, div_up(c_out, grouped::kCols)),
-                       dim3(grouped::kThreads), 0, stream, a);
-    SPIRA_HIP_LAUNCH_CHECK();
-    return kOk;
+    return grouped::launch_rows<T, true>(a, stream);
   });
 }
 
@@ -570,11 +1068,7 @@ int spira_hip_grouped_linear_rows_gradient(int64_t rows, int groups, const int32
     using T = decltype(t);
     if (rows == 0) return kOk;
     grouped::RowsArgs a{{offsets, groups, rows}, nullptr, rows, dz, weights, nullptr, c_out, c_in, 0, dx};
-    const int64_t parts = grouped::most_parts(rows, groups, grouped::kRows) + 1;
-    hipLaunchKernelGGL((grouped::rows_kernel<T, false>), dim3(parts, div_up(c_in, grouped::kCols)),
-                       dim3(grouped::kThreads), 0, stream, a);
-    SPIRA_HIP_LAUNCH_CHECK();
-    return kOk;
+    return grouped::launch_rows<T, false>(a, stream);
   });
 }
 
@@ -602,13 +1096,18 @@ int spira_hip_grouped_linear_weights_gradient(int64_t rows, int groups, const in
     grouped::WeightsArgs a{{offsets, groups, rows}, sources, num_sources, x, dz, c_in, c_out, part,
                            part ? static_cast<float *>(workspace) : nullptr, dw};
     const int64_t z = part ? grouped::most_parts(rows, groups, part) : groups;
-    hipLaunchKernelGGL(grouped::weights_kernel<T>,
+    if (grouped::dma_fits<T>(a)) {
+      const int64_t blocks = z * div_up(c_out, 128) * div_up(c_in, 128);
+      SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear_weights_gradient: too many tiles");
+      hipLaunchKernelGGL((grouped::weights_tile_kernel<T, 128, 128, 64, 64>), dim3(blocks), dim3(256), 0, stream, a);
+    } else
+      hipLaunchKernelGGL(grouped::weights_kernel<T>,
                        dim3(div_up(c_out, grouped::kCols), div_up(c_in, grouped::kRows), z), dim3(grouped::kThreads), 0,
                        stream, a);
     SPIRA_HIP_LAUNCH_CHECK();
     if (part) {
       const int64_t size = static_cast<int64_t>(c_in) * c_out;
-      hipLaunchKernelGGL(grouped::join_kernel<T>, dim3(div_up(size, 1024), groups), dim3(256), 0, stream, a.g, part, z,
+      hipLaunchKernelGGL(grouped::join_kernel<T>, dim3(div_up(size, 64), groups), dim3(256), 0, stream, a.g, part, z,
                          a.partial, size, static_cast<T *>(dw));
       SPIRA_HIP_LAUNCH_CHECK();
     }
@@ -643,7 +1142,7 @@ int spira_hip_grouped_linear_activation_gradient(int64_t rows, int groups, const
       SPIRA_HIP_LAUNCH_CHECK();
     }
     if (dbias) {
-      hipLaunchKernelGGL(grouped::join_kernel<T>, dim3(div_up(c_out, 1024), groups), dim3(256), 0, stream, g,
+      hipLaunchKernelGGL(grouped::join_kernel<T>, dim3(div_up(c_out, 64), groups), dim3(256), 0, stream, g,
                          static_cast<int>(part), parts, partial, static_cast<int64_t>(c_out), static_cast<T *>(dbias));
       SPIRA_HIP_LAUNCH_CHECK();
     }

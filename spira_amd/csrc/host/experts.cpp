@@ -5,9 +5,13 @@
 #include "host_common.h"
 
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 namespace spira_host {
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 using Tensor = torch::Tensor;
 using OptTensor = std::optional<torch::Tensor>;
 
@@ -310,16 +314,200 @@ static Tensor dropout(const Tensor &x, double p, uint64_t seed, uint64_t offset,
   return y;
 }
 
+// ---------------------------------------------------------------------------
+// Gradients.  The functions above take contiguous tensors and know nothing of
+// autograd; those below are what Python calls.  (In C++: with Python's autograd
+// functions a training step of a small operator was bound by the host, 104 us
+// where its kernels take 23.)
+// ---------------------------------------------------------------------------
+static Tensor dense(const Tensor &t) { return t.contiguous(); }
+static OptTensor dense(const OptTensor &t) { return t ? OptTensor(t->contiguous()) : t; }
+
+static bool tracked(std::initializer_list<const OptTensor *> ts) {
+  if (!torch::GradMode::is_enabled()) return false;
+  for (const OptTensor *t : ts)
+    if (*t && (*t)->requires_grad()) return true;
+  return false;
+}
+static bool wants(const OptTensor &t) { return t && t->requires_grad(); }
+
+static Tensor given(const OptTensor &t) { return t ? *t : Tensor(); }
+static OptTensor maybe(const Tensor &t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+// Gradients are of first order: with a graph of them asked for, they carry a
+// node that fails when it is differentiated.
+static variable_list once(variable_list grads, const char *name) {
+  if (!torch::GradMode::is_enabled()) return grads;
+  variable_list some;
+  for (const Tensor &g : grads)
+    if (g.defined()) some.push_back(g.detach().requires_grad_(true));
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string("[Spira] ") + name + ": gradients are of first order", static_cast<int64_t>(some.size()));
+  some = (*error)(std::move(some));
+  size_t i = 0;
+  for (Tensor &g : grads)
+    if (g.defined()) g = some[i++];
+  return grads;
+}
+
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &bias,
+                        const Tensor &offsets, const OptTensor &rows, const OptTensor &slots, bool relu) {
+    Tensor y = grouped_linear(x, w, offsets, rows, bias, relu);
+    ctx->save_for_backward({x, w, offsets, given(rows), given(slots), relu ? y : Tensor()});
+    ctx->saved_data["need"] = int64_t(x.requires_grad()) | int64_t(w.requires_grad()) << 1 | int64_t(wants(bias)) << 2;
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list d) {
+    const variable_list v = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    auto [dx, dw, db] = grouped_linear_backward(v[0], v[1], v[2], maybe(v[3]), maybe(v[4]), maybe(v[5]), dense(d[0]),
+                                                need & 1, need & 2, need & 4);
+    return once({given(dx), given(dw), given(db), Tensor(), Tensor(), Tensor(), Tensor()}, "grouped_linear");
+  }
+};
+
+static Tensor grouped_linear_call(const Tensor &x, const Tensor &w, const Tensor &offsets, const OptTensor &rows,
+                                  const OptTensor &slots, const OptTensor &bias, bool relu) {
+  if (slots) {
+    SPIRA_CHECK_ARG(rows && slots->dim() == 2 && x.dim() == 2 && slots->size(0) == x.size(0) &&
+                        slots->numel() == rows->numel(),
+                    "grouped_linear: routes of ", slots->sizes(), " choices do not fit features of ", x.sizes());
+  }
+  const OptTensor ox = x, ow = w;
+  if (tracked({&ox, &ow, &bias}))
+    return LinearFunction::apply(dense(x), dense(w), dense(bias), dense(offsets), dense(rows), dense(slots), relu);
+  return grouped_linear(dense(x), dense(w), dense(offsets), dense(rows), dense(bias), relu);
+}
+
+struct RouteFunction : torch::autograd::Function<RouteFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &logits, int64_t k, bool renormalize) {
+    auto [weights, chosen, offsets, rows, slots] = route(logits, k, renormalize);
+    ctx->save_for_backward({logits, weights, chosen});
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->mark_non_differentiable({chosen, offsets, rows, slots});
+    ctx->set_materialize_grads(false);  // (four of zeros, for the integers)
+    return {weights, chosen, offsets, rows, slots};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list d) {
+    const variable_list v = ctx->get_saved_variables();
+    return once({route_backward(v[0], v[1], v[2], dense(d[0]), ctx->saved_data["renormalize"].toBool()), Tensor(),
+                 Tensor()},
+                "route_experts");
+  }
+};
+
+static std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_call(const Tensor &logits, int64_t k,
+                                                                     bool renormalize) {
+  const OptTensor l = logits;
+  if (!tracked({&l})) return route(dense(logits), k, renormalize);
+  const variable_list v = RouteFunction::apply(dense(logits), k, renormalize);
+  return {v[0], v[1], v[2], v[3], v[4]};
+}
+
+struct CombineFunction : torch::autograd::Function<CombineFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &h, const Tensor &weights, const Tensor &rows,
+                        const Tensor &slots) {
+    ctx->save_for_backward({h, weights, rows, slots});
+    ctx->saved_data["need"] = int64_t(h.requires_grad()) | int64_t(weights.requires_grad()) << 1;
+    return combine(h, slots, weights);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list d) {
+    const variable_list v = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    auto [dh, dw] = combine_backward(v[0], v[2], v[3], v[1], dense(d[0]), need & 1, need & 2);
+    return once({given(dh), given(dw), Tensor(), Tensor()}, "combine_experts");
+  }
+};
+
+static Tensor combine_call(const Tensor &h, const Tensor &weights, const Tensor &rows, const Tensor &slots) {
+  const OptTensor oh = h, ow = weights;
+  if (tracked({&oh, &ow})) return CombineFunction::apply(dense(h), dense(weights), dense(rows), dense(slots));
+  return combine(dense(h), dense(slots), dense(weights));
+}
+
+struct NormFunction : torch::autograd::Function<NormFunction> {
+  // (the outputs that there are: r, next)
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const OptTensor &h, const OptTensor &weight,
+                               const OptTensor &gate, const OptTensor &next_weight, bool gate_sigmoid, double scale,
+                               double eps) {
+    auto [r, next, inv_h, inv_r] = gated_residual_norm(x, h, weight, gate, gate_sigmoid, scale, next_weight, eps, true);
+    ctx->save_for_backward(
+        {x, given(h), given(weight), given(gate), given(next_weight), given(inv_h), given(inv_r)});
+    ctx->saved_data["need"] = int64_t(x.requires_grad()) | int64_t(wants(h)) << 1 | int64_t(wants(weight)) << 2 |
+                              int64_t(wants(gate)) << 3 | int64_t(wants(next_weight)) << 4;
+    ctx->saved_data["gate_sigmoid"] = gate_sigmoid;
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    variable_list out;
+    if (r) out.push_back(*r);
+    if (next) out.push_back(*next);
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list d) {
+    const variable_list v = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    Tensor dr = v[1].defined() ? d[0] : Tensor(), dn = v[4].defined() ? d.back() : Tensor();
+    auto g = gated_residual_norm_backward(
+        v[0], maybe(v[1]), maybe(v[2]), maybe(v[3]), ctx->saved_data["gate_sigmoid"].toBool(),
+        ctx->saved_data["scale"].toDouble(), maybe(v[4]), maybe(v[5]), maybe(v[6]), dense(maybe(dr)), dense(maybe(dn)),
+        {bool(need & 1), bool(need & 2), bool(need & 4), bool(need & 8), bool(need & 16)});
+    variable_list out;
+    for (const OptTensor &t : g) out.push_back(given(t));
+    out.resize(8);
+    return once(std::move(out), "gated_residual_norm");
+  }
+};
+
+static std::tuple<OptTensor, OptTensor> norm_call(const Tensor &x, const OptTensor &h, const OptTensor &weight,
+                                                  const OptTensor &gate, bool gate_sigmoid, double scale,
+                                                  const OptTensor &next_weight, double eps) {
+  const OptTensor ox = x;
+  if (!tracked({&ox, &h, &weight, &gate, &next_weight})) {
+    auto out = gated_residual_norm(dense(x), dense(h), dense(weight), dense(gate), gate_sigmoid, scale,
+                                   dense(next_weight), eps, false);
+    return {std::get<0>(out), std::get<1>(out)};
+  }
+  const variable_list v = NormFunction::apply(dense(x), dense(h), dense(weight), dense(gate), dense(next_weight),
+                                              gate_sigmoid, scale, eps);
+  return {h ? OptTensor(v[0]) : std::nullopt, next_weight ? OptTensor(v.back()) : std::nullopt};
+}
+
+struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const OptTensor &residual, double p, int64_t seed,
+                        int64_t offset) {
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["need"] = int64_t(x.requires_grad()) | int64_t(wants(residual)) << 1;
+    return dropout(x, p, static_cast<uint64_t>(seed), static_cast<uint64_t>(offset), residual);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list d) {
+    const int64_t need = ctx->saved_data["need"].toInt();
+    Tensor dx;
+    if (need & 1)
+      dx = dropout(dense(d[0]), ctx->saved_data["p"].toDouble(), static_cast<uint64_t>(ctx->saved_data["seed"].toInt()),
+                   static_cast<uint64_t>(ctx->saved_data["offset"].toInt()), std::nullopt);
+    // (the residual's gradient is the output's own, of any order)
+    variable_list own = once({dx}, "dropout");
+    return {own[0], need & 2 ? d[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+static Tensor dropout_call(const Tensor &x, double p, uint64_t seed, uint64_t offset, const OptTensor &residual) {
+  const OptTensor ox = x;
+  if (tracked({&ox, &residual}))
+    return DropoutFunction::apply(dense(x), dense(residual), p, static_cast<int64_t>(seed),
+                                  static_cast<int64_t>(offset));
+  return dropout(dense(x), p, seed, offset, dense(residual));
+}
+
 void register_experts(pybind11::module_ &m) {
-  m.def("grouped_linear", &grouped_linear);
-  m.def("grouped_linear_backward", &grouped_linear_backward);
-  m.def("route_experts", &route);
-  m.def("route_experts_backward", &route_backward);
-  m.def("combine_experts", &combine);
-  m.def("combine_experts_backward", &combine_backward);
-  m.def("gated_residual_norm", &gated_residual_norm);
-  m.def("gated_residual_norm_backward", &gated_residual_norm_backward);
-  m.def("dropout", &dropout);
+  m.def("grouped_linear", &grouped_linear_call);
+  m.def("route_experts", &route_call);
+  m.def("combine_experts", &combine_call);
+  m.def("gated_residual_norm", &norm_call);
+  m.def("dropout", &dropout_call);
 }
 
 }  // namespace spira_host

@@ -14,13 +14,15 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._native import _C
-from .convolution import _c, _gpu
+from .convolution import _gpu
 
 __all__ = ["ExpertRoutes", "route_experts", "grouped_linear", "combine_experts", "gated_residual_norm", "rms_norm",
            "dropout"]
+
+
+_LOW = (1 << 64) - 1
 
 
 class ExpertRoutes(NamedTuple):
@@ -38,26 +40,6 @@ class ExpertRoutes(NamedTuple):
     slots: torch.Tensor    # [T, k] int32: the row of each choice, or -1
 
 
-def _tracked(*tensors: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, k, renormalize):
-        out = _C.route_experts(logits, k, renormalize)
-        ctx.save_for_backward(logits, out[0], out[1])
-        ctx.renormalize = renormalize
-        ctx.mark_non_differentiable(*out[1:])
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dweights, *_):
-        logits, weights, experts = ctx.saved_tensors
-        return _C.route_experts_backward(logits, weights, experts, _c(dweights), ctx.renormalize), None, None
-
-
 def route_experts(logits: torch.Tensor, k: int, *, renormalize: bool = True) -> ExpertRoutes:
     """The k largest of each token's ``logits`` [T, E] (the lowest index first
     among equals) with their softmax weights, over the chosen ones or, without
@@ -68,26 +50,7 @@ def route_experts(logits: torch.Tensor, k: int, *, renormalize: bool = True) -> 
     choices.
     """
     _gpu(logits)
-    logits, k = _c(logits), int(k)
-    if _tracked(logits):
-        return ExpertRoutes(*_Route.apply(logits, k, bool(renormalize)))
-    return ExpertRoutes(*_C.route_experts(logits, k, bool(renormalize)))
-
-
-class _GroupedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, offsets, rows, slots, relu):
-        y = _C.grouped_linear(x, weight, offsets, rows, bias, relu)
-        ctx.save_for_backward(x, weight, offsets, rows, slots, y if relu else None)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, offsets, rows, slots, y = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*_C.grouped_linear_backward(x, weight, offsets, rows, slots, y, _c(dy), *need[:3]), None, None, None,
-                None)
+    return ExpertRoutes(*_C.route_experts(logits, k, renormalize))
 
 
 def grouped_linear(features: torch.Tensor, weight: torch.Tensor, groups: Union[torch.Tensor, ExpertRoutes], *,
@@ -102,30 +65,9 @@ def grouped_linear(features: torch.Tensor, weight: torch.Tensor, groups: Union[t
     number of rows, none included; rows in no group are zero.
     """
     _gpu(features)
-    rows = slots = None
-    offsets = groups
     if isinstance(groups, ExpertRoutes):
-        offsets, rows, slots = groups.offsets, _c(groups.rows), _c(groups.slots)
-        if slots.dim() != 2 or slots.size(0) != features.size(0) or slots.numel() != rows.numel():
-            raise RuntimeError(f"[Spira] grouped_linear: routes of {tuple(slots.shape)} choices and "
-                               f"{rows.numel()} rows do not fit {features.size(0)} tokens")
-    args = _c(features), _c(weight), _c(bias)
-    if _tracked(*args):
-        return _GroupedLinear.apply(*args, _c(offsets), rows, slots, bool(relu))
-    return _C.grouped_linear(args[0], args[1], _c(offsets), rows, args[2], bool(relu))
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, h, weights, rows, slots):
-        ctx.save_for_backward(h, weights, rows, slots)
-        return _C.combine_experts(h, slots, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        h, weights, rows, slots = ctx.saved_tensors
-        return (*_C.combine_experts_backward(h, rows, slots, weights, _c(dy), *ctx.needs_input_grad[:2]), None, None)
+        return _C.grouped_linear(features, weight, groups.offsets, groups.rows, groups.slots, bias, relu)
+    return _C.grouped_linear(features, weight, groups, None, None, bias, relu)
 
 
 def combine_experts(features: torch.Tensor, routes: ExpertRoutes) -> torch.Tensor:
@@ -133,29 +75,7 @@ def combine_experts(features: torch.Tensor, routes: ExpertRoutes) -> torch.Tenso
     features[slots[t, j]]`` over its choices, ``features`` [T * k, C] in the
     routes' order.  Zero for a token without any."""
     _gpu(features)
-    h, weights, slots = _c(features), _c(routes.weights), _c(routes.slots)
-    if _tracked(h, weights):
-        return _Combine.apply(h, weights, _c(routes.rows), slots)
-    return _C.combine_experts(h, slots, weights)
-
-
-class _GatedResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, h, weight, gate, next_weight, gate_sigmoid, scale, eps):
-        r, n, inv_h, inv_r = _C.gated_residual_norm(x, h, weight, gate, gate_sigmoid, scale, next_weight, eps, True)
-        ctx.save_for_backward(x, h, weight, gate, next_weight, inv_h, inv_r)
-        ctx.options = gate_sigmoid, scale
-        ctx.set_materialize_grads(False)
-        return r, n
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dr, dn):
-        x, h, weight, gate, next_weight, inv_h, inv_r = ctx.saved_tensors
-        need = [bool(v) for v in ctx.needs_input_grad[:5]]
-        dx, dh, dw, dg, dnw = _C.gated_residual_norm_backward(
-            x, h, weight, gate, ctx.options[0], ctx.options[1], next_weight, inv_h, inv_r, _c(dr), _c(dn), need)
-        return dx, dh, dw, dg, dnw, None, None, None
+    return _C.combine_experts(features, routes.weights, routes.rows, routes.slots)
 
 
 def gated_residual_norm(residual: torch.Tensor, update: torch.Tensor, *, weight: Optional[torch.Tensor] = None,
@@ -173,35 +93,14 @@ def gated_residual_norm(residual: torch.Tensor, update: torch.Tensor, *, weight:
     channels.
     """
     _gpu(residual)
-    args = _c(residual), _c(update), _c(weight), _c(gate), _c(next_weight)
-    if _tracked(*args):
-        return _GatedResidualNorm.apply(*args, bool(gate_sigmoid), float(scale), float(eps))
-    x, h, weight, gate, next_weight = args
-    return _C.gated_residual_norm(x, h, weight, gate, bool(gate_sigmoid), float(scale), next_weight, float(eps),
-                                  False)[:2]
+    return _C.gated_residual_norm(residual, update, weight, gate, gate_sigmoid, scale, next_weight, eps)
 
 
 def rms_norm(features: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """``features / sqrt(mean(features ** 2) + eps) * weight`` over the channels:
     the entry of a first block."""
     _gpu(features)
-    x, weight = _c(features), _c(weight)
-    if _tracked(x, weight):
-        return _GatedResidualNorm.apply(x, None, None, None, weight, False, 1.0, float(eps))[1]
-    return _C.gated_residual_norm(x, None, None, None, False, 1.0, weight, float(eps), False)[1]
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        ctx.mask = p, seed, offset
-        return _C.dropout(x, p, seed, offset, residual)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        dx = _C.dropout(_c(dy), *ctx.mask, None) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+    return _C.gated_residual_norm(features, None, None, None, False, 1.0, weight, eps)[1]
 
 
 def dropout(features: torch.Tensor, p: float, seed: int, offset: int = 0, *,
@@ -217,8 +116,4 @@ def dropout(features: torch.Tensor, p: float, seed: int, offset: int = 0, *,
     it was captured with.
     """
     _gpu(features)
-    low = (1 << 64) - 1
-    args = _c(features), _c(residual), float(p), int(seed) & low, int(offset) & low
-    if _tracked(*args[:2]):
-        return _Dropout.apply(*args)
-    return _C.dropout(args[0], *args[2:], args[1])
+    return _C.dropout(features, p, seed & _LOW, offset & _LOW, residual)
