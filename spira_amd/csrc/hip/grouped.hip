@@ -103,6 +103,47 @@ __device__ __forceinline__ int64_t count_parts(const Groups &g, int size) {
   return first + count;
 }
 
+// Block w's place among `count` pieces of work so that each of the 8 XCDs (w %
+// 8) takes one range of them; w itself past them.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t w, uint32_t count) {
+  if (w >= count) return w;
+  const uint32_t q = count / 8, r = count % 8, x = w % 8;
+  return x * q + (x < r ? x : r) + w / 8;
+}
+
+// Block w's part and column among parts x cols, in XCD order: the columns of a
+// part together, so that an XCD's L2 holds a few parts' rows and a group's
+// weights.  Past the last, part.begin counts the blocks and `idle` is their number.
+struct Place {
+  Part part;
+  uint32_t col;
+  int64_t idle;
+};
+__device__ __forceinline__ Place find_place(const Groups &g, int size, uint32_t w, uint32_t cols, uint32_t blocks) {
+  if (g.count > 64) {
+    const uint32_t work = static_cast<uint32_t>(count_parts(g, size)) * cols, at = xcd_order(w, work);
+    if (at >= work) return {{-1, at - work, 0}, 0, blocks - work};
+    return {find_part(g, size, at / cols), at % cols, 0};
+  }
+  // (the offsets read once)
+  const int lane = lane_id();
+  const int64_t lo = lane < g.count ? bound(g, lane) : 0, hi = lane < g.count ? bound(g, lane + 1) : 0;
+  const uint32_t parts = hi > lo ? static_cast<uint32_t>(hi - lo + size - 1) / size : 0;
+  uint32_t upto = parts;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const uint32_t u = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += u;
+  }
+  const uint32_t work = uniform(__shfl(upto, 63, 64)) * cols, at = xcd_order(w, work);
+  if (at >= work) return {{-1, at - work, 0}, 0, blocks - work};
+  const uint32_t index = at / cols;
+  const int e = __builtin_ctzll(ballot(upto > index));
+  const int64_t nth = index - (__shfl(upto, e, 64) - __shfl(parts, e, 64));
+  const int64_t begin = __shfl(lo, e, 64) + nth * size, end = __shfl(hi, e, 64);
+  return {{uniform(e), uniform(begin), uniform(begin + size < end ? begin + size : end)}, at % cols, 0};
+}
+
 // most parts that any offsets of `count` groups over `rows` rows can have
 static int64_t most_parts(int64_t rows, int64_t count, int64_t size) {
   return (rows + std::min(rows, count) * (size - 1)) / size;
@@ -566,43 +607,77 @@ template <class T, bool KO> static int launch_stream(const RowsArgs &a, hipStrea
 // ---------------------------------------------------------------------------
 // Tiles fed by DMA: rows and widths of whole 16-byte chunks.  The global loads
 // write LDS themselves (no registers, no address arithmetic but one add a
-// load), a step ahead of the products, in two stages.  The LDS swizzle is made
-// by the order in which the lanes fetch a row's chunks.  Chunks past a row's end
-// and rows that are not there are out of the buffer's range: they load zeros.
+// load), three steps ahead of the products, in a ring of four stages of 64 bytes
+// of the summed index.  (Two stages of 128 bytes leave a load the time of one
+// step to arrive, and the matrix cores busy for 28 % of it.)  The LDS swizzle is
+// made by the order in which the lanes fetch a row's chunks.  Chunks past a
+// row's end and rows that are not there are out of the buffer's range: they load
+// zeros, and so do the steps past the last, so that the loads in flight are
+// always as many.
+//
 // ---------------------------------------------------------------------------
 constexpr uint32_t kOutOfRange = 0x80000000u;
 constexpr int64_t kBufferLimit = int64_t(1) << 31;
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *base, int64_t bytes) {
+// A buffer descriptor: base, bytes, raw.
+__device__ __forceinline__ uintx4_t buffer(const void *base, int64_t bytes) {
   const int64_t n = bytes < 0 ? 0 : bytes < kBufferLimit ? bytes : kBufferLimit - 1;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(n), 0x00020000);
+  const auto at = reinterpret_cast<uint64_t>(base);
+  return {uniform(static_cast<uint32_t>(at)), uniform(static_cast<uint32_t>(at >> 32) & 0xFFFFu),
+          uniform(static_cast<uint32_t>(n)), 0x00020000u};
 }
-// 1 KB to LDS, 16 bytes from each lane's offset
-__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, uint32_t offset, char *to) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void *)to, 16, offset, 0, 0, 0);
+// 1 KB to LDS, 16 bytes from each lane's offset.  In assembly, and waited for by
+// the ring alone: the compiler's own count of such loads is not kept over the
+// ring's loop, it would wait for all of them once a turn.  (No register is
+// written.  What loads the compiler itself waits for, it waits longer.)
+__device__ __forceinline__ void load_lds(uintx4_t from, uint32_t offset, char *to) {
+  const uint32_t at = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)to)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(at), "v"(offset), "s"(from) : "memory", "m0");
+}
+// 256 bytes, 4 from each lane's offset
+__device__ __forceinline__ void load_lds_word(uintx4_t from, uint32_t offset, void *to) {
+  const uint32_t at = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void *)to)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(at), "v"(offset), "s"(from) : "memory", "m0");
+}
+// Until all but the last N loads have landed and this wave's LDS reads are done,
+// then the block's barrier.
+template <int N> __device__ __forceinline__ void wait_loads_and_meet() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | ((N >> 4) << 14));
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
 
-// Block w's place among `count` pieces of work so that each of the 8 XCDs (w %
-// 8) takes one range of them; w itself past them.
-__device__ __forceinline__ int64_t xcd_order(int64_t w, int64_t count) {
-  if (w >= count) return w;
-  const int64_t q = count / 8, r = count % 8, x = w % 8;
-  return x * q + (x < r ? x : r) + w / 8;
-}
+constexpr int kRing = 64;  // bytes of the summed index per stage
+template <class T> constexpr int kRingK = kRing / static_cast<int>(sizeof(T));
 
 template <class T, int M, int N, int WM, int WN> struct Tile {
   static constexpr int NW = (M / WM) * (N / WN), NT = 64 * NW;
   static constexpr int MI = WM / 16, NI = WN / 16;
-  static constexpr int XL = M / 8 / NW, WL = N / 8 / NW;  // loads (1 KB) a wave and step
-  static constexpr int XBYTES = M * kStep, WBYTES = N * kStep;
-  static_assert(XL >= 1 && WL >= 1 && XL * NW * 8 == M && WL * NW * 8 == N, "tile shape");
+  static constexpr int XL = M / 16 / NW, WL = N / 16 / NW;  // loads (1 KB) a wave and stage
+  static constexpr int XBYTES = M * kRing, WBYTES = N * kRing;
+  static_assert(XL >= 1 && WL >= 1 && XL * NW * 16 == M && WL * NW * 16 == N, "tile shape");
 };
 
-// where lane `lane` of a tile's load `i` (1 KB) reads: KC row and chunk; KO row k and chunk
+// KC stage: row r's chunk c (of 4) at r * 64 + (c ^ turn(r)) * 16.  A 16-byte LDS
+// read serves lanes 0-3, 12-15, 20-27 at once (then 4-11, 16-19, 28-31, and so in
+// the upper half): rows 0-3 and 12-15 of one chunk with rows 4-11 of the next.
+// turn() is 0, 2, 3, 1 for the four rows-of-four, which keeps those apart.
+__device__ __forceinline__ int turn(int r) { return ((r >> 1) & 2) ^ (((r >> 3) & 1) * 3); }
+__device__ __forceinline__ int ring_at(int r, int c) { return r * kRing + ((c ^ turn(r)) << 4); }
+__device__ __forceinline__ uintx4_t ring_frag(const char *tile, int r0) {
+  const int lane = lane_id();
+  return *reinterpret_cast<const uintx4_t *>(tile + ring_at(r0 + (lane & 15), lane >> 4));
+}
+
+// where lane `lane` of a stage's load `i` (1 KB) reads: KC row and chunk; KO row k and chunk
 __device__ __forceinline__ void kc_source(int i, int lane, int &r, int &c) {
-  r = i * 8 + (lane >> 3);
-  c = (lane & 7) ^ ((r >> 1) & 7);
+  r = i * 16 + (lane >> 2);
+  c = (lane & 3) ^ turn(r);
 }
 template <class T, int N> __device__ __forceinline__ void ko_source(int i, int lane, int &k, int &c) {
   constexpr int CPR = N * static_cast<int>(sizeof(T)) / 16;
@@ -615,41 +690,167 @@ template <class T, int MI, int NI> struct TileSums {
   floatx4_t v[MI][NI];
 };
 
-template <class T, int MI, int NI, class MFrag, class NFrag>
-__device__ __forceinline__ void multiply_tile(TileSums<T, MI, NI> &acc, MFrag &&mf, NFrag &&nf) {
-#pragma unroll
-  for (int kk = 0; kk < 2; ++kk) {
-    uintx4_t m[MI], n[NI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) n[i] = nf(i, kk);
-#pragma unroll
-    for (int i = 0; i < MI; ++i) m[i] = mf(i, kk);
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) mma<T>(acc.v[i][j], n[j], m[i]);
+// What a wave reads of a stage a step ahead: the channels' fragments, and the
+// first rows'.
+constexpr int kAhead = 2;
+template <int NI> struct Head {
+  uintx4_t n[NI], m[kAhead];
+};
+
+// acc += a stage's products.  The first rows' begin at once behind the barrier, on
+// the head read during the step before (without it the matrix cores wait for
+// 80 KB of LDS reads of eight waves); the others' fragments arrive meanwhile, and
+// then the next step's head.  m(i): rows' fragment i of this stage; ahead(f): the
+// next stage's head.
+template <class T, int MI, int NI, class M, class Ahead>
+__device__ __forceinline__ void multiply_tile(TileSums<T, MI, NI> &acc, const Head<NI> &f, Head<NI> &next, bool busy,
+                                              M &&m, Ahead &&ahead) {
+  if (!busy) {
+    ahead(next);
+    return;
   }
+  constexpr int REST = MI - kAhead, FIRST = REST / 2;
+  static_assert(REST >= 2, "rows of a wave");
+  uintx4_t r[REST];
+  const auto products = [&](int i, uintx4_t x) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) mma<T>(acc.v[i][j], f.n[j], x);
+  };
+#pragma unroll
+  for (int i = 0; i < FIRST; ++i) r[i] = m(kAhead + i);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) products(i, f.m[i]);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = FIRST; i < REST; ++i) r[i] = m(kAhead + i);
+#pragma unroll
+  for (int i = 0; i < FIRST; ++i) products(kAhead + i, r[i]);
+  __builtin_amdgcn_sched_barrier(0);
+  ahead(next);
+#pragma unroll
+  for (int i = FIRST; i < REST; ++i) products(kAhead + i, r[i]);
 }
+
+// issue(step, stage), head(stage, f) and multiply(stage, next stage, f, next f)
+// over `steps` steps; L: loads a wave and step.
+template <int L, class F, class Issue, class ReadHead, class Multiply>
+__device__ __forceinline__ void ring_loop(int steps, Issue &&issue, ReadHead &&head, Multiply &&multiply) {
+  using std::integral_constant;
+  constexpr integral_constant<int, 0> s0;
+  constexpr integral_constant<int, 1> s1;
+  constexpr integral_constant<int, 2> s2;
+  constexpr integral_constant<int, 3> s3;
+  if (steps <= 0) return;
+  issue(0, s0);
+  issue(1, s1);
+  issue(2, s2);
+  F a, b;
+  wait_loads_and_meet<2 * L>();
+  head(s0, a);
+  for (int step = 0;;) {
+    wait_loads_and_meet<L>();
+    issue(step + 3, s3);
+    multiply(s0, s1, a, b);
+    if (++step == steps) break;
+    wait_loads_and_meet<L>();
+    issue(step + 3, s0);
+    multiply(s1, s2, b, a);
+    if (++step == steps) break;
+    wait_loads_and_meet<L>();
+    issue(step + 3, s1);
+    multiply(s2, s3, a, b);
+    if (++step == steps) break;
+    wait_loads_and_meet<L>();
+    issue(step + 3, s2);
+    multiply(s3, s0, b, a);
+    if (++step == steps) break;
+  }
+  wait_loads();  // (none may land in the LDS of a block that follows)
+}
+// stage s of four arrays
+template <int S> __device__ __forceinline__ char *stage_of(char *a, char *b, char *c, char *d) {
+  if constexpr (S == 0) return a;
+  else if constexpr (S == 1) return b;
+  else if constexpr (S == 2) return c;
+  else return d;
+}
+
+// A lane's sums are four channels of each of four 16-channel tiles: quarter q of
+// the wave holds channels 4 q of every tile.  Exchanged between the quarters (a 4
+// x 4 transpose in two rounds of swaps), quarter q holds all 16 of tile q, and the
+// wave writes 16 rows of whole 128-byte lines.  Every lane takes part; `there`:
+// its row is to be written.  n: first of the 64 channels, of `width`.
+template <class T> __device__ __forceinline__ void store_row(T *row, int64_t n, int64_t width, bool there,
+                                                             const floatx4_t (&v)[4]) {
+  constexpr int W = static_cast<int>(sizeof(T));  // words of four values
+  uint32_t u[4][W];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    T t[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t[q] = from_float<T>(v[j][q]);
+    __builtin_memcpy(u[j], t, sizeof(t));
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const auto s = __builtin_amdgcn_permlane32_swap(u[j][w], u[j + 2][w], false, false);
+      u[j][w] = s[0];
+      u[j + 2][w] = s[1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const auto s = __builtin_amdgcn_permlane16_swap(u[j][w], u[j + 1][w], false, false);
+      u[j][w] = s[0];
+      u[j + 1][w] = s[1];
+    }
+  }
+  const int64_t at = n + (lane_id() >> 4) * 16;
+  if (!there) return;
+  const uint32_t *f = &u[0][0];
+#pragma unroll
+  for (int c = 0; c < W; ++c)
+    // (widths are whole chunks)
+    if (at + c * kVec<T> < width)
+      *reinterpret_cast<Unaligned<T> *>(row + at + c * kVec<T>) = uintx4_t{f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]};
+}
+
+// The bias of a lane's channels, read before the products begin.
+template <class T, int NI> struct BiasOf {
+  T v[NI][4];
+  __device__ __forceinline__ void load(const T *bias, int64_t n, int64_t width, int lane) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int64_t at = n + j * 16 + (lane >> 4) * 4;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[j][q] = bias && at < width ? bias[at + q] : static_cast<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ floatx4_t at(int j) const {
+    return {to_float(v[j][0]), to_float(v[j][1]), to_float(v[j][2]), to_float(v[j][3])};
+  }
+};
 
 template <class T, bool KO, int M, int N, int WM, int WN>
 __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) void tile_kernel(const RowsArgs a) {
   using S = Tile<T, M, N, WM, WN>;
-  __shared__ __align__(1024) char x0[S::XBYTES], x1[S::XBYTES], w0[S::WBYTES], w1[S::WBYTES];
+  __shared__ __align__(1024) char x0[S::XBYTES], x1[S::XBYTES], x2[S::XBYTES], x3[S::XBYTES];
+  __shared__ __align__(1024) char w0[S::WBYTES], w1[S::WBYTES], w2[S::WBYTES], w3[S::WBYTES];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t cols = (a.n + N - 1) / N, parts = count_parts(a.g, M);
-  const int64_t place = xcd_order(blockIdx.x, parts * cols);
-  const Part part = find_part(a.g, M, place / cols);
+  const Place place = find_place(a.g, M, blockIdx.x, static_cast<uint32_t>((a.n + N - 1) / N), gridDim.x);
+  const Part part = place.part;
   if (part.group < 0) {
-    clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, place - parts * cols, gridDim.x - parts * cols, S::NT);
+    clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, part.begin, place.idle, S::NT);
     return;
   }
-  const int64_t n0 = place % cols * N;
+  const int64_t n0 = place.col * static_cast<int64_t>(N);
   const uint32_t kbytes = static_cast<uint32_t>(a.k * static_cast<int64_t>(sizeof(T)));
   const uint32_t nbytes = static_cast<uint32_t>(a.n * static_cast<int64_t>(sizeof(T)));
-  const __amdgpu_buffer_rsrc_t xr =
+  const uintx4_t xr =
       a.source ? buffer(a.x, a.num_sources * kbytes)
                : buffer(static_cast<const char *>(a.x) + part.begin * kbytes, (part.end - part.begin) * kbytes);
-  const __amdgpu_buffer_rsrc_t wr =
+  const uintx4_t wr =
       buffer(static_cast<const char *>(a.w) + part.group * a.k * nbytes, a.k * static_cast<int64_t>(nbytes));
   uint32_t xo[S::XL], xc[S::XL], wo[S::WL], wc[S::WL];
 #pragma unroll
@@ -676,62 +877,55 @@ __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) void tile_kernel(const
       wo[i] = n0 + r < a.n ? static_cast<uint32_t>(n0 + r) * kbytes + wc[i] : kOutOfRange;
     }
   }
-  const int steps = static_cast<int>((kbytes + kStep - 1) / kStep);
-  auto issue = [&](int step, char *xs, char *ws) {
-    const uint32_t kb = step * kStep;
+  const int steps = static_cast<int>((kbytes + kRing - 1) / kRing);
+  auto issue = [&](int step, auto stage) {
+    constexpr int st = decltype(stage)::value;
+    char *xs = stage_of<st>(x0, x1, x2, x3), *ws = stage_of<st>(w0, w1, w2, w3);
+    const uint32_t kb = step * kRing;
 #pragma unroll
     for (int i = 0; i < S::XL; ++i)
       load_lds(xr, kb + xc[i] < kbytes ? xo[i] + kb : kOutOfRange, xs + (wave * S::XL + i) * 1024);
-    // (KO weights past the last row of the group: out of range)
-    const uint32_t wb = KO ? step * static_cast<uint32_t>(kStepK<T>) * nbytes : kb;
+    // (KO weights past the group's last row: out of range)
+    const uint32_t wb = KO ? step * static_cast<uint32_t>(kRingK<T>) * nbytes : kb;
 #pragma unroll
     for (int i = 0; i < S::WL; ++i)
       load_lds(wr, KO || kb + wc[i] < kbytes ? wo[i] + wb : kOutOfRange, ws + (wave * S::WL + i) * 1024);
   };
   const int m0 = wave / (N / WN) * WM, c0 = wave % (N / WN) * WN;
+  const bool busy = part.begin + m0 < part.end;  // (a last part's rows may end before this wave's)
   TileSums<T, S::MI, S::NI> acc{};
-  auto compute = [&](const char *xs, const char *ws) {
-    multiply_tile<T, S::MI, S::NI>(
-        acc, [&](int i, int kk) { return kc_frag(xs, m0 + i * 16, kk); },
-        [&](int i, int kk) {
-          if constexpr (KO) return ko_frag<T, N>(ws, c0 + i * 16, kk);
-          else return kc_frag(ws, c0 + i * 16, kk);
-        });
+  BiasOf<T, S::NI> bias;
+  bias.load(a.bias ? static_cast<const T *>(a.bias) + part.group * a.n : nullptr, n0 + c0, a.n, lane);
+  using F = Head<S::NI>;
+  const auto rows_frag = [&](auto stage, int i) {
+    return ring_frag(stage_of<decltype(stage)::value>(x0, x1, x2, x3), m0 + i * 16);
   };
-  issue(0, x0, w0);
-  wait_loads();
-  __syncthreads();
-  for (int step = 0;;) {
-    if (step + 1 < steps) issue(step + 1, x1, w1);
-    compute(x0, w0);
-    if (++step == steps) break;
-    wait_loads();
-    __syncthreads();
-    if (step + 1 < steps) issue(step + 1, x0, w0);
-    compute(x1, w1);
-    if (++step == steps) break;
-    wait_loads();
-    __syncthreads();
-  }
-  const T *bias = a.bias ? static_cast<const T *>(a.bias) + part.group * a.n : nullptr;
+  const auto head = [&](auto stage, F &f) {
+    const char *ws = stage_of<decltype(stage)::value>(w0, w1, w2, w3);
 #pragma unroll
-  for (int j = 0; j < S::NI; ++j) {
-    const int64_t n = n0 + c0 + j * 16 + (lane >> 4) * 4;
-    if (n >= a.n) continue;  // (widths are whole chunks, so that four values are inside or not)
-    floatx4_t b = {0, 0, 0, 0};
-    if (bias)
+    for (int i = 0; i < S::NI; ++i) {
+      if constexpr (KO) f.n[i] = ko_frag<T, N>(ws, c0 + i * 16, 0);
+      else f.n[i] = ring_frag(ws, c0 + i * 16);
+    }
 #pragma unroll
-      for (int v = 0; v < 4; ++v) b[v] = to_float(bias[n + v]);
+    for (int i = 0; i < kAhead; ++i) f.m[i] = rows_frag(stage, i);
+  };
+  ring_loop<S::XL + S::WL, F>(steps, issue, head, [&](auto stage, auto after, const F &f, F &next) {
+    multiply_tile<T>(
+        acc, f, next, busy, [&](int i) { return rows_frag(stage, i); }, [&](F &n) { head(after, n); });
+  });
 #pragma unroll
-    for (int i = 0; i < S::MI; ++i) {
-      const int64_t r = part.begin + m0 + i * 16 + (lane & 15);
-      if (r >= part.end) continue;
-      floatx4_t v = acc.v[i][j] + b;
+  for (int i = 0; i < S::MI; ++i) {
+    const int64_t r = part.begin + m0 + i * 16 + (lane & 15);
+    floatx4_t v[S::NI];
+#pragma unroll
+    for (int j = 0; j < S::NI; ++j) {
+      v[j] = acc.v[i][j] + bias.at(j);
       if (a.relu)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
-      store4(static_cast<T *>(a.y) + r * a.n + n, 4, v);
+        for (int q = 0; q < 4; ++q) v[j][q] = v[j][q] < 0.f ? 0.f : v[j][q];
     }
+    store_row<T>(static_cast<T *>(a.y) + r * a.n, n0 + c0, a.n, r < part.end, v);
   }
 }
 
@@ -755,8 +949,12 @@ template <class T, bool KO, int M, int N, int WM, int WN> static int launch_tile
 template <class T, bool KO> static int launch_rows(const RowsArgs &a, hipStream_t stream) {
   if (streams<T>(a.k, a.n)) return launch_stream<T, KO>(a, stream);
   if (dma_fits<T>(a)) {
+    // The large tile reads each operand half as often from L2 and LDS: 32k rows
+    // 1024 -> 2048 in 16 even groups 141 us, with the small one 197.  It needs
+    // groups that fill its rows, and blocks for every CU.
     if constexpr (sizeof(T) == 2)
-      if (a.g.rows / a.g.count >= 512 && a.n >= 256) return launch_tile<T, KO, 256, 256, 128, 64>(a, stream);
+      if (a.g.rows / a.g.count >= 256 && a.n > 128 && div_up(a.g.rows, 256) * div_up(a.n, 256) >= 256)
+        return launch_tile<T, KO, 256, 256, 128, 64>(a, stream);
     return launch_tile<T, KO, 128, 128, 64, 64>(a, stream);
   }
   hipLaunchKernelGGL((rows_kernel<T, KO>), dim3(most_parts(a.g.rows, a.g.count, kRows) + 1, div_up(a.n, kCols)),
@@ -844,15 +1042,18 @@ template <class T> __global__ __launch_bounds__(kThreads) void weights_kernel(co
     }
 }
 
-// The same fed by DMA, as tile_kernel.
-template <class T, int M, int N, int WM, int WN>
+// The same fed by DMA, as tile_kernel.  The sources of gathered rows come the same
+// way, three steps before the loads that need them, to a ring of each wave's own.
+template <class T, bool GATHER, int M, int N, int WM, int WN>
 __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) __attribute__((amdgpu_waves_per_eu(2))) void weights_tile_kernel(const WeightsArgs a) {
   using S = Tile<T, M, N, WM, WN>;
-  __shared__ __align__(1024) char x0[S::XBYTES], x1[S::XBYTES], z0[S::WBYTES], z1[S::WBYTES];
+  __shared__ __align__(1024) char x0[S::XBYTES], x1[S::XBYTES], x2[S::XBYTES], x3[S::XBYTES];
+  __shared__ __align__(1024) char z0[S::WBYTES], z1[S::WBYTES], z2[S::WBYTES], z3[S::WBYTES];
+  __shared__ int32_t sources[GATHER ? S::NW : 1][4][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t mt = (a.ci + M - 1) / M, nt = (a.co + N - 1) / N, tiles = mt * nt;
   const int64_t parts = a.partial ? count_parts(a.g, a.part_rows) : a.g.count;
-  const int64_t place = xcd_order(blockIdx.x, parts * tiles);
+  const int64_t place = blockIdx.x;
   if (place >= parts * tiles) return;
   const int64_t nth = place / tiles;
   Part part;
@@ -861,7 +1062,7 @@ __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) __attribute__((amdgpu_
   const int64_t m0 = place % tiles / nt * M, n0 = place % nt * N;
   const uint32_t xbytes = static_cast<uint32_t>(a.ci * static_cast<int64_t>(sizeof(T)));
   const uint32_t zbytes = static_cast<uint32_t>(a.co * static_cast<int64_t>(sizeof(T)));
-  const __amdgpu_buffer_rsrc_t gathered = buffer(a.x, a.num_sources * xbytes);
+  const uintx4_t gathered = buffer(a.x, a.num_sources * xbytes);
   int xk[S::XL], zk[S::WL];
   uint32_t xo[S::XL], zo[S::WL];
 #pragma unroll
@@ -878,71 +1079,92 @@ __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) __attribute__((amdgpu_
     zo[i] = static_cast<uint32_t>(n0 * sizeof(T)) + c * 16;
     if (zo[i] >= zbytes) zo[i] = kOutOfRange;
   }
-  // the sources of a step's rows, fetched a step before their loads are issued
-  int32_t src[S::XL];
-  auto look = [&](int64_t r0) {
-#pragma unroll
-    for (int i = 0; i < S::XL; ++i) src[i] = r0 + xk[i] < part.end ? a.source[r0 + xk[i]] : -1;
+  const uintx4_t list = buffer(GATHER ? a.source + part.begin : nullptr, GATHER ? (part.end - part.begin) * 4 : 0);
+  auto look = [&](int step, int slot) {
+    load_lds_word(list, lane < kRingK<T> ? (step * kRingK<T> + lane) * 4u : kOutOfRange, sources[wave][slot]);
   };
-  auto issue = [&](int64_t r0, char *xs, char *zs) {
-    if (a.source) {
+  auto issue = [&](int step, auto stage) {
+    constexpr int st = decltype(stage)::value;
+    char *xs = stage_of<st>(x0, x1, x2, x3), *zs = stage_of<st>(z0, z1, z2, z3);
+    const int64_t r0 = part.begin + static_cast<int64_t>(step) * kRingK<T>;
+    if constexpr (GATHER) {
+      int32_t src[S::XL];
+#pragma unroll
+      for (int i = 0; i < S::XL; ++i) src[i] = sources[wave][st][xk[i]];
 #pragma unroll
       for (int i = 0; i < S::XL; ++i) {
-        const bool in = src[i] >= 0 && src[i] < a.num_sources && xo[i] != kOutOfRange;
-        load_lds(gathered, in ? static_cast<uint32_t>(src[i]) * xbytes + xo[i] : kOutOfRange, xs + (wave * S::XL + i) * 1024);
+        const bool in = r0 + xk[i] < part.end && src[i] >= 0 && src[i] < a.num_sources && xo[i] != kOutOfRange;
+        load_lds(gathered, in ? static_cast<uint32_t>(src[i]) * xbytes + xo[i] : kOutOfRange,
+                 xs + (wave * S::XL + i) * 1024);
       }
-      look(r0 + kStepK<T>);
+      look(step + 3, (st + 3) % 4);
     } else {
-      const __amdgpu_buffer_rsrc_t xr = buffer(static_cast<const char *>(a.x) + r0 * xbytes, (part.end - r0) * xbytes);
+      const uintx4_t xr = buffer(static_cast<const char *>(a.x) + r0 * xbytes, (part.end - r0) * xbytes);
 #pragma unroll
-      for (int i = 0; i < S::XL; ++i)
-        load_lds(xr, xo[i] + xk[i] * xbytes, xs + (wave * S::XL + i) * 1024);
+      for (int i = 0; i < S::XL; ++i) load_lds(xr, xo[i] + xk[i] * xbytes, xs + (wave * S::XL + i) * 1024);
     }
-    const __amdgpu_buffer_rsrc_t zr = buffer(static_cast<const char *>(a.dz) + r0 * zbytes, (part.end - r0) * zbytes);
+    const uintx4_t zr = buffer(static_cast<const char *>(a.dz) + r0 * zbytes, (part.end - r0) * zbytes);
 #pragma unroll
-    for (int i = 0; i < S::WL; ++i)
-      load_lds(zr, zo[i] + zk[i] * zbytes, zs + (wave * S::WL + i) * 1024);
+    for (int i = 0; i < S::WL; ++i) load_lds(zr, zo[i] + zk[i] * zbytes, zs + (wave * S::WL + i) * 1024);
   };
   const int wm = wave / (N / WN) * WM, wn = wave % (N / WN) * WN;
   TileSums<T, S::MI, S::NI> acc{};
-  auto compute = [&](const char *xs, const char *zs) {
-    multiply_tile<T, S::MI, S::NI>(
-        acc, [&](int i, int kk) { return ko_frag<T, M>(xs, wm + i * 16, kk); },
-        [&](int i, int kk) { return ko_frag<T, N>(zs, wn + i * 16, kk); });
-  };
-  if (part.begin < part.end) {
-    if (a.source) look(part.begin);
-    issue(part.begin, x0, z0);
+  const int steps = part.begin < part.end ? static_cast<int>((part.end - part.begin + kRingK<T> - 1) / kRingK<T>) : 0;
+  if constexpr (GATHER) {
+    look(0, 0);
+    look(1, 1);
+    look(2, 2);
     wait_loads();
-    __syncthreads();
-    for (int64_t r0 = part.begin;;) {
-      if (r0 + kStepK<T> < part.end) issue(r0 + kStepK<T>, x1, z1);
-      compute(x0, z0);
-      if ((r0 += kStepK<T>) >= part.end) break;
-      wait_loads();
-      __syncthreads();
-      if (r0 + kStepK<T> < part.end) issue(r0 + kStepK<T>, x0, z0);
-      compute(x1, z1);
-      if ((r0 += kStepK<T>) >= part.end) break;
-      wait_loads();
-      __syncthreads();
-    }
+    asm volatile("" ::: "memory");
   }
+  using F = Head<S::NI>;
+  const auto rows_frag = [&](auto stage, int i) {
+    return ko_frag<T, M>(stage_of<decltype(stage)::value>(x0, x1, x2, x3), wm + i * 16, 0);
+  };
+  const auto head = [&](auto stage, F &f) {
 #pragma unroll
-  for (int i = 0; i < S::MI; ++i)
+    for (int i = 0; i < S::NI; ++i)
+      f.n[i] = ko_frag<T, N>(stage_of<decltype(stage)::value>(z0, z1, z2, z3), wn + i * 16, 0);
 #pragma unroll
-    for (int j = 0; j < S::NI; ++j) {
-      const int64_t m = m0 + wm + i * 16 + (lane & 15), n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (m >= a.ci || n >= a.co) continue;
-      if (a.partial) store4(a.partial + (nth * a.ci + m) * a.co + n, 4, acc.v[i][j]);
-      else store4(static_cast<T *>(a.dw) + (part.group * a.ci + m) * a.co + n, 4, acc.v[i][j]);
-    }
+    for (int i = 0; i < kAhead; ++i) f.m[i] = rows_frag(stage, i);
+  };
+  ring_loop<S::XL + S::WL + (GATHER ? 1 : 0), F>(steps, issue, head,
+                                                 [&](auto stage, auto after, const F &f, F &next) {
+                                                   multiply_tile<T>(
+                                                       acc, f, next, true, [&](int i) { return rows_frag(stage, i); },
+                                                       [&](F &n) { head(after, n); });
+                                                 });
+#pragma unroll
+  for (int i = 0; i < S::MI; ++i) {
+    const int64_t m = m0 + wm + i * 16 + (lane & 15);
+    if (a.partial) store_row<float>(a.partial + (nth * a.ci + m) * a.co, n0 + wn, a.co, m < a.ci, acc.v[i]);
+    else store_row<T>(static_cast<T *>(a.dw) + (part.group * a.ci + m) * a.co, n0 + wn, a.co, m < a.ci, acc.v[i]);
+  }
 }
 
 template <class T> static bool dma_fits(const WeightsArgs &a) {
   const int64_t size = sizeof(T);
   return a.ci % kVec<T> == 0 && a.co % kVec<T> == 0 && aligned(a.x) && aligned(a.dz) && a.ci * size <= (1 << 22) &&
          a.co * size <= (1 << 22) && (!a.source || a.num_sources * a.ci * size < kBufferLimit);
+}
+
+template <class T, int M, int N, int WM, int WN>
+static int launch_weights_tile(const WeightsArgs &a, int64_t parts, hipStream_t stream) {
+  const int64_t blocks = parts * div_up(a.co, N) * div_up(a.ci, M);
+  SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear_weights_gradient: too many tiles");
+  const dim3 threads(Tile<T, M, N, WM, WN>::NT);
+  if (a.source)
+    hipLaunchKernelGGL((weights_tile_kernel<T, true, M, N, WM, WN>), dim3(blocks), threads, 0, stream, a);
+  else
+    hipLaunchKernelGGL((weights_tile_kernel<T, false, M, N, WM, WN>), dim3(blocks), threads, 0, stream, a);
+  SPIRA_HIP_LAUNCH_CHECK();
+  return kOk;
+}
+template <class T> static int launch_weights(const WeightsArgs &a, int64_t parts, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2)
+    if (a.ci > 128 && a.co > 128 && parts * div_up(a.ci, 256) * div_up(a.co, 256) >= 256)
+      return launch_weights_tile<T, 256, 256, 128, 64>(a, parts, stream);
+  return launch_weights_tile<T, 128, 128, 64, 64>(a, parts, stream);
 }
 
 // out[e] = sum of the group's parts (`size` values each): 16 lanes of four values
@@ -1097,9 +1319,7 @@ int spira_hip_grouped_linear_weights_gradient(int64_t rows, int groups, const in
                            part ? static_cast<float *>(workspace) : nullptr, dw};
     const int64_t z = part ? grouped::most_parts(rows, groups, part) : groups;
     if (grouped::dma_fits<T>(a)) {
-      const int64_t blocks = z * div_up(c_out, 128) * div_up(c_in, 128);
-      SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear_weights_gradient: too many tiles");
-      hipLaunchKernelGGL((grouped::weights_tile_kernel<T, 128, 128, 64, 64>), dim3(blocks), dim3(256), 0, stream, a);
+      if (int rc = grouped::launch_weights<T>(a, z, stream)) return rc;
     } else
       hipLaunchKernelGGL(grouped::weights_kernel<T>,
                        dim3(div_up(c_out, grouped::kCols), div_up(c_in, grouped::kRows), z), dim3(grouped::kThreads), 0,
