@@ -9,10 +9,11 @@
 // and weight 0 in the rest.
 //
 // Order: a stable counting sort of the T k assignments by expert, those without
-// one last.  Blocks of 2048 assignments count their experts, one block per
-// expert turns the counts into running sums, and each block ranks its own
-// assignments: lanes of a wave with the same expert find each other by one
-// ballot per bit of the expert's number.  No order depends on atomics.
+// one last.  The blocks that choose count their tokens' experts; then as many
+// blocks sum the counts before their own and rank their assignments: lanes of a
+// wave with the same expert find each other by one ballot per bit of the
+// expert's number.  No order depends on atomics (those on integer counts only
+// add up).  Few tokens take one block and one launch.
 //
 // Bound by launches up to about 100k tokens, by memory past that.
 #include "numeric.hpp"
@@ -25,7 +26,7 @@ namespace route {
 
 constexpr int kMaxExperts = 512;
 constexpr int kMaxChoices = 16;
-constexpr int kTile = 2048;  // assignments per block of the sort
+constexpr int kTile = 2048;  // most assignments per block
 constexpr int kHeld = 8;     // logits per lane
 
 // larger logit, larger key; 0 for nothing left
@@ -104,50 +105,53 @@ __device__ __forceinline__ void choose(const T *logits, int experts, int k, int 
   put(-1, 0, sum);
 }
 
-template <class T, int G>
-__global__ __launch_bounds__(256) void choose_kernel(const T *logits, int64_t tokens, int experts, int k,
-                                                     int renormalize, float *weights, int32_t *chosen) {
-  constexpr int TPB = 256 / G;
-  __shared__ float num[TPB][kMaxChoices + 1];
-  __shared__ int32_t pick[TPB][kMaxChoices + 1];
-  const int lane = threadIdx.x % G, slot = threadIdx.x / G;
-  const int64_t first = blockIdx.x * static_cast<int64_t>(TPB), token = first + slot;
-  if (token < tokens)
-    choose<T, G>(logits + token * experts, experts, k, renormalize, lane, [&](int j, int e, float v) {
-      if (lane != 0) return;
-      num[slot][j < 0 ? kMaxChoices : j] = v;
-      if (j >= 0) pick[slot][j] = e;
-    });
-  __syncthreads();
-  const int n = static_cast<int>(std::min<int64_t>(TPB, tokens - first)) * k;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int t = i / k, j = i % k;
-    const int32_t e = pick[t][j];
-    weights[first * k + i] = e >= 0 ? num[t][j] / num[t][kMaxChoices] : 0.f;
-    chosen[first * k + i] = e;
-  }
-}
-
 // the bin of an assignment: its expert, or `experts` without one (also for
 // numbers that are none, so that no count leaves its place)
 __device__ __forceinline__ int bin_of(int32_t e, int experts) {
   return static_cast<uint32_t>(e) < static_cast<uint32_t>(experts) ? e : experts;
 }
 
-// counts[bin, block]
-__global__ __launch_bounds__(256) void count_kernel(const int32_t *chosen, int64_t n, int experts, int blocks,
-                                                    int32_t *counts) {
-  __shared__ int32_t c[kMaxExperts + 1];
-  for (int e = threadIdx.x; e <= experts; e += 256) c[e] = 0;
-  __syncthreads();
-  const int64_t first = blockIdx.x * static_cast<int64_t>(kTile);
-#pragma unroll
-  for (int i = 0; i < kTile / 256; ++i) {
-    const int64_t a = first + i * 256 + threadIdx.x;
-    if (a < n) atomicAdd(&c[bin_of(chosen[a], experts)], 1);
+// The choices of tokens first to first + count by the block's 256 threads, 256 / G
+// at a time, and their number per bin.
+template <class T, int G>
+__device__ void choose_tokens(const T *logits, int64_t first, int count, int experts, int k, int renormalize,
+                              float *weights, int32_t *chosen, int32_t *bins) {
+  constexpr int TPB = 256 / G;
+  __shared__ float num[TPB][kMaxChoices + 1];
+  __shared__ int32_t pick[TPB][kMaxChoices + 1];
+  const int lane = threadIdx.x % G, slot = threadIdx.x / G;
+  for (int e = threadIdx.x; e <= experts; e += 256) bins[e] = 0;
+  for (int t0 = 0; t0 < count; t0 += TPB) {
+    __syncthreads();
+    if (t0 + slot < count)
+      choose<T, G>(logits + (first + t0 + slot) * experts, experts, k, renormalize, lane, [&](int j, int e, float v) {
+        if (lane != 0) return;
+        num[slot][j < 0 ? kMaxChoices : j] = v;
+        if (j >= 0) pick[slot][j] = e;
+      });
+    __syncthreads();
+    const int n = min(TPB, count - t0) * k;
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const int t = i / k, j = i % k;
+      const int32_t e = pick[t][j];
+      weights[(first + t0) * k + i] = e >= 0 ? num[t][j] / num[t][kMaxChoices] : 0.f;
+      chosen[(first + t0) * k + i] = e;
+      atomicAdd(&bins[bin_of(e, experts)], 1);
+    }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e <= experts; e += 256) counts[e * static_cast<int64_t>(blocks) + blockIdx.x] = c[e];
+}
+
+// choices of `tile` tokens a block, and counts[bin, block]
+template <class T, int G>
+__global__ __launch_bounds__(256) void choose_kernel(const T *logits, int64_t tokens, int tile, int experts, int k,
+                                                     int renormalize, float *weights, int32_t *chosen,
+                                                     int32_t *counts) {
+  __shared__ int32_t bins[kMaxExperts + 1];
+  const int64_t first = blockIdx.x * static_cast<int64_t>(tile);
+  choose_tokens<T, G>(logits, first, static_cast<int>(std::min<int64_t>(tile, tokens - first)), experts, k, renormalize,
+                      weights, chosen, bins);
+  for (int e = threadIdx.x; e <= experts; e += 256) counts[e * static_cast<int64_t>(gridDim.x) + blockIdx.x] = bins[e];
 }
 
 // inclusive sum over the block's threads (NT), with the block's total
@@ -197,61 +201,120 @@ __device__ __forceinline__ uint64_t same(int value, int bits, bool there) {
   return m;
 }
 
-__global__ __launch_bounds__(256) void rank_kernel(const int32_t *chosen, int64_t n, int experts, int k, int bits,
-                                                   int blocks, const int32_t *counts, const int32_t *totals,
-                                                   int32_t *offsets, int32_t *rows, int32_t *slots) {
+struct Order {
+  int experts, k, bits;
+  int32_t *offsets, *rows, *slots;
+};
+
+// Ranks assignments first to last (at most kTile) of `chosen`; begin(e): the
+// first row of bin e for them.  A quarter of them a wave, in order.
+template <class Begin>
+__device__ void rank_tile(const int32_t *chosen, int64_t first, int64_t last, const Order &o, Begin &&begin) {
   __shared__ int32_t base[4][kMaxExperts + 1];  // next row of each bin, per wave
-  __shared__ int32_t shared[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t first = blockIdx.x * static_cast<int64_t>(kTile) + wave * (kTile / 4);
-  for (int i = threadIdx.x; i < 4 * (kMaxExperts + 1); i += 256) (&base[0][0])[i] = 0;
+  const int share = static_cast<int>((last - first + 255) / 256) * 64;
+  const int64_t from = first + wave * share, to = std::min(from + share, last);
+  for (int e = lane; e <= o.experts; e += 64) base[wave][e] = 0;
   __syncthreads();
   int bin[kTile / 256];
 #pragma unroll
   for (int i = 0; i < kTile / 256; ++i) {
-    const int64_t a = first + i * 64 + lane;
-    bin[i] = a < n ? bin_of(chosen[a], experts) : experts;
-    if (a < n) atomicAdd(&base[wave][bin[i]], 1);
+    const int64_t a = from + i * 64 + lane;
+    bin[i] = a < to ? bin_of(chosen[a], o.experts) : o.experts;
+    if (a < to) atomicAdd(&base[wave][bin[i]], 1);
   }
   __syncthreads();
-  // counts of the waves to first rows
-  int32_t sum = 0;
-  for (int e0 = 0; e0 <= experts; e0 += 256) {
-    const int e = e0 + threadIdx.x;
-    const int32_t v = e <= experts ? totals[e] : 0;
-    int32_t total;
-    const int32_t upto = block_scan<256>(v, shared, total);
-    if (e <= experts) {
-      const int32_t begin = sum + upto - v;
-      if (blockIdx.x == 0) offsets[e] = begin;
-      int32_t at = begin + (n > 0 ? counts[e * static_cast<int64_t>(blocks) + blockIdx.x] : 0);
+  for (int e = threadIdx.x; e <= o.experts; e += 256) {
+    int32_t at = begin(e);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int32_t c = base[w][e];
-        base[w][e] = at;
-        at += c;
-      }
+    for (int w = 0; w < 4; ++w) {
+      const int32_t c = base[w][e];
+      base[w][e] = at;
+      at += c;
     }
-    sum += total;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kTile / 256; ++i) {
-    const int64_t a = first + i * 64 + lane;
-    const bool there = a < n;
-    const uint64_t m = same(bin[i], bits, there);
+    const int64_t a = from + i * 64 + lane;
+    const bool there = a < to;
+    if (!ballot(there)) break;
+    const uint64_t m = same(bin[i], o.bits, there);
     if (there) {
-      const int before = lane_prefix(m);
-      const int32_t at = base[wave][bin[i]] + before;
+      const int32_t at = base[wave][bin[i]] + lane_prefix(m);
       // (the last lane of each expert, after all have read; a wave's LDS
       // accesses keep their order)
       if ((m >> lane) == 1) base[wave][bin[i]] = at + 1;
-      const bool held = bin[i] < experts;
-      rows[at] = held ? static_cast<int32_t>(a / k) : -1;
-      slots[a] = held ? at : -1;
+      const bool held = bin[i] < o.experts;
+      o.rows[at] = held ? static_cast<int32_t>(a / o.k) : -1;
+      o.slots[a] = held ? at : -1;
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// first[e] = sum of v[0 .. e - 1] for the experts + 1 bins of a block
+__device__ __forceinline__ void bins_before(const int32_t *v, int32_t *first, int experts, int32_t *shared) {
+  int32_t sum = 0;
+  for (int e0 = 0; e0 <= experts; e0 += 256) {
+    const int e = e0 + threadIdx.x;
+    const int32_t c = e <= experts ? v[e] : 0;
+    int32_t total;
+    const int32_t upto = block_scan<256>(c, shared, total);
+    if (e <= experts) first[e] = sum + upto - c;
+    sum += total;
+  }
+  __syncthreads();
+}
+
+// (totals null: the counts are those of the blocks, and each block sums them;
+// else running_kernel has)
+__global__ __launch_bounds__(256) void rank_kernel(const int32_t *chosen, int64_t n, int tile, int blocks,
+                                                   const int32_t *counts, const int32_t *totals, const Order o) {
+  __shared__ int32_t total[kMaxExperts + 1], before[kMaxExperts + 1], first[kMaxExperts + 1], shared[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (totals) {
+    for (int e = threadIdx.x; e <= o.experts; e += 256) {
+      total[e] = totals[e];
+      before[e] = n > 0 ? counts[e * static_cast<int64_t>(blocks) + blockIdx.x] : 0;
+    }
+  } else {
+    for (int e = wave; e <= o.experts; e += 4) {
+      int32_t all = 0, mine = 0;
+      for (int b = lane; b < blocks; b += 64) {
+        const int32_t c = counts[e * static_cast<int64_t>(blocks) + b];
+        all += c;
+        mine += b < static_cast<int>(blockIdx.x) ? c : 0;
+      }
+#pragma unroll
+      for (int s = 32; s > 0; s >>= 1) {
+        all += __shfl_xor(all, s, 64);
+        mine += __shfl_xor(mine, s, 64);
+      }
+      if (lane == 0) {
+        total[e] = all;
+        before[e] = mine;
+      }
+    }
+  }
+  __syncthreads();
+  bins_before(total, first, o.experts, shared);
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= o.experts; e += 256) o.offsets[e] = first[e];
+  const int64_t a = blockIdx.x * static_cast<int64_t>(tile);
+  rank_tile(chosen, a, std::min<int64_t>(a + tile, n), o, [&](int e) { return first[e] + before[e]; });
+}
+
+// the whole of it by one block
+template <class T, int G>
+__global__ __launch_bounds__(256) void route_kernel(const T *logits, int tokens, int renormalize, float *weights,
+                                                    int32_t *chosen, const Order o) {
+  __shared__ int32_t bins[kMaxExperts + 1], first[kMaxExperts + 1], shared[4];
+  choose_tokens<T, G>(logits, 0, tokens, o.experts, o.k, renormalize, weights, chosen, bins);
+  bins_before(bins, first, o.experts, shared);
+  for (int e = threadIdx.x; e <= o.experts; e += 256) o.offsets[e] = first[e];
+  // (the choices, written by other threads of the block, are visible behind the barriers)
+  rank_tile(chosen, 0, static_cast<int64_t>(tokens) * o.k, o, [&](int e) { return first[e]; });
 }
 
 // dlogits.  Over the chosen: w (d - sum d w) at them, 0 elsewhere; over all
@@ -391,6 +454,18 @@ template <class F> int with_lanes(int experts, F &&f) {
   return f(integral_constant<int, 64>{});
 }
 
+// Tokens per block: one pass of the block's threads while that leaves the sort
+// no more than 256 blocks' counts, then more, up to kTile assignments; all of
+// them where four passes of one block do.
+static int tile_tokens(int64_t tokens, int experts, int k) {
+  int lanes = 1;
+  while (lanes * kHeld < experts) lanes *= 2;
+  const int pass = std::min(256 / lanes, kTile / k);
+  if (tokens <= 4 * pass && tokens * k <= kTile) return static_cast<int>(std::max<int64_t>(tokens, 1));
+  const int64_t even = round_up(div_up(tokens, 256), pass);
+  return static_cast<int>(std::max<int64_t>(std::min<int64_t>(even, kTile / k / pass * pass), pass));
+}
+
 static int check(int64_t tokens, int experts, int k) {
   SPIRA_HIP_REQUIRE(experts > 0 && experts <= kMaxExperts, "route: needs 1 to 512 experts");
   SPIRA_HIP_REQUIRE(k > 0 && k <= kMaxChoices && k <= experts, "route: needs 1 to 16 choices, at most the experts");
@@ -408,7 +483,7 @@ extern "C" {
 
 int spira_hip_route_workspace(int64_t tokens, int experts, int k, size_t *bytes) {
   if (int rc = route::check(tokens, experts, k)) return rc;
-  const int64_t blocks = div_up(tokens * k, route::kTile);
+  const int64_t blocks = div_up(tokens, route::tile_tokens(tokens, experts, k));
   *bytes = static_cast<size_t>((blocks + 1) * (experts + 1)) * sizeof(int32_t);
   return kOk;
 }
@@ -418,34 +493,42 @@ int spira_hip_route(const void *logits, int64_t tokens, int experts, int k, int 
                     size_t workspace_bytes, hipStream_t stream) {
   if (int rc = route::check(tokens, experts, k)) return rc;
   const int64_t n = tokens * k;
-  const int blocks = static_cast<int>(div_up(n, route::kTile));
+  const int tile = route::tile_tokens(tokens, experts, k);
+  const int blocks = static_cast<int>(div_up(tokens, tile));
   SPIRA_HIP_REQUIRE(workspace && workspace_bytes >= static_cast<size_t>((blocks + int64_t(1)) * (experts + 1)) * 4,
                     "route: workspace too small (spira_hip_route_workspace)");
   SPIRA_HIP_REQUIRE(offsets && (n == 0 || (logits && weights && chosen && rows && slots)), "route: null tensor");
   auto *totals = static_cast<int32_t *>(workspace);
   int32_t *counts = totals + experts + 1;
+  int bits = 0;
+  while ((1 << bits) <= experts) ++bits;
+  const route::Order o{experts, k, bits, offsets, rows, slots};
   return with_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    if (n > 0) {
-      const int rc = route::with_lanes(experts, [&](auto G) -> int {
-        constexpr int g = decltype(G)::value;
-        hipLaunchKernelGGL((route::choose_kernel<T, g>), dim3(div_up(tokens, 256 / g)), dim3(256), 0, stream,
-                           static_cast<const T *>(logits), tokens, experts, k, renormalize, weights, chosen);
+    return route::with_lanes(experts, [&](auto G) -> int {
+      constexpr int g = decltype(G)::value;
+      const T *l = static_cast<const T *>(logits);
+      if (blocks <= 1) {
+        hipLaunchKernelGGL((route::route_kernel<T, g>), dim3(1), dim3(256), 0, stream, l, static_cast<int>(tokens),
+                           renormalize, weights, chosen, o);
         SPIRA_HIP_LAUNCH_CHECK();
         return kOk;
-      });
-      if (rc) return rc;
-      hipLaunchKernelGGL(route::count_kernel, dim3(blocks), dim3(256), 0, stream, chosen, n, experts, blocks, counts);
+      }
+      hipLaunchKernelGGL((route::choose_kernel<T, g>), dim3(blocks), dim3(256), 0, stream, l, tokens, tile, experts, k,
+                         renormalize, weights, chosen, counts);
       SPIRA_HIP_LAUNCH_CHECK();
-    }
-    hipLaunchKernelGGL(route::running_kernel, dim3(experts + 1), dim3(256), 0, stream, blocks, counts, totals);
-    SPIRA_HIP_LAUNCH_CHECK();
-    int bits = 0;
-    while ((1 << bits) <= experts) ++bits;
-    hipLaunchKernelGGL(route::rank_kernel, dim3(std::max(blocks, 1)), dim3(256), 0, stream, chosen, n, experts, k,
-                       bits, blocks, counts, totals, offsets, rows, slots);
-    SPIRA_HIP_LAUNCH_CHECK();
-    return kOk;
+      // Each block of the second launch reads all counts, a wave a bin: worth it
+      // while that is a few microseconds (one launch costs about four).
+      const bool summed = (experts + 1) * div_up(blocks, 64) <= 128;
+      if (!summed) {
+        hipLaunchKernelGGL(route::running_kernel, dim3(experts + 1), dim3(256), 0, stream, blocks, counts, totals);
+        SPIRA_HIP_LAUNCH_CHECK();
+      }
+      hipLaunchKernelGGL(route::rank_kernel, dim3(blocks), dim3(256), 0, stream, chosen, n, tile * k, blocks, counts,
+                         summed ? nullptr : totals, o);
+      SPIRA_HIP_LAUNCH_CHECK();
+      return kOk;
+    });
   });
 }
 
