@@ -481,14 +481,24 @@ __global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(
       }
   };
   find_rows(part.begin + wave * 16 * MT);
+  fetch();
   if constexpr (KO) {
     // as they lie in memory, [KF FK, quads 64], zeros past their ends; then, all
     // in registers between two barriers, to fragments
-    const int cpr = quads * 64 / kVec<T>;
-    for (int id = threadIdx.x; id < KF * FK * cpr; id += kStreamThreads) {
-      const int k = id / cpr, c = id - k * cpr;
-      const T *p = w + k * a.n + c * kVec<T>;
-      *reinterpret_cast<uintx4_t *>(wlds + id * 16) = load_raw(p, k < a.k ? a.n - c * kVec<T> : 0);
+    // (nine loads of a thread at a time under way)
+    const int cpr = quads * 64 / kVec<T>, chunks = KF * FK * cpr;
+    for (int first = threadIdx.x; first < chunks; first += 9 * kStreamThreads) {
+      uintx4_t v[9];
+#pragma unroll
+      for (int q = 0; q < 9; ++q) {
+        const int id = first + q * kStreamThreads, k = id / cpr, c = id - k * cpr;
+        v[q] = load_raw(w + k * a.n + c * kVec<T>, k < a.k ? a.n - c * kVec<T> : 0);
+      }
+#pragma unroll
+      for (int q = 0; q < 9; ++q) {
+        const int id = first + q * kStreamThreads;
+        if (id < chunks) *reinterpret_cast<uintx4_t *>(wlds + id * 16) = v[q];
+      }
     }
     __syncthreads();
     uintx4_t v[MOST];
@@ -522,7 +532,6 @@ __global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(
       *reinterpret_cast<uintx4_t *>(wlds + id * 1024 + lane * 16) = load_raw(w + n * a.k + k, n < a.n ? a.k - k : 0);
     }
   }
-  fetch();
   __syncthreads();
   const T *bias = a.bias ? static_cast<const T *>(a.bias) + part.group * a.n : nullptr;
   for (int64_t r0 = part.begin + wave * 16 * MT; r0 < part.end; r0 += kStreamWaves * 16 * MT) {
@@ -578,7 +587,7 @@ template <class T, bool KO> static int launch_stream(const RowsArgs &a, hipStrea
   const auto go = [&](auto KF, auto MT) -> int {
     constexpr int kf = decltype(KF)::value, mt = decltype(MT)::value;
     const size_t lds = static_cast<size_t>(kf) * 4 * div_up(a.n, 64) * 1024;
-    // a part gives each wave one or two tiles
+    // a part gives each wave one tile, or two where that leaves parts for every CU
     const int rows = kStreamWaves * 16 * mt * (a.g.rows >= 65536 ? 2 : 1);
     const auto kernel = stream_kernel<T, KO, kf, mt>;
     SPIRA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -591,13 +600,17 @@ template <class T, bool KO> static int launch_stream(const RowsArgs &a, hipStrea
   using std::integral_constant;
   const int64_t f = div_up(a.k * static_cast<int64_t>(sizeof(T)), 64);
   constexpr integral_constant<int, 1> one;
-  constexpr integral_constant<int, 2> two;
+  // tiles of 32 rows halve the reads of the weights from LDS; of 16 rows they
+  // give twice the waves work where there are few
+  const auto either = [&](auto KF) {
+    return a.g.rows >= 65536 ? go(KF, integral_constant<int, 2>{}) : go(KF, one);
+  };
   switch (f) {
-    case 1: return go(integral_constant<int, 1>{}, two);
-    case 2: return go(integral_constant<int, 2>{}, two);
-    case 3: return go(integral_constant<int, 3>{}, two);
-    case 4: return go(integral_constant<int, 4>{}, two);
-    case 5: case 6: return go(integral_constant<int, 6>{}, two);
+    case 1: return either(integral_constant<int, 1>{});
+    case 2: return either(integral_constant<int, 2>{});
+    case 3: return either(integral_constant<int, 3>{});
+    case 4: return either(integral_constant<int, 4>{});
+    case 5: case 6: return either(integral_constant<int, 6>{});
     case 7: case 8: return go(integral_constant<int, 8>{}, one);
     case 9: case 10: case 11: case 12: return go(integral_constant<int, 12>{}, one);
     default: return go(integral_constant<int, 16>{}, one);
@@ -1253,7 +1266,7 @@ static int weight_parts(int64_t rows, int64_t groups, int64_t ci, int64_t co) {
   const int64_t tiles = div_up(ci, kRows) * div_up(co, kCols) * groups;
   const int64_t want = 4 * 256;
   if (tiles >= want || rows == 0) return 0;
-  const int64_t size = std::max<int64_t>(round_up(div_up(rows * div_up(ci, kRows) * div_up(co, kCols), want), 64), 256);
+  const int64_t size = std::max<int64_t>(round_up(div_up(rows * div_up(ci, kRows) * div_up(co, kCols), want), 64), 128);
   return static_cast<int>(launch_limit(rows, groups, size));
 }
 

@@ -57,20 +57,27 @@ template <int G> __device__ __forceinline__ float row_sum(float v, float *shared
 template <class T, int NV> struct Row {
   float v[NV][kVec<T>];
 };
+// a row as it lies in memory: half the registers, unpacked where it is used
+template <int NV> struct Raw {
+  uintx4_t v[NV];
+};
 
 template <class T, int G, int NV>
-__device__ __forceinline__ Row<T, NV> load_row(const void *base, int64_t row, int c, int lane, float none = 0.f) {
-  Row<T, NV> r;
+__device__ __forceinline__ Raw<NV> load_row(const void *base, int64_t row, int c, int lane) {
+  Raw<NV> r;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int at = (lane + i * G) * kVec<T>;
-    Chunk<T> k;
-    if (base) {
-      k = load_chunk(static_cast<const T *>(base) + row * c + at, c - at);
-    } else {
+    r.v[i] = load_raw(static_cast<const T *>(base) + row * c + at, base ? c - at : 0);
+  }
+  return r;
+}
+
+template <class T, int NV> __device__ __forceinline__ Row<T, NV> unpack_row(const Raw<NV> &raw) {
+  Row<T, NV> r;
 #pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) k.v[j] = none;
-    }
+  for (int i = 0; i < NV; ++i) {
+    const Chunk<T> k = unpack<T>(raw.v[i]);
 #pragma unroll
     for (int j = 0; j < kVec<T>; ++j) r.v[i][j] = k.v[j];
   }
@@ -97,120 +104,174 @@ template <class T, int NV, class F> __device__ __forceinline__ void each(F &&f) 
     for (int j = 0; j < kVec<T>; ++j) f(i, j);
 }
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+// (the hardware's exponential and reciprocal, good to one unit each: at |v| up to
+// 20 within 3e-6 of the value; the library's take 17 us of a 16k x 1024 call)
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+}
 
-// the row's gate (raw)
+// a row's part of the gate as it lies in memory: its channels, or its one value
 template <class T, int G, int NV>
-__device__ __forceinline__ Row<T, NV> load_gate(const Args &a, int64_t row, int lane, const Row<T, NV> &channel) {
+__device__ __forceinline__ Raw<NV> load_gate(const Args &a, int64_t row, int lane) {
   if (a.gate_form == kFull) return load_row<T, G, NV>(a.gate, row, a.c, lane);
-  if (a.gate_form != kRow) return channel;
+  Raw<NV> g{};
+  if (a.gate_form == kRow) g.v[0] = load_raw(static_cast<const T *>(a.gate) + row, 1);
+  return g;
+}
+// the gate's values, through its sigmoid if it has one; `channel`: a gate per channel
+template <class T, int NV>
+__device__ __forceinline__ Row<T, NV> gate_of(const Args &a, const Raw<NV> &own, const Raw<NV> &channel) {
   Row<T, NV> g;
-  const float v = to_float(static_cast<const T *>(a.gate)[row]);
-  each<T, NV>([&](int i, int j) { g.v[i][j] = v; });
+  if (a.gate_form == kNone) {
+    each<T, NV>([&](int i, int j) { g.v[i][j] = 1.f; });
+    return g;
+  }
+  g = unpack_row<T>(a.gate_form == kChannel ? channel : own);
+  if (a.gate_form == kRow) {
+    const float v = g.v[0][0];
+    each<T, NV>([&](int i, int j) { g.v[i][j] = v; });
+  }
+  if (a.sigmoid) each<T, NV>([&](int i, int j) { g.v[i][j] = sigmoid(g.v[i][j]); });
   return g;
 }
 
+// Each group of lanes walks rows, with the next row's loads under way while it
+// computes; weights stay in registers.  (Every group takes as many turns, so that
+// a block's barriers meet.)
 template <class T, int G, int NV, int NT>
 __global__ __launch_bounds__(NT) void forward_kernel(const Args a) {
   __shared__ float shared[NT / 64];
   constexpr int RPB = NT / G;
   const int lane = threadIdx.x % G;
   const float inv_c = 1.f / static_cast<float>(a.c);
-  const int64_t row = blockIdx.x * static_cast<int64_t>(RPB) + threadIdx.x / G;
-  if (row >= a.n) return;  // (whole groups of lanes; blocks of one row keep all of theirs)
-  Row<T, NV> r = load_row<T, G, NV>(a.x, row, a.c, lane);
-  if (a.h) {
-    Row<T, NV> z = load_row<T, G, NV>(a.h, row, a.c, lane);
-    const Row<T, NV> w = load_row<T, G, NV>(a.w, 0, a.c, lane, 1.f);
-    Row<T, NV> g = load_row<T, G, NV>(a.gate_form == kChannel ? a.gate : nullptr, 0, a.c, lane, 1.f);
-    g = load_gate<T, G, NV>(a, row, lane, g);
-    if (a.w) {
-      float ss = 0;
-      each<T, NV>([&](int i, int j) { ss += z.v[i][j] * z.v[i][j]; });
-      const float inv = rsqrtf(row_sum<G>(ss, shared) * inv_c + a.eps);
-      if (a.inv_h && lane == 0) a.inv_h[row] = inv;
-      each<T, NV>([&](int i, int j) { z.v[i][j] *= inv * w.v[i][j]; });
+  const int64_t turn = gridDim.x * static_cast<int64_t>(RPB);
+  const Raw<NV> w_raw = load_row<T, G, NV>(a.w, 0, a.c, lane), next_raw = load_row<T, G, NV>(a.w_next, 0, a.c, lane);
+  const Raw<NV> channel = load_row<T, G, NV>(a.gate_form == kChannel ? a.gate : nullptr, 0, a.c, lane);
+  int64_t first = blockIdx.x * static_cast<int64_t>(RPB);
+  Raw<NV> x, h, gate;
+  const auto fetch = [&](int64_t from) {
+    const int64_t row = std::min<int64_t>(from + threadIdx.x / G, a.n - 1);
+    x = load_row<T, G, NV>(a.x, row, a.c, lane);
+    if (a.h) {
+      h = load_row<T, G, NV>(a.h, row, a.c, lane);
+      gate = load_gate<T, G, NV>(a, row, lane);
     }
-    if (a.gate_form != kNone && a.sigmoid) each<T, NV>([&](int i, int j) { g.v[i][j] = sigmoid(g.v[i][j]); });
-    each<T, NV>([&](int i, int j) { r.v[i][j] += a.scale * g.v[i][j] * z.v[i][j]; });
-    store_row<T, G, NV>(a.r, row, a.c, lane, r);
-  }
-  if (a.next) {
-    const Row<T, NV> w = load_row<T, G, NV>(a.w_next, 0, a.c, lane);
-    float ss = 0;
-    each<T, NV>([&](int i, int j) { ss += r.v[i][j] * r.v[i][j]; });
-    // (lanes past the row hold zeros)
-    const float inv = rsqrtf(row_sum<G>(ss, shared) * inv_c + a.eps);
-    if (a.inv_r && lane == 0) a.inv_r[row] = inv;
-    each<T, NV>([&](int i, int j) { r.v[i][j] *= inv * w.v[i][j]; });
-    store_row<T, G, NV>(a.next, row, a.c, lane, r);
+  };
+  fetch(first);
+  for (; first < a.n; first += turn) {
+    const int64_t row = first + threadIdx.x / G;
+    const bool there = row < a.n;
+    Row<T, NV> r = unpack_row<T>(x), z = unpack_row<T>(h);
+    const Raw<NV> own = gate;
+    if (first + turn < a.n) fetch(first + turn);
+    if (a.h) {
+      if (a.w) {
+        float ss = 0;
+        each<T, NV>([&](int i, int j) { ss += z.v[i][j] * z.v[i][j]; });
+        const float inv = rsqrtf(row_sum<G>(ss, shared) * inv_c + a.eps);
+        if (there && a.inv_h && lane == 0) a.inv_h[row] = inv;
+        const Row<T, NV> w = unpack_row<T>(w_raw);
+        each<T, NV>([&](int i, int j) { z.v[i][j] *= inv * w.v[i][j]; });
+      }
+      const Row<T, NV> g = gate_of<T>(a, own, channel);
+      each<T, NV>([&](int i, int j) { r.v[i][j] += a.scale * g.v[i][j] * z.v[i][j]; });
+      if (there) store_row<T, G, NV>(a.r, row, a.c, lane, r);
+    }
+    if (a.next) {
+      float ss = 0;
+      each<T, NV>([&](int i, int j) { ss += r.v[i][j] * r.v[i][j]; });
+      // (lanes past the row hold zeros)
+      const float inv = rsqrtf(row_sum<G>(ss, shared) * inv_c + a.eps);
+      if (there && a.inv_r && lane == 0) a.inv_r[row] = inv;
+      const Row<T, NV> w = unpack_row<T>(next_raw);
+      each<T, NV>([&](int i, int j) { r.v[i][j] *= inv * w.v[i][j]; });
+      if (there) store_row<T, G, NV>(a.next, row, a.c, lane, r);
+    }
   }
 }
 
-template <class T, int G, int NV, int NT>
+// CHANNEL: a gate per channel, whose gradient is a sum over the rows
+template <class T, int G, int NV, int NT, bool CHANNEL>
 __global__ __launch_bounds__(NT) void backward_kernel(const Args a) {
   constexpr int RPB = NT / G, VEC = kVec<T>, NW = NT / 64;
   __shared__ float shared[NW];
-  __shared__ float sums[G < 64 || NW > G / 64 ? NW * G * NV * VEC : 1];
+  __shared__ float sums[NT > G ? NW * G * NV * VEC : 1];
   const int lane = threadIdx.x % G;
   const float inv_c = 1.f / static_cast<float>(a.c);
-  const Row<T, NV> w = load_row<T, G, NV>(a.w, 0, a.c, lane, 1.f);
-  const Row<T, NV> w_next = load_row<T, G, NV>(a.dnext ? a.w_next : nullptr, 0, a.c, lane);
-  const Row<T, NV> channel =
-      load_row<T, G, NV>(a.gate_form == kChannel ? a.gate : nullptr, 0, a.c, lane, 1.f);
+  const int64_t turn = gridDim.x * static_cast<int64_t>(RPB);
+  const Raw<NV> w_raw = load_row<T, G, NV>(a.w, 0, a.c, lane), next_raw = load_row<T, G, NV>(a.w_next, 0, a.c, lane);
+  const Raw<NV> channel = load_row<T, G, NV>(CHANNEL ? a.gate : nullptr, 0, a.c, lane);
   Row<T, NV> dw{}, dw_next{}, dg_sum{};
-  // (every group of lanes walks as many rows, so that a block's barriers meet)
-  for (int64_t first = blockIdx.x * static_cast<int64_t>(RPB); first < a.n;
-       first += gridDim.x * static_cast<int64_t>(RPB)) {
-    const int64_t own = first + threadIdx.x / G;
-    const bool there = own < a.n;
-    const int64_t row = there ? own : a.n - 1;
-    Row<T, NV> r = load_row<T, G, NV>(a.x, row, a.c, lane), hh{}, g{};
-    Row<T, NV> d = load_row<T, G, NV>(a.dr, row, a.c, lane);
-    float inv_h = 1.f;
+  int64_t first = blockIdx.x * static_cast<int64_t>(RPB);
+  Raw<NV> x, h, gate, dr, dnext;
+  float inv_h, inv_r;
+  const auto fetch = [&](int64_t from) {
+    const int64_t row = std::min<int64_t>(from + threadIdx.x / G, a.n - 1);
+    x = load_row<T, G, NV>(a.x, row, a.c, lane);
     if (a.h) {
-      hh = load_row<T, G, NV>(a.h, row, a.c, lane);
-      g = load_gate<T, G, NV>(a, row, lane, channel);
-      if (a.gate_form != kNone && a.sigmoid) each<T, NV>([&](int i, int j) { g.v[i][j] = sigmoid(g.v[i][j]); });
-      if (a.w) inv_h = a.inv_h[row];
+      h = load_row<T, G, NV>(a.h, row, a.c, lane);
+      gate = load_gate<T, G, NV>(a, row, lane);
+    }
+    dr = load_row<T, G, NV>(a.dr, row, a.c, lane);
+    if (a.dnext) dnext = load_row<T, G, NV>(a.dnext, row, a.c, lane);
+    inv_h = a.w ? a.inv_h[row] : 1.f;
+    inv_r = a.dnext ? a.inv_r[row] : 1.f;
+  };
+  fetch(first);
+  for (; first < a.n; first += turn) {
+    const int64_t row = first + threadIdx.x / G;
+    const bool there = row < a.n;
+    Row<T, NV> r = unpack_row<T>(x), d = unpack_row<T>(dr), hh{}, g{};
+    const float ih = inv_h, ir = inv_r;
+    if (a.h) {
+      hh = unpack_row<T>(h);
+      g = gate_of<T>(a, gate, channel);
+      // (z is w hhat, or h)
+      const Row<T, NV> w = unpack_row<T>(w_raw);
       each<T, NV>([&](int i, int j) {
-        hh.v[i][j] *= inv_h;
-        r.v[i][j] += a.scale * g.v[i][j] * (hh.v[i][j] * w.v[i][j]);
+        hh.v[i][j] *= ih;
+        r.v[i][j] += a.scale * g.v[i][j] * (a.w ? hh.v[i][j] * w.v[i][j] : hh.v[i][j]);
       });
     }
+    Row<T, NV> dn = unpack_row<T>(dnext);
+    if (first + turn < a.n) fetch(first + turn);
     if (a.dnext) {
-      const Row<T, NV> dn = load_row<T, G, NV>(a.dnext, row, a.c, lane);
-      const float inv_r = a.inv_r[row];
+      const Row<T, NV> w = unpack_row<T>(next_raw);
       float s = 0;
       each<T, NV>([&](int i, int j) {
-        r.v[i][j] *= inv_r;
-        s += dn.v[i][j] * w_next.v[i][j] * r.v[i][j];
+        r.v[i][j] *= ir;
         if (there) dw_next.v[i][j] += dn.v[i][j] * r.v[i][j];
+        dn.v[i][j] *= w.v[i][j];
+        s += dn.v[i][j] * r.v[i][j];
       });
       s = row_sum<G>(s, shared) * inv_c;
-      each<T, NV>([&](int i, int j) { d.v[i][j] += inv_r * (dn.v[i][j] * w_next.v[i][j] - r.v[i][j] * s); });
+      each<T, NV>([&](int i, int j) { d.v[i][j] += ir * (dn.v[i][j] - r.v[i][j] * s); });
     }
     if (there && a.dx) store_row<T, G, NV>(a.dx, row, a.c, lane, d);
     if (!a.h) continue;
     // d becomes dz, g the gate's gradient
     float along = 0;
-    each<T, NV>([&](int i, int j) {
-      const float dz = a.scale * g.v[i][j] * d.v[i][j];
-      float dg = a.scale * (hh.v[i][j] * w.v[i][j]) * d.v[i][j];
-      if (a.sigmoid) dg *= g.v[i][j] * (1.f - g.v[i][j]);
-      g.v[i][j] = dg;
-      along += dg;
-      d.v[i][j] = dz;
-    });
-    if (a.gate_form == kFull) {
+    {
+      const Row<T, NV> w = unpack_row<T>(w_raw);
+      each<T, NV>([&](int i, int j) {
+        const float dz = a.scale * g.v[i][j] * d.v[i][j];
+        float dg = a.scale * (a.w ? hh.v[i][j] * w.v[i][j] : hh.v[i][j]) * d.v[i][j];
+        if (a.sigmoid) dg *= g.v[i][j] * (1.f - g.v[i][j]);
+        g.v[i][j] = dg;
+        along += dg;
+        d.v[i][j] = dz;
+      });
+    }
+    if constexpr (CHANNEL) {
+      if (there) each<T, NV>([&](int i, int j) { dg_sum.v[i][j] += g.v[i][j]; });
+    } else if (a.gate_form == kFull) {
       if (there && a.dgate) store_row<T, G, NV>(a.dgate, row, a.c, lane, g);
     } else if (a.gate_form == kRow) {
       along = row_sum<G>(along, shared);
       if (there && a.dgate && lane == 0) static_cast<T *>(a.dgate)[row] = from_float<T>(along);
-    } else if (there) {
-      each<T, NV>([&](int i, int j) { dg_sum.v[i][j] += g.v[i][j]; });
     }
     if (a.w) {
+      const Row<T, NV> w = unpack_row<T>(w_raw);
       float s = 0;
       each<T, NV>([&](int i, int j) {
         if (there) dw.v[i][j] += d.v[i][j] * hh.v[i][j];
@@ -218,7 +279,7 @@ __global__ __launch_bounds__(NT) void backward_kernel(const Args a) {
         s += d.v[i][j] * hh.v[i][j];
       });
       s = row_sum<G>(s, shared) * inv_c;
-      each<T, NV>([&](int i, int j) { d.v[i][j] = inv_h * (d.v[i][j] - hh.v[i][j] * s); });
+      each<T, NV>([&](int i, int j) { d.v[i][j] = ih * (d.v[i][j] - hh.v[i][j] * s); });
     }
     if (there && a.dh) store_row<T, G, NV>(a.dh, row, a.c, lane, d);
   }
@@ -251,7 +312,7 @@ __global__ __launch_bounds__(NT) void backward_kernel(const Args a) {
   };
   if (a.w) out(dw, 0);
   if (a.dnext) out(dw_next, 1);
-  if (a.gate_form == kChannel) out(dg_sum, 2);
+  if constexpr (CHANNEL) out(dg_sum, 2);
 }
 
 // columns of the blocks' sums: 16 columns a block, 64 threads to each, joined in
@@ -296,8 +357,11 @@ template <class T, class F> int with_shape(int c, F &&f) {
   return kInvalidArgument;
 }
 
-// blocks of the backward pass: enough to fill the chip twice over, each with
-// its partial sums of the columns
+// Blocks: what the CUs hold at once, each walking rows.  The backward pass's write
+// their partial sums of the columns.
+static int64_t forward_blocks(int64_t n, int rows_per_block) {
+  return std::min<int64_t>(div_up(n, rows_per_block), 2048);
+}
 static int64_t backward_blocks(int64_t n, int rows_per_block) {
   return std::min<int64_t>(div_up(n, rows_per_block), 512);
 }
@@ -337,7 +401,7 @@ int spira_hip_gated_residual_norm(const void *x, const void *h, int64_t n, int c
     using T = decltype(t);
     return norm::with_shape<T>(c, [&](auto G, auto NV, auto NT) -> int {
       constexpr int g = decltype(G)::value, nt = decltype(NT)::value;
-      hipLaunchKernelGGL((norm::forward_kernel<T, g, decltype(NV)::value, nt>), dim3(div_up(n, nt / g)), dim3(nt), 0,
+      hipLaunchKernelGGL((norm::forward_kernel<T, g, decltype(NV)::value, nt>), dim3(norm::forward_blocks(n, nt / g)), dim3(nt), 0,
                          stream, a);
       SPIRA_HIP_LAUNCH_CHECK();
       return kOk;
@@ -385,8 +449,12 @@ int spira_hip_gated_residual_norm_backward(const void *x, const void *h, int64_t
         a.partial = static_cast<float *>(workspace);
       }
       if (n > 0) {
-        hipLaunchKernelGGL((norm::backward_kernel<T, g, decltype(NV)::value, nt>), dim3(blocks), dim3(nt), 0, stream,
-                           a);
+        if (channel)
+          hipLaunchKernelGGL((norm::backward_kernel<T, g, decltype(NV)::value, nt, true>), dim3(blocks), dim3(nt), 0,
+                             stream, a);
+        else
+          hipLaunchKernelGGL((norm::backward_kernel<T, g, decltype(NV)::value, nt, false>), dim3(blocks), dim3(nt), 0,
+                             stream, a);
         SPIRA_HIP_LAUNCH_CHECK();
       }
       if (sums) {

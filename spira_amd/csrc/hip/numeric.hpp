@@ -35,11 +35,16 @@ template <class T> struct Chunk {
 // n: how many of the chunk's values lie inside the row (any number; values
 // past it are zero, or not written)
 template <class T> __device__ __forceinline__ uintx4_t load_raw(const T *p, int64_t n) {
-  if (n >= kVec<T>) return *reinterpret_cast<const Unaligned<T> *>(p);
-  Packed<T> r;
+  uintx4_t raw = {0, 0, 0, 0};
+  if (n >= kVec<T>) {
+    raw = *reinterpret_cast<const Unaligned<T> *>(p);
+  } else if (n > 0) {  // (few lanes; those wholly past the row skip it)
+    Packed<T> r;
 #pragma unroll
-  for (int i = 0; i < kVec<T>; ++i) r.v[i] = i < n ? p[i] : static_cast<T>(0.f);
-  return __builtin_bit_cast(uintx4_t, r);
+    for (int i = 0; i < kVec<T>; ++i) r.v[i] = i < n ? p[i] : static_cast<T>(0.f);
+    raw = __builtin_bit_cast(uintx4_t, r);
+  }
+  return raw;
 }
 template <class T> __device__ __forceinline__ Chunk<T> unpack(uintx4_t raw) {
   const Packed<T> r = __builtin_bit_cast(Packed<T>, raw);
@@ -57,7 +62,7 @@ template <class T> __device__ __forceinline__ void store_chunk(T *p, int64_t n, 
   for (int i = 0; i < kVec<T>; ++i) r.v[i] = from_float<T>(c.v[i]);
   if (n >= kVec<T>) {
     *reinterpret_cast<Unaligned<T> *>(p) = __builtin_bit_cast(uintx4_t, r);
-  } else {
+  } else if (n > 0) {
 #pragma unroll
     for (int i = 0; i < kVec<T>; ++i)
       if (i < n) p[i] = r.v[i];
