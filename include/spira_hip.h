@@ -569,7 +569,8 @@ int spira_hip_grouped_linear_weights_gradient(int64_t rows, int groups, const in
 /* With y (the outputs of a relu): dz = dy where y > 0, else 0, for the groups'
  * rows; without, dz is dy and not written.  dbias[e] = sum of the group's dz,
  * or null. */
-int spira_hip_grouped_linear_activation_gradient_workspace(int64_t rows, int groups, int c_out, size_t *bytes);
+int spira_hip_grouped_linear_activation_gradient_workspace(int64_t rows, int groups, int c_out, int dtype,
+                                                           size_t *bytes);
 int spira_hip_grouped_linear_activation_gradient(int64_t rows, int groups, const int32_t *offsets, const void *dy,
                                                  const void *y, int c_out, int dtype, void *dz, void *dbias,
                                                  void *workspace, size_t workspace_bytes, hipStream_t stream);

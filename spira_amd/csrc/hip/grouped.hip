@@ -430,7 +430,7 @@ template <class T, bool KO> __global__ __launch_bounds__(kThreads) void rows_ker
 // from registers.
 // ---------------------------------------------------------------------------
 constexpr int kStreamWaves = 8, kStreamThreads = 64 * kStreamWaves;
-constexpr int kMostStreamFragments = 144;  // 1 KB each: 16 KB of the LDS left
+constexpr int kMostStreamFragments = 144;  // 1 KB each; at most 9 KB of bias beside them
 
 // the channel (of 64) of operand row i of fragment j
 __device__ __forceinline__ int dealt(int j, int i) { return (i >> 2) * 16 + j * 4 + (i & 3); }
@@ -440,9 +440,10 @@ struct StreamArgs {
   int part_rows;
 };
 
-// KF: fragments (64 bytes) of a row; MT: 16-row tiles a wave takes at a time
-template <class T, bool KO, int KF, int MT>
-__global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(KF * MT <= 8 ? 4 : 2))) void stream_kernel(const StreamArgs sa) {
+// KF: fragments (64 bytes) of a row.  A wave takes 16 rows at a time (32 halve the
+// reads of the weights from LDS and measure the same).
+template <class T, bool KO, int KF>
+__global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(KF <= 8 ? 4 : 2))) void stream_kernel(const StreamArgs sa) {
   constexpr int FK = 64 / static_cast<int>(sizeof(T));  // values of the summed index per fragment
   constexpr int MOST = kMostStreamFragments / kStreamWaves;
   extern __shared__ __align__(1024) char wlds[];
@@ -457,31 +458,27 @@ __global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(
   const int quads = static_cast<int>((a.n + 63) / 64);  // of fragments
   const int fragments = quads * 4 * KF;
   // the first tile's rows are on their way while the weights are laid out
-  const T *row[MT];
-  uintx4_t next[MT][KF];
-  auto find_rows = [&](int64_t r0) {
+  uintx4_t next[KF];
+  auto fetch = [&](int64_t r0) {
+    const int64_t r = r0 + l16;
+    int64_t s = r < part.end ? r : -1;
+    if (s >= 0 && a.source) {
+      s = a.source[r];
+      if (s >= a.num_sources) s = -1;
+    }
+    const T *row = s >= 0 ? static_cast<const T *>(a.x) + s * a.k : nullptr;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int64_t r = r0 + m * 16 + l16;
-      int64_t s = r < part.end ? r : -1;
-      if (s >= 0 && a.source) {
-        s = a.source[r];
-        if (s >= a.num_sources) s = -1;
-      }
-      row[m] = s >= 0 ? static_cast<const T *>(a.x) + s * a.k : nullptr;
+    for (int f = 0; f < KF; ++f) {
+      const int64_t k = f * FK + lq * kVec<T>;
+      next[f] = load_raw(row + k, row ? a.k - k : 0);
     }
   };
-  auto fetch = [&] {
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int f = 0; f < KF; ++f) {
-        const int64_t k = f * FK + lq * kVec<T>;
-        next[m][f] = load_raw(row[m] + k, row[m] ? a.k - k : 0);
-      }
-  };
-  find_rows(part.begin + wave * 16 * MT);
-  fetch();
+  fetch(part.begin + wave * 16);
+  // the bias too lies in LDS: a load from memory in the loop below would wait for
+  // the rows under way before it
+  float *bias = reinterpret_cast<float *>(wlds + fragments * 1024);
+  for (int n = threadIdx.x; n < quads * 64; n += kStreamThreads)
+    bias[n] = a.bias && n < a.n ? to_float(static_cast<const T *>(a.bias)[part.group * a.n + n]) : 0.f;
   if constexpr (KO) {
     // as they lie in memory, [KF FK, quads 64], zeros past their ends; then, all
     // in registers between two barriers, to fragments
@@ -533,44 +530,31 @@ __global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(
     }
   }
   __syncthreads();
-  const T *bias = a.bias ? static_cast<const T *>(a.bias) + part.group * a.n : nullptr;
-  for (int64_t r0 = part.begin + wave * 16 * MT; r0 < part.end; r0 += kStreamWaves * 16 * MT) {
-    uintx4_t x[MT][KF];
+  for (int64_t r0 = part.begin + wave * 16; r0 < part.end; r0 += kStreamWaves * 16) {
+    uintx4_t x[KF];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int f = 0; f < KF; ++f) x[m][f] = next[m][f];
-    find_rows(r0 + kStreamWaves * 16 * MT);
-    fetch();
+    for (int f = 0; f < KF; ++f) x[f] = next[f];
+    fetch(r0 + kStreamWaves * 16);
+    const int64_t r = r0 + l16;
     for (int q = 0; q < quads; ++q) {
-      floatx4_t acc[MT][4] = {};
+      floatx4_t acc[4] = {};
       const char *wq = wlds + q * 4 * KF * 1024 + lane * 16;
 #pragma unroll
       for (int f = 0; f < KF; ++f)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uintx4_t b = *reinterpret_cast<const uintx4_t *>(wq + (j * KF + f) * 1024);
-#pragma unroll
-          for (int m = 0; m < MT; ++m) mma<T>(acc[m][j], b, x[m][f]);
-        }
+        for (int j = 0; j < 4; ++j)
+          mma<T>(acc[j], *reinterpret_cast<const uintx4_t *>(wq + (j * KF + f) * 1024), x[f]);
       const int64_t n = q * 64 + lq * 16;
-      if (n >= a.n) continue;
+      if (n >= a.n || r >= part.end) continue;
 #pragma unroll
       for (int h = 0; h < 16 / kVec<T>; ++h) {
-        Chunk<T> b{};
-        if (bias) b = load_chunk(bias + n + h * kVec<T>, a.n - n - h * kVec<T>);
+        Chunk<T> c;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const int64_t r = r0 + m * 16 + l16;
-          if (r >= part.end) continue;
-          Chunk<T> c;
-#pragma unroll
-          for (int v = 0; v < kVec<T>; ++v) {
-            const float s = acc[m][(h * kVec<T> + v) / 4][v % 4] + b.v[v];
-            c.v[v] = a.relu && s < 0.f ? 0.f : s;
-          }
-          store_chunk(static_cast<T *>(a.y) + r * a.n + n + h * kVec<T>, a.n - n - h * kVec<T>, c);
+        for (int v = 0; v < kVec<T>; ++v) {
+          const float s = acc[(h * kVec<T> + v) / 4][v % 4] + bias[n + h * kVec<T> + v];
+          c.v[v] = a.relu && s < 0.f ? 0.f : s;
         }
+        store_chunk(static_cast<T *>(a.y) + r * a.n + n + h * kVec<T>, a.n - n - h * kVec<T>, c);
       }
     }
   }
@@ -584,36 +568,32 @@ template <class T> static bool streams(int64_t k, int64_t n) {
 }
 
 template <class T, bool KO> static int launch_stream(const RowsArgs &a, hipStream_t stream) {
-  const auto go = [&](auto KF, auto MT) -> int {
-    constexpr int kf = decltype(KF)::value, mt = decltype(MT)::value;
-    const size_t lds = static_cast<size_t>(kf) * 4 * div_up(a.n, 64) * 1024;
-    // a part gives each wave one tile, or two where that leaves parts for every CU
-    const int rows = kStreamWaves * 16 * mt * (a.g.rows >= 65536 ? 2 : 1);
-    const auto kernel = stream_kernel<T, KO, kf, mt>;
+  const auto go = [&](auto KF) -> int {
+    constexpr int kf = decltype(KF)::value;
+    const size_t lds = div_up(a.n, 64) * (static_cast<size_t>(kf) * 4 * 1024 + 64 * sizeof(float));
+    // Parts for all blocks that the CUs hold at once (two each, or one where the
+    // weights take more than half the LDS), in one round: 200k rows 96 -> 384 in
+    // parts of 512 rows 44.7 us, of 256 51.5, of 128 57.8; 40k rows 128 19.4, 512 28.5.
+    const int64_t held = lds > 80 * 1024 ? 256 : 512, wave_rows = kStreamWaves * 16;
+    const int rows = static_cast<int>(round_up(std::max<int64_t>(div_up(a.g.rows, held), 1), wave_rows));
+    const auto kernel = stream_kernel<T, KO, kf>;
     SPIRA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, kMostStreamFragments * 1024));
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     hipLaunchKernelGGL(kernel, dim3(most_parts(a.g.rows, a.g.count, rows) + 1), dim3(kStreamThreads), lds, stream,
                        StreamArgs{a, rows});
     SPIRA_HIP_LAUNCH_CHECK();
     return kOk;
   };
   using std::integral_constant;
-  const int64_t f = div_up(a.k * static_cast<int64_t>(sizeof(T)), 64);
-  constexpr integral_constant<int, 1> one;
-  // tiles of 32 rows halve the reads of the weights from LDS; of 16 rows they
-  // give twice the waves work where there are few
-  const auto either = [&](auto KF) {
-    return a.g.rows >= 65536 ? go(KF, integral_constant<int, 2>{}) : go(KF, one);
-  };
-  switch (f) {
-    case 1: return either(integral_constant<int, 1>{});
-    case 2: return either(integral_constant<int, 2>{});
-    case 3: return either(integral_constant<int, 3>{});
-    case 4: return either(integral_constant<int, 4>{});
-    case 5: case 6: return either(integral_constant<int, 6>{});
-    case 7: case 8: return go(integral_constant<int, 8>{}, one);
-    case 9: case 10: case 11: case 12: return go(integral_constant<int, 12>{}, one);
-    default: return go(integral_constant<int, 16>{}, one);
+  switch (div_up(a.k * static_cast<int64_t>(sizeof(T)), 64)) {
+    case 1: return go(integral_constant<int, 1>{});
+    case 2: return go(integral_constant<int, 2>{});
+    case 3: return go(integral_constant<int, 3>{});
+    case 4: return go(integral_constant<int, 4>{});
+    case 5: case 6: return go(integral_constant<int, 6>{});
+    case 7: case 8: return go(integral_constant<int, 8>{});
+    case 9: case 10: case 11: case 12: return go(integral_constant<int, 12>{});
+    default: return go(integral_constant<int, 16>{});
   }
 }
 
@@ -1270,7 +1250,11 @@ static int weight_parts(int64_t rows, int64_t groups, int64_t ci, int64_t co) {
   return static_cast<int>(launch_limit(rows, groups, size));
 }
 
-constexpr int kSumRows = 256;  // rows per part of the column sums
+// Rows per part of the column sums: blocks for every CU, at most 256 rows each.
+template <class T> static int64_t sum_rows(int64_t rows, int64_t groups, int64_t co) {
+  const int64_t size = round_up(div_up(rows * div_up(co, 16 * kVec<T>), 1024), 16);
+  return launch_limit(rows, groups, std::min<int64_t>(std::max<int64_t>(size, 32), 256));
+}
 
 }  // namespace grouped
 
@@ -1348,10 +1332,13 @@ int spira_hip_grouped_linear_weights_gradient(int64_t rows, int groups, const in
   });
 }
 
-int spira_hip_grouped_linear_activation_gradient_workspace(int64_t rows, int groups, int c_out, size_t *bytes) {
-  const int64_t part = grouped::launch_limit(rows, groups, grouped::kSumRows);
-  *bytes = grouped::most_parts(rows, groups, part) * static_cast<size_t>(c_out) * sizeof(float);
-  return kOk;
+int spira_hip_grouped_linear_activation_gradient_workspace(int64_t rows, int groups, int c_out, int dtype,
+                                                           size_t *bytes) {
+  return with_type(dtype, [&](auto t) -> int {
+    const int64_t part = grouped::sum_rows<decltype(t)>(rows, groups, c_out);
+    *bytes = grouped::most_parts(rows, groups, part) * static_cast<size_t>(c_out) * sizeof(float);
+    return kOk;
+  });
 }
 
 int spira_hip_grouped_linear_activation_gradient(int64_t rows, int groups, const int32_t *offsets, const void *dy,
@@ -1360,12 +1347,12 @@ int spira_hip_grouped_linear_activation_gradient(int64_t rows, int groups, const
   if (int rc = grouped::check(rows, groups, offsets, 1, c_out)) return rc;
   SPIRA_HIP_REQUIRE((rows == 0 || dy) && (y == nullptr || dz || rows == 0) && (y || dbias),
                     "grouped_linear_activation_gradient: null tensor");
-  const int64_t part = grouped::launch_limit(rows, groups, grouped::kSumRows);
-  const int64_t parts = grouped::most_parts(rows, groups, part);
-  SPIRA_HIP_REQUIRE(!dbias || workspace_bytes >= static_cast<size_t>(parts) * c_out * sizeof(float),
-                    "grouped_linear_activation_gradient: workspace too small");
   return with_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
+    const int64_t part = grouped::sum_rows<T>(rows, groups, c_out);
+    const int64_t parts = grouped::most_parts(rows, groups, part);
+    SPIRA_HIP_REQUIRE(!dbias || workspace_bytes >= static_cast<size_t>(parts) * c_out * sizeof(float),
+                      "grouped_linear_activation_gradient: workspace too small");
     const grouped::Groups g{offsets, groups, rows};
     auto *partial = dbias ? static_cast<float *>(workspace) : nullptr;
     if (rows > 0) {

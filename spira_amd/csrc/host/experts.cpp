@@ -103,7 +103,8 @@ static std::tuple<OptTensor, OptTensor, OptTensor> grouped_linear_backward(
     if (y) dz = like(x, {l.rows, l.co});
     if (need_db) db = like(x, {l.groups, l.co});
     size_t bytes = 0;
-    check_rc(spira_hip_grouped_linear_activation_gradient_workspace(l.rows, l.groups, l.co, &bytes), "grouped_linear");
+    check_rc(spira_hip_grouped_linear_activation_gradient_workspace(l.rows, l.groups, l.co, dtype, &bytes),
+             "grouped_linear");
     Tensor ws = workspace(bytes, x.device());
     check_rc(spira_hip_grouped_linear_activation_gradient(l.rows, l.groups, off, dy.data_ptr(), ptr(y), l.co, dtype,
                                                           dz.data_ptr(), db ? db->data_ptr() : nullptr, ws.data_ptr(),
