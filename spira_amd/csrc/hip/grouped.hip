@@ -458,21 +458,25 @@ __global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(
   const int quads = static_cast<int>((a.n + 63) / 64);  // of fragments
   const int fragments = quads * 4 * KF;
   // the first tile's rows are on their way while the weights are laid out
+  // (and the sources of the rows after them)
   uintx4_t next[KF];
+  int32_t source = -1;
+  auto look = [&](int64_t r0) {
+    if (a.source) source = r0 + l16 < part.end ? a.source[r0 + l16] : -1;
+  };
   auto fetch = [&](int64_t r0) {
     const int64_t r = r0 + l16;
     int64_t s = r < part.end ? r : -1;
-    if (s >= 0 && a.source) {
-      s = a.source[r];
-      if (s >= a.num_sources) s = -1;
-    }
+    if (a.source) s = source < a.num_sources ? source : -1;
     const T *row = s >= 0 ? static_cast<const T *>(a.x) + s * a.k : nullptr;
+    look(r0 + kStreamWaves * 16);
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
       const int64_t k = f * FK + lq * kVec<T>;
       next[f] = load_raw(row + k, row ? a.k - k : 0);
     }
   };
+  look(part.begin + wave * 16);
   fetch(part.begin + wave * 16);
   // the bias too lies in LDS: a load from memory in the loop below would wait for
   // the rows under way before it
