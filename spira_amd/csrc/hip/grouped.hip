@@ -232,7 +232,9 @@ template <int N> struct Staged {
   uintx4_t v[N];
 };
 
-// 128 x 128 outputs by four waves, 64 x 64 each
+// Tiles through registers, for what DMA cannot feed: rows or views off 16-byte
+// boundaries, odd widths, and tensors of 2 GiB and more under one descriptor.
+// 128 x 128 outputs by four waves, 64 x 64 each.
 constexpr int kRows = 128, kCols = 128, kThreads = 256;
 
 template <class T> struct Product {
@@ -420,7 +422,8 @@ template <class T, bool KO> __global__ __launch_bounds__(kThreads) void rows_ker
 
 // ---------------------------------------------------------------------------
 // Rows streamed past weights that stay in LDS.  Where a group's weights fit
-// there, the operator is bound by its rows' bytes: a block lays the weights out
+// there, the operator is bound by its rows' bytes (200k rows 96 -> 384, gathered:
+// 46 us where its bytes take 33; tiles of both operands 123): a block lays the weights out
 // once, one 1 KB block per MFMA fragment in lane order, and its eight waves then
 // walk the rows of its part on their own, without barriers, each holding a
 // tile's rows in registers and fetching the next tile's meanwhile.
@@ -1157,6 +1160,8 @@ static int launch_weights_tile(const WeightsArgs &a, int64_t parts, hipStream_t 
   SPIRA_HIP_LAUNCH_CHECK();
   return kOk;
 }
+// The large tile where there are blocks for every CU: 32k rows 1024 -> 2048 in 16
+// groups 172 us, with the small one 185.
 template <class T> static int launch_weights(const WeightsArgs &a, int64_t parts, hipStream_t stream) {
   if constexpr (sizeof(T) == 2)
     if (a.ci > 128 && a.co > 128 && parts * div_up(a.ci, 256) * div_up(a.co, 256) >= 256)
@@ -1232,20 +1237,22 @@ __global__ __launch_bounds__(256) void activation_kernel(const Groups g, int par
 
 static int check(int64_t rows, int groups, const int32_t *offsets, int64_t ci, int64_t co) {
   SPIRA_HIP_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) - 256, "grouped_linear: bad number of rows");
-  SPIRA_HIP_REQUIRE(groups > 0 && groups <= 65535, "grouped_linear: needs 1 to 65535 groups");
+  SPIRA_HIP_REQUIRE(groups > 0 && groups <= 32767, "grouped_linear: needs 1 to 32767 groups");
   SPIRA_HIP_REQUIRE(ci > 0 && co > 0 && ci <= (1 << 20) && co <= (1 << 20), "grouped_linear: bad widths");
   SPIRA_HIP_REQUIRE(offsets, "grouped_linear: no offsets");
   return kOk;
 }
 
-// (grids have 65535 blocks in y and z: larger parts for more rows than that)
+// (grids have 65535 blocks in y and z: larger parts for more rows than that; the
+// groups alone are at most half as many)
 static int64_t launch_limit(int64_t rows, int64_t groups, int64_t size) {
   while (most_parts(rows, groups, size) > 65535 - 1) size *= 2;
   return size;
 }
 
 // Rows per part of the weights' gradient; 0: whole groups, no parts.  Parts are
-// cut where the weights' tiles alone would leave the chip idle.
+// cut where the weights' tiles alone would leave the chip idle, at least 128 rows
+// each: 20k fp32 rows 63 -> 130 in parts of 128 31 us, of 256 42.
 static int weight_parts(int64_t rows, int64_t groups, int64_t ci, int64_t co) {
   const int64_t tiles = div_up(ci, kRows) * div_up(co, kCols) * groups;
   const int64_t want = 4 * 256;

@@ -67,7 +67,7 @@ static Linear check_linear(const Tensor &x, const Tensor &w, const Tensor &offse
   Linear l{sources ? sources->size(0) : x.size(0), w.size(0), w.size(1), w.size(2)};
   SPIRA_CHECK_ARG(l.groups > 0 && l.ci > 0 && l.co > 0, "weight must not be empty");
   SPIRA_CHECK_ARG(l.ci <= (1 << 20) && l.co <= (1 << 20), "weight is too wide");
-  SPIRA_CHECK_ARG(l.groups <= 65535, "grouped_linear: needs 1 to 65535 groups");
+  SPIRA_CHECK_ARG(l.groups <= 32767, "grouped_linear: needs 1 to 32767 groups");
   return l;
 }
 

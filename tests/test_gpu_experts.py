@@ -162,6 +162,36 @@ def test_grouped_linear_long_group_and_odd_views(dev):
     assert torch.count_nonzero(y[19_003:]) == 0 and torch.count_nonzero(dx[19_003:]) == 0
 
 
+@pytest.mark.parametrize("dtype,groups,rows,ci,co", [
+    ("bf16", 12, 17_000, 1032, 1032),  # large tiles both ways
+    ("f16", 100, 9_000, 256, 328),     # more groups than lanes
+    ("f32", 5, 3_000, 320, 260), ("f16", 3, 40_000, 384, 512), ("bf16", 2, 300, 2048, 136)])
+def test_grouped_linear_wide(dev, dtype, groups, rows, ci, co):
+    """Weights too large for LDS: gathered rows, groups of any size, tokens without an expert."""
+    dt = DTYPES[dtype]
+    logits = randn((rows, groups), torch.float32, 1) + torch.linspace(2, 0, groups)
+    logits[::7] = -math.inf
+    routes = F.route_experts(logits.to(dev), 1)
+    x, w = randn((rows, ci), dt, 2).to(dev), randn((groups, ci, co), dt, 3, ci ** -0.5).to(dev)
+    b, dy = randn((groups, co), dt, 4, 0.1).to(dev), randn((rows, co), dt, 5).to(dev)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = F.grouped_linear(x, w, routes, bias=b, relu=True)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    offsets, at = routes.offsets.tolist(), routes.rows.long()
+    used = torch.zeros(rows, dtype=torch.bool, device=dev)
+    for e in range(groups):
+        lo, hi = offsets[e], offsets[e + 1]
+        source = at[lo:hi]
+        used[source] = True
+        xe, we, be = x[source].detach().double(), w[e].detach().double(), b[e].detach().double()
+        ze = dy[lo:hi].double() * (y[lo:hi] > 0)
+        close(y[lo:hi], (xe @ we + be).clamp(min=0), xe.abs() @ we.abs() + be.abs(), ci, f"y {e}")
+        close(dx[source], ze @ we.T, ze.abs() @ we.T.abs(), co, f"dx {e}")
+        close(dw[e], xe.T @ ze, xe.T.abs() @ ze.abs(), hi - lo, f"dw {e}")
+        close(db[e], ze.sum(0), ze.abs().sum(0), hi - lo, f"db {e}")
+    assert torch.count_nonzero(dx[~used]) == 0 and torch.count_nonzero(y[offsets[-1]:]) == 0
+
+
 def test_grouped_linear_nonfinite_rows_stay_in_their_rows(dev):
     """Infinities and NaN of one row, or outside the groups, reach no other row."""
     x = randn((200, 72), torch.float16, 1)
