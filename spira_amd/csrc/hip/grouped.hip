@@ -929,6 +929,113 @@ __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) void tile_kernel(const
   }
 }
 
+// Few rows to a group (a serving step's): the weights' bytes are all there is, and
+// what counts is how many of them are under way.  A block takes 16 rows and 64
+// columns, each of its four waves every fourth step with a ring of its own, without
+// barriers; their sums are added in order at the end.
+constexpr int kFewDepth = 4, kFewWaves = 4;
+template <class T, bool KO> __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const RowsArgs a) {
+  using S = Tile<T, 16, 64, 16, 64>;
+  constexpr int STAGE = S::XBYTES + S::WBYTES, L = S::XL + S::WL;
+  static_assert(S::NW == 1 && (kFewDepth - 1) * L < 64, "a wave's own loads, counted");
+  __shared__ __align__(1024) char rings[kFewWaves][kFewDepth * STAGE];
+  static_assert(sizeof(rings) >= kFewWaves * 4096, "the sums of the waves");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char *ring = rings[wave];
+  const Place place = find_place(a.g, 16, blockIdx.x, static_cast<uint32_t>((a.n + 63) / 64), gridDim.x);
+  const Part part = place.part;
+  if (part.group < 0) {
+    clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, part.begin, place.idle, 64 * kFewWaves);
+    return;
+  }
+  const int64_t n0 = place.col * static_cast<int64_t>(64);
+  const uint32_t kbytes = static_cast<uint32_t>(a.k * static_cast<int64_t>(sizeof(T)));
+  const uint32_t nbytes = static_cast<uint32_t>(a.n * static_cast<int64_t>(sizeof(T)));
+  const uintx4_t xr =
+      a.source ? buffer(a.x, a.num_sources * kbytes)
+               : buffer(static_cast<const char *>(a.x) + part.begin * kbytes, (part.end - part.begin) * kbytes);
+  const uintx4_t wr =
+      buffer(static_cast<const char *>(a.w) + part.group * a.k * nbytes, a.k * static_cast<int64_t>(nbytes));
+  uint32_t xo[S::XL], xc[S::XL], wo[S::WL], wc[S::WL];
+#pragma unroll
+  for (int i = 0; i < S::XL; ++i) {
+    int r, c;
+    kc_source(i, lane, r, c);
+    xc[i] = c * 16;
+    xo[i] = kOutOfRange;
+    if (part.begin + r < part.end) {
+      const int64_t s = a.source ? a.source[part.begin + r] : r;
+      if (s >= 0 && (!a.source || s < a.num_sources)) xo[i] = static_cast<uint32_t>(s) * kbytes + xc[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < S::WL; ++i) {
+    int r, c;
+    if constexpr (KO) {
+      ko_source<T, 64>(i, lane, r, c);
+      wc[i] = 0;
+      wo[i] = r * nbytes + static_cast<uint32_t>(n0 * sizeof(T)) + c * 16;
+    } else {
+      kc_source(i, lane, r, c);
+      wc[i] = c * 16;
+      wo[i] = n0 + r < a.n ? static_cast<uint32_t>(n0 + r) * kbytes + wc[i] : kOutOfRange;
+    }
+  }
+  BiasOf<T, 4> bias;
+  bias.load(a.bias ? static_cast<const T *>(a.bias) + part.group * a.n : nullptr, n0, a.n, lane);
+  const int steps = static_cast<int>((kbytes + kRing - 1) / kRing);
+  auto issue = [&](int turn) {
+    const int step = turn * kFewWaves + wave;
+    char *xs = ring + turn % kFewDepth * STAGE, *ws = xs + S::XBYTES;
+    const uint32_t kb = step * kRing;
+#pragma unroll
+    for (int i = 0; i < S::XL; ++i) load_lds(xr, kb + xc[i] < kbytes ? xo[i] + kb : kOutOfRange, xs + i * 1024);
+    const uint32_t wb = KO ? step * static_cast<uint32_t>(kRingK<T>) * nbytes : kb;
+#pragma unroll
+    for (int i = 0; i < S::WL; ++i)
+      load_lds(wr, kb + wc[i] < kbytes ? wo[i] + wb : kOutOfRange, ws + i * 1024);
+  };
+  for (int turn = 0; turn < kFewDepth; ++turn) issue(turn);
+  floatx4_t acc[4] = {};
+  for (int turn = 0; turn * kFewWaves + wave < steps; ++turn) {
+    __builtin_amdgcn_s_waitcnt((((kFewDepth - 1) * L) & 15) | (7 << 4) | (15 << 8) | ((((kFewDepth - 1) * L) >> 4) << 14));
+    asm volatile("" ::: "memory");
+    const char *xs = ring + turn % kFewDepth * STAGE, *ws = xs + S::XBYTES;
+    uintx4_t n[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (KO) n[j] = ko_frag<T, 64>(ws, j * 16, 0);
+      else n[j] = ring_frag(ws, j * 16);
+    }
+    const uintx4_t m = ring_frag(xs, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mma<T>(acc[j], n[j], m);
+    // (the stage is read before it is loaded again)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    issue(turn + kFewDepth);
+  }
+  wait_loads();  // (none may land in what follows)
+  asm volatile("" ::: "memory");
+  __syncthreads();
+  auto *sums = reinterpret_cast<floatx4_t *>(&rings[0][0]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sums[(wave * 4 + j) * 64 + lane] = acc[j];
+  __syncthreads();
+  if (wave != 0) return;
+  floatx4_t v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] = bias.at(j);
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) v[j] += sums[(w * 4 + j) * 64 + lane];
+    if (a.relu)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[j][q] = v[j][q] < 0.f ? 0.f : v[j][q];
+  }
+  const int64_t r = part.begin + (lane & 15);
+  store_row<T>(static_cast<T *>(a.y) + r * a.n, n0, a.n, r < part.end, v);
+}
+
 static bool aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Whether DMA can feed the tiles.
@@ -946,7 +1053,21 @@ template <class T, bool KO, int M, int N, int WM, int WN> static int launch_tile
   return kOk;
 }
 
+template <class T, bool KO> static int launch_few(const RowsArgs &a, hipStream_t stream) {
+  const int64_t blocks = most_parts(a.g.rows, a.g.count, 16) * div_up(a.n, 64) + 1;
+  SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear: too many tiles");
+  hipLaunchKernelGGL((few_kernel<T, KO>), dim3(blocks), dim3(64 * kFewWaves), 0, stream, a);
+  SPIRA_HIP_LAUNCH_CHECK();
+  return kOk;
+}
+
 template <class T, bool KO> static int launch_rows(const RowsArgs &a, hipStream_t stream) {
+  // Few rows to a group (us, against the large forms below): bf16 16 rows 2048 ->
+  // 512 in 32 groups 10.2 and 22.5, fp32 19 and 138; 16 a group 96 -> 384 5.7 and
+  // 10.1, 62 a group 64 -> 64 5.2 and 6.8; but bf16 32 a group 1024 -> 2048 27.6 and
+  // 17.2 (fp32 57 and 78), where every 16 rows read wide weights again.
+  const int64_t few = streams<T>(a.k, a.n) ? 64 : sizeof(T) == 4 ? 32 : 16;
+  if (a.g.rows <= few * a.g.count && dma_fits<T>(a)) return launch_few<T, KO>(a, stream);
   if (streams<T>(a.k, a.n)) return launch_stream<T, KO>(a, stream);
   if (dma_fits<T>(a)) {
     // The large tile reads each operand half as often from L2 and LDS: 32k rows
