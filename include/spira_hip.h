@@ -559,6 +559,15 @@ int spira_hip_grouped_linear(int64_t rows, int groups, const int32_t *offsets, c
 int spira_hip_grouped_linear_rows_gradient(int64_t rows, int groups, const int32_t *offsets, const void *dz, int c_out,
                                            const void *weights, int c_in, int dtype, void *dx, hipStream_t stream);
 
+/* dx[t] = sum over the slots in [0, rows) of token t, in their order, of
+ * dz[slot] @ transpose(weights[e]), e the slot's group: slots [tokens, k].  The
+ * rows' shares stay fp32 until they are added (in the workspace). */
+int spira_hip_grouped_linear_tokens_gradient_workspace(int64_t rows, int k, int c_in, size_t *bytes);
+int spira_hip_grouped_linear_tokens_gradient(int64_t rows, int groups, const int32_t *offsets, const int32_t *slots,
+                                             int64_t tokens, int k, const void *dz, int c_out, const void *weights,
+                                             int c_in, int dtype, void *dx, void *workspace, size_t workspace_bytes,
+                                             hipStream_t stream);
+
 /* dw[e] = sum over the group's rows of transpose(x[s]) dz[r]. */
 int spira_hip_grouped_linear_weights_gradient_workspace(int64_t rows, int groups, int c_in, int c_out, size_t *bytes);
 int spira_hip_grouped_linear_weights_gradient(int64_t rows, int groups, const int32_t *offsets, const int32_t *sources,

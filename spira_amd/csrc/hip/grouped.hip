@@ -336,8 +336,9 @@ struct RowsArgs {
   void *y;
 };
 
-// Forward (KO weights [k, n]) and rows' gradient (KC weights [n, k]).
-template <class T, bool KO> __global__ __launch_bounds__(kThreads) void rows_kernel(const RowsArgs a) {
+// Forward (KO weights [k, n]) and rows' gradient (KC weights [n, k]).  O: type of
+// the outputs, the operands' own or, for shares that are yet to be added, fp32.
+template <class T, bool KO, class O> __global__ __launch_bounds__(kThreads) void rows_kernel(const RowsArgs a) {
   using P = Product<T>;
   __shared__ __align__(1024) char lds[4 * P::TILE];  // two stages of both tiles
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -345,7 +346,7 @@ template <class T, bool KO> __global__ __launch_bounds__(kThreads) void rows_ker
   if (part.group < 0) {
     if (blockIdx.y == 0) {
       const int64_t used = blockIdx.x - part.begin;
-      clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, part.begin, gridDim.x - used, kThreads);
+      clear_ungrouped(a.g, static_cast<O *>(a.y), a.n, part.begin, gridDim.x - used, kThreads);
     }
     return;
   }
@@ -415,7 +416,7 @@ template <class T, bool KO> __global__ __launch_bounds__(kThreads) void rows_ker
       if (a.relu)
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
-      store4(static_cast<T *>(a.y) + r * a.n + n, a.n - n, v);
+      store4(static_cast<O *>(a.y) + r * a.n + n, a.n - n, v);
     }
   }
 }
@@ -445,7 +446,7 @@ struct StreamArgs {
 
 // KF: fragments (64 bytes) of a row.  A wave takes 16 rows at a time (32 halve the
 // reads of the weights from LDS and measure the same).
-template <class T, bool KO, int KF>
+template <class T, bool KO, int KF, class O>
 __global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(KF <= 8 ? 4 : 2))) void stream_kernel(const StreamArgs sa) {
   constexpr int FK = 64 / static_cast<int>(sizeof(T));  // values of the summed index per fragment
   constexpr int MOST = kMostStreamFragments / kStreamWaves;
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, lq = lane >> 4;
   const Part part = find_part(a.g, sa.part_rows, blockIdx.x);
   if (part.group < 0) {
-    clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, part.begin, gridDim.x - (blockIdx.x - part.begin), kStreamThreads);
+    clear_ungrouped(a.g, static_cast<O *>(a.y), a.n, part.begin, gridDim.x - (blockIdx.x - part.begin), kStreamThreads);
     return;
   }
   const T *w = static_cast<const T *>(a.w) + part.group * a.k * a.n;
@@ -554,14 +555,14 @@ __global__ __launch_bounds__(kStreamThreads) __attribute__((amdgpu_waves_per_eu(
       const int64_t n = q * 64 + lq * 16;
       if (n >= a.n || r >= part.end) continue;
 #pragma unroll
-      for (int h = 0; h < 16 / kVec<T>; ++h) {
-        Chunk<T> c;
+      for (int h = 0; h < 16 / kVec<O>; ++h) {
+        Chunk<O> c;
 #pragma unroll
-        for (int v = 0; v < kVec<T>; ++v) {
-          const float s = acc[(h * kVec<T> + v) / 4][v % 4] + bias[n + h * kVec<T> + v];
+        for (int v = 0; v < kVec<O>; ++v) {
+          const float s = acc[(h * kVec<O> + v) / 4][v % 4] + bias[n + h * kVec<O> + v];
           c.v[v] = a.relu && s < 0.f ? 0.f : s;
         }
-        store_chunk(static_cast<T *>(a.y) + r * a.n + n + h * kVec<T>, a.n - n - h * kVec<T>, c);
+        store_chunk(static_cast<O *>(a.y) + r * a.n + n + h * kVec<O>, a.n - n - h * kVec<O>, c);
       }
     }
   }
@@ -574,7 +575,7 @@ template <class T> static bool streams(int64_t k, int64_t n) {
   return f <= 16 && kf * 4 * div_up(n, 64) <= kMostStreamFragments;
 }
 
-template <class T, bool KO> static int launch_stream(const RowsArgs &a, hipStream_t stream) {
+template <class T, bool KO, class O> static int launch_stream(const RowsArgs &a, hipStream_t stream) {
   const auto go = [&](auto KF) -> int {
     constexpr int kf = decltype(KF)::value;
     const size_t lds = div_up(a.n, 64) * (static_cast<size_t>(kf) * 4 * 1024 + 64 * sizeof(float));
@@ -583,7 +584,7 @@ template <class T, bool KO> static int launch_stream(const RowsArgs &a, hipStrea
     // parts of 512 rows 44.7 us, of 256 51.5, of 128 57.8; 40k rows 128 19.4, 512 28.5.
     const int64_t held = lds > 80 * 1024 ? 256 : 512, wave_rows = kStreamWaves * 16;
     const int rows = static_cast<int>(round_up(std::max<int64_t>(div_up(a.g.rows, held), 1), wave_rows));
-    const auto kernel = stream_kernel<T, KO, kf>;
+    const auto kernel = stream_kernel<T, KO, kf, O>;
     SPIRA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
     hipLaunchKernelGGL(kernel, dim3(most_parts(a.g.rows, a.g.count, rows) + 1), dim3(kStreamThreads), lds, stream,
@@ -832,7 +833,7 @@ template <class T, int NI> struct BiasOf {
   }
 };
 
-template <class T, bool KO, int M, int N, int WM, int WN>
+template <class T, bool KO, class O, int M, int N, int WM, int WN>
 __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) void tile_kernel(const RowsArgs a) {
   using S = Tile<T, M, N, WM, WN>;
   __shared__ __align__(1024) char x0[S::XBYTES], x1[S::XBYTES], x2[S::XBYTES], x3[S::XBYTES];
@@ -841,7 +842,7 @@ __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) void tile_kernel(const
   const Place place = find_place(a.g, M, blockIdx.x, static_cast<uint32_t>((a.n + N - 1) / N), gridDim.x);
   const Part part = place.part;
   if (part.group < 0) {
-    clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, part.begin, place.idle, S::NT);
+    clear_ungrouped(a.g, static_cast<O *>(a.y), a.n, part.begin, place.idle, S::NT);
     return;
   }
   const int64_t n0 = place.col * static_cast<int64_t>(N);
@@ -925,7 +926,7 @@ __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) void tile_kernel(const
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[j][q] = v[j][q] < 0.f ? 0.f : v[j][q];
     }
-    store_row<T>(static_cast<T *>(a.y) + r * a.n, n0 + c0, a.n, r < part.end, v);
+    store_row<O>(static_cast<O *>(a.y) + r * a.n, n0 + c0, a.n, r < part.end, v);
   }
 }
 
@@ -934,7 +935,7 @@ __global__ __launch_bounds__((Tile<T, M, N, WM, WN>::NT)) void tile_kernel(const
 // columns, each of its four waves every fourth step with a ring of its own, without
 // barriers; their sums are added in order at the end.
 constexpr int kFewDepth = 4, kFewWaves = 4;
-template <class T, bool KO> __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const RowsArgs a) {
+template <class T, bool KO, class O> __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const RowsArgs a) {
   using S = Tile<T, 16, 64, 16, 64>;
   constexpr int STAGE = S::XBYTES + S::WBYTES, L = S::XL + S::WL;
   static_assert(S::NW == 1 && (kFewDepth - 1) * L < 64, "a wave's own loads, counted");
@@ -945,7 +946,7 @@ template <class T, bool KO> __global__ __launch_bounds__(64 * kFewWaves) void fe
   const Place place = find_place(a.g, 16, blockIdx.x, static_cast<uint32_t>((a.n + 63) / 64), gridDim.x);
   const Part part = place.part;
   if (part.group < 0) {
-    clear_ungrouped(a.g, static_cast<T *>(a.y), a.n, part.begin, place.idle, 64 * kFewWaves);
+    clear_ungrouped(a.g, static_cast<O *>(a.y), a.n, part.begin, place.idle, 64 * kFewWaves);
     return;
   }
   const int64_t n0 = place.col * static_cast<int64_t>(64);
@@ -1033,7 +1034,7 @@ template <class T, bool KO> __global__ __launch_bounds__(64 * kFewWaves) void fe
       for (int q = 0; q < 4; ++q) v[j][q] = v[j][q] < 0.f ? 0.f : v[j][q];
   }
   const int64_t r = part.begin + (lane & 15);
-  store_row<T>(static_cast<T *>(a.y) + r * a.n, n0, a.n, r < part.end, v);
+  store_row<O>(static_cast<O *>(a.y) + r * a.n, n0, a.n, r < part.end, v);
 }
 
 static bool aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -1045,40 +1046,40 @@ template <class T> static bool dma_fits(const RowsArgs &a) {
          a.k * size <= (1 << 22) && (!a.source || a.num_sources * a.k * size < kBufferLimit);
 }
 
-template <class T, bool KO, int M, int N, int WM, int WN> static int launch_tile(const RowsArgs &a, hipStream_t stream) {
+template <class T, bool KO, class O, int M, int N, int WM, int WN> static int launch_tile(const RowsArgs &a, hipStream_t stream) {
   const int64_t blocks = (most_parts(a.g.rows, a.g.count, M)) * div_up(a.n, N) + 1;
   SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear: too many tiles");
-  hipLaunchKernelGGL((tile_kernel<T, KO, M, N, WM, WN>), dim3(blocks), dim3(Tile<T, M, N, WM, WN>::NT), 0, stream, a);
+  hipLaunchKernelGGL((tile_kernel<T, KO, O, M, N, WM, WN>), dim3(blocks), dim3(Tile<T, M, N, WM, WN>::NT), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();
   return kOk;
 }
 
-template <class T, bool KO> static int launch_few(const RowsArgs &a, hipStream_t stream) {
+template <class T, bool KO, class O> static int launch_few(const RowsArgs &a, hipStream_t stream) {
   const int64_t blocks = most_parts(a.g.rows, a.g.count, 16) * div_up(a.n, 64) + 1;
   SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear: too many tiles");
-  hipLaunchKernelGGL((few_kernel<T, KO>), dim3(blocks), dim3(64 * kFewWaves), 0, stream, a);
+  hipLaunchKernelGGL((few_kernel<T, KO, O>), dim3(blocks), dim3(64 * kFewWaves), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();
   return kOk;
 }
 
-template <class T, bool KO> static int launch_rows(const RowsArgs &a, hipStream_t stream) {
+template <class T, bool KO, class O = T> static int launch_rows(const RowsArgs &a, hipStream_t stream) {
   // Few rows to a group (us, against the large forms below): bf16 16 rows 2048 ->
   // 512 in 32 groups 10.2 and 22.5, fp32 19 and 138; 16 a group 96 -> 384 5.7 and
   // 10.1, 62 a group 64 -> 64 5.2 and 6.8; but bf16 32 a group 1024 -> 2048 27.6 and
   // 17.2 (fp32 57 and 78), where every 16 rows read wide weights again.
   const int64_t few = streams<T>(a.k, a.n) ? 64 : sizeof(T) == 4 ? 32 : 16;
-  if (a.g.rows <= few * a.g.count && dma_fits<T>(a)) return launch_few<T, KO>(a, stream);
-  if (streams<T>(a.k, a.n)) return launch_stream<T, KO>(a, stream);
+  if (a.g.rows <= few * a.g.count && dma_fits<T>(a)) return launch_few<T, KO, O>(a, stream);
+  if (streams<T>(a.k, a.n)) return launch_stream<T, KO, O>(a, stream);
   if (dma_fits<T>(a)) {
     // The large tile reads each operand half as often from L2 and LDS: 32k rows
     // 1024 -> 2048 in 16 even groups 141 us, with the small one 197.  It needs
     // groups that fill its rows, and blocks for every CU.
     if constexpr (sizeof(T) == 2)
       if (a.g.rows / a.g.count >= 256 && a.n > 128 && div_up(a.g.rows, 256) * div_up(a.n, 256) >= 256)
-        return launch_tile<T, KO, 256, 256, 128, 64>(a, stream);
-    return launch_tile<T, KO, 128, 128, 64, 64>(a, stream);
+        return launch_tile<T, KO, O, 256, 256, 128, 64>(a, stream);
+    return launch_tile<T, KO, O, 128, 128, 64, 64>(a, stream);
   }
-  hipLaunchKernelGGL((rows_kernel<T, KO>), dim3(most_parts(a.g.rows, a.g.count, kRows) + 1, div_up(a.n, kCols)),
+  hipLaunchKernelGGL((rows_kernel<T, KO, O>), dim3(most_parts(a.g.rows, a.g.count, kRows) + 1, div_up(a.n, kCols)),
                      dim3(kThreads), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();
   return kOk;
@@ -1420,6 +1421,41 @@ int spira_hip_grouped_linear_rows_gradient(int64_t rows, int groups, const int32
     if (rows == 0) return kOk;
     grouped::RowsArgs a{{offsets, groups, rows}, nullptr, rows, dz, weights, nullptr, c_out, c_in, 0, dx};
     return grouped::launch_rows<T, false>(a, stream);
+  });
+}
+
+int spira_hip_grouped_linear_tokens_gradient_workspace(int64_t rows, int k, int c_in, size_t *bytes) {
+  SPIRA_HIP_REQUIRE(rows >= 0 && k > 0 && c_in > 0, "grouped_linear_tokens_gradient: bad sizes");
+  *bytes = static_cast<size_t>(rows) * c_in * sizeof(float);
+  return kOk;
+}
+
+int spira_hip_grouped_linear_tokens_gradient(int64_t rows, int groups, const int32_t *offsets, const int32_t *slots,
+                                             int64_t tokens, int k, const void *dz, int c_out, const void *weights,
+                                             int c_in, int dtype, void *dx, void *workspace, size_t workspace_bytes,
+                                             hipStream_t stream) {
+  if (int rc = grouped::check(rows, groups, offsets, c_in, c_out)) return rc;
+  SPIRA_HIP_REQUIRE(tokens >= 0 && k > 0, "grouped_linear_tokens_gradient: bad sizes");
+  SPIRA_HIP_REQUIRE(weights && (rows == 0 || dz) && (tokens == 0 || (slots && dx)),
+                    "grouped_linear_tokens_gradient: null tensor");
+  size_t need = 0;
+  if (int rc = spira_hip_grouped_linear_tokens_gradient_workspace(rows, k, c_in, &need)) return rc;
+  SPIRA_HIP_REQUIRE(workspace_bytes >= need && (workspace || need == 0),
+                    "grouped_linear_tokens_gradient: workspace too small");
+  return with_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    grouped::RowsArgs a{{offsets, groups, rows}, nullptr, rows, dz, weights, nullptr, c_out, c_in, 0, workspace};
+    // (one share a token is the sum: it is rounded at once, and takes half the bytes)
+    if (k == 1) {
+      if (rows > 0)
+        if (int rc = grouped::launch_rows<T, false>(a, stream)) return rc;
+      return spira_hip_combine(workspace, rows, slots, nullptr, tokens, k, c_in, dtype, dx, stream);
+    }
+    // (more stay fp32: 16 bits would round shares that cancel, and lose those past 65504.  It costs their bytes,
+    // 585 -> 638 us for a step of 16k tokens, two choices, 1024 -> 2048)
+    if (rows > 0)
+      if (int rc = grouped::launch_rows<T, false, float>(a, stream)) return rc;
+    return sum_slots(static_cast<const float *>(workspace), rows, slots, tokens, k, c_in, dtype, dx, stream);
   });
 }
 

@@ -77,6 +77,10 @@ template <int G> __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// y[t] = sum_j h[slots[t, j]] over the slots in [0, rows), y in `dtype` (route.hip)
+int sum_slots(const float *h, int64_t rows, const int32_t *slots, int64_t tokens, int k, int c, int dtype, void *y,
+              hipStream_t stream);
+
 // f(T{}) for the storage type that `dtype` names
 template <class F> int with_type(int dtype, F &&f) {
   switch (dtype) {

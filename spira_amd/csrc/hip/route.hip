@@ -380,9 +380,10 @@ __global__ __launch_bounds__(256) void choose_backward_kernel(const T *logits, c
   }
 }
 
-// y[t] = sum_j w[t, j] h[slots[t, j]]: a thread per chunk of a token's row
-template <class T>
-__global__ __launch_bounds__(256) void combine_kernel(const T *h, int64_t rows, const int32_t *slots,
+// y[t] = sum_j w[t, j] h[slots[t, j]]: a thread per chunk of a token's row.  I: type
+// of h, the outputs' or fp32
+template <class T, class I>
+__global__ __launch_bounds__(256) void combine_kernel(const I *h, int64_t rows, const int32_t *slots,
                                                       const float *weights, int64_t tokens, int k, int c, T *y) {
   const int chunks = (c + kVec<T> - 1) / kVec<T>;
   const int64_t i = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x;
@@ -394,9 +395,13 @@ __global__ __launch_bounds__(256) void combine_kernel(const T *h, int64_t rows, 
     const int32_t s = slots[t * k + j];
     if (s < 0 || s >= rows) continue;
     const float w = weights ? weights[t * k + j] : 1.f;
-    const Chunk<T> v = load_chunk(h + static_cast<int64_t>(s) * c + at, c - at);
+    const I *row = h + static_cast<int64_t>(s) * c + at;
 #pragma unroll
-    for (int q = 0; q < kVec<T>; ++q) sum.v[q] += w * v.v[q];
+    for (int p = 0; p < kVec<T>; p += kVec<I>) {
+      const Chunk<I> v = load_chunk(row + p, c - at - p);
+#pragma unroll
+      for (int q = 0; q < kVec<I>; ++q) sum.v[p + q] += w * v.v[q];
+    }
   }
   store_chunk(y + t * c + at, c - at, sum);
 }
@@ -466,6 +471,18 @@ static int tile_tokens(int64_t tokens, int experts, int k) {
   return static_cast<int>(std::max<int64_t>(std::min<int64_t>(even, kTile / k / pass * pass), pass));
 }
 
+template <class T, class I>
+static int launch_combine(const I *h, int64_t rows, const int32_t *slots, const float *weights, int64_t tokens, int k,
+                          int c, T *y, hipStream_t stream) {
+  const int64_t blocks = div_up(tokens * div_up(c, kVec<T>), 256);
+  if (blocks == 0) return kOk;
+  SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "combine: too many values");
+  hipLaunchKernelGGL((combine_kernel<T, I>), dim3(blocks), dim3(256), 0, stream, h, rows, slots, weights, tokens, k, c,
+                     y);
+  SPIRA_HIP_LAUNCH_CHECK();
+  return kOk;
+}
+
 static int check(int64_t tokens, int experts, int k) {
   SPIRA_HIP_REQUIRE(experts > 0 && experts <= kMaxExperts, "route: needs 1 to 512 experts");
   SPIRA_HIP_REQUIRE(k > 0 && k <= kMaxChoices && k <= experts, "route: needs 1 to 16 choices, at most the experts");
@@ -474,6 +491,14 @@ static int check(int64_t tokens, int experts, int k) {
 }
 
 }  // namespace route
+
+int sum_slots(const float *h, int64_t rows, const int32_t *slots, int64_t tokens, int k, int c, int dtype, void *y,
+              hipStream_t stream) {
+  return with_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return route::launch_combine<T, float>(h, rows, slots, nullptr, tokens, k, c, static_cast<T *>(y), stream);
+  });
+}
 
 }  // namespace spira_hip
 
@@ -558,13 +583,8 @@ int spira_hip_combine(const void *h, int64_t num_rows, const int32_t *slots, con
   SPIRA_HIP_REQUIRE(tokens == 0 || (slots && y && (h || num_rows == 0)), "combine: null tensor");
   return with_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const int64_t blocks = div_up(tokens * div_up(c, kVec<T>), 256);
-    if (blocks == 0) return kOk;
-    SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "combine: too many values");
-    hipLaunchKernelGGL(route::combine_kernel<T>, dim3(blocks), dim3(256), 0, stream, static_cast<const T *>(h),
-                       num_rows, slots, weights, tokens, k, c, static_cast<T *>(y));
-    SPIRA_HIP_LAUNCH_CHECK();
-    return kOk;
+    return route::launch_combine<T, T>(static_cast<const T *>(h), num_rows, slots, weights, tokens, k, c,
+                                       static_cast<T *>(y), stream);
   });
 }
 

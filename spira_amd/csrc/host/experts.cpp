@@ -112,23 +112,22 @@ static std::tuple<OptTensor, OptTensor, OptTensor> grouped_linear_backward(
              "grouped_linear");
   }
   if (need_dx) {
-    // (with slots, each row's share is rounded to the features' type before the
-    // few of a token are added in fp32: half the bytes of fp32 shares, and at
-    // most 1.41 times the rounding error of one rounding at the end)
-    Tensor d = like(x, {l.rows, l.ci});
-    check_rc(spira_hip_grouped_linear_rows_gradient(l.rows, l.groups, off, dz.data_ptr(), l.co, w.data_ptr(), l.ci,
-                                                    dtype, d.data_ptr(), current_stream()),
-             "grouped_linear");
-    if (slots) {
-      dx = like(x, x.sizes());
-      if (slots->size(1) > 0)
-        check_rc(spira_hip_combine(d.data_ptr(), l.rows, slots->data_ptr<int32_t>(), nullptr, x.size(0),
-                                   slots->size(1), l.ci, dtype, dx->data_ptr(), current_stream()),
-                 "grouped_linear");
-      else
-        dx->zero_();
+    dx = like(x, x.sizes());
+    if (!slots) {
+      check_rc(spira_hip_grouped_linear_rows_gradient(l.rows, l.groups, off, dz.data_ptr(), l.co, w.data_ptr(), l.ci,
+                                                      dtype, dx->data_ptr(), current_stream()),
+               "grouped_linear");
+    } else if (slots->size(1) > 0) {
+      size_t bytes = 0;
+      check_rc(spira_hip_grouped_linear_tokens_gradient_workspace(l.rows, slots->size(1), l.ci, &bytes),
+               "grouped_linear");
+      Tensor ws = workspace(bytes, x.device());
+      check_rc(spira_hip_grouped_linear_tokens_gradient(l.rows, l.groups, off, slots->data_ptr<int32_t>(), x.size(0),
+                                                        slots->size(1), dz.data_ptr(), l.co, w.data_ptr(), l.ci, dtype,
+                                                        dx->data_ptr(), ws.data_ptr(), bytes, current_stream()),
+               "grouped_linear");
     } else {
-      dx = d;
+      dx->zero_();
     }
   }
   if (need_dw) {

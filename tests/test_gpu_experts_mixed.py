@@ -1,0 +1,67 @@
+"""The row operators where a first set of tests does not reach: shares of a token
+that cancel, loops over many rows, long sums in 16 bits, groups far from even,
+and the ways of autograd around a call.
+
+Tolerances as in test_gpu_experts.py: an output's own rounding, u |ref|, and the
+error of a sum of n terms in fp32, n 2^-24 times the sum of their magnitudes
+(twice that, for the roundings of the terms themselves)."""
+import pytest
+import torch
+
+from spira_amd.nn import functional as F
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+TINY = {torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133, torch.float32: 2.0 ** -149}
+
+
+def close(got, ref, magnitude, terms, what=""):
+    """got within its rounding of ref plus a sum of `terms` terms of total magnitude `magnitude`."""
+    got, dtype = got.detach().double(), got.dtype
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    tol = UNIT[dtype] * ref.abs() * 1.001 + 2 * (terms + 16) * 2.0 ** -24 * magnitude + TINY[dtype]
+    bad = ~((got - ref).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), torch.nonzero(bad)[0].tolist(), got[bad][0].item(), ref[bad][0].item())
+
+
+def randn(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,k,experts,ci,co", [
+    (9, 2, 2, 64, 64),          # few rows to a group
+    (400, 3, 4, 48, 64),        # streamed
+    (500, 2, 2, 512, 256),      # tiles
+    (9000, 2, 2, 1032, 64),     # large tiles
+    (300, 2, 3, 1031, 65)])     # tiles through registers
+def test_gradient_of_shares_that_cancel(dev, tokens, k, experts, ci, co, dtype):
+    """A token's share of each of its experts is some 60000, past the largest fp16
+    number for many, and their sum a few hundred: the shares may not be rounded to
+    the features' type before they are added."""
+    dt = DTYPES[dtype]
+    routes = F.route_experts(randn((tokens, experts), torch.float32, 5).to(dev), k)
+    size = 60000 / co ** 0.5
+    common, own = randn((ci, co), dt, 1, size), randn((experts, ci, co), torch.float32, 2, size / 128)
+    # (every second expert's weights are the others' negative, and a little of its own)
+    sign = torch.tensor([1.0, -1.0] * experts)[:experts, None, None]
+    w = (sign * common.float() + own).to(dt).to(dev)
+    dy = randn((tokens, co), dt, 3).to(dev)
+    x = torch.zeros(tokens, ci, dtype=dt, device=dev, requires_grad=True)
+    slots, chosen = routes.slots.long(), routes.experts.long()
+    given = torch.zeros(tokens * k, co, dtype=dt, device=dev)
+    given[slots.reshape(-1)] = dy.repeat_interleave(k, 0)
+    (dx,) = torch.autograd.grad(F.grouped_linear(x, w, routes), x, given)
+    ref = torch.zeros(tokens, ci, dtype=torch.float64, device=dev)
+    magnitude = torch.zeros_like(ref)
+    for e in range(experts):
+        of = (chosen == e).any(1)
+        d = dy[of].double()
+        ref[of] += d @ w[e].double().T
+        magnitude[of] += d.abs() @ w[e].double().T.abs()
+    fits = ref.abs() < 65000 if dtype == "f16" else torch.ones_like(ref, dtype=torch.bool)
+    assert fits.float().mean() > 0.5
+    close(dx[fits], ref[fits], magnitude[fits], k * co, "dx")
