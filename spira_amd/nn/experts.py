@@ -21,8 +21,13 @@ class ExpertBlock(nn.Module):
     parameters have the features' type (``.half()``, ``.bfloat16()``).
 
     Dropout acts in training mode.  Its mask follows from ``seed`` and the
-    number of training calls so far, which is part of the state_dict.
+    number of training calls so far, which is part of the state_dict.  A call
+    that a backward pass computes again (``torch.utils.checkpoint``) has its
+    first mask; it is known by a draw of each call from torch's CPU generator,
+    whose state checkpointing restores (``preserve_rng_state``, the default).
     """
+
+    _KEPT = 4096  # calls whose numbers are kept for a backward pass
 
     def __init__(self, channels: int, hidden: int, experts: int, choices: int = 2, *, dropout: float = 0.0,
                  scale: float = 1.0, eps: float = 1e-6, seed: int = 0):
@@ -37,6 +42,7 @@ class ExpertBlock(nn.Module):
         self.exit = nn.Parameter(torch.ones(channels))
         self.gate = nn.Parameter(torch.full((channels,), 0.1))
         self.register_buffer("calls", torch.zeros((), dtype=torch.int64, device="cpu"))
+        self._numbers = {}  # of recent training calls, by their draws
 
     def _apply(self, fn, recurse=True):
         # (the count of calls is read on the host: it stays there)
@@ -44,6 +50,21 @@ class ExpertBlock(nn.Module):
         super()._apply(fn, recurse)
         self._buffers["calls"] = calls
         return self
+
+    def _number(self) -> int:
+        """The number of this training call, or of the one that it computes again."""
+        draw = int(torch.randint(2 ** 63 - 1, (), dtype=torch.int64, device="cpu"))
+        if torch._C._current_graph_task_id() >= 0:  # within a backward pass
+            if draw not in self._numbers:
+                raise RuntimeError("[Spira] ExpertBlock: a training call within a backward pass that repeats none "
+                                   "before it (checkpointing has to preserve the state of torch's generator)")
+            return self._numbers[draw]
+        self._numbers.pop(draw, None)
+        self._numbers[draw] = number = int(self.calls)
+        if len(self._numbers) > self._KEPT:
+            del self._numbers[next(iter(self._numbers))]
+        self.calls += 1
+        return number
 
     def forward(self, input: SparseTensor) -> SparseTensor:
         x = input.features
@@ -53,7 +74,6 @@ class ExpertBlock(nn.Module):
         h = F.grouped_linear(h, self.down, routes.offsets, bias=self.down_bias)
         h = F.combine_experts(h, routes)
         if self.training and self.dropout > 0:
-            h = F.dropout(h, self.dropout, self.seed, int(self.calls))
-            self.calls += 1
+            h = F.dropout(h, self.dropout, self.seed, self._number())
         y, _ = F.gated_residual_norm(x, h, weight=self.exit, gate=self.gate, scale=self.scale, eps=self.eps)
         return SparseTensor(coordinates=input.coordinates, features=y, stride=input.stride)
