@@ -2,6 +2,8 @@
 gate, dropout and residual.  No reference counterpart."""
 from __future__ import annotations
 
+from typing import Optional, Tuple
+
 import torch
 from torch import nn
 
@@ -20,17 +22,23 @@ class ExpertBlock(nn.Module):
     ``SparseTensor`` of the same coordinates, behind any ``SparseConv`` block;
     parameters have the features' type (``.half()``, ``.bfloat16()``).
 
-    Dropout acts in training mode.  Its mask follows from ``seed`` and the
-    number of training calls so far, which is part of the state_dict.  A call
-    that a backward pass computes again (``torch.utils.checkpoint``) has its
-    first mask; it is known by a draw of each call from torch's CPU generator,
-    whose state checkpointing restores (``preserve_rng_state``, the default).
+    Dropout acts in training mode.  Without a ``seed`` each call's mask is drawn
+    from torch's CPU generator: another in every call, block and, where their
+    generators differ, process.  With one it follows from the seed and the
+    number of training calls so far, which is part of the state_dict; blocks of
+    one width (copies among them) and ranks then need seeds of their own, or
+    they drop the same positions.
+
+    A call that a backward pass computes again (``torch.utils.checkpoint``) has
+    its first mask, by torch's generator, whose state checkpointing restores
+    (``preserve_rng_state``, the default).  A captured graph replays the mask
+    that it was captured with.
     """
 
     _KEPT = 4096  # calls whose numbers are kept for a backward pass
 
     def __init__(self, channels: int, hidden: int, experts: int, choices: int = 2, *, dropout: float = 0.0,
-                 scale: float = 1.0, eps: float = 1e-6, seed: int = 0):
+                 scale: float = 1.0, eps: float = 1e-6, seed: Optional[int] = None):
         super().__init__()
         self.choices, self.dropout, self.scale, self.eps, self.seed = choices, dropout, scale, eps, seed
         self.entry = nn.Parameter(torch.ones(channels))
@@ -51,20 +59,22 @@ class ExpertBlock(nn.Module):
         self._buffers["calls"] = calls
         return self
 
-    def _number(self) -> int:
-        """The number of this training call, or of the one that it computes again."""
-        draw = int(torch.randint(2 ** 63 - 1, (), dtype=torch.int64, device="cpu"))
-        if torch._C._current_graph_task_id() >= 0:  # within a backward pass
-            if draw not in self._numbers:
-                raise RuntimeError("[Spira] ExpertBlock: a training call within a backward pass that repeats none "
-                                   "before it (checkpointing has to preserve the state of torch's generator)")
-            return self._numbers[draw]
-        self._numbers.pop(draw, None)
-        self._numbers[draw] = number = int(self.calls)
-        if len(self._numbers) > self._KEPT:
-            del self._numbers[next(iter(self._numbers))]
-        self.calls += 1
-        return number
+    def _mask(self) -> Tuple[int, int]:
+        """Seed and offset of this training call's mask."""
+        draw = tuple(torch.randint(2 ** 63 - 1, (2,), dtype=torch.int64, device="cpu").tolist())
+        again = torch._C._current_graph_task_id() >= 0  # within a backward pass: a call computed again
+        if not again:
+            self._numbers.pop(draw, None)
+            self._numbers[draw] = int(self.calls)
+            if len(self._numbers) > self._KEPT:
+                del self._numbers[next(iter(self._numbers))]
+            self.calls += 1
+        if self.seed is None:
+            return draw
+        if draw not in self._numbers:
+            raise RuntimeError("[Spira] ExpertBlock: a training call within a backward pass that repeats none before it "
+                               "(checkpointing has to preserve the state of torch's generator)")
+        return self.seed, self._numbers[draw]
 
     def forward(self, input: SparseTensor) -> SparseTensor:
         x = input.features
@@ -74,6 +84,6 @@ class ExpertBlock(nn.Module):
         h = F.grouped_linear(h, self.down, routes.offsets, bias=self.down_bias)
         h = F.combine_experts(h, routes)
         if self.training and self.dropout > 0:
-            h = F.dropout(h, self.dropout, self.seed, self._number())
+            h = F.dropout(h, self.dropout, *self._mask())
         y, _ = F.gated_residual_norm(x, h, weight=self.exit, gate=self.gate, scale=self.scale, eps=self.eps)
         return SparseTensor(coordinates=input.coordinates, features=y, stride=input.stride)

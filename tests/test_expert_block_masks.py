@@ -1,5 +1,7 @@
 """The dropout masks of ``ExpertBlock``: which call has which.  On the CPU, with
 plain forms in place of the kernels; and once more with the kernels."""
+import copy
+
 import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
@@ -122,6 +124,49 @@ def test_a_recomputation_that_cannot_be_known_is_refused(plain):
     y = checkpoint(lambda f: block(SparseTensor(coords, f)).features, x, use_reentrant=False, preserve_rng_state=False)
     with pytest.raises(RuntimeError, match="repeats none"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_calls_without_a_seed(plain, reentrant):
+    check_recomputation("cpu", reentrant)
+    first, again = plain[:4], plain[4:]
+    assert again[:4] == first and sorted(again[4:]) == sorted(first)
+
+
+def test_blocks_have_masks_of_their_own(plain):
+    """Without a seed: two blocks, a copy of one, and every call of each; and the same again from the same state of
+    torch's generator.  With a seed: the number of the call."""
+    coords, x = voxels()
+    torch.manual_seed(0)
+    a, b = (spnn.ExpertBlock(12, 24, 4, 2, dropout=0.5) for _ in range(2))
+    blocks = [a, b, copy.deepcopy(a)]
+    runs = []
+    for _ in range(2):
+        torch.manual_seed(9)
+        del plain[:]
+        for block in blocks + blocks:
+            block(SparseTensor(coords, x))
+        assert len(set(plain)) == 6
+        runs.append(list(plain))
+    assert runs[0] == runs[1] and [int(block.calls) for block in blocks] == [4, 4, 4]
+    del plain[:]
+    a, b = (spnn.ExpertBlock(12, 24, 4, 2, dropout=0.5, seed=s) for s in (0, 1))
+    for block in (a, b, a):
+        block(SparseTensor(coords, x))
+    assert plain == [(0, 0), (1, 0), (0, 1)]
+
+
+@pytest.mark.gpu
+def test_blocks_drop_positions_of_their_own(dev):
+    """Of two default blocks of one width, the kept positions agree as often as independent ones do: half of 4096 x 64
+    at p = 0.5, within 6 deviations (of 256 each)."""
+    x = torch.randn(4096, 64, generator=torch.Generator().manual_seed(3)).to(dev)
+    kept = []
+    for _ in range(2):
+        block = spnn.ExpertBlock(64, 64, 4, 2, dropout=0.5).to(dev)
+        y = block(SparseTensor(torch.arange(4096, device=dev), x)).features
+        kept.append(y != x)
+    assert abs(int((kept[0] == kept[1]).sum()) - 2 ** 17) < 6 * 256
 
 
 @pytest.mark.gpu
