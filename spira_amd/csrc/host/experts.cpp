@@ -4,6 +4,7 @@
 // caching allocator on the current stream; nothing is read back on the host.
 #include "host_common.h"
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -323,7 +324,12 @@ static Tensor dropout(const Tensor &x, double p, uint64_t seed, uint64_t offset,
 static Tensor dense(const Tensor &t) { return t.contiguous(); }
 static OptTensor dense(const OptTensor &t) { return t ? OptTensor(t->contiguous()) : t; }
 
-static bool tracked(std::initializer_list<const OptTensor *> ts) {
+// Whether the call needs a node in the graph.  A tangent of forward mode would be
+// lost without a word, here and within a node, and read as zero: it is refused.
+static bool tracked(const char *name, std::initializer_list<const OptTensor *> ts) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (const OptTensor *t : ts)
+      SPIRA_CHECK_ARG(!*t || !(*t)->_fw_grad(0).defined(), name, ": there are no derivatives of forward mode");
   if (!torch::GradMode::is_enabled()) return false;
   for (const OptTensor *t : ts)
     if (*t && (*t)->requires_grad()) return true;
@@ -375,7 +381,7 @@ static Tensor grouped_linear_call(const Tensor &x, const Tensor &w, const Tensor
                     "grouped_linear: routes of ", slots->sizes(), " choices do not fit features of ", x.sizes());
   }
   const OptTensor ox = x, ow = w;
-  if (tracked({&ox, &ow, &bias}))
+  if (tracked("grouped_linear", {&ox, &ow, &bias}))
     return LinearFunction::apply(dense(x), dense(w), dense(bias), dense(offsets), dense(rows), dense(slots), relu);
   return grouped_linear(dense(x), dense(w), dense(offsets), dense(rows), dense(bias), relu);
 }
@@ -400,7 +406,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
 static std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_call(const Tensor &logits, int64_t k,
                                                                      bool renormalize) {
   const OptTensor l = logits;
-  if (!tracked({&l})) return route(dense(logits), k, renormalize);
+  if (!tracked("route_experts", {&l})) return route(dense(logits), k, renormalize);
   const variable_list v = RouteFunction::apply(dense(logits), k, renormalize);
   return {v[0], v[1], v[2], v[3], v[4]};
 }
@@ -422,7 +428,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
 
 static Tensor combine_call(const Tensor &h, const Tensor &weights, const Tensor &rows, const Tensor &slots) {
   const OptTensor oh = h, ow = weights;
-  if (tracked({&oh, &ow})) return CombineFunction::apply(dense(h), dense(weights), dense(rows), dense(slots));
+  if (tracked("combine_experts", {&oh, &ow})) return CombineFunction::apply(dense(h), dense(weights), dense(rows), dense(slots));
   return combine(dense(h), dense(slots), dense(weights));
 }
 
@@ -463,7 +469,7 @@ static std::tuple<OptTensor, OptTensor> norm_call(const Tensor &x, const OptTens
                                                   const OptTensor &gate, bool gate_sigmoid, double scale,
                                                   const OptTensor &next_weight, double eps) {
   const OptTensor ox = x;
-  if (!tracked({&ox, &h, &weight, &gate, &next_weight})) {
+  if (!tracked("gated_residual_norm", {&ox, &h, &weight, &gate, &next_weight})) {
     auto out = gated_residual_norm(dense(x), dense(h), dense(weight), dense(gate), gate_sigmoid, scale,
                                    dense(next_weight), eps, false);
     return {std::get<0>(out), std::get<1>(out)};
@@ -496,7 +502,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
 
 static Tensor dropout_call(const Tensor &x, double p, uint64_t seed, uint64_t offset, const OptTensor &residual) {
   const OptTensor ox = x;
-  if (tracked({&ox, &residual}))
+  if (tracked("dropout", {&ox, &residual}))
     return DropoutFunction::apply(dense(x), dense(residual), p, static_cast<int64_t>(seed),
                                   static_cast<int64_t>(offset));
   return dropout(dense(x), p, seed, offset, dense(residual));

@@ -65,3 +65,36 @@ def test_gradient_of_shares_that_cancel(dev, tokens, k, experts, ci, co, dtype):
     fits = ref.abs() < 65000 if dtype == "f16" else torch.ones_like(ref, dtype=torch.bool)
     assert fits.float().mean() > 0.5
     close(dx[fits], ref[fits], magnitude[fits], k * co, "dx")
+
+
+def operators(dev):
+    """Each operator as a function of its floating arguments, and those."""
+    routes = F.route_experts(randn((12, 4), torch.float32, 1).to(dev), 2)
+    calls = {
+        "grouped_linear": (lambda x, w, b: F.grouped_linear(x, w, routes, bias=b), (12, 16), (4, 16, 8), (4, 8)),
+        "route_experts": (lambda l: F.route_experts(l, 2).weights, (12, 4)),
+        "combine_experts": (lambda h, w: F.combine_experts(h, routes._replace(weights=w)), (24, 16), (12, 2)),
+        "gated_residual_norm": (lambda x, h, w, g, n: F.gated_residual_norm(x, h, weight=w, gate=g, next_weight=n)[1],
+                                (12, 16), (12, 16), (16,), (12, 16), (16,)),
+        "rms_norm": (F.rms_norm, (12, 16), (16,)),
+        "dropout": (lambda x, r: F.dropout(x, 0.5, 1, residual=r), (12, 16), (12, 16)),
+    }
+    for name, (f, *shapes) in calls.items():
+        yield name, f, [randn(s, torch.float32, 10 + i).to(dev) for i, s in enumerate(shapes)]
+
+
+@pytest.mark.parametrize("wants", [False, True])
+def test_tangents_of_forward_mode_are_refused(dev, wants):
+    """Of each argument, with and without a gradient asked for; where forward mode is off they do not matter."""
+    from torch.autograd import forward_ad
+    for name, f, args in operators(dev):
+        for i in range(len(args)):
+            with forward_ad.dual_level():
+                dual = [forward_ad.make_dual(t.clone().requires_grad_(wants), torch.ones_like(t)) if j == i else t
+                        for j, t in enumerate(args)]
+                with pytest.raises(RuntimeError, match=r"\[Spira\].*forward mode"):
+                    f(*dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match=r"\[Spira\].*forward mode"):
+                    f(*dual)
+                with forward_ad._set_fwd_grad_enabled(False):
+                    assert torch.equal(f(*dual).detach(), f(*args)), (name, i)
