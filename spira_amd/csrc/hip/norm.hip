@@ -104,10 +104,13 @@ template <class T, int NV, class F> __device__ __forceinline__ void each(F &&f) 
     for (int j = 0; j < kVec<T>; ++j) f(i, j);
 }
 
-// (the hardware's exponential and reciprocal, good to one unit each: at |v| up to
-// 20 within 3e-6 of the value; the library's take 17 us of a 16k x 1024 call)
-__device__ __forceinline__ float sigmoid(float v) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+// For 16 bits the hardware's exponential and reciprocal, good to one unit each: at
+// |v| up to 20 within 3e-6 of the value, a hundredth of an output's rounding (the
+// library's take 17 us of a 16k x 1024 call).  For fp32 that would be tens of units:
+// the library's exponential and a rounded division (16k x 1024 forward 64.5 -> 67.5 us).
+template <class T> __device__ __forceinline__ float sigmoid(float v) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * v));
+  else return 1.f / (1.f + expf(-v));
 }
 
 // a row's part of the gate as it lies in memory: its channels, or its one value
@@ -131,7 +134,7 @@ __device__ __forceinline__ Row<T, NV> gate_of(const Args &a, const Raw<NV> &own,
     const float v = g.v[0][0];
     each<T, NV>([&](int i, int j) { g.v[i][j] = v; });
   }
-  if (a.sigmoid) each<T, NV>([&](int i, int j) { g.v[i][j] = sigmoid(g.v[i][j]); });
+  if (a.sigmoid) each<T, NV>([&](int i, int j) { g.v[i][j] = sigmoid<T>(g.v[i][j]); });
   return g;
 }
 

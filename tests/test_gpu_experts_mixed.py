@@ -98,3 +98,14 @@ def test_tangents_of_forward_mode_are_refused(dev, wants):
                     f(*dual)
                 with forward_ad._set_fwd_grad_enabled(False):
                     assert torch.equal(f(*dual).detach(), f(*args)), (name, i)
+
+
+def test_sigmoid_gate_in_fp32(dev):
+    """The gate alone (residual 0, update 1): the exponential is good to one ulp (2^-23 of it), the sum and the
+    division to half of one each, so that the gate is within 2^-22 of its value."""
+    n, c = 64, 1024
+    gate = torch.linspace(-80, 80, n * c, dtype=torch.float32, device=dev).view(n, c)
+    r, _ = F.gated_residual_norm(torch.zeros_like(gate), torch.ones_like(gate), gate=gate, gate_sigmoid=True)
+    ref = 1 / (1 + torch.exp(-gate.double()))
+    off = ((r.double() - ref).abs() / ref).max().item()
+    assert off <= 2.0 ** -22, off
