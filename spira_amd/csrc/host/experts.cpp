@@ -397,6 +397,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list d) {
     const variable_list v = ctx->get_saved_variables();
+    if (!d[0].defined()) return {Tensor(), Tensor(), Tensor()};  // (what follows had no gradient of the weights)
     return once({route_backward(v[0], v[1], v[2], dense(d[0]), ctx->saved_data["renormalize"].toBool()), Tensor(),
                  Tensor()},
                 "route_experts");

@@ -109,3 +109,24 @@ def test_sigmoid_gate_in_fp32(dev):
     ref = 1 / (1 + torch.exp(-gate.double()))
     off = ((r.double() - ref).abs() / ref).max().item()
     assert off <= 2.0 ** -22, off
+
+
+class Cut(torch.autograd.Function):
+    """Passes values on, and no gradient back."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, d):
+        return None
+
+
+def test_no_gradient_comes_back(dev):
+    """A function behind an operator that returns no gradient leaves those of the rest as they are."""
+    for name, f, args in operators(dev):
+        leaves = [t.requires_grad_(True) for t in args]
+        grads = torch.autograd.grad(Cut.apply(f(*leaves)).sum() + sum(t.sum() for t in leaves), leaves)
+        for i, g in enumerate(grads):
+            assert torch.equal(g, torch.ones_like(g)), (name, i)
