@@ -1063,13 +1063,26 @@ template <class T, bool KO, class O> static int launch_few(const RowsArgs &a, hi
 }
 
 template <class T, bool KO, class O = T> static int launch_rows(const RowsArgs &a, hipStream_t stream) {
-  // Few rows to a group (us, against the large forms below): bf16 16 rows 2048 ->
-  // 512 in 32 groups 10.2 and 22.5, fp32 19 and 138; 16 a group 96 -> 384 5.7 and
-  // 10.1, 62 a group 64 -> 64 5.2 and 6.8; but bf16 32 a group 1024 -> 2048 27.6 and
-  // 17.2 (fp32 57 and 78), where every 16 rows read wide weights again.
-  const int64_t few = streams<T>(a.k, a.n) ? 64 : sizeof(T) == 4 ? 32 : 16;
-  if (a.g.rows <= few * a.g.count && dma_fits<T>(a)) return launch_few<T, KO, O>(a, stream);
-  if (streams<T>(a.k, a.n)) return launch_stream<T, KO, O>(a, stream);
+  // Few rows to a group, on average: how the rows lie, only the device knows.  A
+  // block of few_kernel reads its weights for 16 rows only, so the few form is
+  // taken where most of its blocks, however uneven the groups, run at once (512 do):
+  // then it costs its latency, which is the shortest.  us against the large forms
+  // below, groups of even sizes / sizes falling by 0.8 each:
+  //   bf16 16 a group, 32 groups, 2048 -> 512 (496 blocks) 14.6 / 18.2 and 22.3 / 23.7
+  //   4 a group, 32 groups, 512 -> 2048 (1216) 15.6 / 13.2 and 13.9 / 11.3
+  //   16 a group, 256 groups, 1024 -> 1024 (8k) 130 / 80 and 111 / 32
+  //   streamed weights: 16 a group, 64 groups, 96 -> 384 (744) 5.5 / 6.3 and 10.1 / 10.6;
+  //   64 a group 256 -> 256 (1264) 10.5 / 12.4 and 18.0 / 18.7, 96 -> 384 (1896) 13.5 / 15.5 and 10.5 / 10.9
+  // Tiles of fp32 take the matrix cores four times the rows that are there: 16 a group,
+  // 128 groups, 2048 -> 2048 390 / 352 and 1009 / 440, 32 a group 634 / 634 and 1009 /
+  // 515, of any number of blocks.  (All rows in one group: 582 and 270.)
+  const bool stream_fits = streams<T>(a.k, a.n);
+  const int64_t few = stream_fits ? 64 : sizeof(T) == 4 ? 32 : 16;
+  const int64_t most_blocks = stream_fits ? 1280 : sizeof(T) == 4 ? INT64_MAX : 1024;
+  if (a.g.rows <= few * a.g.count && most_parts(a.g.rows, a.g.count, 16) * div_up(a.n, 64) <= most_blocks &&
+      dma_fits<T>(a))
+    return launch_few<T, KO, O>(a, stream);
+  if (stream_fits) return launch_stream<T, KO, O>(a, stream);
   if (dma_fits<T>(a)) {
     // The large tile reads each operand half as often from L2 and LDS: 32k rows
     // 1024 -> 2048 in 16 even groups 141 us, with the small one 197.  It needs

@@ -193,8 +193,10 @@ def test_weights_gradient_without_parts(dev, groups, rows, ci, co, gathered, dty
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["uneven", "one"])
-@pytest.mark.parametrize("groups,rows,ci,co", [(32, 16, 2048, 512), (32, 512, 1000, 136), (20, 300, 4096, 72)])
+@pytest.mark.parametrize("groups,rows,ci,co", [(32, 16, 2048, 512), (32, 512, 1000, 136), (20, 300, 4096, 72),
+                                               (40, 640, 1024, 1096)])
 def test_few_rows_long_sums(dev, groups, rows, ci, co, kind, dtype):
-    """Sums past the depth at which each wave's ring of stages is used again; all rows in one of many groups."""
+    """Sums past the depth at which each wave's ring of stages is used again; all rows in one of many groups.  The last
+    has more blocks of 16 rows than run at once: tiles, in 16 bits."""
     check_linear(dev, dtype, rows, sizes_of(kind, groups, rows), ci, co, False)
     check_linear(dev, dtype, rows, sizes_of(kind, groups, rows), ci, co, True)
