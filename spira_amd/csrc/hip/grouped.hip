@@ -1370,10 +1370,14 @@ __global__ __launch_bounds__(256) void activation_kernel(const Groups g, int par
   }
 }
 
-static int check(int64_t rows, int groups, const int32_t *offsets, int64_t ci, int64_t co) {
+static int check_sizes(int64_t rows, int groups, int64_t ci, int64_t co) {
   SPIRA_HIP_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) - 256, "grouped_linear: bad number of rows");
   SPIRA_HIP_REQUIRE(groups > 0 && groups <= 32767, "grouped_linear: needs 1 to 32767 groups");
   SPIRA_HIP_REQUIRE(ci > 0 && co > 0 && ci <= (1 << 20) && co <= (1 << 20), "grouped_linear: bad widths");
+  return kOk;
+}
+static int check(int64_t rows, int groups, const int32_t *offsets, int64_t ci, int64_t co) {
+  if (int rc = check_sizes(rows, groups, ci, co)) return rc;
   SPIRA_HIP_REQUIRE(offsets, "grouped_linear: no offsets");
   return kOk;
 }
@@ -1438,7 +1442,8 @@ int spira_hip_grouped_linear_rows_gradient(int64_t rows, int groups, const int32
 }
 
 int spira_hip_grouped_linear_tokens_gradient_workspace(int64_t rows, int k, int c_in, size_t *bytes) {
-  SPIRA_HIP_REQUIRE(rows >= 0 && k > 0 && c_in > 0, "grouped_linear_tokens_gradient: bad sizes");
+  if (int rc = grouped::check_sizes(rows, 1, c_in, 1)) return rc;
+  SPIRA_HIP_REQUIRE(k > 0, "grouped_linear_tokens_gradient: bad sizes");
   *bytes = static_cast<size_t>(rows) * c_in * sizeof(float);
   return kOk;
 }
@@ -1473,6 +1478,7 @@ int spira_hip_grouped_linear_tokens_gradient(int64_t rows, int groups, const int
 }
 
 int spira_hip_grouped_linear_weights_gradient_workspace(int64_t rows, int groups, int c_in, int c_out, size_t *bytes) {
+  if (int rc = grouped::check_sizes(rows, groups, c_in, c_out)) return rc;
   const int part = grouped::weight_parts(rows, groups, c_in, c_out);
   *bytes = part == 0 ? 0 : grouped::most_parts(rows, groups, part) * static_cast<size_t>(c_in) * c_out * sizeof(float);
   return kOk;
@@ -1515,6 +1521,7 @@ int spira_hip_grouped_linear_weights_gradient(int64_t rows, int groups, const in
 
 int spira_hip_grouped_linear_activation_gradient_workspace(int64_t rows, int groups, int c_out, int dtype,
                                                            size_t *bytes) {
+  if (int rc = grouped::check_sizes(rows, groups, 1, c_out)) return rc;
   return with_type(dtype, [&](auto t) -> int {
     const int64_t part = grouped::sum_rows<decltype(t)>(rows, groups, c_out);
     *bytes = grouped::most_parts(rows, groups, part) * static_cast<size_t>(c_out) * sizeof(float);

@@ -413,10 +413,11 @@ int spira_hip_gated_residual_norm(const void *x, const void *h, int64_t n, int c
 }
 
 int spira_hip_gated_residual_norm_backward_workspace(int64_t n, int c, int dtype, size_t *bytes) {
+  SPIRA_HIP_REQUIRE(n >= 0 && c > 0, "gated_residual_norm: bad sizes");
   return with_type(dtype, [&](auto t) -> int {
     return norm::with_shape<decltype(t)>(c, [&](auto G, auto, auto NT) -> int {
       constexpr int rows = decltype(NT)::value / decltype(G)::value;
-      *bytes = static_cast<size_t>(norm::backward_blocks(std::max<int64_t>(n, 0), rows)) * 3 * c * sizeof(float);
+      *bytes = static_cast<size_t>(norm::backward_blocks(n, rows)) * 3 * c * sizeof(float);
       return kOk;
     });
   });
