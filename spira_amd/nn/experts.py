@@ -49,15 +49,25 @@ class ExpertBlock(nn.Module):
         self.down_bias = nn.Parameter(torch.zeros(experts, channels))
         self.exit = nn.Parameter(torch.ones(channels))
         self.gate = nn.Parameter(torch.full((channels,), 0.1))
-        self.register_buffer("calls", torch.zeros((), dtype=torch.int64, device="cpu"))
+        # (no buffer: it is read on the host and stays there, where a data-parallel wrapper over RCCL could not send it)
+        self.calls = torch.zeros((), dtype=torch.int64, device="cpu")
         self._numbers = {}  # of recent training calls, by their draws
 
-    def _apply(self, fn, recurse=True):
-        # (the count of calls is read on the host: it stays there)
-        calls = self._buffers.pop("calls")
-        super()._apply(fn, recurse)
-        self._buffers["calls"] = calls
-        return self
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "calls"] = self.calls.detach()
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                                      error_msgs)
+        key = prefix + "calls"
+        if key in state_dict:
+            self.calls.fill_(int(state_dict[key]))
+        elif strict:
+            missing_keys.append(key)
+        if key in unexpected_keys:
+            unexpected_keys.remove(key)
 
     def _mask(self) -> Tuple[int, int]:
         """Seed and offset of this training call's mask."""

@@ -156,6 +156,52 @@ def test_blocks_have_masks_of_their_own(plain):
     assert plain == [(0, 0), (1, 0), (0, 1)]
 
 
+def test_the_count_of_calls_in_state_dicts(plain):
+    """Saved and loaded with the parameters, alone and within another module; missed where it is not there."""
+    coords, x = voxels()
+    block = spnn.ExpertBlock(12, 24, 4, 2, dropout=0.5)
+    for _ in range(3):
+        block(SparseTensor(coords, x))
+    saved = block.state_dict()
+    assert int(saved["calls"]) == 3 and not list(block.buffers())
+    for outer in (lambda b: b, lambda b: torch.nn.Sequential(torch.nn.Linear(2, 2), b)):
+        state = outer(block).state_dict()
+        other = spnn.ExpertBlock(12, 24, 4, 2, dropout=0.5)
+        state = {k: v.clone() for k, v in state.items()}
+        assert not any(outer(other).load_state_dict(state)) and int(other.calls) == 3
+        assert other.double().calls.dtype == torch.int64
+        (key,) = [k for k in state if k.endswith("calls")]
+        del state[key]
+        with pytest.raises(RuntimeError, match="calls"):
+            outer(other).load_state_dict(state)
+        assert outer(other).load_state_dict(state, strict=False).missing_keys == [key]
+
+
+@pytest.mark.gpu
+def test_data_parallel_over_rccl(dev, tmp_path):
+    """A block within DistributedDataParallel, of one rank: its parameters and buffers are sent, its count is not."""
+    import torch.distributed as dist
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.block = spnn.ExpertBlock(12, 24, 4, 2, dropout=0.5)
+
+        def forward(self, coords, x):
+            return self.block(SparseTensor(coords, x)).features
+
+    dist.init_process_group("nccl", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        net = torch.nn.parallel.DistributedDataParallel(Net().to(dev), device_ids=[0])
+        coords, x = voxels(device=dev)
+        for _ in range(2):
+            net(coords, x).sum().backward()
+        torch.cuda.synchronize()
+        assert int(net.module.block.calls) == 2 and net.module.block.up.grad is not None
+    finally:
+        dist.destroy_process_group()
+
+
 @pytest.mark.gpu
 def test_blocks_drop_positions_of_their_own(dev):
     """Of two default blocks of one width, the kept positions agree as often as independent ones do: half of 4096 x 64
