@@ -11,6 +11,7 @@ when repeated.  Errors are ``RuntimeError("[Spira] ...")``; CPU tensors raise
 """
 from __future__ import annotations
 
+from operator import index
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -116,4 +117,4 @@ def dropout(features: torch.Tensor, p: float, seed: int, offset: int = 0, *,
     it was captured with.
     """
     _gpu(features)
-    return _C.dropout(features, p, seed & _LOW, offset & _LOW, residual)
+    return _C.dropout(features, p, index(seed) & _LOW, index(offset) & _LOW, residual)

@@ -5,6 +5,7 @@ and the ways of autograd around a call.
 Tolerances as in test_gpu_experts.py: an output's own rounding, u |ref|, and the
 error of a sum of n terms in fp32, n 2^-24 times the sum of their magnitudes
 (twice that, for the roundings of the terms themselves)."""
+import numpy as np
 import pytest
 import torch
 
@@ -130,3 +131,16 @@ def test_no_gradient_comes_back(dev):
         grads = torch.autograd.grad(Cut.apply(f(*leaves)).sum() + sum(t.sum() for t in leaves), leaves)
         for i, g in enumerate(grads):
             assert torch.equal(g, torch.ones_like(g)), (name, i)
+
+
+def test_seeds_of_other_integer_types(dev):
+    """NumPy's integers and tensors of one value, as a program's counters are; other numbers are refused."""
+    x = randn((40, 16), torch.float32, 1).to(dev)
+    for seed in (5, -5, 2 ** 62 + 1):
+        ref = F.dropout(x, 0.5, seed, 7)
+        assert torch.equal(F.dropout(x, 0.5, np.int64(seed), np.int32(7)), ref)
+        assert torch.equal(F.dropout(x, 0.5, torch.tensor(seed), torch.tensor(7)), ref)
+    with pytest.raises(TypeError):
+        F.dropout(x, 0.5, 5.0)
+    with pytest.raises(TypeError):
+        F.dropout(x, 0.5, 5, 0.5)
