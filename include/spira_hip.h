@@ -550,7 +550,8 @@ int spira_hip_finalize(const float *acc, int64_t num_targets, int c_out, int dty
  * weights [groups, c_in, c_out]; bias [groups, c_out] or null; act: relu or
  * none; s = sources[r], or r without sources (an s outside [0, num_sources)
  * stands for a row of zeros).  offsets [groups + 1] int32 on the device,
- * ascending; rows of no group get zeros.  1 to 32767 groups. */
+ * ascending; rows of no group get zeros.  1 to 32767 groups, up to 2^31 - 2^23
+ * rows. */
 int spira_hip_grouped_linear(int64_t rows, int groups, const int32_t *offsets, const int32_t *sources,
                              int64_t num_sources, const void *x, int c_in, const void *weights, const void *bias,
                              int c_out, int dtype, int relu, void *y, hipStream_t stream);

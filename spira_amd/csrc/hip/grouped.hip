@@ -1048,7 +1048,7 @@ template <class T> static bool dma_fits(const RowsArgs &a) {
 
 template <class T, bool KO, class O, int M, int N, int WM, int WN> static int launch_tile(const RowsArgs &a, hipStream_t stream) {
   const int64_t blocks = (most_parts(a.g.rows, a.g.count, M)) * div_up(a.n, N) + 1;
-  SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear: too many tiles");
+  SPIRA_HIP_REQUIRE(launchable(blocks, Tile<T, M, N, WM, WN>::NT), "grouped_linear: too many tiles");
   hipLaunchKernelGGL((tile_kernel<T, KO, O, M, N, WM, WN>), dim3(blocks), dim3(Tile<T, M, N, WM, WN>::NT), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();
   return kOk;
@@ -1056,7 +1056,7 @@ template <class T, bool KO, class O, int M, int N, int WM, int WN> static int la
 
 template <class T, bool KO, class O> static int launch_few(const RowsArgs &a, hipStream_t stream) {
   const int64_t blocks = most_parts(a.g.rows, a.g.count, 16) * div_up(a.n, 64) + 1;
-  SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear: too many tiles");
+  SPIRA_HIP_REQUIRE(launchable(blocks, 64 * kFewWaves), "grouped_linear: too many tiles");
   hipLaunchKernelGGL((few_kernel<T, KO, O>), dim3(blocks), dim3(64 * kFewWaves), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();
   return kOk;
@@ -1286,8 +1286,8 @@ template <class T> static bool dma_fits(const WeightsArgs &a) {
 template <class T, int M, int N, int WM, int WN>
 static int launch_weights_tile(const WeightsArgs &a, int64_t parts, hipStream_t stream) {
   const int64_t blocks = parts * div_up(a.co, N) * div_up(a.ci, M);
-  SPIRA_HIP_REQUIRE(blocks < (int64_t(1) << 31), "grouped_linear_weights_gradient: too many tiles");
   const dim3 threads(Tile<T, M, N, WM, WN>::NT);
+  SPIRA_HIP_REQUIRE(launchable(blocks, threads.x), "grouped_linear_weights_gradient: too many tiles");
   if (a.source)
     hipLaunchKernelGGL((weights_tile_kernel<T, true, M, N, WM, WN>), dim3(blocks), threads, 0, stream, a);
   else
@@ -1371,7 +1371,8 @@ __global__ __launch_bounds__(256) void activation_kernel(const Groups g, int par
 }
 
 static int check_sizes(int64_t rows, int groups, int64_t ci, int64_t co) {
-  SPIRA_HIP_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) - 256, "grouped_linear: bad number of rows");
+  // (2^23 short of 31 bits: rows_kernel has 256 threads to 128 rows, and a block more to each group)
+  SPIRA_HIP_REQUIRE(rows >= 0 && rows <= (int64_t(1) << 31) - (1 << 23), "grouped_linear: bad number of rows");
   SPIRA_HIP_REQUIRE(groups > 0 && groups <= 32767, "grouped_linear: needs 1 to 32767 groups");
   SPIRA_HIP_REQUIRE(ci > 0 && co > 0 && ci <= (1 << 20) && co <= (1 << 20), "grouped_linear: bad widths");
   return kOk;

@@ -81,6 +81,12 @@ template <int G> __device__ __forceinline__ float group_sum(float v) {
 int sum_slots(const float *h, int64_t rows, const int32_t *slots, int64_t tokens, int k, int c, int dtype, void *y,
               hipStream_t stream);
 
+// A launch has fewer than 2^32 threads (in x): of more, some do not run, and no error
+// says so.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks * threads < (int64_t(1) << 32); }
+// Blocks (of 256) to launch for this many turns, which the blocks walk.
+inline dim3 walking_blocks(int64_t turns) { return dim3(static_cast<uint32_t>(turns < (1 << 23) ? turns : 1 << 23)); }
+
 // f(T{}) for the storage type that `dtype` names
 template <class F> int with_type(int dtype, F &&f) {
   switch (dtype) {

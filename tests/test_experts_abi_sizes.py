@@ -9,7 +9,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB = ctypes.CDLL(os.path.join(ROOT, "spira_amd", "libspira_hip.so"))
 LIB.spira_hip_last_error.restype = ctypes.c_char_p
 I64, NULL, SOME = ctypes.c_int64, ctypes.c_void_p(), ctypes.c_void_p(256)
-FP16 = 0
+FP16, FP32 = 0, 1
 
 
 def refused(code, text):
@@ -53,3 +53,15 @@ def test_tokens_gradient():
     refused(call(workspace=NULL), "workspace")
     refused(call(bytes_=4 * 10 * 8 - 1), "workspace")
     refused(call(dtype=7), "dtype")
+
+
+def test_launches_of_too_many_threads():
+    """Past 2^32 threads some would not run: refused on the host."""
+    def linear(rows, groups, ci, co, dtype):
+        return LIB.spira_hip_grouped_linear(I64(rows), groups, SOME, NULL, I64(rows), SOME, ci, SOME, NULL, co, dtype, 0,
+                                            SOME, NULL)
+    refused(linear(40_000, 32767, 8, 65536, FP16), "too many tiles")   # tiles of 128 rows
+    refused(linear(16_384, 32767, 8, 65536, FP32), "too many tiles")   # few rows
+    refused(linear((1 << 31) - 1000, 1, 513, 1, FP16), "number of rows")
+    refused(LIB.spira_hip_grouped_linear_weights_gradient(I64(40_000), 32767, SOME, NULL, I64(40_000), SOME, 8, SOME, 65_664,
+                                                          FP16, SOME, NULL, ctypes.c_size_t(0), NULL), "too many tiles")

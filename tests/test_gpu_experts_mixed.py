@@ -144,3 +144,23 @@ def test_seeds_of_other_integer_types(dev):
         F.dropout(x, 0.5, 5.0)
     with pytest.raises(TypeError):
         F.dropout(x, 0.5, 5, 0.5)
+
+
+def test_combine_gradient_of_more_rows_than_a_launch_has_threads_for(dev):
+    """2^27 tokens and as many rows, 16 threads to each: past 2^32 threads, which is what one launch can have."""
+    n = (1 << 27) + 21
+    slots = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=dev)
+    rows = slots.clone()  # (row r is that of token n - 1 - r)
+    slots[::1000], rows[(n - 1 - torch.arange(0, n, 1000, device=dev))] = -1, -1
+    offsets = torch.zeros(2, dtype=torch.int32, device=dev)
+    h = (torch.arange(n, device=dev) % 61).half().view(n, 1).requires_grad_(True)
+    weights = (torch.arange(n, device=dev) % 7 + 1).float().view(n, 1).requires_grad_(True)
+    y = F.combine_experts(h, F.ExpertRoutes(weights, slots.view(n, 1), offsets, rows, slots.view(n, 1)))
+    dy = (torch.arange(n, device=dev) % 5).half().view(n, 1)
+    dh, dw = torch.autograd.grad(y, (h, weights), dy)
+    # (small whole numbers throughout: exact)
+    there = (slots >= 0).view(n, 1)
+    taken = h.detach().flip(0)
+    assert torch.equal(y, (taken * weights.half()).masked_fill(~there, 0))
+    assert torch.equal(dw, (taken * dy).float().masked_fill(~there, 0))
+    assert torch.equal(dh.flip(0), (weights.half() * dy).masked_fill(~there, 0))
