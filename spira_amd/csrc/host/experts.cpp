@@ -428,6 +428,9 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
 };
 
 static Tensor combine_call(const Tensor &h, const Tensor &weights, const Tensor &rows, const Tensor &slots) {
+  // (a slot past the features' rows would count as none)
+  SPIRA_CHECK_ARG(h.dim() == 2 && rows.numel() == h.size(0) && slots.numel() == rows.numel(),
+                  "combine_experts: routes of ", slots.sizes(), " choices do not fit features of ", h.sizes());
   const OptTensor oh = h, ow = weights;
   if (tracked("combine_experts", {&oh, &ow})) return CombineFunction::apply(dense(h), dense(weights), dense(rows), dense(slots));
   return combine(dense(h), dense(slots), dense(weights));

@@ -164,3 +164,15 @@ def test_combine_gradient_of_more_rows_than_a_launch_has_threads_for(dev):
     assert torch.equal(y, (taken * weights.half()).masked_fill(~there, 0))
     assert torch.equal(dw, (taken * dy).float().masked_fill(~there, 0))
     assert torch.equal(dh.flip(0), (weights.half() * dy).masked_fill(~there, 0))
+
+
+def test_combine_refuses_features_of_other_routes(dev):
+    routes = F.route_experts(randn((10, 4), torch.float32, 1).to(dev), 2)
+    for rows in (10, 19, 21):
+        for grad in (False, True):
+            with pytest.raises(RuntimeError, match=r"\[Spira\].*do not fit"):
+                F.combine_experts(torch.zeros(rows, 8, device=dev, requires_grad=grad), routes)
+    with pytest.raises(RuntimeError, match=r"\[Spira\].*do not fit"):
+        F.combine_experts(torch.zeros(20, device=dev), routes)
+    with torch.inference_mode():
+        assert F.combine_experts(torch.zeros(20, 8, device=dev), routes).shape == (10, 8)
