@@ -37,24 +37,24 @@ __device__ __forceinline__ Words philox(uint64_t counter, uint64_t offset, uint6
 // (threshold: 2^32 where nothing is kept.  A dropped value is not multiplied, so
 // that what it holds, infinities and NaN too, does not come through.)
 template <class T>
-__global__ __launch_bounds__(256) void dropout_kernel(const T *x, const T *residual, int64_t n, uint64_t threshold,
-                                                      float scale, uint64_t seed, uint64_t offset, T *y) {
-  const int64_t turn = gridDim.x * static_cast<int64_t>(256 * kVec<T>);
-  for (int64_t i = (blockIdx.x * static_cast<int64_t>(256) + threadIdx.x) * kVec<T>; i < n; i += turn) {
-    Chunk<T> c = load_chunk(x + i, n - i);
+__global__ __launch_bounds__(256) void dropout_kernel(const T *x, const T *residual, int64_t first, int64_t n,
+                                                      uint64_t threshold, float scale, uint64_t seed, uint64_t offset,
+                                                      T *y) {
+  const int64_t i = ((first + blockIdx.x) * 256 + threadIdx.x) * kVec<T>;
+  if (i >= n) return;
+  Chunk<T> c = load_chunk(x + i, n - i);
 #pragma unroll
-    for (int w = 0; w < kVec<T> / 4; ++w) {
-      const Words r = philox(static_cast<uint64_t>(i / 4 + w), offset, seed);
+  for (int w = 0; w < kVec<T> / 4; ++w) {
+    const Words r = philox(static_cast<uint64_t>(i / 4 + w), offset, seed);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c.v[4 * w + j] = r.v[j] >= threshold ? c.v[4 * w + j] * scale : 0.f;
-    }
-    if (residual) {
-      const Chunk<T> add = load_chunk(residual + i, n - i);
-#pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) c.v[j] += add.v[j];
-    }
-    store_chunk(y + i, n - i, c);
+    for (int j = 0; j < 4; ++j) c.v[4 * w + j] = r.v[j] >= threshold ? c.v[4 * w + j] * scale : 0.f;
   }
+  if (residual) {
+    const Chunk<T> add = load_chunk(residual + i, n - i);
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) c.v[j] += add.v[j];
+  }
+  store_chunk(y + i, n - i, c);
 }
 
 }  // namespace dropout
@@ -73,10 +73,10 @@ extern "C" int spira_hip_dropout(const void *x, const void *residual, int64_t n,
     SPIRA_HIP_REQUIRE(x && y, "dropout: null features");
     const auto threshold = static_cast<uint64_t>(p * 4294967296.0);
     const float scale = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.f;
-    hipLaunchKernelGGL(dropout::dropout_kernel<T>, walking_blocks(div_up(n, 256 * kVec<T>)), dim3(256), 0, stream,
-                       static_cast<const T *>(x), static_cast<const T *>(residual), n, threshold, scale, seed, offset,
-                       static_cast<T *>(y));
-    SPIRA_HIP_LAUNCH_CHECK();
-    return kOk;
+    return in_slices(div_up(n, 256 * kVec<T>), [&](int64_t first, dim3 blocks) {
+      hipLaunchKernelGGL(dropout::dropout_kernel<T>, blocks, dim3(256), 0, stream, static_cast<const T *>(x),
+                         static_cast<const T *>(residual), first, n, threshold, scale, seed, offset,
+                         static_cast<T *>(y));
+    });
   });
 }

@@ -84,8 +84,17 @@ int sum_slots(const float *h, int64_t rows, const int32_t *slots, int64_t tokens
 // A launch has fewer than 2^32 threads (in x): of more, some do not run, and no error
 // says so.
 inline bool launchable(int64_t blocks, int64_t threads) { return blocks * threads < (int64_t(1) << 32); }
-// Blocks (of 256) to launch for this many turns, which the blocks walk.
-inline dim3 walking_blocks(int64_t turns) { return dim3(static_cast<uint32_t>(turns < (1 << 23) ? turns : 1 << 23)); }
+// launch(first block, blocks) for so many blocks of 256 in all, in slices of 2^23
+// (a kernel that walks its blocks instead takes 5 % longer: dropout of 200k x 96
+// 20.1 us, 19.1 this way)
+template <class F> int in_slices(int64_t blocks, F &&launch) {
+  constexpr int64_t most = int64_t(1) << 23;
+  for (int64_t first = 0; first < blocks; first += most) {
+    launch(first, dim3(static_cast<uint32_t>(blocks - first < most ? blocks - first : most)));
+    SPIRA_HIP_LAUNCH_CHECK();
+  }
+  return kOk;
+}
 
 // f(T{}) for the storage type that `dtype` names
 template <class F> int with_type(int dtype, F &&f) {

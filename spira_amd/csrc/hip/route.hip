@@ -322,62 +322,61 @@ __global__ __launch_bounds__(256) void route_kernel(const T *logits, int tokens,
 template <class T, int G>
 __global__ __launch_bounds__(256) void choose_backward_kernel(const T *logits, const float *weights,
                                                               const int32_t *chosen, const float *dweights,
-                                                              int64_t tokens, int experts, int k, int renormalize,
-                                                              T *dlogits) {
+                                                              int64_t first, int64_t tokens, int experts, int k,
+                                                              int renormalize, T *dlogits) {
   const int lane = threadIdx.x % G;
-  const int64_t turn = gridDim.x * static_cast<int64_t>(256 / G);
-  for (int64_t token = blockIdx.x * static_cast<int64_t>(256 / G) + threadIdx.x / G; token < tokens; token += turn) {
-    float p[kHeld] = {}, d[kHeld] = {};
-    float mean = 0;
-    for (int j = 0; j < k; ++j) {
-      const int e = chosen[token * k + j];
-      if (e < 0) continue;
-      const float dj = dweights[token * k + j], w = weights[token * k + j];
-      mean += dj * w;
+  const int64_t token = (first + blockIdx.x) * (256 / G) + threadIdx.x / G;
+  if (token >= tokens) return;
+  float p[kHeld] = {}, d[kHeld] = {};
+  float mean = 0;
+  for (int j = 0; j < k; ++j) {
+    const int e = chosen[token * k + j];
+    if (e < 0) continue;
+    const float dj = dweights[token * k + j], w = weights[token * k + j];
+    mean += dj * w;
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i)
-        if (e == lane * kHeld + i) {
-          d[i] = dj;
-          p[i] = w;
-        }
-    }
-    if (!renormalize) {
-      float top = -INFINITY, sum = 0;
-#pragma unroll
-      for (int i = 0; i < kHeld / kVec<T>; ++i) {
-        const int at = lane * kHeld + i * kVec<T>;
-        const Chunk<T> c = load_chunk(logits + token * experts + at, experts - at);
-#pragma unroll
-        for (int j = 0; j < kVec<T>; ++j) p[i * kVec<T> + j] = at + j < experts ? c.v[j] : -INFINITY;
+    for (int i = 0; i < kHeld; ++i)
+      if (e == lane * kHeld + i) {
+        d[i] = dj;
+        p[i] = w;
       }
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) top = fmaxf(top, p[i]);
-#pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-      if (top == -INFINITY) top = 0;  // (no expert: every p is 0)
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        p[i] = expf(p[i] - top);
-        sum += p[i];
-      }
-      sum = group_sum<G>(sum);
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) p[i] *= inv;
-    }
+  }
+  if (!renormalize) {
+    float top = -INFINITY, sum = 0;
 #pragma unroll
     for (int i = 0; i < kHeld / kVec<T>; ++i) {
       const int at = lane * kHeld + i * kVec<T>;
-      Chunk<T> c;
+      const Chunk<T> c = load_chunk(logits + token * experts + at, experts - at);
 #pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) c.v[j] = p[i * kVec<T> + j] * (d[i * kVec<T> + j] - mean);
-      if (renormalize) {
-#pragma unroll
-        for (int j = 0; j < kVec<T>; ++j)
-          if (p[i * kVec<T> + j] == 0.f) c.v[j] = 0.f;
-      }
-      store_chunk(dlogits + token * experts + at, experts - at, c);
+      for (int j = 0; j < kVec<T>; ++j) p[i * kVec<T> + j] = at + j < experts ? c.v[j] : -INFINITY;
     }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) top = fmaxf(top, p[i]);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (top == -INFINITY) top = 0;  // (no expert: every p is 0)
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      p[i] = expf(p[i] - top);
+      sum += p[i];
+    }
+    sum = group_sum<G>(sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) p[i] *= inv;
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld / kVec<T>; ++i) {
+    const int at = lane * kHeld + i * kVec<T>;
+    Chunk<T> c;
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) c.v[j] = p[i * kVec<T> + j] * (d[i * kVec<T> + j] - mean);
+    if (renormalize) {
+#pragma unroll
+      for (int j = 0; j < kVec<T>; ++j)
+        if (p[i * kVec<T> + j] == 0.f) c.v[j] = 0.f;
+    }
+    store_chunk(dlogits + token * experts + at, experts - at, c);
   }
 }
 
@@ -385,70 +384,68 @@ __global__ __launch_bounds__(256) void choose_backward_kernel(const T *logits, c
 // of h, the outputs' or fp32
 template <class T, class I>
 __global__ __launch_bounds__(256) void combine_kernel(const I *h, int64_t rows, const int32_t *slots,
-                                                      const float *weights, int64_t tokens, int k, int c, T *y) {
+                                                      const float *weights, int64_t first, int64_t tokens, int k, int c,
+                                                      T *y) {
   const int chunks = (c + kVec<T> - 1) / kVec<T>;
-  const int64_t turn = gridDim.x * static_cast<int64_t>(256);
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x; i < tokens * chunks; i += turn) {
-    const int64_t t = i / chunks;
-    const int at = static_cast<int>(i - t * chunks) * kVec<T>;
-    Chunk<T> sum{};
-    for (int j = 0; j < k; ++j) {
-      const int32_t s = slots[t * k + j];
-      if (s < 0 || s >= rows) continue;
-      const float w = weights ? weights[t * k + j] : 1.f;
-      const I *row = h + static_cast<int64_t>(s) * c + at;
+  const int64_t i = (first + blockIdx.x) * 256 + threadIdx.x;
+  if (i >= tokens * chunks) return;
+  const int64_t t = i / chunks;
+  const int at = static_cast<int>(i - t * chunks) * kVec<T>;
+  Chunk<T> sum{};
+  for (int j = 0; j < k; ++j) {
+    const int32_t s = slots[t * k + j];
+    if (s < 0 || s >= rows) continue;
+    const float w = weights ? weights[t * k + j] : 1.f;
+    const I *row = h + static_cast<int64_t>(s) * c + at;
 #pragma unroll
-      for (int p = 0; p < kVec<T>; p += kVec<I>) {
-        const Chunk<I> v = load_chunk(row + p, c - at - p);
+    for (int p = 0; p < kVec<T>; p += kVec<I>) {
+      const Chunk<I> v = load_chunk(row + p, c - at - p);
 #pragma unroll
-        for (int q = 0; q < kVec<I>; ++q) sum.v[p + q] += w * v.v[q];
-      }
+      for (int q = 0; q < kVec<I>; ++q) sum.v[p + q] += w * v.v[q];
     }
-    store_chunk(y + t * c + at, c - at, sum);
   }
+  store_chunk(y + t * c + at, c - at, sum);
 }
 
 // dh[slots[t, j]] = w dy[t], dw[t, j] = <dy[t], h[slots[t, j]]>: 16 lanes per
-// token; then (with dh) zeros in the rows of no token
+// token; then zeros in the rows of no token
 template <class T>
 __global__ __launch_bounds__(256) void combine_backward_kernel(const T *h, int64_t rows, const int32_t *rows_of,
                                                                const int32_t *slots, const float *weights,
-                                                               const T *dy, int64_t tokens, int k, int c,
-                                                               int64_t token_blocks, int64_t blocks, T *dh,
-                                                               float *dweights) {
+                                                               const T *dy, int64_t first, int64_t tokens, int k,
+                                                               int c, int64_t token_blocks, T *dh, float *dweights) {
   constexpr int G = 16;
   const int lane = threadIdx.x % G;
-  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-    if (block >= token_blocks) {
-      const int64_t r = (block - token_blocks) * (256 / G) + threadIdx.x / G;
-      if (r >= rows || rows_of[r] >= 0) continue;
-      for (int at = lane * kVec<T>; at < c; at += G * kVec<T>) store_chunk(dh + r * c + at, c - at, Chunk<T>{});
-      continue;
-    }
-    const int64_t t = block * (256 / G) + threadIdx.x / G;
-    if (t >= tokens) continue;
-    for (int j = 0; j < k; ++j) {
-      const int32_t s = slots[t * k + j];
-      float dot = 0;
-      if (s >= 0 && s < rows) {
-        const float w = weights[t * k + j];
-        for (int at = lane * kVec<T>; at < c; at += G * kVec<T>) {
-          Chunk<T> g = load_chunk(dy + t * c + at, c - at);
-          if (dweights) {
-            const Chunk<T> v = load_chunk(h + static_cast<int64_t>(s) * c + at, c - at);
+  const int64_t block = first + blockIdx.x;
+  if (block >= token_blocks) {
+    const int64_t r = (block - token_blocks) * (256 / G) + threadIdx.x / G;
+    if (!dh || r >= rows || rows_of[r] >= 0) return;
+    for (int at = lane * kVec<T>; at < c; at += G * kVec<T>) store_chunk(dh + r * c + at, c - at, Chunk<T>{});
+    return;
+  }
+  const int64_t t = block * (256 / G) + threadIdx.x / G;
+  if (t >= tokens) return;
+  for (int j = 0; j < k; ++j) {
+    const int32_t s = slots[t * k + j];
+    float dot = 0;
+    if (s >= 0 && s < rows) {
+      const float w = weights[t * k + j];
+      for (int at = lane * kVec<T>; at < c; at += G * kVec<T>) {
+        Chunk<T> g = load_chunk(dy + t * c + at, c - at);
+        if (dweights) {
+          const Chunk<T> v = load_chunk(h + static_cast<int64_t>(s) * c + at, c - at);
 #pragma unroll
-            for (int q = 0; q < kVec<T>; ++q) dot += g.v[q] * v.v[q];
-          }
-          if (dh) {
+          for (int q = 0; q < kVec<T>; ++q) dot += g.v[q] * v.v[q];
+        }
+        if (dh) {
 #pragma unroll
-            for (int q = 0; q < kVec<T>; ++q) g.v[q] *= w;
-            store_chunk(dh + static_cast<int64_t>(s) * c + at, c - at, g);
-          }
+          for (int q = 0; q < kVec<T>; ++q) g.v[q] *= w;
+          store_chunk(dh + static_cast<int64_t>(s) * c + at, c - at, g);
         }
       }
-      dot = group_sum<G>(dot);
-      if (dweights && lane == 0) dweights[t * k + j] = dot;
     }
+    dot = group_sum<G>(dot);
+    if (dweights && lane == 0) dweights[t * k + j] = dot;
   }
 }
 
@@ -479,12 +476,10 @@ static int tile_tokens(int64_t tokens, int experts, int k) {
 template <class T, class I>
 static int launch_combine(const I *h, int64_t rows, const int32_t *slots, const float *weights, int64_t tokens, int k,
                           int c, T *y, hipStream_t stream) {
-  const int64_t blocks = div_up(tokens * div_up(c, kVec<T>), 256);
-  if (blocks == 0) return kOk;
-  hipLaunchKernelGGL((combine_kernel<T, I>), walking_blocks(blocks), dim3(256), 0, stream, h, rows, slots, weights, tokens, k, c,
-                     y);
-  SPIRA_HIP_LAUNCH_CHECK();
-  return kOk;
+  return in_slices(div_up(tokens * div_up(c, kVec<T>), 256), [&](int64_t first, dim3 blocks) {
+    hipLaunchKernelGGL((combine_kernel<T, I>), blocks, dim3(256), 0, stream, h, rows, slots, weights, first, tokens, k,
+                       c, y);
+  });
 }
 
 static int check(int64_t tokens, int experts, int k) {
@@ -571,11 +566,11 @@ int spira_hip_route_backward(const void *logits, int64_t tokens, int experts, in
     if (tokens == 0) return kOk;
     return route::with_lanes(experts, [&](auto G) -> int {
       constexpr int g = decltype(G)::value;
-      hipLaunchKernelGGL((route::choose_backward_kernel<T, g>), walking_blocks(div_up(tokens, 256 / g)), dim3(256), 0, stream,
-                         static_cast<const T *>(logits), weights, chosen, dweights, tokens, experts, k, renormalize,
-                         static_cast<T *>(dlogits));
-      SPIRA_HIP_LAUNCH_CHECK();
-      return kOk;
+      return in_slices(div_up(tokens, 256 / g), [&](int64_t first, dim3 blocks) {
+        hipLaunchKernelGGL((route::choose_backward_kernel<T, g>), blocks, dim3(256), 0, stream,
+                           static_cast<const T *>(logits), weights, chosen, dweights, first, tokens, experts, k,
+                           renormalize, static_cast<T *>(dlogits));
+      });
     });
   });
 }
@@ -602,12 +597,11 @@ int spira_hip_combine_backward(const void *h, int64_t num_rows, const int32_t *r
   const int64_t token_blocks = div_up(tokens, 16), blocks = token_blocks + (dh ? div_up(num_rows, 16) : 0);
   return with_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    if (blocks == 0) return kOk;
-    hipLaunchKernelGGL(route::combine_backward_kernel<T>, walking_blocks(blocks), dim3(256), 0, stream,
-                       static_cast<const T *>(h), num_rows, rows, slots, weights, static_cast<const T *>(dy), tokens, k,
-                       c, token_blocks, blocks, static_cast<T *>(dh), dweights);
-    SPIRA_HIP_LAUNCH_CHECK();
-    return kOk;
+    return in_slices(blocks, [&](int64_t first, dim3 slice) {
+      hipLaunchKernelGGL(route::combine_backward_kernel<T>, slice, dim3(256), 0, stream, static_cast<const T *>(h),
+                         num_rows, rows, slots, weights, static_cast<const T *>(dy), first, tokens, k, c, token_blocks,
+                         static_cast<T *>(dh), dweights);
+    });
   });
 }
 
