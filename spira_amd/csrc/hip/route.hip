@@ -15,7 +15,11 @@
 // expert's number.  No order depends on atomics (those on integer counts only
 // add up).  Few tokens take one block and one launch.
 //
-// Bound by launches up to about 100k tokens, by memory past that.
+// Few tokens are bound by the launch (8 of 32 experts: 4.4 us).  100k tokens of 16
+// experts, two choices: 10.0 us to choose and 10.7 to rank, where the bytes of both
+// take about 1: the blocks' barriers, and counts and choices that go through memory
+// between the two; the gradient 4.0 us.  The sum of 100k tokens' rows and its
+// gradient (12.0 and 20.8 us, 96 channels) are bound by memory.
 #include "numeric.hpp"
 
 #include <algorithm>

@@ -7,7 +7,8 @@ fp16, bf16 and fp32 features (all floating inputs of a call share one type, the
 routing weights are fp32); sums are taken in fp32 and outputs rounded once.
 Calls run on the current stream, read nothing back and give identical results
 when repeated.  Errors are ``RuntimeError("[Spira] ...")``; CPU tensors raise
-``NotImplementedError``.  Gradients are of first order.
+``NotImplementedError``.  Gradients are of first order; tangents of forward
+mode are refused.
 """
 from __future__ import annotations
 
