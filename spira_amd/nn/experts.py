@@ -51,7 +51,7 @@ class ExpertBlock(nn.Module):
         self.gate = nn.Parameter(torch.full((channels,), 0.1))
         # (no buffer: it is read on the host and stays there, where a data-parallel wrapper over RCCL could not send it)
         self.calls = torch.zeros((), dtype=torch.int64, device="cpu")
-        self._numbers = {}  # of recent training calls with a seed, by their draws
+        self._numbers = {}  # of recent training calls, by their draws
 
     def _save_to_state_dict(self, destination, prefix, keep_vars):
         super()._save_to_state_dict(destination, prefix, keep_vars)
@@ -72,12 +72,12 @@ class ExpertBlock(nn.Module):
     def _mask(self) -> Tuple[int, int]:
         """Seed and offset of this training call's mask."""
         draw = tuple(torch.randint(2 ** 63 - 1, (2,), dtype=torch.int64, device="cpu").tolist())
-        if torch._C._current_graph_task_id() < 0:  # (not within a backward pass, which computes a call again)
-            if self.seed is not None:
-                self._numbers.pop(draw, None)
-                self._numbers[draw] = int(self.calls)
-                if len(self._numbers) > self._KEPT:
-                    del self._numbers[next(iter(self._numbers))]
+        again = torch._C._current_graph_task_id() >= 0  # within a backward pass: a call computed again
+        if not again:
+            self._numbers.pop(draw, None)
+            self._numbers[draw] = int(self.calls)
+            if len(self._numbers) > self._KEPT:
+                del self._numbers[next(iter(self._numbers))]
             self.calls += 1
         if self.seed is None:
             return draw
