@@ -79,12 +79,10 @@ class ExpertBlock(nn.Module):
             if len(self._numbers) > self._KEPT:
                 del self._numbers[next(iter(self._numbers))]
             self.calls += 1
-        if self.seed is None:
-            return draw
         if draw not in self._numbers:
             raise RuntimeError("[Spira] ExpertBlock: a training call within a backward pass that repeats none before it "
                                "(checkpointing has to preserve the state of torch's generator)")
-        return self.seed, self._numbers[draw]
+        return draw if self.seed is None else (self.seed, self._numbers[draw])
 
     def forward(self, input: SparseTensor) -> SparseTensor:
         x = input.features

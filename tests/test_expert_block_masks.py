@@ -118,9 +118,10 @@ def test_recomputed_calls_have_their_first_masks(plain, reentrant):
     assert again[:4] == first and sorted(again[4:]) == sorted(first)
 
 
-def test_a_recomputation_that_cannot_be_known_is_refused(plain):
+@pytest.mark.parametrize("seed", [5, None])
+def test_a_recomputation_that_cannot_be_known_is_refused(plain, seed):
     coords, x = voxels()
-    block = spnn.ExpertBlock(12, 24, 4, 2, dropout=0.5, seed=5)
+    block = spnn.ExpertBlock(12, 24, 4, 2, dropout=0.5, seed=seed)
     y = checkpoint(lambda f: block(SparseTensor(coords, f)).features, x, use_reentrant=False, preserve_rng_state=False)
     with pytest.raises(RuntimeError, match="repeats none"):
         y.sum().backward()
