@@ -644,6 +644,75 @@ int spira_hip_gated_residual_norm_backward(const void *x, const void *h, int64_t
 int spira_hip_dropout(const void *x, const void *residual, int64_t n, int dtype, double p, uint64_t seed,
                       uint64_t offset, void *y, hipStream_t stream);
 
+/* Attention over packed sequences with grouped heads.  Sequence b has the queries
+ * offsets[b] to offsets[b + 1] and the first key_counts[b] (null: all) of the keys
+ * key_offsets[b] to key_offsets[b + 1], int32 on the device, ascending; what lies
+ * behind a sequence's keys is not read.  Query head h reads key head h kv_heads /
+ * heads.  causal: query i of n sees key j of m if j <= i + m - n.  head_dim: 1 to
+ * 128 values, consecutive; rows and heads at any stride (in values).  A query
+ * without visible keys, or in no sequence, gets zeros. */
+typedef struct {
+  int64_t rows, keys; /* of queries, of keys and values */
+  int sequences, heads, kv_heads, head_dim, dtype, causal;
+  float scale; /* of the scores, positive */
+  const int32_t *offsets, *key_offsets, *key_counts;
+  const void *queries, *key, *value;
+  int64_t query_row, query_head, key_row, key_head, value_row, value_head;
+} spira_hip_attention_t;
+
+/* Workspace bytes of spira_hip_attention without statistics, or of its gradient. */
+int spira_hip_attention_workspace(const spira_hip_attention_t *x, int gradient, size_t *bytes);
+
+/* out [rows, heads, head_dim]; stats (null without a gradient): fp32 [heads, rows],
+ * of fp32 features [2, heads, rows].  A call with stats needs no workspace. */
+int spira_hip_attention(const spira_hip_attention_t *x, void *out, float *stats, void *workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
+/* The gradients (any may be null) from dout, with out and stats of the forward pass:
+ * dqueries [rows, heads, head_dim], dkey and dvalue [keys, kv_heads, head_dim], zeros
+ * in rows of no sequence and behind a sequence's keys. */
+int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out, const float *stats, const void *dout,
+                                 void *dqueries, void *dkey, void *dvalue, void *workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
+
+/* For each head of each row, n = x / sqrt(mean(x^2) + eps) * weight (weight
+ * [head_dim]; null: n = x), then, with axes > 0, each pair of n turned by an angle.
+ * Pair p of head_dim / 2 is (p, p + head_dim / 2), or (2 p, 2 p + 1) interleaved; the
+ * pairs fall into a band for each axis, pairs a (head_dim / 2) / axes up to the next's,
+ * and pair j of n in band a turns by positions[row, a] base^(-j / n) radians.
+ * head_dim: 1 to 128 values, consecutive, even with a rotation; rows and heads at any
+ * stride (in values).  Outputs [rows, heads, head_dim] and [rows, kv_heads, head_dim]. */
+typedef struct {
+  int64_t rows;
+  int heads, kv_heads, head_dim, dtype, axes, interleaved;
+  float eps;
+  double base;
+  const void *queries, *key, *query_weight, *key_weight;
+  int64_t query_row, query_head, key_row, key_head;
+  const int32_t *positions; /* [rows, axes] */
+} spira_hip_heads_t;
+
+int spira_hip_norm_rotate_heads(const spira_hip_heads_t *x, void *queries, void *key, hipStream_t stream);
+
+/* The gradients (any may be null) from those of the outputs (null: none of that side
+ * is wanted). */
+int spira_hip_norm_rotate_heads_backward_workspace(const spira_hip_heads_t *x, size_t *bytes);
+int spira_hip_norm_rotate_heads_backward(const spira_hip_heads_t *x, const void *dout_queries, const void *dout_key,
+                                         void *dqueries, void *dkey, void *dquery_weight, void *dkey_weight,
+                                         void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The balance loss of a router: experts * sum_e share[e] probabilities[e], with
+ * counts[e] = offsets[e + 1] - offsets[e] (those of spira_hip_route), share[e] =
+ * counts[e] over their sum, and probabilities[e] the mean of softmax(logits[t])[e]
+ * over the tokens that have a logit above -inf.  kept [experts + 1] holds what the
+ * gradient needs.  1 to 512 experts. */
+int spira_hip_balance_workspace(int64_t tokens, int experts, size_t *bytes);
+int spira_hip_balance(const void *logits, int64_t tokens, int experts, int dtype, const int32_t *offsets, float *loss,
+                      int32_t *counts, float *probabilities, float *kept, void *workspace, size_t workspace_bytes,
+                      hipStream_t stream);
+int spira_hip_balance_backward(const void *logits, int64_t tokens, int experts, int dtype, const float *kept,
+                               const float *dloss, void *dlogits, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

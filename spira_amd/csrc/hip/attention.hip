@@ -1,0 +1,475 @@
+// Attention over packed sequences (gfx950), forward:
+//
+//   s_ij = scale q_i . k_j,  p_ij = exp(s_ij) / sum over the visible j of exp(s_ij),  o_i = sum_j p_ij v_j
+//
+// with `group` query heads to a key head; causal: query i of n sees key j of m if
+// j <= i + m - n.  A row that sees no key gets zeros.
+//
+// Two forms.  Prompts: a block owns 128 columns (a key head's query heads and
+// their queries, heads fastest), four waves of 32, and walks the keys in tiles
+// that it holds in LDS, the next one under way while it multiplies.  Few tokens:
+// the keys of a sequence are cut into parts, a block's four waves walk a part's
+// tiles each on their own (without barriers) for the same 32 columns, and the
+// parts are joined by a second launch.
+//
+// The softmax is taken in one pass with a running maximum and sum in fp32.  The
+// maximum moves only when a score passes it by 2^8 (in exp2): the sums are exact
+// under any reference, and columns are seldom scaled anew.
+#include "attention.hpp"
+
+#include <algorithm>
+
+namespace spira_hip {
+
+namespace attention {
+
+constexpr float kSlack = 8.f;
+
+// keys of a tile
+template <class T> constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
+
+// a wave's 32 columns on their way: output, reference maximum of the raw scores
+// (-inf: nothing seen) and this half's share of the sum
+template <int DP> struct Columns {
+  floatx16 o[DP / 32];
+  float m, l;
+};
+
+// One tile of KT keys.  limit: how many of them this lane's column sees (any
+// number); whole: every column of the wave sees all.
+template <class T, int DP, int KT>
+__device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[DP / 16], lds_char *kt, lds_char *vt,
+                                            float scale2, int limit, bool whole) {
+  const int h = lane_id() >> 5;
+  floatx16 s[KT / 32];
+#pragma unroll
+  for (int u = 0; u < KT / 32; ++u) {
+    s[u] = floatx16{};
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) mma(s[u], row_frag<T, DP>(kt, 32 * u, st), q[st]);
+  }
+  if (!whole) {
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[u][r] = 32 * u + 8 * (r / 4) + r % 4 < limit - 4 * h ? s[u][r] : -__builtin_inff();
+  }
+  float top = s[0][0];
+#pragma unroll
+  for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[u][r]);
+  top = __builtin_fmaxf(top, other_half(top));
+  // (each column by its own scores: a result does not depend on the wave's others)
+  const bool moves = (top - c.m) * scale2 > kSlack;
+  if (ballot(moves)) {
+    const float m = moves ? top : c.m, by = moves ? __builtin_amdgcn_exp2f((c.m - m) * scale2) : 1.f;
+    c.l *= by;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) c.o[n][r] *= by;
+    c.m = m;
+  }
+  const float base = c.m == -__builtin_inff() ? 0.f : -c.m * scale2;
+  float sum = 0;
+#pragma unroll
+  for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale2, base));
+      sum += s[u][r];
+    }
+  c.l += sum;
+  Frag<T> p[KT / 16];
+#pragma unroll
+  for (int st = 0; st < KT / 16; ++st) p[st] = as_operand<T>(s[st / 2], st % 2);
+#pragma unroll
+  for (int st = 0; st < KT / 16; ++st)
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) mma(c.o[n], col_frag<T, DP>(vt, 16 * st, n), p[st]);
+}
+
+// keys that query i of a sequence sees
+__device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) {
+  if (!a.causal) return s.nk;
+  const int n = i + 1 + s.nk - s.nq;
+  return n < 0 ? 0 : n < s.nk ? n : s.nk;
+}
+
+// ---------------------------------------------------------------------------
+// prompts
+// ---------------------------------------------------------------------------
+constexpr int kColumns = 128;
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(const Args a) {
+  using R = Rows<T, DP>;
+  constexpr int KT = kKeys<T>, TILE = KT * R::PITCH;
+  __shared__ __align__(1024) char lds[4 * TILE];
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id();
+  T *o = static_cast<T *>(a.o);
+  clear_uncovered(a.s.offsets, a.s.count, a.s.rows, o, static_cast<int64_t>(a.heads) * a.d, blockIdx.x, gridDim.x);
+  // (key heads fastest: where their number divides 8 or 8 it, an XCD's blocks share
+  // few heads' keys)
+  const int kv = blockIdx.x % a.kv_heads;
+  const Found f = find_piece(a.s.count, blockIdx.x / a.kv_heads,
+                             [&](int b) { return (queries_of(a.s, b) * a.group + kColumns - 1) / kColumns; });
+  if (f.sequence < 0) return;
+  const Sequence s = sequence_at(a.s, f.sequence);
+  // (the last tile first: it sees the most keys)
+  const int total = s.nq * a.group, c0 = (f.of - 1 - f.nth) * kColumns, w0 = c0 + wave * 32;
+  const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
+  const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i);
+  const int least = visible(a, s, std::min(w0, total - 1) / a.group);
+  const int most = w0 < total ? visible(a, s, std::min(w0 + 31, total - 1) / a.group) : 0;
+  const int fewest = visible(a, s, c0 / a.group), end = visible(a, s, std::min(c0 + kColumns - 1, total - 1) / a.group);
+  const int steps = (end + KT - 1) / KT, own = (most + KT - 1) / KT;
+  const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
+  const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + s.k0 * a.k_row + kv * a.k_head);
+  const char *values = reinterpret_cast<const char *>(static_cast<const T *>(a.v) + s.k0 * a.v_row + kv * a.v_head);
+  const auto issue = [&](int t) {
+    lds_char *to = (lds_char *)lds + (t & 1) * 2 * TILE;
+    fetch_tile<T, DP, KT, 256>(keys + t * (KT * kstride), kstride, s.nk - t * KT, a.d, a.dma & 1, to, threadIdx.x);
+    fetch_tile<T, DP, KT, 256>(values + t * (KT * vstride), vstride, s.nk - t * KT, a.d, a.dma & 1, to + TILE,
+                               threadIdx.x);
+  };
+  if (steps > 0) issue(0);
+  Frag<T> q[DP / 16];
+  {
+    const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) q[st] = load_frag(row, a.d, st);
+  }
+  Columns<DP> c{};
+  c.m = -__builtin_inff();
+  for (int t = 0; t < steps; ++t) {
+    wait_loads_and_meet<0>();
+    if (t + 1 < steps) issue(t + 1);
+    lds_char *kt = (lds_char *)lds + (t & 1) * 2 * TILE;
+    // (the same for the whole block)
+    const bool hides = a.causal && fewest < (t + 1) * KT;
+    const bool found = hides && __syncthreads_or(clear_not_finite<T, DP, KT, 256>(kt + TILE, threadIdx.x));
+    if (t < own) {
+      const int mine = limit - t * KT;
+      attend_tile<T, DP, KT>(c, q, kt, kt + TILE, a.scale2, mine, least >= (t + 1) * KT);
+      if (found)
+        add_not_finite<T, DP>(c.o, values + t * (KT * vstride), vstride, std::min(s.nk - t * KT, KT), a.d,
+                              [&](int x) { return x < mine; });
+    }
+  }
+  const float l = c.l + other_half(c.l);
+  const bool there = column < total;
+  store_column<T, DP>(o + ((s.q0 + i) * a.heads + head) * a.d, a.d, there, c.o, l == 0.f ? 0.f : 1.f / l);
+  if (a.stats && there && lane < 32) {
+    float *to = a.stats + head * a.s.rows + s.q0 + i;
+    const float base = c.m == -__builtin_inff() ? 0.f : c.m * a.scale2;
+    if constexpr (sizeof(T) == 2) {
+      *to = l == 0.f ? __builtin_inff() : base + __builtin_amdgcn_logf(l);
+    } else {
+      to[0] = base;
+      to[a.heads * a.s.rows] = l == 0.f ? 0.f : 1.f / l;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// few tokens
+// ---------------------------------------------------------------------------
+template <class T, int DP> constexpr int kTokenWaves = Rows<T, DP>::PITCH >= 512 ? 2 : 4;
+
+// DIRECT: no sequence has more than one part; the outputs themselves
+template <class T, int DP, bool DIRECT>
+__global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)) void token_kernel(const Args a) {
+  using R = Rows<T, DP>;
+  constexpr int KT = 32, TILE = KT * R::PITCH, NW = kTokenWaves<T, DP>, NT = 64 * NW;
+  constexpr int LOADS = 2 * KT * R::CPR / 64, OPITCH = DP + 4;  // (of the sums in LDS)
+  static_assert(32 * OPITCH * 4 <= 4 * TILE, "a wave's sums take its stages' place");
+  __shared__ __align__(1024) char lds[NW][4 * TILE];
+  __shared__ float wm[NW][32], wl[NW][32], top[32], total_l[32];
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id();
+  lds_char *mine = (lds_char *)lds[wave];
+  T *o = static_cast<T *>(a.o);
+  if constexpr (DIRECT)
+    clear_uncovered(a.s.offsets, a.s.count, a.s.rows, o, static_cast<int64_t>(a.heads) * a.d,
+                    blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x,
+                    static_cast<int64_t>(gridDim.x) * gridDim.y);
+  const int kv = blockIdx.x % a.kv_heads;
+  // (a sequence without keys has a part of none where its outputs are written here)
+  const Found f = find_piece(a.s.count, blockIdx.x / a.kv_heads, [&](int b) {
+    const int n = (keys_of(a.s, b) + a.part_keys - 1) / a.part_keys;
+    return queries_of(a.s, b) == 0 ? 0 : DIRECT ? 1 : n;
+  });
+  if (f.sequence < 0) return;
+  const Sequence s = sequence_at(a.s, f.sequence);
+  const int first = f.nth * a.part_keys, total = s.nq * a.group;
+  const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
+  const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + (s.k0 + first) * a.k_row + kv * a.k_head);
+  const char *values =
+      reinterpret_cast<const char *>(static_cast<const T *>(a.v) + (s.k0 + first) * a.v_row + kv * a.v_head);
+  const int part = std::min(s.nk - first, a.part_keys);
+  for (int w0 = blockIdx.y * 32; w0 < total; w0 += gridDim.y * 32) {
+    const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
+    const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i) - first;
+    const int least = visible(a, s, w0 / a.group) - first;
+    const int most = visible(a, s, std::min(w0 + 31, total - 1) / a.group) - first;
+    const int end = std::min(part, most), steps = end > 0 ? (end + KT - 1) / KT : 0;
+    const auto issue = [&](int t, int stage) {
+      lds_char *to = mine + stage * 2 * TILE;
+      const int64_t n = t < steps ? part - t * KT : 0;
+      fetch_tile<T, DP, KT, 64>(keys + t * (KT * kstride), kstride, n, a.d, a.dma & 1, to, lane);
+      fetch_tile<T, DP, KT, 64>(values + t * (KT * vstride), vstride, n, a.d, a.dma & 1, to + TILE, lane);
+    };
+    issue(wave, 0);
+    Frag<T> q[DP / 16];
+    const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) q[st] = load_frag(row, a.d, st);
+    Columns<DP> c{};
+    c.m = -__builtin_inff();
+    for (int t = wave, stage = 0; t < steps; t += NW, stage ^= 1) {
+      issue(t + NW, stage ^ 1);
+      // until this tile's loads have landed (the next one's are on their way)
+      __builtin_amdgcn_s_waitcnt((LOADS & 15) | (7 << 4) | ((LOADS >> 4) << 14));
+      asm volatile("" ::: "memory");
+      lds_char *kt = mine + stage * 2 * TILE;
+      const bool hides = a.causal && least < (t + 1) * KT;
+      const bool found = hides && ballot(clear_not_finite<T, DP, KT, 64>(kt + TILE, lane)) != 0;
+      const int seen = std::min(limit, part) - t * KT;
+      attend_tile<T, DP, KT>(c, q, kt, kt + TILE, a.scale2, seen, std::min(least, part) >= (t + 1) * KT);
+      if (found)
+        add_not_finite<T, DP>(c.o, values + t * (KT * vstride), vstride, std::min(part - t * KT, KT), a.d,
+                              [&](int x) { return x < seen; });
+    }
+    wait_loads();
+    asm volatile("" ::: "memory");
+    // the waves' columns to LDS, and their sum from there
+    float *sums = reinterpret_cast<float *>(lds[wave]) + (lane & 31) * OPITCH + 4 * (lane >> 5);
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<floatx4_t *>(sums + 32 * n + 8 * g) =
+            floatx4_t{c.o[n][4 * g], c.o[n][4 * g + 1], c.o[n][4 * g + 2], c.o[n][4 * g + 3]};
+    const float l = c.l + other_half(c.l);
+    if (lane < 32) {
+      wm[wave][lane] = c.m;
+      wl[wave][lane] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      float m = wm[0][lane], sum = 0;
+#pragma unroll
+      for (int w = 1; w < NW; ++w) m = __builtin_fmaxf(m, wm[w][lane]);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float by = wm[w][lane] == m ? 1.f : __builtin_amdgcn_exp2f((wm[w][lane] - m) * a.scale2);
+        sum += wl[w][lane] * by;
+        wm[w][lane] = by;
+      }
+      top[lane] = m;
+      total_l[lane] = sum;
+    }
+    __syncthreads();
+    const int columns = std::min(32, total - w0);
+    for (int k = threadIdx.x; k < columns * a.d; k += NT) {
+      const int col = k / a.d, d = k - col * a.d;
+      float v = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) v += wm[w][col] * reinterpret_cast<const float *>(lds[w])[col * OPITCH + d];
+      const int q_at = (w0 + col) / a.group, h_at = kv * a.group + (w0 + col - q_at * a.group);
+      const int64_t at = (s.q0 + q_at) * a.heads + h_at;
+      const float sum = total_l[col];
+      if constexpr (DIRECT) o[at * a.d + d] = from_float<T>(sum == 0.f ? 0.f : v / sum);
+      else a.partial[(f.nth * a.s.rows * a.heads + at) * a.d + d] = v;
+    }
+    if constexpr (!DIRECT)
+      if (static_cast<int>(threadIdx.x) < columns) {
+        const int q_at = (w0 + lane) / a.group, h_at = kv * a.group + (w0 + lane - q_at * a.group);
+        float *to = a.partial_stats + (f.nth * a.s.rows * a.heads + (s.q0 + q_at) * a.heads + h_at) * 2;
+        to[0] = top[lane] == -__builtin_inff() ? top[lane] : top[lane] * a.scale2;
+        to[1] = total_l[lane];
+      }
+    __syncthreads();  // (the next columns' tiles take the sums' place)
+  }
+}
+
+// The parts of a row joined: a wave to a row of one head.
+template <class T> __global__ __launch_bounds__(256) void join_kernel(const Args a) {
+  const int lane = lane_id();
+  const int64_t at = blockIdx.x * static_cast<int64_t>(4) + (threadIdx.x >> 6), all = a.s.rows * a.heads;
+  if (at >= all) return;
+  const int64_t row = at / a.heads;
+  int parts = 0;
+  for (int first = 0; first < a.s.count; first += 64) {
+    const int b = first + lane;
+    const bool mine = b < a.s.count && row >= a.s.offsets[b] && row < a.s.offsets[b + 1];
+    const uint64_t found = ballot(mine);
+    if (found) {
+      parts = (keys_of(a.s, first + __builtin_ctzll(found)) + a.part_keys - 1) / a.part_keys;
+      break;
+    }
+  }
+  float m = -__builtin_inff(), l = 0;
+  for (int p = lane; p < parts; p += 64) {
+    const float *from = a.partial_stats + (p * all + at) * 2;
+    const float pm = from[0], higher = __builtin_fmaxf(m, pm);
+    l = (m == higher ? l : l * __builtin_amdgcn_exp2f(m - higher)) +
+        (pm == higher ? from[1] : from[1] * __builtin_amdgcn_exp2f(pm - higher));
+    m = higher;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float om = __shfl_xor(m, o, 64), ol = __shfl_xor(l, o, 64), higher = __builtin_fmaxf(m, om);
+    l = (m == higher ? l : l * __builtin_amdgcn_exp2f(m - higher)) +
+        (om == higher ? ol : ol * __builtin_amdgcn_exp2f(om - higher));
+    m = higher;
+  }
+  float v[kMostHeadDim / 64] = {};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float pm = a.partial_stats[(p * all + at) * 2];
+    const float by = pm == m ? 1.f : __builtin_amdgcn_exp2f(pm - m);
+#pragma unroll
+    for (int i = 0; i < kMostHeadDim / 64; ++i) {
+      const int d = i * 64 + lane;
+      if (d < a.d) v[i] += by * a.partial[(p * all + at) * a.d + d];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kMostHeadDim / 64; ++i) {
+    const int d = i * 64 + lane;
+    if (d < a.d) static_cast<T *>(a.o)[at * a.d + d] = from_float<T>(l == 0.f ? 0.f : v[i] / l);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+static int check(const spira_hip_attention_t &x) {
+  SPIRA_HIP_REQUIRE(x.rows >= 0 && x.rows < (int64_t(1) << 31) && x.keys >= 0 && x.keys < (int64_t(1) << 31),
+                    "attention: bad number of rows");
+  SPIRA_HIP_REQUIRE(x.sequences > 0 && x.sequences <= (1 << 24), "attention: needs 1 to 2^24 sequences");
+  SPIRA_HIP_REQUIRE(x.heads > 0 && x.kv_heads > 0 && x.heads <= 65536 && x.heads % x.kv_heads == 0,
+                    "attention: the number of query heads must be a multiple of the key heads'");
+  SPIRA_HIP_REQUIRE(x.head_dim > 0 && x.head_dim <= kMostHeadDim, "attention: needs heads of 1 to 128 values");
+  SPIRA_HIP_REQUIRE(x.rows * (x.heads / x.kv_heads) < (int64_t(1) << 31) - kColumns, "attention: too many queries");
+  SPIRA_HIP_REQUIRE(x.scale > 0 && x.scale < __builtin_inff(), "attention: the scale must be positive and finite");
+  SPIRA_HIP_REQUIRE(x.offsets && x.key_offsets, "attention: null offsets");
+  SPIRA_HIP_REQUIRE((x.rows == 0 || x.queries) && (x.keys == 0 || (x.key && x.value)), "attention: null features");
+  return kOk;
+}
+
+int arguments(const spira_hip_attention_t &x, Args &a, int size) {
+  if (int rc = check(x)) return rc;
+  a = Args{};
+  a.s = {x.offsets, x.key_offsets, x.key_counts, x.sequences, x.rows, x.keys};
+  a.heads = x.heads;
+  a.kv_heads = x.kv_heads;
+  a.group = x.heads / x.kv_heads;
+  a.d = x.head_dim;
+  a.causal = x.causal;
+  a.scale = x.scale;
+  a.scale2 = static_cast<float>(static_cast<double>(x.scale) * 1.4426950408889634);
+  a.q = x.queries; a.q_row = x.query_row; a.q_head = x.query_head;
+  a.k = x.key; a.k_row = x.key_row; a.k_head = x.key_head;
+  a.v = x.value; a.v_row = x.value_row; a.v_head = x.value_head;
+  // (bit 0: keys and values, bit 2: queries)
+  a.dma = (dma_rows(x.key, x.key_row, x.key_head, x.head_dim, size, 64) &&
+                   dma_rows(x.value, x.value_row, x.value_head, x.head_dim, size, 64)
+               ? 1
+               : 0) |
+          (dma_rows(x.queries, x.query_row, x.query_head, x.head_dim, size, 64) ? 4 : 0);
+  return kOk;
+}
+
+// The form and, for few tokens, its parts.
+struct Plan {
+  bool tokens;
+  int part_keys;
+  int64_t parts;  // most of a sequence
+};
+static Plan plan(const spira_hip_attention_t &x) {
+  const int64_t group = x.heads / x.kv_heads, columns = div_up(x.rows * group, x.sequences);
+  if (columns > 64) return {false, 0, 0};
+  const int64_t tiles = div_up(columns, 32);
+  const int64_t size = round_up(std::max<int64_t>(div_up(x.keys * x.kv_heads * tiles, 1024), 256), 128);
+  // (partial sums of at most 256 MB)
+  int64_t part = size;
+  while (x.rows * x.heads * div_up(x.keys, part) * (x.head_dim + 2) * 4 > (int64_t(1) << 28) && part < x.keys)
+    part *= 2;
+  return {true, static_cast<int>(std::min<int64_t>(part, int64_t(1) << 30)), div_up(x.keys, part)};
+}
+
+static size_t partial_bytes(const spira_hip_attention_t &x, const Plan &p) {
+  return p.tokens && p.parts > 1 ? static_cast<size_t>(p.parts) * x.rows * x.heads * (x.head_dim + 2) * sizeof(float) : 0;
+}
+
+template <class T, int DP> static int launch(const Args &base, const Plan &p, hipStream_t stream) {
+  Args a = base;
+  if (!p.tokens) {
+    const int64_t blocks = (a.s.rows * a.group / kColumns + a.s.count) * a.kv_heads;
+    SPIRA_HIP_REQUIRE(launchable(blocks, 256), "attention: too many tiles for a launch");
+    hipLaunchKernelGGL((prompt_kernel<T, DP>), dim3(blocks), dim3(256), 0, stream, a);
+    SPIRA_HIP_LAUNCH_CHECK();
+    return kOk;
+  }
+  a.part_keys = p.part_keys;
+  constexpr int threads = 64 * kTokenWaves<T, DP>;
+  const bool direct = p.parts <= 1;
+  const int64_t blocks = (direct ? a.s.count : a.s.keys / p.part_keys + a.s.count) * a.kv_heads;
+  const uint32_t y = static_cast<uint32_t>(div_up(div_up(a.s.rows * a.group, a.s.count), 32));
+  SPIRA_HIP_REQUIRE(launchable(blocks * y, threads), "attention: too many tiles for a launch");
+  if (direct)
+    hipLaunchKernelGGL((token_kernel<T, DP, true>), dim3(blocks, y), dim3(threads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((token_kernel<T, DP, false>), dim3(blocks, y), dim3(threads), 0, stream, a);
+  SPIRA_HIP_LAUNCH_CHECK();
+  if (direct) return kOk;
+  const int64_t joins = div_up(a.s.rows * a.heads, 4);
+  SPIRA_HIP_REQUIRE(launchable(joins, 256), "attention: too many rows for a launch");
+  hipLaunchKernelGGL(join_kernel<T>, dim3(joins), dim3(256), 0, stream, a);
+  SPIRA_HIP_LAUNCH_CHECK();
+  return kOk;
+}
+
+}  // namespace attention
+
+}  // namespace spira_hip
+
+using namespace spira_hip;
+
+extern "C" {
+
+int spira_hip_attention_workspace(const spira_hip_attention_t *x, int gradient, size_t *bytes) {
+  SPIRA_HIP_REQUIRE(x && bytes, "attention: null arguments");
+  if (int rc = attention::check(*x)) return rc;
+  *bytes = gradient ? static_cast<size_t>(x->rows) * x->heads * sizeof(float)
+                    : attention::partial_bytes(*x, attention::plan(*x));
+  return kOk;
+}
+
+int spira_hip_attention(const spira_hip_attention_t *x, void *out, float *stats, void *workspace,
+                        size_t workspace_bytes, hipStream_t stream) {
+  SPIRA_HIP_REQUIRE(x, "attention: null arguments");
+  attention::Args a;
+  if (int rc = attention::arguments(*x, a, x->dtype == SPIRA_F32 ? 4 : 2)) return rc;
+  if (x->rows == 0) return kOk;
+  SPIRA_HIP_REQUIRE(out, "attention: null output");
+  // (a gradient's statistics come from the prompts' form)
+  const attention::Plan p = stats ? attention::Plan{false, 0, 0} : attention::plan(*x);
+  const size_t need = attention::partial_bytes(*x, p);
+  SPIRA_HIP_REQUIRE(workspace_bytes >= need && (workspace || need == 0), "attention: workspace too small");
+  a.o = out;
+  a.stats = stats;
+  a.partial = static_cast<float *>(workspace);
+  a.partial_stats = a.partial ? a.partial + p.parts * x->rows * x->heads * x->head_dim : nullptr;
+  return with_type(x->dtype, [&](auto t) -> int {
+    return attention::with_width(x->head_dim, [&](auto W) -> int {
+      return attention::launch<decltype(t), decltype(W)::value>(a, p, stream);
+    });
+  });
+}
+
+}  // extern "C"

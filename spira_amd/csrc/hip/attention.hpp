@@ -1,0 +1,374 @@
+// What the attention kernels share: packed sequences and their tiles, tiles of
+// rows in LDS, fragments of the 32 x 32 matrix instructions.
+//
+// All products put the rows that a tile holds (keys; in the keys' gradient,
+// queries) first and the columns that a wave owns (queries; keys) second, so that
+// a lane's sums belong to one column, that of lane % 32:
+//
+//   scores  S^T = K Q^T        (a lane: 16 of 32 keys, the lane 32 on the others)
+//   output  O^T += V^T P^T     (P^T: the scores' registers as they are)
+//
+// Statistics of a column need no broadcast, and P goes from the first product's
+// sums to the second's operand without a move: in the sums, register r of half h =
+// lane / 32 is row 8 (r / 4) + 4 h + r % 4, so a step of 16 rows takes registers 8
+// s to 8 s + 7, and the other operand's fragment takes rows 4 h + {0..3} and 8 + 4
+// h + {0..3}, which two transposing LDS reads give (ds_read_b64_tr_b16).
+#pragma once
+
+#include "tiles.hpp"
+
+namespace spira_hip {
+
+namespace attention {
+
+using namespace tiles;
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.44269504f;
+constexpr int kMostHeadDim = 128;
+
+// ---------------------------------------------------------------------------
+// sequences
+// ---------------------------------------------------------------------------
+// Sequence b has the queries offsets[b] to offsets[b + 1] and the first
+// key_counts[b] (or all) of the keys key_offsets[b] to key_offsets[b + 1].
+struct Sequences {
+  const int32_t *offsets, *key_offsets, *key_counts;
+  int count;
+  int64_t rows, keys;
+};
+struct Sequence {
+  int64_t q0, k0;  // first query and key
+  int nq, nk;
+  int room;  // keys and the room behind them
+};
+
+// (whatever the numbers are, no row outside the tensors)
+__device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t most) { return v < 0 ? 0 : v > most ? most : v; }
+__device__ __forceinline__ int queries_of(const Sequences &s, int b) {
+  const int64_t lo = clamp_row(s.offsets[b], s.rows), hi = clamp_row(s.offsets[b + 1], s.rows);
+  return hi > lo ? static_cast<int>(hi - lo) : 0;
+}
+__device__ __forceinline__ int room_of(const Sequences &s, int b) {
+  const int64_t lo = clamp_row(s.key_offsets[b], s.keys), hi = clamp_row(s.key_offsets[b + 1], s.keys);
+  return hi > lo ? static_cast<int>(hi - lo) : 0;
+}
+__device__ __forceinline__ int keys_of(const Sequences &s, int b) {
+  const int room = room_of(s, b);
+  if (!s.key_counts) return room;
+  const int n = s.key_counts[b];
+  return n < 0 ? 0 : n < room ? n : room;
+}
+__device__ __forceinline__ Sequence sequence_at(const Sequences &s, int b) {
+  return {uniform(clamp_row(s.offsets[b], s.rows)), uniform(clamp_row(s.key_offsets[b], s.keys)),
+          uniform(queries_of(s, b)), uniform(keys_of(s, b)), uniform(room_of(s, b))};
+}
+
+struct Found {
+  int sequence;  // -1: past the last
+  int nth, of;   // the piece within its sequence, and their number
+};
+// Piece `index` of the sequences cut into pieces(b) each, the same on every lane.
+template <class Pieces> __device__ __forceinline__ Found find_piece(int count, int64_t index, Pieces &&pieces) {
+  const int lane = lane_id();
+  int64_t before = 0;
+  for (int first = 0; first < count; first += 64) {
+    const int b = first + lane, n = b < count ? pieces(b) : 0;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int u = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += u;
+    }
+    const uint64_t past = ballot(before + upto > index);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int of = __shfl(n, at, 64);
+      return {uniform(first + at), uniform(static_cast<int>(index - before - (__shfl(upto, at, 64) - of))), uniform(of)};
+    }
+    before += __shfl(upto, 63, 64);
+  }
+  return {-1, 0, 0};
+}
+
+// zeros in the rows (of `width` values) that no sequence covers, by the launch's
+// blocks together
+template <class T>
+__device__ void clear_uncovered(const int32_t *offsets, int count, int64_t rows, T *y, int64_t width, int64_t block,
+                                int64_t blocks) {
+  const int64_t lo = clamp_row(offsets[0], rows), last = clamp_row(offsets[count], rows), hi = last > lo ? last : lo;
+  const int64_t chunks = (width + kVec<T> - 1) / kVec<T>, open = lo + rows - hi;
+  for (int64_t i = block * blockDim.x + threadIdx.x; i < open * chunks; i += blocks * blockDim.x) {
+    const int64_t k = i / chunks, r = k < lo ? k : hi + k - lo, at = (i - k * chunks) * kVec<T>;
+    store_chunk(y + r * width + at, width - at, Chunk<T>{});
+  }
+}
+
+// ---------------------------------------------------------------------------
+// tiles of rows in LDS
+// ---------------------------------------------------------------------------
+// Rows of DP values (the head's, rounded up to 32) at a pitch of a power of two.
+// The 16-byte chunk c of row r lies at slot c ^ swizzle(r): 16 consecutive rows'
+// chunk c, and four consecutive rows' 64 bytes, each meet all banks once.
+template <class T, int DP> struct Rows {
+  static constexpr int SIZE = static_cast<int>(sizeof(T));
+  static constexpr int PITCH = (DP == 96 ? 128 : DP) * SIZE;  // bytes
+  static constexpr int CPR = PITCH / 16;                      // chunks a row
+  static constexpr int STEPS = DP / 16, TILES = DP / 32;
+  __device__ static __forceinline__ int swizzle(int r) {
+    if constexpr (PITCH == 64) return (r >> 2) & 3;
+    else if constexpr (PITCH == 128) return ((r & 2) << 1) | ((r >> 2) & 3);
+    else return ((r & 3) << 2) | ((r >> 2) & 3);
+  }
+  __device__ static __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ swizzle(r)) << 4); }
+};
+
+// eight values of the summed index
+template <class T> struct Frag {
+  uintx4_t v[sizeof(T) / 2];
+};
+
+template <class T> __device__ __forceinline__ void mma(floatx16 &d, const Frag<T> &a, const Frag<T> &b) {
+  if constexpr (std::is_same_v<T, _Float16>) {
+    d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a.v[0]), __builtin_bit_cast(half8, b.v[0]), d,
+                                               0, 0, 0);
+  } else if constexpr (std::is_same_v<T, __bf16>) {
+    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a.v[0]), __builtin_bit_cast(bf8, b.v[0]), d, 0,
+                                                0, 0);
+  } else {
+    // (element i of both halves' eight: the summed index in another order, the same
+    // for both operands)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const floatx4_t x = __builtin_bit_cast(floatx4_t, a.v[i]), y = __builtin_bit_cast(floatx4_t, b.v[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], d, 0, 0, 0);
+    }
+  }
+}
+
+// Registers 8 s to 8 s + 7 of sums as an operand.  For 16 bits each is rounded to
+// the inputs' type, as the matrix instructions take it: half a step of a term of
+// the sum that follows, which itself is rounded to that type once.
+template <class T> __device__ __forceinline__ Frag<T> as_operand(const floatx16 &p, int s) {
+  Frag<T> f;
+  if constexpr (sizeof(T) == 2) {
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = from_float<T>(p[8 * s + i]);
+    __builtin_memcpy(&f, t, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      f.v[i] = __builtin_bit_cast(uintx4_t, floatx4_t{p[8 * s + 4 * i], p[8 * s + 4 * i + 1], p[8 * s + 4 * i + 2],
+                                                      p[8 * s + 4 * i + 3]});
+  }
+  return f;
+}
+
+// rows r0 to r0 + 31 as the first operand of step st of 16 values
+template <class T, int DP> __device__ __forceinline__ Frag<T> row_frag(lds_char *tile, int r0, int st) {
+  const int lane = lane_id(), r = r0 + (lane & 31), h = lane >> 5;
+  Frag<T> f;
+#pragma unroll
+  for (int i = 0; i < Rows<T, DP>::SIZE / 2; ++i)
+    f.v[i] = *(lds_chunk *)(tile + Rows<T, DP>::at(r, (st * 2 + h) * (Rows<T, DP>::SIZE / 2) + i));
+  return f;
+}
+// values 32 n to 32 n + 31 as the first operand, summed over rows r0 to r0 + 15
+template <class T, int DP> __device__ __forceinline__ Frag<T> col_frag(lds_char *tile, int r0, int n) {
+  using R = Rows<T, DP>;
+  const int lane = lane_id(), h = lane >> 5;
+  Frag<T> f;
+  if constexpr (sizeof(T) == 2) {
+    const int i = lane & 15, r = r0 + 4 * h + (i >> 2), c = n * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+    const auto lo = read_tr(tile + R::at(r, c) + (i & 1) * 8), hi = read_tr(tile + R::at(r + 8, c) + (i & 1) * 8);
+    const uintx2_t a = __builtin_bit_cast(uintx2_t, lo), b = __builtin_bit_cast(uintx2_t, hi);
+    f.v[0] = {a[0], a[1], b[0], b[1]};
+  } else {
+    const int d = n * 32 + (lane & 31);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      f.v[i / 4][i % 4] =
+          *(lds_word *)(tile + R::at(r0 + (i / 4) * 8 + 4 * h + i % 4, d >> 2) + (d & 3) * 4);
+  }
+  return f;
+}
+// a column's row of memory as the second operand of step st, zeros past d and
+// without a row
+template <class T> __device__ __forceinline__ Frag<T> load_frag(const T *row, int d, int st) {
+  Frag<T> f;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+    const int at = st * 16 + (lane_id() >> 5) * 8 + i * kVec<T>;
+    f.v[i] = load_raw(row + at, row ? d - at : 0);
+  }
+  return f;
+}
+
+// A tile of R rows from memory to LDS by NT threads (of which this is `thread`):
+// rows [0, n) of `stride` bytes, zeros behind them and behind a row's d values.
+// DMA (rows, strides and addresses of whole 16-byte chunks: `dma`): under way on
+// return, a load of 1 KB per wave and instruction; chunks outside are out of the
+// buffer's range.  Else through registers, written on return.
+template <class T, int DP, int R, int NT>
+__device__ __forceinline__ void fetch_tile(const char *rows, int64_t stride, int64_t n, int d, bool dma, lds_char *tile,
+                                           int thread) {
+  using S = Rows<T, DP>;
+  constexpr int LOADS = R * S::CPR / NT;
+  static_assert(LOADS >= 1 && LOADS * NT == R * S::CPR, "tile shape");
+  const int dbytes = d * S::SIZE;
+  n = n < 0 ? 0 : n > R ? R : n;
+  if (dma) {
+    const uintx4_t from = buffer(rows, n > 0 ? (n - 1) * stride + dbytes : 0);
+    lds_char *to = tile + (thread & ~63) * 16;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int id = i * NT + thread, r = id / S::CPR, c = (id % S::CPR) ^ S::swizzle(r);
+      const uint32_t offset = static_cast<uint32_t>(r) * static_cast<uint32_t>(stride) + c * 16;
+      load_lds(from, c * 16 < dbytes ? offset : kOutOfRange, (lds_void *)(to + i * NT * 16));
+    }
+  } else {
+    uintx4_t v[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int id = i * NT + thread, r = id / S::CPR, c = (id % S::CPR) ^ S::swizzle(r);
+      v[i] = load_raw(reinterpret_cast<const T *>(rows + r * stride) + c * kVec<T>, r < n ? d - c * kVec<T> : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) *(lds_chunk *)(tile + (i * NT + thread) * 16) = v[i];
+  }
+}
+
+// the larger (or the sum) of the two halves' values of a column
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// ---------------------------------------------------------------------------
+// infinities and NaN where the mask hides them
+// ---------------------------------------------------------------------------
+// A hidden row's weight is 0, and 0 times an infinity or NaN is NaN: where some
+// columns see a row and others do not, such values are taken out of the tile before
+// its product and added to the columns that see them, from memory.
+
+// Zeros for what is not finite in a tile's R rows, by NT threads; whether this one
+// found any.
+template <class T, int DP, int R, int NT> __device__ __forceinline__ bool clear_not_finite(lds_char *tile, int thread) {
+  constexpr uint32_t E = sizeof(T) == 4 ? 0x7F800000u : std::is_same_v<T, _Float16> ? 0x7C00u : 0x7F80u;
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < R * Rows<T, DP>::CPR / NT; ++i) {
+    lds_chunk *at = (lds_chunk *)(tile + (i * NT + thread) * 16);
+    uintx4_t v = *at;
+    bool here = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if ((v[j] & E) == E) {
+        v[j] &= sizeof(T) == 4 ? 0u : 0xFFFF0000u;
+        here = true;
+      }
+      if (sizeof(T) == 2 && ((v[j] >> 16) & E) == E) {
+        v[j] &= 0xFFFFu;
+        here = true;
+      }
+    }
+    if (here) *at = v;
+    found |= here;
+  }
+  return found;
+}
+
+// acc += what is not finite in n rows of memory, for the columns that see the row
+// (sees(i): whether this lane's does)
+template <class T, int DP, class Sees>
+__device__ __forceinline__ void add_not_finite(floatx16 (&acc)[DP / 32], const char *rows, int64_t stride, int n, int d,
+                                               Sees &&sees) {
+  const int h = lane_id() >> 5;
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    const T *row = reinterpret_cast<const T *>(rows + i * stride) + 4 * h;
+    const bool seen = sees(i);
+#pragma unroll
+    for (int m = 0; m < DP / 32; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at = 32 * m + 8 * (r / 4) + r % 4;
+        const float v = at + 4 * h < d ? to_float(row[at]) : 0.f;
+        if (seen && !(__builtin_fabsf(v) < __builtin_inff())) acc[m][r] += v;
+        if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (few registers: it is a rare path)
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// columns to memory
+// ---------------------------------------------------------------------------
+// A column's sums times `by` to its row of d values.  The halves exchange groups of
+// four values, so that each lane writes eight consecutive ones.  Every lane takes
+// part; `there`: its column is to be written.
+template <class T, int DP>
+__device__ __forceinline__ void store_column(T *row, int d, bool there, const floatx16 (&acc)[DP / 32], float by) {
+  const int h = lane_id() >> 5;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, acc[n][8 * m + i] * by),
+                                                        __builtin_bit_cast(uint32_t, acc[n][8 * m + 4 + i] * by), false,
+                                                        false);
+        v[i] = __builtin_bit_cast(float, static_cast<uint32_t>(s[0]));
+        v[4 + i] = __builtin_bit_cast(float, static_cast<uint32_t>(s[1]));
+      }
+      const int at = 32 * n + 8 * (2 * m + h);
+#pragma unroll
+      for (int c = 0; c < 8 / kVec<T>; ++c) {
+        Chunk<T> k;
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) k.v[i] = v[c * kVec<T> + i];
+        if (there) store_chunk(row + at + c * kVec<T>, d - at - c * kVec<T>, k);
+      }
+    }
+}
+
+// whether tiles of such rows can be fetched by DMA
+inline bool dma_rows(const void *p, int64_t row, int64_t head, int d, int size, int64_t tile_rows) {
+  const auto whole = [&](int64_t values) { return values * size % 16 == 0; };
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && whole(row) && whole(head) && whole(d) &&
+         row * size * tile_rows < kBufferLimit / 2;
+}
+
+// f of the head's padded width
+template <class F> int with_width(int d, F &&f) {
+  using std::integral_constant;
+  if (d <= 32) return f(integral_constant<int, 32>{});
+  if (d <= 64) return f(integral_constant<int, 64>{});
+  if (d <= 96) return f(integral_constant<int, 96>{});
+  return f(integral_constant<int, 128>{});
+}
+
+// Strides in values.
+struct Args {
+  Sequences s;
+  int heads, kv_heads, group, d, causal, dma;
+  float scale;   // of the scores
+  float scale2;  // scale log2 e
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  void *o;       // [rows, heads, d]
+  float *stats;  // [heads, rows] log2 of the sum of exp2 of a row's scaled scores; fp32: [2, heads, rows], their
+                 // largest and the inverse of the sum beside it
+  // few tokens
+  float *partial, *partial_stats;
+  int part_keys;  // keys a part
+  // backward
+  const void *dout, *out;
+  float *delta;  // [heads, rows]
+  void *dq, *dk, *dv;
+};
+
+}  // namespace attention
+
+}  // namespace spira_hip

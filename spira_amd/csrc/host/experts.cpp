@@ -2,58 +2,9 @@
 // its experts' rows, the gated residual norm and dropout, forward and gradients
 // (no counterparts in the reference).  Outputs and workspaces come from the
 // caching allocator on the current stream; nothing is read back on the host.
-#include "host_common.h"
-
-#include <c10/core/AutogradState.h>
-#include <c10/core/DeviceGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include "rows.h"
 
 namespace spira_host {
-
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-using Tensor = torch::Tensor;
-using OptTensor = std::optional<torch::Tensor>;
-
-static int row_dtype(const Tensor &t) {
-  switch (t.scalar_type()) {
-    case torch::kHalf: return SPIRA_F16;
-    case torch::kBFloat16: return SPIRA_BF16;
-    case torch::kFloat: return SPIRA_F32;
-    default: fail("Cannot find implementation for feature dtype ", t.scalar_type());
-  }
-}
-
-static const void *ptr(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
-
-// t is a contiguous tensor of this type, on x's device, of these sizes (-1: any)
-static void require(const Tensor &t, const char *name, const Tensor &x, torch::ScalarType type,
-                    std::initializer_list<int64_t> sizes) {
-  require_device(t, name);
-  SPIRA_CHECK_ARG(t.device() == x.device(), name, " must be on ", x.device());
-  SPIRA_CHECK_ARG(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
-  bool fits = t.dim() == static_cast<int64_t>(sizes.size());
-  int64_t d = 0;
-  for (int64_t s : sizes) {
-    if (fits && s >= 0 && t.size(d) != s) fits = false;
-    ++d;
-  }
-  if (!fits) {
-    std::ostringstream os;
-    for (int64_t s : sizes) os << (os.tellp() > 0 ? ", " : "") << (s < 0 ? std::string("any") : std::to_string(s));
-    fail(name, " must have the shape [", os.str(), "], got ", t.sizes());
-  }
-}
-static void require(const OptTensor &t, const char *name, const Tensor &x, torch::ScalarType type,
-                    std::initializer_list<int64_t> sizes) {
-  if (t) require(*t, name, x, type, sizes);
-}
-
-static Tensor like(const Tensor &x, torch::IntArrayRef sizes) { return torch::empty(sizes, x.options()); }
-static Tensor floats(const Tensor &x, torch::IntArrayRef sizes) {
-  return torch::empty(sizes, x.options().dtype(torch::kFloat));
-}
 
 struct Linear {
   int64_t rows, groups, ci, co;
@@ -315,47 +266,43 @@ static Tensor dropout(const Tensor &x, double p, uint64_t seed, uint64_t offset,
   return y;
 }
 
+// (loss, counts, mean probabilities, what the gradient needs)
+static std::tuple<Tensor, Tensor, Tensor, Tensor> balance(const Tensor &logits, const Tensor &offsets) {
+  require(logits, "logits", logits, logits.scalar_type(), {-1, -1});
+  const int dtype = row_dtype(logits);
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  SPIRA_CHECK_ARG(experts > 0 && experts <= 512, "balance_loss: needs 1 to 512 experts, got ", experts);
+  require(offsets, "offsets", logits, torch::kInt, {experts + 1});
+  const c10::DeviceGuard guard(logits.device());
+  size_t bytes = 0;
+  check_rc(spira_hip_balance_workspace(tokens, experts, &bytes), "balance_loss");
+  Tensor loss = floats(logits, {}), counts = empty_i32({experts}, logits.device()), mean = floats(logits, {experts});
+  Tensor kept = floats(logits, {experts + 1}), ws = workspace(bytes, logits.device());
+  check_rc(spira_hip_balance(logits.data_ptr(), tokens, experts, dtype, offsets.data_ptr<int32_t>(),
+                             loss.data_ptr<float>(), counts.data_ptr<int32_t>(), mean.data_ptr<float>(),
+                             kept.data_ptr<float>(), ws.data_ptr(), bytes, current_stream()),
+           "balance_loss");
+  return {loss, counts, mean, kept};
+}
+
+static Tensor balance_backward(const Tensor &logits, const Tensor &kept, const Tensor &dloss) {
+  require(logits, "logits", logits, logits.scalar_type(), {-1, -1});
+  require(kept, "sums", logits, torch::kFloat, {logits.size(1) + 1});
+  require(dloss, "gradient", logits, torch::kFloat, {});
+  const c10::DeviceGuard guard(logits.device());
+  Tensor d = like(logits, logits.sizes());
+  check_rc(spira_hip_balance_backward(logits.data_ptr(), logits.size(0), logits.size(1), row_dtype(logits),
+                                      kept.data_ptr<float>(), dloss.data_ptr<float>(), d.data_ptr(), current_stream()),
+           "balance_loss");
+  return d;
+}
+
 // ---------------------------------------------------------------------------
 // Gradients.  The functions above take contiguous tensors and know nothing of
 // autograd; those below are what Python calls.  (In C++: with Python's autograd
 // functions a training step of a small operator was bound by the host, 104 us
 // where its kernels take 23.)
 // ---------------------------------------------------------------------------
-static Tensor dense(const Tensor &t) { return t.contiguous(); }
-static OptTensor dense(const OptTensor &t) { return t ? OptTensor(t->contiguous()) : t; }
-
-// Whether the call needs a node in the graph.  A tangent of forward mode would be
-// lost without a word, here and within a node, and read as zero: it is refused.
-static bool tracked(const char *name, std::initializer_list<const OptTensor *> ts) {
-  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
-    for (const OptTensor *t : ts)
-      SPIRA_CHECK_ARG(!*t || !(*t)->_fw_grad(0).defined(), name, ": there are no derivatives of forward mode");
-  if (!torch::GradMode::is_enabled()) return false;
-  for (const OptTensor *t : ts)
-    if (*t && (*t)->requires_grad()) return true;
-  return false;
-}
-static bool wants(const OptTensor &t) { return t && t->requires_grad(); }
-
-static Tensor given(const OptTensor &t) { return t ? *t : Tensor(); }
-static OptTensor maybe(const Tensor &t) { return t.defined() ? OptTensor(t) : std::nullopt; }
-
-// Gradients are of first order: with a graph of them asked for, they carry a
-// node that fails when it is differentiated.
-static variable_list once(variable_list grads, const char *name) {
-  if (!torch::GradMode::is_enabled()) return grads;
-  variable_list some;
-  for (const Tensor &g : grads)
-    if (g.defined()) some.push_back(g.detach().requires_grad_(true));
-  auto error = std::make_shared<torch::autograd::DelayedError>(
-      std::string("[Spira] ") + name + ": gradients are of first order", static_cast<int64_t>(some.size()));
-  some = (*error)(std::move(some));
-  size_t i = 0;
-  for (Tensor &g : grads)
-    if (g.defined()) g = some[i++];
-  return grads;
-}
-
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const OptTensor &bias,
                         const Tensor &offsets, const OptTensor &rows, const OptTensor &slots, bool relu) {
@@ -512,12 +459,38 @@ static Tensor dropout_call(const Tensor &x, double p, uint64_t seed, uint64_t of
   return dropout(dense(x), p, seed, offset, dense(residual));
 }
 
+struct BalanceFunction : torch::autograd::Function<BalanceFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &offsets) {
+    auto [loss, counts, mean, kept] = balance(logits, offsets);
+    ctx->save_for_backward({logits, kept});
+    ctx->mark_non_differentiable({counts, mean});
+    ctx->set_materialize_grads(false);
+    return {loss, counts, mean};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list d) {
+    const variable_list v = ctx->get_saved_variables();
+    if (!d[0].defined()) return {Tensor(), Tensor()};
+    return once({balance_backward(v[0], v[1], dense(d[0])), Tensor()}, "balance_loss");
+  }
+};
+
+static std::tuple<Tensor, Tensor, Tensor> balance_call(const Tensor &logits, const Tensor &offsets) {
+  const OptTensor l = logits;
+  if (!tracked("balance_loss", {&l})) {
+    auto out = balance(dense(logits), dense(offsets));
+    return {std::get<0>(out), std::get<1>(out), std::get<2>(out)};
+  }
+  const variable_list v = BalanceFunction::apply(dense(logits), dense(offsets));
+  return {v[0], v[1], v[2]};
+}
+
 void register_experts(pybind11::module_ &m) {
   m.def("grouped_linear", &grouped_linear_call);
   m.def("route_experts", &route_call);
   m.def("combine_experts", &combine_call);
   m.def("gated_residual_norm", &norm_call);
   m.def("dropout", &dropout_call);
+  m.def("balance_loss", &balance_call);
 }
 
 }  // namespace spira_host

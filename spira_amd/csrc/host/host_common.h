@@ -130,5 +130,6 @@ void register_coords(pybind11::module_ &m);
 void register_mapping(pybind11::module_ &m);
 void register_conv(pybind11::module_ &m);
 void register_experts(pybind11::module_ &m);
+void register_attention(pybind11::module_ &m);
 
 }  // namespace spira_host

@@ -9,4 +9,5 @@ PYBIND11_MODULE(_C, m) {
   spira_host::register_mapping(m);
   spira_host::register_conv(m);
   spira_host::register_experts(m);
+  spira_host::register_attention(m);
 }

@@ -21,7 +21,7 @@ from ._native import _C
 from .convolution import _gpu
 
 __all__ = ["ExpertRoutes", "route_experts", "grouped_linear", "combine_experts", "gated_residual_norm", "rms_norm",
-           "dropout"]
+           "dropout", "BalanceLoss", "balance_loss"]
 
 
 _LOW = (1 << 64) - 1
@@ -53,6 +53,26 @@ def route_experts(logits: torch.Tensor, k: int, *, renormalize: bool = True) -> 
     """
     _gpu(logits)
     return ExpertRoutes(*_C.route_experts(logits, k, renormalize))
+
+
+class BalanceLoss(NamedTuple):
+    """What a router's choices over T tokens say of its E experts' use."""
+    loss: torch.Tensor           # [] fp32, differentiable: 1 where all are used alike, up to E
+    counts: torch.Tensor         # [E] int32: assignments to each expert
+    probabilities: torch.Tensor  # [E] fp32: mean of the router's softmax over the tokens
+
+
+def balance_loss(logits: torch.Tensor, groups: Union[torch.Tensor, ExpertRoutes]) -> BalanceLoss:
+    """``E * sum_e share[e] * probabilities[e]``: the loss that keeps a router's
+    experts in use.
+
+    ``logits`` [T, E] are the router's, ``groups`` its ``ExpertRoutes`` or their
+    offsets [E + 1] int32.  share[e] is expert e's part of the assignments (it has
+    no gradient), probabilities[e] the mean of softmax(logits)[:, e] over the
+    tokens that have an expert (a logit above -inf).  Up to 512 experts.
+    """
+    _gpu(logits)
+    return BalanceLoss(*_C.balance_loss(logits, groups.offsets if isinstance(groups, ExpertRoutes) else groups))
 
 
 def grouped_linear(features: torch.Tensor, weight: torch.Tensor, groups: Union[torch.Tensor, ExpertRoutes], *,
