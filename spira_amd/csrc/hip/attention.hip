@@ -35,25 +35,24 @@ template <int DP> struct Columns {
   float m, l;
 };
 
-// One tile of KT keys.  limit: how many of them this lane's column sees (any
-// number); whole: every column of the wave sees all.
-template <class T, int DP, int KT>
-__device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[DP / 16], lds_char *kt, lds_char *vt,
-                                            float scale2, int limit, bool whole) {
-  const int h = lane_id() >> 5;
+// One tile of KT keys.  MASKED: this lane's column sees the first `limit` of them (any
+// number); else every column of the wave sees all.
+template <bool MASKED, class T, int DP, int KT>
+__device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[DP / 16], const Reader<T, DP> &read,
+                                            lds_char *kt, lds_char *vt, float scale2, int limit) {
   floatx16 s[KT / 32];
 #pragma unroll
   for (int u = 0; u < KT / 32; ++u) {
     s[u] = floatx16{};
 #pragma unroll
-    for (int st = 0; st < DP / 16; ++st) mma(s[u], row_frag<T, DP>(kt, 32 * u, st), q[st]);
+    for (int st = 0; st < DP / 16; ++st) mma(s[u], read.rows(kt, 32 * u, st), q[st]);
   }
-  if (!whole) {
+  if constexpr (MASKED) {
+    const int mine = limit - 4 * (lane_id() >> 5);
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[u][r] = 32 * u + 8 * (r / 4) + r % 4 < limit - 4 * h ? s[u][r] : -__builtin_inff();
+      for (int r = 0; r < 16; ++r) s[u][r] = 32 * u + 8 * (r / 4) + r % 4 < mine ? s[u][r] : -__builtin_inff();
   }
   float top = s[0][0];
 #pragma unroll
@@ -73,22 +72,22 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
     c.m = m;
   }
   const float base = c.m == -__builtin_inff() ? 0.f : -c.m * scale2;
-  float sum = 0;
 #pragma unroll
-  for (int u = 0; u < KT / 32; ++u)
+  for (int u = 0; u < KT / 32; ++u) {
+    float sum = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale2, base));
       sum += s[u][r];
     }
-  c.l += sum;
-  Frag<T> p[KT / 16];
+    c.l += sum;
 #pragma unroll
-  for (int st = 0; st < KT / 16; ++st) p[st] = as_operand<T>(s[st / 2], st % 2);
+    for (int st = 0; st < 2; ++st) {
+      const Frag<T> p = as_operand<T>(s[u], st);
 #pragma unroll
-  for (int st = 0; st < KT / 16; ++st)
-#pragma unroll
-    for (int n = 0; n < DP / 32; ++n) mma(c.o[n], col_frag<T, DP>(vt, 16 * st, n), p[st]);
+      for (int n = 0; n < DP / 32; ++n) mma(c.o[n], read.cols(vt, 32 * u + 16 * st, n), p);
+    }
+  }
 }
 
 // keys that query i of a sequence sees
@@ -103,7 +102,7 @@ __device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) 
 // ---------------------------------------------------------------------------
 constexpr int kColumns = 128;
 
-template <class T, int DP>
+template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(const Args a) {
   using R = Rows<T, DP>;
   constexpr int KT = kKeys<T>, TILE = KT * R::PITCH;
@@ -122,20 +121,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   const int total = s.nq * a.group, c0 = (f.of - 1 - f.nth) * kColumns, w0 = c0 + wave * 32;
   const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
   const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i);
-  const int least = visible(a, s, std::min(w0, total - 1) / a.group);
   const int most = w0 < total ? visible(a, s, std::min(w0 + 31, total - 1) / a.group) : 0;
   const int fewest = visible(a, s, c0 / a.group), end = visible(a, s, std::min(c0 + kColumns - 1, total - 1) / a.group);
   const int steps = (end + KT - 1) / KT, own = (most + KT - 1) / KT;
   const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
   const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + s.k0 * a.k_row + kv * a.k_head);
   const char *values = reinterpret_cast<const char *>(static_cast<const T *>(a.v) + s.k0 * a.v_row + kv * a.v_head);
-  const auto issue = [&](int t) {
-    lds_char *to = (lds_char *)lds + (t & 1) * 2 * TILE;
-    fetch_tile<T, DP, KT, 256>(keys + t * (KT * kstride), kstride, s.nk - t * KT, a.d, a.dma & 1, to, threadIdx.x);
-    fetch_tile<T, DP, KT, 256>(values + t * (KT * vstride), vstride, s.nk - t * KT, a.d, a.dma & 1, to + TILE,
-                               threadIdx.x);
+  const Fetch<T, DP, KT, 256, DMA> fetch_keys(kstride, a.d, threadIdx.x), fetch_values(vstride, a.d, threadIdx.x);
+  const auto issue = [&](int t, int stage) {
+    lds_char *to = (lds_char *)lds + stage * 2 * TILE;
+    fetch_keys(keys + t * (KT * kstride), s.nk - t * KT, to);
+    fetch_values(values + t * (KT * vstride), s.nk - t * KT, to + TILE);
   };
-  if (steps > 0) issue(0);
+  if (steps > 0) issue(0, 0);
   Frag<T> q[DP / 16];
   {
     const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
@@ -144,16 +142,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   }
   Columns<DP> c{};
   c.m = -__builtin_inff();
-  for (int t = 0; t < steps; ++t) {
+  const Reader<T, DP> read;
+  // tiles that every column sees whole
+  const int whole = std::min(fewest / KT, steps);
+  int t = 0;
+  const auto step = [&](auto STAGE) {
+    constexpr int stage = decltype(STAGE)::value;
     wait_loads_and_meet<0>();
-    if (t + 1 < steps) issue(t + 1);
+    if (t + 1 < steps) issue(t + 1, stage ^ 1);
+    lds_char *kt = (lds_char *)lds + stage * 2 * TILE;
+    attend_tile<false, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, 0);
+  };
+  while (t < whole) {
+    step(std::integral_constant<int, 0>{});
+    if (++t == whole) break;
+    step(std::integral_constant<int, 1>{});
+    ++t;
+  }
+  // the others
+  for (; t < steps; ++t) {
+    wait_loads_and_meet<0>();
+    if (t + 1 < steps) issue(t + 1, (t + 1) & 1);
     lds_char *kt = (lds_char *)lds + (t & 1) * 2 * TILE;
     // (the same for the whole block)
-    const bool hides = a.causal && fewest < (t + 1) * KT;
-    const bool found = hides && __syncthreads_or(clear_not_finite<T, DP, KT, 256>(kt + TILE, threadIdx.x));
+    const bool found = a.causal && __syncthreads_or(clear_not_finite<T, DP, KT, 256>(kt + TILE, threadIdx.x));
     if (t < own) {
       const int mine = limit - t * KT;
-      attend_tile<T, DP, KT>(c, q, kt, kt + TILE, a.scale2, mine, least >= (t + 1) * KT);
+      attend_tile<true, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, mine);
       if (found)
         add_not_finite<T, DP>(c.o, values + t * (KT * vstride), vstride, std::min(s.nk - t * KT, KT), a.d,
                               [&](int x) { return x < mine; });
@@ -180,7 +195,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
 template <class T, int DP> constexpr int kTokenWaves = Rows<T, DP>::PITCH >= 512 ? 2 : 4;
 
 // DIRECT: no sequence has more than one part; the outputs themselves
-template <class T, int DP, bool DIRECT>
+template <class T, int DP, bool DIRECT, bool DMA>
 __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)) void token_kernel(const Args a) {
   using R = Rows<T, DP>;
   constexpr int KT = 32, TILE = KT * R::PITCH, NW = kTokenWaves<T, DP>, NT = 64 * NW;
@@ -209,6 +224,8 @@ __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)
   const char *values =
       reinterpret_cast<const char *>(static_cast<const T *>(a.v) + (s.k0 + first) * a.v_row + kv * a.v_head);
   const int part = std::min(s.nk - first, a.part_keys);
+  const Fetch<T, DP, KT, 64, DMA> fetch_keys(kstride, a.d, lane), fetch_values(vstride, a.d, lane);
+  const Reader<T, DP> read;
   for (int w0 = blockIdx.y * 32; w0 < total; w0 += gridDim.y * 32) {
     const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
     const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i) - first;
@@ -218,8 +235,8 @@ __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)
     const auto issue = [&](int t, int stage) {
       lds_char *to = mine + stage * 2 * TILE;
       const int64_t n = t < steps ? part - t * KT : 0;
-      fetch_tile<T, DP, KT, 64>(keys + t * (KT * kstride), kstride, n, a.d, a.dma & 1, to, lane);
-      fetch_tile<T, DP, KT, 64>(values + t * (KT * vstride), vstride, n, a.d, a.dma & 1, to + TILE, lane);
+      fetch_keys(keys + t * (KT * kstride), n, to);
+      fetch_values(values + t * (KT * vstride), n, to + TILE);
     };
     issue(wave, 0);
     Frag<T> q[DP / 16];
@@ -234,10 +251,13 @@ __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)
       __builtin_amdgcn_s_waitcnt((LOADS & 15) | (7 << 4) | ((LOADS >> 4) << 14));
       asm volatile("" ::: "memory");
       lds_char *kt = mine + stage * 2 * TILE;
-      const bool hides = a.causal && least < (t + 1) * KT;
-      const bool found = hides && ballot(clear_not_finite<T, DP, KT, 64>(kt + TILE, lane)) != 0;
+      if (std::min(least, part) >= (t + 1) * KT) {
+        attend_tile<false, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, 0);
+        continue;
+      }
+      const bool found = a.causal && ballot(clear_not_finite<T, DP, KT, 64>(kt + TILE, lane)) != 0;
       const int seen = std::min(limit, part) - t * KT;
-      attend_tile<T, DP, KT>(c, q, kt, kt + TILE, a.scale2, seen, std::min(least, part) >= (t + 1) * KT);
+      attend_tile<true, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, seen);
       if (found)
         add_not_finite<T, DP>(c.o, values + t * (KT * vstride), vstride, std::min(part - t * KT, KT), a.d,
                               [&](int x) { return x < seen; });
@@ -375,12 +395,9 @@ int arguments(const spira_hip_attention_t &x, Args &a, int size) {
   a.q = x.queries; a.q_row = x.query_row; a.q_head = x.query_head;
   a.k = x.key; a.k_row = x.key_row; a.k_head = x.key_head;
   a.v = x.value; a.v_row = x.value_row; a.v_head = x.value_head;
-  // (bit 0: keys and values, bit 2: queries)
-  a.dma = (dma_rows(x.key, x.key_row, x.key_head, x.head_dim, size, 64) &&
-                   dma_rows(x.value, x.value_row, x.value_head, x.head_dim, size, 64)
-               ? 1
-               : 0) |
-          (dma_rows(x.queries, x.query_row, x.query_head, x.head_dim, size, 64) ? 4 : 0);
+  const auto whole = [&](const void *p, int64_t row, int64_t head) { return dma_rows(p, row, head, x.head_dim, size); };
+  a.dma = (whole(x.key, x.key_row, x.key_head) && whole(x.value, x.value_row, x.value_head) ? kKeysByDma : 0) |
+          (whole(x.queries, x.query_row, x.query_head) ? kQueriesByDma : 0);
   return kOk;
 }
 
@@ -406,12 +423,12 @@ static size_t partial_bytes(const spira_hip_attention_t &x, const Plan &p) {
   return p.tokens && p.parts > 1 ? static_cast<size_t>(p.parts) * x.rows * x.heads * (x.head_dim + 2) * sizeof(float) : 0;
 }
 
-template <class T, int DP> static int launch(const Args &base, const Plan &p, hipStream_t stream) {
+template <class T, int DP, bool DMA> static int launch_form(const Args &base, const Plan &p, hipStream_t stream) {
   Args a = base;
   if (!p.tokens) {
     const int64_t blocks = (a.s.rows * a.group / kColumns + a.s.count) * a.kv_heads;
     SPIRA_HIP_REQUIRE(launchable(blocks, 256), "attention: too many tiles for a launch");
-    hipLaunchKernelGGL((prompt_kernel<T, DP>), dim3(blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((prompt_kernel<T, DP, DMA>), dim3(blocks), dim3(256), 0, stream, a);
     SPIRA_HIP_LAUNCH_CHECK();
     return kOk;
   }
@@ -422,9 +439,9 @@ template <class T, int DP> static int launch(const Args &base, const Plan &p, hi
   const uint32_t y = static_cast<uint32_t>(div_up(div_up(a.s.rows * a.group, a.s.count), 32));
   SPIRA_HIP_REQUIRE(launchable(blocks * y, threads), "attention: too many tiles for a launch");
   if (direct)
-    hipLaunchKernelGGL((token_kernel<T, DP, true>), dim3(blocks, y), dim3(threads), 0, stream, a);
+    hipLaunchKernelGGL((token_kernel<T, DP, true, DMA>), dim3(blocks, y), dim3(threads), 0, stream, a);
   else
-    hipLaunchKernelGGL((token_kernel<T, DP, false>), dim3(blocks, y), dim3(threads), 0, stream, a);
+    hipLaunchKernelGGL((token_kernel<T, DP, false, DMA>), dim3(blocks, y), dim3(threads), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();
   if (direct) return kOk;
   const int64_t joins = div_up(a.s.rows * a.heads, 4);
@@ -432,6 +449,10 @@ template <class T, int DP> static int launch(const Args &base, const Plan &p, hi
   hipLaunchKernelGGL(join_kernel<T>, dim3(joins), dim3(256), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();
   return kOk;
+}
+
+template <class T, int DP> static int launch(const Args &a, const Plan &p, hipStream_t stream) {
+  return a.dma & kKeysByDma ? launch_form<T, DP, true>(a, p, stream) : launch_form<T, DP, false>(a, p, stream);
 }
 
 }  // namespace attention

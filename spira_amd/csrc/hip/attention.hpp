@@ -154,10 +154,14 @@ template <class T> __device__ __forceinline__ void mma(floatx16 &d, const Frag<T
 template <class T> __device__ __forceinline__ Frag<T> as_operand(const floatx16 &p, int s) {
   Frag<T> f;
   if constexpr (sizeof(T) == 2) {
-    T t[8];
+    typedef float float2v __attribute__((ext_vector_type(2)));
+    typedef T pair __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = from_float<T>(p[8 * s + i]);
-    __builtin_memcpy(&f, t, 16);
+    for (int i = 0; i < 4; ++i) {
+      // (two at a time: one instruction)
+      const pair t = __builtin_convertvector((float2v{p[8 * s + 2 * i], p[8 * s + 2 * i + 1]}), pair);
+      f.v[0][i] = __builtin_bit_cast(uint32_t, t);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -167,34 +171,48 @@ template <class T> __device__ __forceinline__ Frag<T> as_operand(const floatx16 
   return f;
 }
 
-// rows r0 to r0 + 31 as the first operand of step st of 16 values
-template <class T, int DP> __device__ __forceinline__ Frag<T> row_frag(lds_char *tile, int r0, int st) {
-  const int lane = lane_id(), r = r0 + (lane & 31), h = lane >> 5;
-  Frag<T> f;
-#pragma unroll
-  for (int i = 0; i < Rows<T, DP>::SIZE / 2; ++i)
-    f.v[i] = *(lds_chunk *)(tile + Rows<T, DP>::at(r, (st * 2 + h) * (Rows<T, DP>::SIZE / 2) + i));
-  return f;
-}
-// values 32 n to 32 n + 31 as the first operand, summed over rows r0 to r0 + 15
-template <class T, int DP> __device__ __forceinline__ Frag<T> col_frag(lds_char *tile, int r0, int n) {
+// Where a lane reads of a tile.  What a fragment's number changes of an address is
+// bits that the swizzle has not moved together: an exclusive or of a constant, and
+// a constant offset.
+template <class T, int DP> struct Reader {
   using R = Rows<T, DP>;
-  const int lane = lane_id(), h = lane >> 5;
-  Frag<T> f;
-  if constexpr (sizeof(T) == 2) {
-    const int i = lane & 15, r = r0 + 4 * h + (i >> 2), c = n * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
-    const auto lo = read_tr(tile + R::at(r, c) + (i & 1) * 8), hi = read_tr(tile + R::at(r + 8, c) + (i & 1) * 8);
-    const uintx2_t a = __builtin_bit_cast(uintx2_t, lo), b = __builtin_bit_cast(uintx2_t, hi);
-    f.v[0] = {a[0], a[1], b[0], b[1]};
-  } else {
-    const int d = n * 32 + (lane & 31);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      f.v[i / 4][i % 4] =
-          *(lds_word *)(tile + R::at(r0 + (i / 4) * 8 + 4 * h + i % 4, d >> 2) + (d & 3) * 4);
+  uint32_t row, col;  // LDS addresses in the tile
+  __device__ __forceinline__ explicit Reader() {
+    const int lane = lane_id(), h = lane >> 5;
+    row = R::at(lane & 31, h * (R::SIZE / 2));
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15;
+      col = R::at(4 * h + (i >> 2), ((lane >> 4) & 1) * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+    } else {
+      col = R::at(4 * h, (lane & 31) >> 2) + (lane & 3) * 4;
+    }
   }
-  return f;
-}
+  // rows r0 to r0 + 31 as the first operand of step st of 16 values
+  __device__ __forceinline__ Frag<T> rows(lds_char *tile, int r0, int st) const {
+    Frag<T> f;
+#pragma unroll
+    for (int i = 0; i < R::SIZE / 2; ++i) f.v[i] = *(lds_chunk *)(tile + r0 * R::PITCH + (row ^ (st * 16 * R::SIZE + i * 16)));
+    return f;
+  }
+  // values 32 n to 32 n + 31 as the first operand, summed over rows r0 to r0 + 15
+  __device__ __forceinline__ Frag<T> cols(lds_char *tile, int r0, int n) const {
+    Frag<T> f;
+    lds_char *at = tile + r0 * R::PITCH;
+    if constexpr (sizeof(T) == 2) {
+      const auto lo = read_tr(at + (col ^ (n * 64))), hi = read_tr(at + 8 * R::PITCH + (col ^ (n * 64 + 32)));
+      const uintx2_t a = __builtin_bit_cast(uintx2_t, lo), b = __builtin_bit_cast(uintx2_t, hi);
+      f.v[0] = {a[0], a[1], b[0], b[1]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // (row i % 4 and the rows 8 behind change the swizzle as R::at says)
+        const int r = (i / 4) * 8 + i % 4;
+        f.v[i / 4][i % 4] = *(lds_word *)(at + r * R::PITCH + (col ^ (n * 128) ^ (R::swizzle(r) << 4)));
+      }
+    }
+    return f;
+  }
+};
 // a column's row of memory as the second operand of step st, zeros past d and
 // without a row
 template <class T> __device__ __forceinline__ Frag<T> load_frag(const T *row, int d, int st) {
@@ -207,39 +225,59 @@ template <class T> __device__ __forceinline__ Frag<T> load_frag(const T *row, in
   return f;
 }
 
-// A tile of R rows from memory to LDS by NT threads (of which this is `thread`):
-// rows [0, n) of `stride` bytes, zeros behind them and behind a row's d values.
-// DMA (rows, strides and addresses of whole 16-byte chunks: `dma`): under way on
-// return, a load of 1 KB per wave and instruction; chunks outside are out of the
-// buffer's range.  Else through registers, written on return.
-template <class T, int DP, int R, int NT>
-__device__ __forceinline__ void fetch_tile(const char *rows, int64_t stride, int64_t n, int d, bool dma, lds_char *tile,
-                                           int thread) {
+// Tiles of R rows from memory to LDS by NT threads (of which this is `thread`): n rows
+// of `stride` bytes, zeros behind them and behind a row's d values.
+// DMA (rows, strides and addresses of whole 16-byte chunks): under way on return, a
+// load of 1 KB per wave and instruction; chunks outside are out of the buffer's
+// range.  Else through registers, written on return.
+template <class T, int DP, int R, int NT, bool DMA> struct Fetch {
   using S = Rows<T, DP>;
-  constexpr int LOADS = R * S::CPR / NT;
+  static constexpr int LOADS = R * S::CPR / NT;
+  // rows from one load to the next, whose chunks a thread takes in the same order where
+  // these are whole swizzles
+  static constexpr int TURN = NT / S::CPR;
+  static constexpr bool SAME = TURN % 16 == 0;
   static_assert(LOADS >= 1 && LOADS * NT == R * S::CPR, "tile shape");
-  const int dbytes = d * S::SIZE;
-  n = n < 0 ? 0 : n > R ? R : n;
-  if (dma) {
-    const uintx4_t from = buffer(rows, n > 0 ? (n - 1) * stride + dbytes : 0);
-    lds_char *to = tile + (thread & ~63) * 16;
+  int64_t stride;
+  int thread, d;
+  uint32_t first[SAME ? 1 : LOADS];
+  __device__ __forceinline__ Fetch(int64_t stride, int d, int thread) : stride(stride), thread(thread), d(d) {
+    if constexpr (DMA) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int id = i * NT + thread, r = id / S::CPR, c = (id % S::CPR) ^ S::swizzle(r);
-      const uint32_t offset = static_cast<uint32_t>(r) * static_cast<uint32_t>(stride) + c * 16;
-      load_lds(from, c * 16 < dbytes ? offset : kOutOfRange, (lds_void *)(to + i * NT * 16));
+      for (int i = 0; i < (SAME ? 1 : LOADS); ++i) {
+        const int id = i * NT + thread, r = id / S::CPR, c = (id % S::CPR) ^ S::swizzle(r);
+        first[i] = c * 16 < d * S::SIZE ? static_cast<uint32_t>(r) * static_cast<uint32_t>(stride) + c * 16 : kOutOfRange;
+      }
     }
-  } else {
-    uintx4_t v[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int id = i * NT + thread, r = id / S::CPR, c = (id % S::CPR) ^ S::swizzle(r);
-      v[i] = load_raw(reinterpret_cast<const T *>(rows + r * stride) + c * kVec<T>, r < n ? d - c * kVec<T> : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) *(lds_chunk *)(tile + (i * NT + thread) * 16) = v[i];
   }
-}
+  __device__ __forceinline__ void operator()(const char *rows, int64_t n, lds_char *tile) const {
+    if constexpr (DMA) {
+      lds_char *to = tile + (thread & ~63) * 16;
+      const auto bytes = [&](int64_t m, int64_t most) {
+        m = m < most ? m : most;
+        return m > 0 ? (m - 1) * stride + d * S::SIZE : int64_t(0);
+      };
+      if constexpr (SAME) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+          load_lds(buffer(rows + i * TURN * stride, bytes(n - i * TURN, TURN)), first[0], (lds_void *)(to + i * NT * 16));
+      } else {
+        const uintx4_t from = buffer(rows, bytes(n, R));
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load_lds(from, first[i], (lds_void *)(to + i * NT * 16));
+      }
+    } else {
+      uintx4_t v[LOADS];
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int id = i * NT + thread, r = id / S::CPR, c = (id % S::CPR) ^ S::swizzle(r);
+        v[i] = load_raw(reinterpret_cast<const T *>(rows + r * stride) + c * kVec<T>, r < n ? d - c * kVec<T> : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) *(lds_chunk *)(tile + (i * NT + thread) * 16) = v[i];
+    }
+  }
+};
 
 // the larger (or the sum) of the two halves' values of a column
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
@@ -333,11 +371,11 @@ __device__ __forceinline__ void store_column(T *row, int d, bool there, const fl
     }
 }
 
-// whether tiles of such rows can be fetched by DMA
-inline bool dma_rows(const void *p, int64_t row, int64_t head, int d, int size, int64_t tile_rows) {
+// whether tiles (of at most 64 rows) can be fetched by DMA
+inline bool dma_rows(const void *p, int64_t row, int64_t head, int d, int size) {
   const auto whole = [&](int64_t values) { return values * size % 16 == 0; };
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && whole(row) && whole(head) && whole(d) &&
-         row * size * tile_rows < kBufferLimit / 2;
+         row * size * 64 < kBufferLimit / 2;
 }
 
 // f of the head's padded width
@@ -348,6 +386,8 @@ template <class F> int with_width(int d, F &&f) {
   if (d <= 96) return f(integral_constant<int, 96>{});
   return f(integral_constant<int, 128>{});
 }
+
+constexpr int kKeysByDma = 1, kQueriesByDma = 2;
 
 // Strides in values.
 struct Args {

@@ -38,7 +38,7 @@ __device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) 
   return n < 0 ? 0 : n < s.nk ? n : s.nk;
 }
 
-template <class T, int DP>
+template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(const Args a) {
   using R = Rows<T, DP>;
   constexpr int KT = kKeys<T>, TILE = KT * R::PITCH;
@@ -55,20 +55,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
   const int total = s.nq * a.group, c0 = (f.of - 1 - f.nth) * kColumns, w0 = c0 + wave * 32;
   const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
   const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i);
-  const int least = visible(a, s, std::min(w0, total - 1) / a.group);
-  const int most = w0 < total ? visible(a, s, std::min(w0 + 31, total - 1) / a.group) : 0;
   const int fewest = visible(a, s, c0 / a.group), end = dq ? visible(a, s, std::min(c0 + kColumns - 1, total - 1) / a.group) : 0;
-  const int steps = (end + KT - 1) / KT, own = (most + KT - 1) / KT;
+  const int steps = (end + KT - 1) / KT;
   const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
   const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + s.k0 * a.k_row + kv * a.k_head);
   const char *values = reinterpret_cast<const char *>(static_cast<const T *>(a.v) + s.k0 * a.v_row + kv * a.v_head);
-  const auto issue = [&](int t) {
-    lds_char *to = (lds_char *)lds + (t & 1) * 2 * TILE;
-    fetch_tile<T, DP, KT, 256>(keys + t * (KT * kstride), kstride, s.nk - t * KT, a.d, a.dma & 1, to, threadIdx.x);
-    fetch_tile<T, DP, KT, 256>(values + t * (KT * vstride), vstride, s.nk - t * KT, a.d, a.dma & 1, to + TILE,
-                               threadIdx.x);
+  const Fetch<T, DP, KT, 256, DMA> fetch_keys(kstride, a.d, threadIdx.x), fetch_values(vstride, a.d, threadIdx.x);
+  const auto issue = [&](int t, int stage) {
+    lds_char *to = (lds_char *)lds + stage * 2 * TILE;
+    fetch_keys(keys + t * (KT * kstride), s.nk - t * KT, to);
+    fetch_values(values + t * (KT * vstride), s.nk - t * KT, to + TILE);
   };
-  if (steps > 0) issue(0);
+  if (steps > 0) issue(0, 0);
   const int64_t at = (s.q0 + i) * a.heads + head;
   Frag<T> q[DP / 16], g[DP / 16];
   const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
@@ -92,42 +90,68 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
   Stat<T> r{a.stats[stat], 1.f};
   if constexpr (sizeof(T) == 4) r.by = a.stats[a.heads * a.s.rows + stat];
   floatx16 acc[DP / 32] = {};
-  for (int t = 0; t < steps; ++t) {
+  const Reader<T, DP> read;
+  // ds of 32 keys (MASKED: of which this lane's column sees the first `seen`), in place of their scores
+  const auto gradients = [&](auto MASKED, lds_char *kt, lds_char *vt, int seen, floatx16 &ds) {
+    floatx16 p{}, dp{};
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) {
+      mma(p, read.rows(kt, 0, st), q[st]);
+      mma(dp, read.rows(vt, 0, st), g[st]);
+    }
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const float w = weight(p[x], a.scale2, r) * (dp[x] - delta);
+      ds[x] = !decltype(MASKED)::value || 8 * (x / 4) + x % 4 < seen - 4 * h ? w : 0.f;
+    }
+  };
+  const auto accumulate = [&](lds_char *kt, const floatx16 &ds) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const Frag<T> f = as_operand<T>(ds, st);
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n) mma(acc[n], read.cols(kt, 16 * st, n), f);
+    }
+  };
+  const int whole = std::min(fewest / KT, steps);  // tiles that every column sees whole
+  int t = 0;
+  const auto step = [&](auto STAGE) {
+    constexpr int stage = decltype(STAGE)::value;
     wait_loads_and_meet<0>();
-    if (t + 1 < steps) issue(t + 1);
-    // (the same for the whole block, which then stays together)
-    const bool hides = a.causal && fewest < (t + 1) * KT;
-    if (t >= own && !hides) continue;
-    lds_char *kt = (lds_char *)lds + (t & 1) * 2 * TILE, *vt = kt + TILE;
-    const bool whole = least >= (t + 1) * KT;
+    if (t + 1 < steps) issue(t + 1, stage ^ 1);
+    lds_char *kt = (lds_char *)lds + stage * 2 * TILE;
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u) {
-      floatx16 p{}, dp{};
-#pragma unroll
-      for (int st = 0; st < DP / 16; ++st) {
-        mma(p, row_frag<T, DP>(kt, 32 * u, st), q[st]);
-        mma(dp, row_frag<T, DP>(vt, 32 * u, st), g[st]);
-      }
-      const int mine = limit - t * KT - 32 * u;
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const float ds = weight(p[x], a.scale2, r) * (dp[x] - delta);
-        p[x] = whole || 8 * (x / 4) + x % 4 < mine - 4 * h ? ds : 0.f;
-      }
-      Frag<T> ds[2] = {as_operand<T>(p, 0), as_operand<T>(p, 1)};
-      lds_char *tile = kt + 32 * u * R::PITCH;
+      floatx16 ds;
+      gradients(std::false_type{}, kt + 32 * u * R::PITCH, kt + TILE + 32 * u * R::PITCH, 0, ds);
+      accumulate(kt + 32 * u * R::PITCH, ds);
+    }
+  };
+  while (t < whole) {
+    step(std::integral_constant<int, 0>{});
+    if (++t == whole) break;
+    step(std::integral_constant<int, 1>{});
+    ++t;
+  }
+  // the others; the block stays together
+  for (; t < steps; ++t) {
+    wait_loads_and_meet<0>();
+    if (t + 1 < steps) issue(t + 1, (t + 1) & 1);
+#pragma unroll 1
+    for (int u = 0; u < KT / 32; ++u) {
+      lds_char *kt = (lds_char *)lds + (t & 1) * 2 * TILE + 32 * u * R::PITCH;
+      const int first = t * KT + 32 * u, seen = limit - first;
+      floatx16 ds;
+      gradients(std::true_type{}, kt, kt + TILE, seen, ds);
       bool found = false;
-      if (hides) {
+      if (a.causal) {
         __syncthreads();  // (every wave has the scores)
-        found = __syncthreads_or(clear_not_finite<T, DP, 32, 256>(tile, threadIdx.x));
+        found = __syncthreads_or(clear_not_finite<T, DP, 32, 256>(kt, threadIdx.x));
       }
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int n = 0; n < DP / 32; ++n) mma(acc[n], col_frag<T, DP>(tile, 16 * st, n), ds[st]);
+      accumulate(kt, ds);
       if (found)
-        add_not_finite<T, DP>(acc, keys + (t * KT + 32 * u) * kstride, kstride, std::min(s.nk - t * KT - 32 * u, 32), a.d,
-                              [&](int x) { return x < mine; });
+        add_not_finite<T, DP>(acc, keys + first * kstride, kstride, std::min(s.nk - first, 32), a.d,
+                              [&](int x) { return x < seen; });
     }
   }
   if (dq) store_column<T, DP>(dq + at * a.d, a.d, there, acc, a.scale);
@@ -139,7 +163,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
 constexpr int kOwnKeys = 128;
 template <class T> constexpr int kQueries = sizeof(T) == 2 ? 64 : 32;
 
-template <class T, int DP>
+template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_kernel(const Args a) {
   using R = Rows<T, DP>;
   constexpr int QT = kQueries<T>, TILE = QT * R::PITCH;
@@ -158,9 +182,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   // (the first tile first: the most queries see it)
   const int c0 = f.nth * kOwnKeys, w0 = c0 + wave * 32, key = w0 + (lane & 31);
   const bool there = key < s.nk;
-  // the first query that sees this lane's key, the wave's first and last, the block's first
+  // the first query that sees a key
   const auto first_of = [&](int k) { return a.causal ? std::max(0, k - (s.nk - s.nq)) : 0; };
-  const int first = first_of(key), earliest = first_of(w0), latest = first_of(w0 + 31), begin = first_of(c0) / QT;
+  const int first = first_of(key), begin = first_of(c0) / QT;
+  const int latest = first_of(std::min(c0 + kOwnKeys, s.nk) - 1);  // (from here on all of the block's keys are seen)
   const int end = (s.nq + QT - 1) / QT, span = c0 < s.nk ? std::max(0, end - begin) : 0, steps = span * a.group;
   const int64_t qstride = a.q_row * R::SIZE, gstride = static_cast<int64_t>(a.heads) * a.d * R::SIZE;
   const auto queries_of_head = [&](int head) {
@@ -169,21 +194,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   const auto gradients_of = [&](int head) {
     return reinterpret_cast<const char *>(static_cast<const T *>(a.dout) + static_cast<int64_t>(head) * a.d);
   };
-  const auto issue = [&](int step, int g, int t) {
-    lds_char *to = (lds_char *)lds + (step & 1) * 2 * TILE;
+  const Fetch<T, DP, QT, 256, DMA> fetch_queries(qstride, a.d, threadIdx.x), fetch_gradients(gstride, a.d, threadIdx.x);
+  const auto issue = [&](int stage, int g, int t) {
+    lds_char *to = (lds_char *)lds + stage * 2 * TILE;
     const int head = kv * a.group + g;
     const int64_t q0 = s.q0 + t * QT;
     const int n = s.nq - t * QT;
-    fetch_tile<T, DP, QT, 256>(queries_of_head(head) + q0 * qstride, qstride, n, a.d, a.dma & 4, to, threadIdx.x);
-    fetch_tile<T, DP, QT, 256>(gradients_of(head) + q0 * gstride, gstride, n, a.d, a.dma & 4, to + TILE, threadIdx.x);
+    fetch_queries(queries_of_head(head) + q0 * qstride, n, to);
+    fetch_gradients(gradients_of(head) + q0 * gstride, n, to + TILE);
     // (rows past the last: zeros, of which every product is zero)
     const int64_t bytes = std::min(n, QT) * 4;
     const uint32_t at = lane < QT ? lane * 4 : kOutOfRange;
     const int64_t row = head * a.s.rows + q0;
-    if (wave == 0) load_lds_word(buffer(a.stats + row, bytes), at, rows[step & 1][0]);
-    if (wave == 1) load_lds_word(buffer(a.delta + row, bytes), at, rows[step & 1][1]);
+    if (wave == 0) load_lds_word(buffer(a.stats + row, bytes), at, rows[stage][0]);
+    if (wave == 1) load_lds_word(buffer(a.delta + row, bytes), at, rows[stage][1]);
     if (sizeof(T) == 4 && wave == 2)
-      load_lds_word(buffer(a.stats + a.heads * a.s.rows + row, bytes), at, rows[step & 1][2]);
+      load_lds_word(buffer(a.stats + a.heads * a.s.rows + row, bytes), at, rows[stage][2]);
   };
   int g = 0, t = begin;  // of the step to be issued
   const auto advance = [&] {
@@ -205,72 +231,92 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
     }
   }
   floatx16 ak[DP / 32] = {}, av[DP / 32] = {};
+  const Reader<T, DP> read;
+  // p and ds of 32 queries from row `row` of the tile on; MASKED: this lane's key is seen from the `mine`th on
+  const auto weights = [&](auto MASKED, int stage, int row, int mine, floatx16 &p, floatx16 &ds) {
+    lds_char *qt = (lds_char *)lds + stage * 2 * TILE + row * R::PITCH, *gt = qt + TILE;
+    p = floatx16{};
+    ds = floatx16{};
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) {
+      mma(p, read.rows(qt, 0, st), k[st]);
+      mma(ds, read.rows(gt, 0, st), v[st]);
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float *at = &rows[stage][0][row + 8 * x + 4 * h];
+      const floatx4_t base = *reinterpret_cast<const floatx4_t *>(at);
+      const floatx4_t delta = *reinterpret_cast<const floatx4_t *>(at + 64);
+      floatx4_t by{};
+      if constexpr (sizeof(T) == 4) by = *reinterpret_cast<const floatx4_t *>(at + 128);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float w = weight(p[4 * x + y], a.scale2, Stat<T>{base[y], by[y]});
+        const bool seen = !decltype(MASKED)::value || 8 * x + y >= mine - 4 * h;
+        ds[4 * x + y] = seen ? w * (ds[4 * x + y] - delta[y]) : 0.f;
+        p[4 * x + y] = seen ? w : 0.f;
+      }
+    }
+  };
+  const auto accumulate = [&](floatx16 (&acc)[DP / 32], lds_char *tile, const floatx16 &p) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const Frag<T> f = as_operand<T>(p, st);
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n) mma(acc[n], read.cols(tile, 16 * st, n), f);
+    }
+  };
   int now = begin, at_head = 0;  // of the step at hand
-  for (int step = 0; step < steps; ++step) {
+  const auto step = [&](int index, auto STAGE) {
+    constexpr int stage = decltype(STAGE)::value;
     wait_loads_and_meet<0>();
-    if (step + 1 < steps) {
-      issue(step + 1, g, t);
+    if (index + 1 < steps) {
+      issue(stage ^ 1, g, t);
       advance();
     }
-    const int q0 = now * QT, of_head = at_head;
+    const int q0 = now * QT, head = kv * a.group + at_head;
     if (++now == end) {
       now = begin;
       ++at_head;
     }
-    // (the same for the whole block, which then stays together)
-    const bool hides = a.causal && q0 < first_of(std::min(c0 + kOwnKeys, s.nk) - 1);
-    if (w0 >= s.nk && !hides) continue;
-    lds_char *tiles = (lds_char *)lds + (step & 1) * 2 * TILE;
+    lds_char *qt = (lds_char *)lds + stage * 2 * TILE, *gt = qt + TILE;
+    if (q0 >= latest) {
+      if (w0 < s.nk)
 #pragma unroll
-    for (int u = 0; u < QT / 32; ++u) {
-      const int r0 = q0 + 32 * u;
-      if ((r0 + 32 <= earliest || r0 >= s.nq) && !hides) continue;  // (hidden from all keys, or past the last)
-      lds_char *qt = tiles + 32 * u * R::PITCH, *gt = qt + TILE;
-      floatx16 p{}, dp{};
-#pragma unroll
-      for (int st = 0; st < DP / 16; ++st) {
-        mma(p, row_frag<T, DP>(qt, 0, st), k[st]);
-        mma(dp, row_frag<T, DP>(gt, 0, st), v[st]);
-      }
-      const bool whole = r0 >= latest;
-      const int mine = first - r0;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float *at = &rows[step & 1][0][32 * u + 8 * x + 4 * h];
-        const floatx4_t base = *reinterpret_cast<const floatx4_t *>(at);
-        const floatx4_t delta = *reinterpret_cast<const floatx4_t *>(at + 64);
-        floatx4_t by{};
-        if constexpr (sizeof(T) == 4) by = *reinterpret_cast<const floatx4_t *>(at + 128);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float w = weight(p[4 * x + y], a.scale2, Stat<T>{base[y], by[y]});
-          const bool seen = whole || 8 * x + y >= mine - 4 * h;
-          dp[4 * x + y] = seen ? w * (dp[4 * x + y] - delta[y]) : 0.f;
-          p[4 * x + y] = seen ? w : 0.f;
+        for (int u = 0; u < QT / 32; ++u) {
+          floatx16 p, ds;
+          weights(std::false_type{}, stage, 32 * u, 0, p, ds);
+          accumulate(av, gt + 32 * u * R::PITCH, p);
+          accumulate(ak, qt + 32 * u * R::PITCH, ds);
         }
-      }
-      const Frag<T> pf[2] = {as_operand<T>(p, 0), as_operand<T>(p, 1)}, ds[2] = {as_operand<T>(dp, 0), as_operand<T>(dp, 1)};
-      bool found = false;
-      if (hides) {
-        __syncthreads();  // (every wave has the scores)
-        const bool x = clear_not_finite<T, DP, 32, 256>(qt, threadIdx.x), y = clear_not_finite<T, DP, 32, 256>(gt, threadIdx.x);
-        found = __syncthreads_or(x || y);
-      }
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int n = 0; n < DP / 32; ++n) mma(av[n], col_frag<T, DP>(gt, 16 * st, n), pf[st]);
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int n = 0; n < DP / 32; ++n) mma(ak[n], col_frag<T, DP>(qt, 16 * st, n), ds[st]);
+      return;
+    }
+    // (the block stays together)
+#pragma unroll 1
+    for (int u = 0; u < QT / 32; ++u) {
+      const int mine = first - q0 - 32 * u;
+      floatx16 p, ds;
+      weights(std::true_type{}, stage, 32 * u, mine, p, ds);
+      lds_char *qu = qt + 32 * u * R::PITCH, *gu = gt + 32 * u * R::PITCH;
+      __syncthreads();  // (every wave has the scores)
+      const bool x = clear_not_finite<T, DP, 32, 256>(qu, threadIdx.x), y = clear_not_finite<T, DP, 32, 256>(gu, threadIdx.x);
+      const bool found = __syncthreads_or(x || y);
+      accumulate(av, gu, p);
+      accumulate(ak, qu, ds);
       if (found) {
-        const int head = kv * a.group + of_head, n = std::min(s.nq - r0, 32);
-        const auto sees = [&](int x) { return x >= mine; };
-        add_not_finite<T, DP>(av, gradients_of(head) + (s.q0 + r0) * gstride, gstride, n, a.d, sees);
-        add_not_finite<T, DP>(ak, queries_of_head(head) + (s.q0 + r0) * qstride, qstride, n, a.d, sees);
+        const int64_t r0 = s.q0 + q0 + 32 * u;
+        const int n = std::min(s.nq - q0 - 32 * u, 32);
+        const auto sees = [&](int r) { return r >= mine; };
+        add_not_finite<T, DP>(av, gradients_of(head) + r0 * gstride, gstride, n, a.d, sees);
+        add_not_finite<T, DP>(ak, queries_of_head(head) + r0 * qstride, qstride, n, a.d, sees);
       }
     }
+  };
+  for (int index = 0; index < steps;) {
+    step(index, std::integral_constant<int, 0>{});
+    if (++index == steps) break;
+    step(index, std::integral_constant<int, 1>{});
+    ++index;
   }
   // (keys that are none, in the room behind the others, get zeros)
   if (!there) {
@@ -288,13 +334,19 @@ template <class T, int DP> static int launch(const Args &a, hipStream_t stream) 
   if (a.s.rows > 0) {
     const int64_t blocks = (a.s.rows * a.group / kColumns + a.s.count) * a.kv_heads;
     SPIRA_HIP_REQUIRE(launchable(blocks, 256), "attention: too many tiles for a launch");
-    hipLaunchKernelGGL((queries_kernel<T, DP>), dim3(blocks), dim3(256), 0, stream, a);
+    if (a.dma & kKeysByDma)
+      hipLaunchKernelGGL((queries_kernel<T, DP, true>), dim3(blocks), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((queries_kernel<T, DP, false>), dim3(blocks), dim3(256), 0, stream, a);
     SPIRA_HIP_LAUNCH_CHECK();
   }
   if (a.s.keys > 0 && (a.dk || a.dv)) {
     const int64_t blocks = (a.s.keys / kOwnKeys + a.s.count) * a.kv_heads;
     SPIRA_HIP_REQUIRE(launchable(blocks, 256), "attention: too many tiles for a launch");
-    hipLaunchKernelGGL((keys_kernel<T, DP>), dim3(blocks), dim3(256), 0, stream, a);
+    if (a.dma & kQueriesByDma)
+      hipLaunchKernelGGL((keys_kernel<T, DP, true>), dim3(blocks), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((keys_kernel<T, DP, false>), dim3(blocks), dim3(256), 0, stream, a);
     SPIRA_HIP_LAUNCH_CHECK();
   }
   return kOk;
@@ -325,8 +377,8 @@ int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out
   a.dq = dqueries;
   a.dk = dkey;
   a.dv = dvalue;
-  if (!attention::dma_rows(dout, static_cast<int64_t>(x->heads) * x->head_dim, x->head_dim, x->head_dim, size, 64))
-    a.dma &= ~4;
+  if (!attention::dma_rows(dout, static_cast<int64_t>(x->heads) * x->head_dim, x->head_dim, x->head_dim, size))
+    a.dma &= ~attention::kQueriesByDma;
   return with_type(x->dtype, [&](auto t) -> int {
     return attention::with_width(x->head_dim, [&](auto W) -> int {
       return attention::launch<decltype(t), decltype(W)::value>(a, stream);
