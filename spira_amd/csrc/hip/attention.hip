@@ -419,6 +419,8 @@ static Plan plan(const spira_hip_attention_t &x) {
   return {true, static_cast<int>(std::min<int64_t>(part, int64_t(1) << 30)), div_up(x.keys, part)};
 }
 
+size_t gradient_bytes(const spira_hip_attention_t &x);  // (attention_backward.hip)
+
 static size_t partial_bytes(const spira_hip_attention_t &x, const Plan &p) {
   return p.tokens && p.parts > 1 ? static_cast<size_t>(p.parts) * x.rows * x.heads * (x.head_dim + 2) * sizeof(float) : 0;
 }
@@ -466,8 +468,7 @@ extern "C" {
 int spira_hip_attention_workspace(const spira_hip_attention_t *x, int gradient, size_t *bytes) {
   SPIRA_HIP_REQUIRE(x && bytes, "attention: null arguments");
   if (int rc = attention::check(*x)) return rc;
-  *bytes = gradient ? static_cast<size_t>(x->rows) * x->heads * sizeof(float)
-                    : attention::partial_bytes(*x, attention::plan(*x));
+  *bytes = gradient ? attention::gradient_bytes(*x) : attention::partial_bytes(*x, attention::plan(*x));
   return kOk;
 }
 

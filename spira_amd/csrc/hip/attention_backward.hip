@@ -163,7 +163,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
 constexpr int kOwnKeys = 128;
 template <class T> constexpr int kQueries = sizeof(T) == 2 ? 64 : 32;
 
-template <class T, int DP, bool DMA>
+// SPLIT: a block takes every `splits`th step of its keys', from blockIdx.y on, and writes its
+// sums in fp32 to be joined.
+template <class T, int DP, bool DMA, bool SPLIT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_kernel(const Args a) {
   using R = Rows<T, DP>;
   constexpr int QT = kQueries<T>, TILE = QT * R::PITCH;
@@ -172,8 +174,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id(), h = lane >> 5;
   T *dk = static_cast<T *>(a.dk), *dv = static_cast<T *>(a.dv);
   const int64_t width = static_cast<int64_t>(a.kv_heads) * a.d;
-  if (dk) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dk, width, blockIdx.x, gridDim.x);
-  if (dv) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dv, width, blockIdx.x, gridDim.x);
+  if (!SPLIT && dk) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dk, width, blockIdx.x, gridDim.x);
+  if (!SPLIT && dv) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dv, width, blockIdx.x, gridDim.x);
   const int kv = blockIdx.x % a.kv_heads;
   const Found f = find_piece(a.s.count, blockIdx.x / a.kv_heads,
                              [&](int b) { return static_cast<int>((room_of(a.s, b) + int64_t(kOwnKeys) - 1) / kOwnKeys); });
@@ -186,7 +188,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   const auto first_of = [&](int k) { return a.causal ? std::max(0, k - (s.nk - s.nq)) : 0; };
   const int first = first_of(key), begin = first_of(c0) / QT;
   const int latest = first_of(std::min(c0 + kOwnKeys, s.nk) - 1);  // (from here on all of the block's keys are seen)
-  const int end = (s.nq + QT - 1) / QT, span = c0 < s.nk ? std::max(0, end - begin) : 0, steps = span * a.group;
+  const int end = (s.nq + QT - 1) / QT, span = c0 < s.nk ? std::max(0, end - begin) : 0;
+  const int splits = SPLIT ? static_cast<int>(gridDim.y) : 1, part = SPLIT ? static_cast<int>(blockIdx.y) : 0;
+  const int64_t all = static_cast<int64_t>(span) * a.group;
+  const int steps = static_cast<int>(all > part ? (all - part + splits - 1) / splits : 0);
   const int64_t qstride = a.q_row * R::SIZE, gstride = static_cast<int64_t>(a.heads) * a.d * R::SIZE;
   const auto queries_of_head = [&](int head) {
     return reinterpret_cast<const char *>(static_cast<const T *>(a.q) + head * a.q_head);
@@ -211,15 +216,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
     if (sizeof(T) == 4 && wave == 2)
       load_lds_word(buffer(a.stats + a.heads * a.s.rows + row, bytes), at, rows[stage][2]);
   };
-  int g = 0, t = begin;  // of the step to be issued
-  const auto advance = [&] {
-    if (++t == end) {
-      t = begin;
-      ++g;
+  // the head and tile of a step, and of the one that follows
+  struct Where {
+    int g, t;
+  };
+  const auto advance = [&](Where &w) {
+    w.t += splits;
+    while (w.t >= end) {
+      w.t -= span;
+      ++w.g;
     }
   };
-  if (steps > 0) issue(0, g, t);
-  advance();
+  Where next{0, begin + part};
+  if (steps > 0) {
+    while (next.t >= end) {
+      next.t -= span;
+      ++next.g;
+    }
+    issue(0, next.g, next.t);
+  }
+  Where now = next;  // of the step at hand
+  if (steps > 1) advance(next);
   Frag<T> k[DP / 16], v[DP / 16];
   {
     const T *krow = there ? static_cast<const T *>(a.k) + (s.k0 + key) * a.k_row + kv * a.k_head : nullptr;
@@ -266,19 +283,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       for (int n = 0; n < DP / 32; ++n) mma(acc[n], read.cols(tile, 16 * st, n), f);
     }
   };
-  int now = begin, at_head = 0;  // of the step at hand
   const auto step = [&](int index, auto STAGE) {
     constexpr int stage = decltype(STAGE)::value;
     wait_loads_and_meet<0>();
     if (index + 1 < steps) {
-      issue(stage ^ 1, g, t);
-      advance();
+      issue(stage ^ 1, next.g, next.t);
     }
-    const int q0 = now * QT, head = kv * a.group + at_head;
-    if (++now == end) {
-      now = begin;
-      ++at_head;
-    }
+    const int q0 = now.t * QT, head = kv * a.group + now.g;
+    now = next;
+    if (index + 2 < steps) advance(next);
     lds_char *qt = (lds_char *)lds + stage * 2 * TILE, *gt = qt + TILE;
     if (q0 >= latest) {
       if (w0 < s.nk)
@@ -324,13 +337,87 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
     for (int n = 0; n < DP / 32; ++n) ak[n] = av[n] = floatx16{};
   }
   const int64_t to = ((s.k0 + key) * a.kv_heads + kv) * a.d;
+  if constexpr (SPLIT) {
+    float *sums = a.partial + part * 2 * a.s.keys * width + to;
+    store_column<float, DP>(sums, a.d, there, ak, a.scale);
+    store_column<float, DP>(sums + a.s.keys * width, a.d, there, av, 1.f);
+    return;
+  }
   if (dk) store_column<T, DP>(dk + to, a.d, key < s.room, ak, a.scale);
   if (dv) store_column<T, DP>(dv + to, a.d, key < s.room, av, 1.f);
 }
 
+// dk (blockIdx.y 0) and dv from the splits' sums, in their order; zeros in rows that are no keys
+template <class T> __global__ __launch_bounds__(256) void sums_kernel(const Args a, int splits) {
+  const int64_t width = static_cast<int64_t>(a.kv_heads) * a.d, chunks = (width + kVec<T> - 1) / kVec<T>;
+  const int64_t id = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x, row = id / chunks, at = (id - row * chunks) * kVec<T>;
+  T *to = static_cast<T *>(blockIdx.y == 0 ? a.dk : a.dv);
+  if (!to || row >= a.s.keys) return;
+  bool there = false;
+  // (sequences are ascending: the last that begins at or before the row)
+  int lo = 0, hi = a.s.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.s.key_offsets[mid] <= row) lo = mid;
+    else hi = mid;
+  }
+  const int64_t first = clamp_row(a.s.key_offsets[lo], a.s.keys);
+  there = row >= first && row < first + keys_of(a.s, lo);
+  Chunk<T> sum{};
+  if (there) {
+    const float *from = a.partial + blockIdx.y * a.s.keys * width + row * width + at;
+    for (int p = 0; p < splits; ++p, from += 2 * a.s.keys * width)
+#pragma unroll
+      for (int c = 0; c < kVec<T> / 4; ++c) {
+        const Chunk<float> x = load_chunk(from + 4 * c, width - at - 4 * c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum.v[4 * c + i] += x.v[i];
+      }
+  }
+  store_chunk(to + row * width + at, width - at, sum);
+}
+
 int arguments(const spira_hip_attention_t &x, Args &a, int size);
 
-template <class T, int DP> static int launch(const Args &a, hipStream_t stream) {
+// Parts of the keys' steps.  A block of 128 keys has as many steps as its sequence has
+// queries (times the group's heads, over 64): a long sequence's blocks run on alone when
+// the others are done.  With parts for 8 blocks a CU, however long the sequences, at
+// most 8 of them (their sums in fp32 are written and read again).
+static int key_splits(const spira_hip_attention_t &x) {
+  const int64_t blocks = (x.keys / kOwnKeys + x.sequences) * x.kv_heads;
+  const int64_t steps = div_up(x.rows, 64) * (x.heads / x.kv_heads);
+  const int64_t bytes = 2 * x.keys * x.kv_heads * x.head_dim * 4;
+  int64_t splits = std::min<int64_t>({2048 / std::max<int64_t>(blocks, 1), steps, 8});
+  if (bytes > 0) splits = std::min<int64_t>(splits, (int64_t(1) << 30) / bytes);
+  return static_cast<int>(std::max<int64_t>(splits, 1));
+}
+static size_t delta_bytes(const spira_hip_attention_t &x) {
+  return round_up(static_cast<int64_t>(x.rows) * x.heads * static_cast<int64_t>(sizeof(float)), 256);
+}
+static size_t sums_bytes(const spira_hip_attention_t &x) {
+  const int splits = key_splits(x);
+  return splits > 1 ? static_cast<size_t>(splits) * 2 * x.keys * x.kv_heads * x.head_dim * sizeof(float) : 0;
+}
+size_t gradient_bytes(const spira_hip_attention_t &x) { return delta_bytes(x) + sums_bytes(x); }
+
+template <class T, int DP, bool DMA> static int launch_keys(const Args &a, int splits, hipStream_t stream) {
+  const int64_t blocks = (a.s.keys / kOwnKeys + a.s.count) * a.kv_heads;
+  SPIRA_HIP_REQUIRE(launchable(blocks * splits, 256), "attention: too many tiles for a launch");
+  if (splits == 1) {
+    hipLaunchKernelGGL((keys_kernel<T, DP, DMA, false>), dim3(blocks), dim3(256), 0, stream, a);
+    SPIRA_HIP_LAUNCH_CHECK();
+    return kOk;
+  }
+  hipLaunchKernelGGL((keys_kernel<T, DP, DMA, true>), dim3(blocks, splits), dim3(256), 0, stream, a);
+  SPIRA_HIP_LAUNCH_CHECK();
+  const int64_t sums = div_up(a.s.keys * div_up(static_cast<int64_t>(a.kv_heads) * a.d, kVec<T>), 256);
+  SPIRA_HIP_REQUIRE(launchable(sums * 2, 256), "attention: too many rows for a launch");
+  hipLaunchKernelGGL(sums_kernel<T>, dim3(sums, 2), dim3(256), 0, stream, a, splits);
+  SPIRA_HIP_LAUNCH_CHECK();
+  return kOk;
+}
+
+template <class T, int DP> static int launch(const Args &a, int splits, hipStream_t stream) {
   if (a.s.rows > 0) {
     const int64_t blocks = (a.s.rows * a.group / kColumns + a.s.count) * a.kv_heads;
     SPIRA_HIP_REQUIRE(launchable(blocks, 256), "attention: too many tiles for a launch");
@@ -340,15 +427,8 @@ template <class T, int DP> static int launch(const Args &a, hipStream_t stream) 
       hipLaunchKernelGGL((queries_kernel<T, DP, false>), dim3(blocks), dim3(256), 0, stream, a);
     SPIRA_HIP_LAUNCH_CHECK();
   }
-  if (a.s.keys > 0 && (a.dk || a.dv)) {
-    const int64_t blocks = (a.s.keys / kOwnKeys + a.s.count) * a.kv_heads;
-    SPIRA_HIP_REQUIRE(launchable(blocks, 256), "attention: too many tiles for a launch");
-    if (a.dma & kQueriesByDma)
-      hipLaunchKernelGGL((keys_kernel<T, DP, true>), dim3(blocks), dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL((keys_kernel<T, DP, false>), dim3(blocks), dim3(256), 0, stream, a);
-    SPIRA_HIP_LAUNCH_CHECK();
-  }
+  if (a.s.keys > 0 && (a.dk || a.dv))
+    return a.dma & kQueriesByDma ? launch_keys<T, DP, true>(a, splits, stream) : launch_keys<T, DP, false>(a, splits, stream);
   return kOk;
 }
 
@@ -368,12 +448,14 @@ int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out
   attention::Args a;
   if (int rc = attention::arguments(*x, a, size)) return rc;
   SPIRA_HIP_REQUIRE(x->rows == 0 || (out && stats && dout), "attention: null outputs of the forward pass");
-  const size_t need = static_cast<size_t>(x->rows) * x->heads * sizeof(float);
+  const size_t need = attention::gradient_bytes(*x);
+  const int splits = attention::key_splits(*x);
   SPIRA_HIP_REQUIRE(workspace_bytes >= need && (workspace || need == 0), "attention: workspace too small");
   a.out = out;
   a.dout = dout;
   a.stats = const_cast<float *>(stats);
   a.delta = static_cast<float *>(workspace);
+  a.partial = splits > 1 ? a.delta + attention::delta_bytes(*x) / sizeof(float) : nullptr;
   a.dq = dqueries;
   a.dk = dkey;
   a.dv = dvalue;
@@ -381,7 +463,7 @@ int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out
     a.dma &= ~attention::kQueriesByDma;
   return with_type(x->dtype, [&](auto t) -> int {
     return attention::with_width(x->head_dim, [&](auto W) -> int {
-      return attention::launch<decltype(t), decltype(W)::value>(a, stream);
+      return attention::launch<decltype(t), decltype(W)::value>(a, splits, stream);
     });
   });
 }

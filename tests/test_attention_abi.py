@@ -67,7 +67,7 @@ def test_attention_outputs_and_workspaces():
     refused(LIB.spira_hip_attention(ctypes.byref(attention(dtype=7)), P(SOME), None, None, SIZE(0), None), "dtype")
     refused(LIB.spira_hip_attention_backward(ctypes.byref(x), P(SOME), None, P(SOME), P(SOME), P(SOME), P(SOME), P(SOME),
                                              SIZE(1 << 40), None), "null")
-    assert LIB.spira_hip_attention_workspace(ctypes.byref(x), 1, ctypes.byref(size)) == 0 and size.value == 100 * 4 * 4
+    assert LIB.spira_hip_attention_workspace(ctypes.byref(x), 1, ctypes.byref(size)) == 0 and size.value >= 100 * 4 * 4
     refused(LIB.spira_hip_attention_backward(ctypes.byref(x), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME),
                                              SIZE(size.value - 1), None), "workspace")
     # few tokens against a long cache: the parts' sums
