@@ -25,9 +25,6 @@ namespace attention {
 
 constexpr float kSlack = 8.f;
 
-// keys of a tile
-template <class T> constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
-
 // a wave's 32 columns on their way: output, reference maximum of the raw scores
 // (-inf: nothing seen) and this half's share of the sum
 template <int DP> struct Columns {
@@ -90,23 +87,16 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
   }
 }
 
-// keys that query i of a sequence sees
-__device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) {
-  if (!a.causal) return s.nk;
-  const int n = i + 1 + s.nk - s.nq;
-  return n < 0 ? 0 : n < s.nk ? n : s.nk;
-}
-
 // ---------------------------------------------------------------------------
 // prompts
 // ---------------------------------------------------------------------------
-constexpr int kColumns = 128;
-
 template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(const Args a) {
   using R = Rows<T, DP>;
-  constexpr int KT = kKeys<T>, TILE = KT * R::PITCH;
-  __shared__ __align__(1024) char lds[4 * TILE];
+  constexpr int KT = kKeys<T>, TILE = KT * R::PITCH, STAGES = kStages<T, DP>;
+  using Fetcher = Fetch<T, DP, KT, 256, DMA>;
+  constexpr int AHEAD = DMA ? 2 * Fetcher::LOADS * (STAGES - 2) : 0;  // loads under way behind a stage's own
+  __shared__ __align__(1024) char lds[STAGES * 2 * TILE];
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id();
   T *o = static_cast<T *>(a.o);
   clear_uncovered(a.s.offsets, a.s.count, a.s.rows, o, static_cast<int64_t>(a.heads) * a.d, blockIdx.x, gridDim.x);
@@ -127,13 +117,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
   const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + s.k0 * a.k_row + kv * a.k_head);
   const char *values = reinterpret_cast<const char *>(static_cast<const T *>(a.v) + s.k0 * a.v_row + kv * a.v_head);
-  const Fetch<T, DP, KT, 256, DMA> fetch_keys(kstride, a.d, threadIdx.x), fetch_values(vstride, a.d, threadIdx.x);
+  const Fetcher fetch_keys(kstride, a.d, threadIdx.x), fetch_values(vstride, a.d, threadIdx.x);
   const auto issue = [&](int t, int stage) {
     lds_char *to = (lds_char *)lds + stage * 2 * TILE;
     fetch_keys(keys + t * (KT * kstride), s.nk - t * KT, to);
     fetch_values(values + t * (KT * vstride), s.nk - t * KT, to + TILE);
   };
-  if (steps > 0) issue(0, 0);
+  if (steps > 0)
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
   Frag<T> q[DP / 16];
   {
     const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
@@ -145,25 +137,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   const Reader<T, DP> read;
   // tiles that every column sees whole
   const int whole = std::min(fewest / KT, steps);
-  int t = 0;
-  const auto step = [&](auto STAGE) {
+  ring<STAGES>(whole, 0, [&](int t, auto STAGE) {
     constexpr int stage = decltype(STAGE)::value;
-    wait_loads_and_meet<0>();
-    if (t + 1 < steps) issue(t + 1, stage ^ 1);
+    wait_loads_and_meet<AHEAD>();
+    issue(t + STAGES - 1, (stage + STAGES - 1) % STAGES);
     lds_char *kt = (lds_char *)lds + stage * 2 * TILE;
     attend_tile<false, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, 0);
-  };
-  while (t < whole) {
-    step(std::integral_constant<int, 0>{});
-    if (++t == whole) break;
-    step(std::integral_constant<int, 1>{});
-    ++t;
-  }
+  });
   // the others
-  for (; t < steps; ++t) {
-    wait_loads_and_meet<0>();
-    if (t + 1 < steps) issue(t + 1, (t + 1) & 1);
-    lds_char *kt = (lds_char *)lds + (t & 1) * 2 * TILE;
+  for (int t = whole; t < steps; ++t) {
+    wait_loads_and_meet<AHEAD>();
+    issue(t + STAGES - 1, (t + STAGES - 1) % STAGES);
+    lds_char *kt = (lds_char *)lds + t % STAGES * 2 * TILE;
     // (the same for the whole block)
     const bool found = a.causal && __syncthreads_or(clear_not_finite<T, DP, KT, 256>(kt + TILE, threadIdx.x));
     if (t < own) {
@@ -174,6 +159,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
                               [&](int x) { return x < mine; });
     }
   }
+  wait_loads();  // (none may land in the LDS of a block that follows)
   const float l = c.l + other_half(c.l);
   const bool there = column < total;
   store_column<T, DP>(o + ((s.q0 + i) * a.heads + head) * a.d, a.d, there, c.o, l == 0.f ? 0.f : 1.f / l);
@@ -419,8 +405,6 @@ static Plan plan(const spira_hip_attention_t &x) {
   return {true, static_cast<int>(std::min<int64_t>(part, int64_t(1) << 30)), div_up(x.keys, part)};
 }
 
-size_t gradient_bytes(const spira_hip_attention_t &x);  // (attention_backward.hip)
-
 static size_t partial_bytes(const spira_hip_attention_t &x, const Plan &p) {
   return p.tokens && p.parts > 1 ? static_cast<size_t>(p.parts) * x.rows * x.heads * (x.head_dim + 2) * sizeof(float) : 0;
 }
@@ -468,7 +452,7 @@ extern "C" {
 int spira_hip_attention_workspace(const spira_hip_attention_t *x, int gradient, size_t *bytes) {
   SPIRA_HIP_REQUIRE(x && bytes, "attention: null arguments");
   if (int rc = attention::check(*x)) return rc;
-  *bytes = gradient ? attention::gradient_bytes(*x) : attention::partial_bytes(*x, attention::plan(*x));
+  *bytes = gradient ? attention::delta_bytes(*x) + attention::key_sums_bytes(*x) : attention::partial_bytes(*x, attention::plan(*x));
   return kOk;
 }
 

@@ -279,6 +279,32 @@ template <class T, int DP, int R, int NT, bool DMA> struct Fetch {
   }
 };
 
+// Stages of two tiles each that a block holds: what is fetched arrives one step later
+// with two of them, two steps later with three.
+template <class T, int DP> constexpr int kStages = Rows<T, DP>::PITCH <= 128 ? 3 : 2;
+
+// step(t, stage) for t in [0, n), the stages in turn from `first` on
+template <int STAGES, class Step> __device__ __forceinline__ void ring(int n, int first, Step &&step) {
+  using std::integral_constant;
+  int skip = first;
+  for (int t = 0; t < n;) {
+    if (skip-- <= 0) {
+      step(t, integral_constant<int, 0>{});
+      if (++t == n) break;
+    }
+    if (skip-- <= 0) {
+      step(t, integral_constant<int, 1>{});
+      if (++t == n) break;
+    }
+    if constexpr (STAGES == 3)
+      if (skip-- <= 0) {
+        step(t, integral_constant<int, 2>{});
+        ++t;
+      }
+    skip = 0;
+  }
+}
+
 // the larger (or the sum) of the two halves' values of a column
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
@@ -408,6 +434,41 @@ struct Args {
   float *delta;  // [heads, rows]
   void *dq, *dk, *dv;
 };
+
+// ---------------------------------------------------------------------------
+// columns of queries
+// ---------------------------------------------------------------------------
+constexpr int kColumns = 128;  // of a block: a key head's query heads and their queries, heads fastest
+// keys of a tile
+template <class T> constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
+
+// keys that query i of a sequence sees
+__device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) {
+  if (!a.causal) return s.nk;
+  const int n = i + 1 + s.nk - s.nq;
+  return n < 0 ? 0 : n < s.nk ? n : s.nk;
+}
+
+// a row's statistics, and p from a raw score
+template <class T> struct Stat {
+  float base, by;
+};
+template <class T> __device__ __forceinline__ float weight(float s, float scale2, const Stat<T> &r) {
+  const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale2, -r.base));
+  // (in fp32 the logarithm of the sum would be rounded to as much as 1e-6 of p)
+  return sizeof(T) == 2 ? e : e * r.by;
+}
+
+int arguments(const spira_hip_attention_t &x, Args &a, int size);  // (attention.hip)
+// (attention_keys.hip)
+int key_splits(const spira_hip_attention_t &x);
+size_t key_sums_bytes(const spira_hip_attention_t &x);
+int key_gradients(const spira_hip_attention_t &x, const Args &a, hipStream_t stream);
+
+// bytes of the gradients' workspace before the keys' sums: delta
+inline size_t delta_bytes(const spira_hip_attention_t &x) {
+  return round_up(static_cast<int64_t>(x.rows) * x.heads * static_cast<int64_t>(sizeof(float)), 256);
+}
 
 }  // namespace attention
 
