@@ -92,6 +92,40 @@ template <class Pieces> __device__ __forceinline__ Found find_piece(int count, i
   return {-1, 0, 0};
 }
 
+// Piece `index` in the order of what is left of its sequence from it on, the most
+// first: with a causal mask that is a piece's work, and the longest begin first.  nth
+// is what is left behind it (0: the sequence's last).  Lanes hold the sequences; of more
+// than 64, sequence by sequence.
+template <class Pieces> __device__ __forceinline__ Found find_longest(int count, int64_t index, Pieces &&pieces) {
+  if (count > 64) {
+    Found f = find_piece(count, index, pieces);
+    f.nth = f.of - 1 - f.nth;
+    return f;
+  }
+  const int lane = lane_id(), n = lane < count ? pieces(lane) : 0;
+  // pieces with more than r left behind them and themselves: the sum of max(0, n - r)
+  const auto longer = [&](int r) {
+    int64_t sum = n > r ? n - r : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    return uniform(sum);
+  };
+  int most = n;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) most = std::max(most, __shfl_xor(most, o, 64));
+  int lo = 0, hi = uniform(most);  // longer(lo) > index >= longer(hi)
+  if (longer(0) <= index) return {-1, 0, 0};
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (longer(mid) > index) lo = mid;
+    else hi = mid;
+  }
+  const int64_t rank = index - longer(hi);
+  const uint64_t held = ballot(n >= hi);
+  const int b = __builtin_ctzll(ballot((held >> lane & 1) && lane_prefix(held) == rank));
+  return {uniform(b), hi - 1, uniform(__shfl(n, b, 64))};
+}
+
 // zeros in the rows (of `width` values) that no sequence covers, by the launch's
 // blocks together
 template <class T>
@@ -279,29 +313,19 @@ template <class T, int DP, int R, int NT, bool DMA> struct Fetch {
   }
 };
 
-// Stages of two tiles each that a block holds: what is fetched arrives one step later
-// with two of them, two steps later with three.
-template <class T, int DP> constexpr int kStages = Rows<T, DP>::PITCH <= 128 ? 3 : 2;
-
-// step(t, stage) for t in [0, n), the stages in turn from `first` on
-template <int STAGES, class Step> __device__ __forceinline__ void ring(int n, int first, Step &&step) {
+// step(t, stage) for t in [0, n), the two stages in turn from `first` on
+template <class Step> __device__ __forceinline__ void ring(int n, int first, Step &&step) {
   using std::integral_constant;
-  int skip = first;
-  for (int t = 0; t < n;) {
-    if (skip-- <= 0) {
-      step(t, integral_constant<int, 0>{});
-      if (++t == n) break;
-    }
-    if (skip-- <= 0) {
-      step(t, integral_constant<int, 1>{});
-      if (++t == n) break;
-    }
-    if constexpr (STAGES == 3)
-      if (skip-- <= 0) {
-        step(t, integral_constant<int, 2>{});
-        ++t;
-      }
-    skip = 0;
+  int t = 0;
+  if (first == 1 && n > 0) {
+    step(0, integral_constant<int, 1>{});
+    t = 1;
+  }
+  while (t < n) {
+    step(t, integral_constant<int, 0>{});
+    if (++t == n) break;
+    step(t, integral_constant<int, 1>{});
+    ++t;
   }
 }
 

@@ -22,20 +22,18 @@ namespace attention {
 template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(const Args a) {
   using R = Rows<T, DP>;
-  constexpr int KT = kKeys<T>, TILE = KT * R::PITCH, STAGES = kStages<T, DP>;
-  using Fetcher = Fetch<T, DP, KT, 256, DMA>;
-  constexpr int AHEAD = DMA ? 2 * Fetcher::LOADS * (STAGES - 2) : 0;  // loads under way behind a stage's own
-  __shared__ __align__(1024) char lds[STAGES * 2 * TILE];
+  constexpr int KT = kKeys<T>, TILE = KT * R::PITCH;
+  __shared__ __align__(1024) char lds[4 * TILE];
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id(), h = lane >> 5;
   T *dq = static_cast<T *>(a.dq);
   if (dq)
     clear_uncovered(a.s.offsets, a.s.count, a.s.rows, dq, static_cast<int64_t>(a.heads) * a.d, blockIdx.x, gridDim.x);
   const int kv = blockIdx.x % a.kv_heads;
-  const Found f = find_piece(a.s.count, blockIdx.x / a.kv_heads,
-                             [&](int b) { return (queries_of(a.s, b) * a.group + kColumns - 1) / kColumns; });
+  const Found f = find_longest(a.s.count, blockIdx.x / a.kv_heads,
+                               [&](int b) { return (queries_of(a.s, b) * a.group + kColumns - 1) / kColumns; });
   if (f.sequence < 0) return;
   const Sequence s = sequence_at(a.s, f.sequence);
-  const int total = s.nq * a.group, c0 = (f.of - 1 - f.nth) * kColumns, w0 = c0 + wave * 32;
+  const int total = s.nq * a.group, c0 = f.nth * kColumns, w0 = c0 + wave * 32;
   const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
   const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i);
   const int fewest = visible(a, s, c0 / a.group), end = dq ? visible(a, s, std::min(c0 + kColumns - 1, total - 1) / a.group) : 0;
@@ -43,15 +41,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
   const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
   const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + s.k0 * a.k_row + kv * a.k_head);
   const char *values = reinterpret_cast<const char *>(static_cast<const T *>(a.v) + s.k0 * a.v_row + kv * a.v_head);
-  const Fetcher fetch_keys(kstride, a.d, threadIdx.x), fetch_values(vstride, a.d, threadIdx.x);
+  const Fetch<T, DP, KT, 256, DMA> fetch_keys(kstride, a.d, threadIdx.x), fetch_values(vstride, a.d, threadIdx.x);
   const auto issue = [&](int t, int stage) {
     lds_char *to = (lds_char *)lds + stage * 2 * TILE;
     fetch_keys(keys + t * (KT * kstride), s.nk - t * KT, to);
     fetch_values(values + t * (KT * vstride), s.nk - t * KT, to + TILE);
   };
-  if (steps > 0)
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
+  if (steps > 0) issue(0, 0);
   const int64_t at = (s.q0 + i) * a.heads + head;
   Frag<T> q[DP / 16], g[DP / 16];
   const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
@@ -99,10 +95,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
     }
   };
   const int whole = std::min(fewest / KT, steps);  // tiles that every column sees whole
-  ring<STAGES>(whole, 0, [&](int t, auto STAGE) {
+  ring(whole, 0, [&](int t, auto STAGE) {
     constexpr int stage = decltype(STAGE)::value;
-    wait_loads_and_meet<AHEAD>();
-    issue(t + STAGES - 1, (stage + STAGES - 1) % STAGES);
+    wait_loads_and_meet<0>();
+    if (t + 1 < steps) issue(t + 1, stage ^ 1);
     lds_char *kt = (lds_char *)lds + stage * 2 * TILE;
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u) {
@@ -113,11 +109,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
   });
   // the others; the block stays together
   for (int t = whole; t < steps; ++t) {
-    wait_loads_and_meet<AHEAD>();
-    issue(t + STAGES - 1, (t + STAGES - 1) % STAGES);
+    wait_loads_and_meet<0>();
+    if (t + 1 < steps) issue(t + 1, (t + 1) & 1);
 #pragma unroll 1
     for (int u = 0; u < KT / 32; ++u) {
-      lds_char *kt = (lds_char *)lds + t % STAGES * 2 * TILE + 32 * u * R::PITCH;
+      lds_char *kt = (lds_char *)lds + (t & 1) * 2 * TILE + 32 * u * R::PITCH;
       const int first = t * KT + 32 * u, seen = limit - first;
       floatx16 ds;
       gradients(std::true_type{}, kt, kt + TILE, seen, ds);
@@ -132,7 +128,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
                               [&](int x) { return x < seen; });
     }
   }
-  wait_loads();  // (none may land in the LDS of a block that follows)
   if (dq) store_column<T, DP>(dq + at * a.d, a.d, there, acc, a.scale);
 }
 

@@ -24,24 +24,20 @@ template <class T> constexpr int kQueries = sizeof(T) == 2 ? 64 : 32;
 template <class T, int DP, bool DMA, bool SPLIT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_kernel(const Args a) {
   using R = Rows<T, DP>;
-  constexpr int QT = kQueries<T>, TILE = QT * R::PITCH, STAGES = kStages<T, DP>;
-  using Fetcher = Fetch<T, DP, QT, 256, DMA>;
-  // loads under way behind a stage's own: two tiles' and a wave's row of statistics
-  constexpr int AHEAD = (DMA ? 2 * Fetcher::LOADS + 1 : 1) * (STAGES - 2);
-  __shared__ __align__(1024) char lds[STAGES * 2 * TILE];
-  __shared__ __align__(256) float rows[STAGES][4][64];  // statistics, delta and the sum's inverse of a tile's rows
+  constexpr int QT = kQueries<T>, TILE = QT * R::PITCH;
+  __shared__ __align__(1024) char lds[4 * TILE];
+  __shared__ __align__(256) float rows[2][4][64];  // statistics, delta and the sum's inverse of a tile's rows
   const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id(), h = lane >> 5;
   T *dk = static_cast<T *>(a.dk), *dv = static_cast<T *>(a.dv);
   const int64_t width = static_cast<int64_t>(a.kv_heads) * a.d;
   if (!SPLIT && dk) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dk, width, blockIdx.x, gridDim.x);
   if (!SPLIT && dv) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dv, width, blockIdx.x, gridDim.x);
   const int kv = blockIdx.x % a.kv_heads;
-  const Found f = find_piece(a.s.count, blockIdx.x / a.kv_heads,
-                             [&](int b) { return static_cast<int>((room_of(a.s, b) + int64_t(kOwnKeys) - 1) / kOwnKeys); });
+  const Found f = find_longest(a.s.count, blockIdx.x / a.kv_heads,
+                               [&](int b) { return static_cast<int>((room_of(a.s, b) + int64_t(kOwnKeys) - 1) / kOwnKeys); });
   if (f.sequence < 0) return;
   const Sequence s = sequence_at(a.s, f.sequence);
-  // (the first tile first: the most queries see it)
-  const int c0 = f.nth * kOwnKeys, w0 = c0 + wave * 32, key = w0 + (lane & 31);
+  const int c0 = (f.of - 1 - f.nth) * kOwnKeys, w0 = c0 + wave * 32, key = w0 + (lane & 31);
   const bool there = key < s.nk;
   // the first query that sees a key
   const auto first_of = [&](int k) { return a.causal ? std::max(0, k - (s.nk - s.nq)) : 0; };
@@ -61,7 +57,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   const auto gradients_of = [&](int head) {
     return reinterpret_cast<const char *>(static_cast<const T *>(a.dout) + static_cast<int64_t>(head) * a.d);
   };
-  const Fetcher fetch_queries(qstride, a.d, threadIdx.x), fetch_gradients(gstride, a.d, threadIdx.x);
+  const Fetch<T, DP, QT, 256, DMA> fetch_queries(qstride, a.d, threadIdx.x), fetch_gradients(gstride, a.d, threadIdx.x);
   const auto issue = [&](int stage, int g, int t) {
     lds_char *to = (lds_char *)lds + stage * 2 * TILE;
     const int head = kv * a.group + g;
@@ -95,12 +91,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   Where next{0, begin, 0};  // to be fetched
   if (steps > 0) advance(next, part);
   Where now = next;  // at hand
-  if (steps > 0)
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      issue(i, next.g, i < steps ? next.t : end);
-      advance(next, splits);
-    }
+  if (steps > 0) {
+    issue(0, next.g, next.t);
+    advance(next, splits);
+  }
   Frag<T> k[DP / 16], v[DP / 16];
   {
     const T *krow = there ? static_cast<const T *>(a.k) + (s.k0 + key) * a.k_row + kv * a.k_head : nullptr;
@@ -147,10 +141,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
     }
   };
   for (int index = 0; index < hidden; ++index) {
-    wait_loads_and_meet<AHEAD>();
-    issue((index + STAGES - 1) % STAGES, next.g, index + STAGES - 1 < steps ? next.t : end);
-    advance(next, splits);
-    const int stage = index % STAGES, q0 = now.t * QT, head = kv * a.group + now.g;
+    wait_loads_and_meet<0>();
+    if (index + 1 < steps) {
+      issue((index + 1) & 1, next.g, next.t);
+      advance(next, splits);
+    }
+    const int stage = index & 1, q0 = now.t * QT, head = kv * a.group + now.g;
     advance(now, splits);
 #pragma unroll 1
     for (int u = 0; u < QT / 32; ++u) {
@@ -172,11 +168,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       }
     }
   }
-  ring<STAGES>(steps - hidden, hidden % STAGES, [&](int index, auto STAGE) {
+  ring(steps - hidden, hidden & 1, [&](int index, auto STAGE) {
     constexpr int stage = decltype(STAGE)::value;
-    wait_loads_and_meet<AHEAD>();
-    issue((stage + STAGES - 1) % STAGES, next.g, hidden + index + STAGES - 1 < steps ? next.t : end);
-    advance(next, splits);
+    wait_loads_and_meet<0>();
+    if (hidden + index + 1 < steps) {
+      issue(stage ^ 1, next.g, next.t);
+      advance(next, splits);
+    }
     if (w0 >= s.nk) return;
     lds_char *qt = (lds_char *)lds + stage * 2 * TILE, *gt = qt + TILE;
 #pragma unroll
@@ -187,7 +185,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       accumulate(ak, qt + 32 * u * R::PITCH, ds);
     }
   });
-  wait_loads();  // (none may land in the LDS of a block that follows)
   // (keys that are none, in the room behind the others, get zeros)
   if (!there) {
 #pragma unroll
