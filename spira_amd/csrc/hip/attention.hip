@@ -87,6 +87,19 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
   }
 }
 
+// a row's statistics for the gradients, from its reference and sum
+template <class T>
+__device__ __forceinline__ void put_statistics(const Args &a, int head, int64_t row, float m, float l) {
+  float *to = a.stats + head * a.s.rows + row;
+  const float base = m == -__builtin_inff() ? 0.f : m * a.scale2;
+  if constexpr (sizeof(T) == 2) {
+    *to = l == 0.f ? __builtin_inff() : base + __builtin_amdgcn_logf(l);
+  } else {
+    to[0] = base;
+    to[a.heads * a.s.rows] = l == 0.f ? 0.f : 1.f / l;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // prompts
 // ---------------------------------------------------------------------------
@@ -101,11 +114,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   // (key heads fastest: where their number divides 8 or 8 it, an XCD's blocks share
   // few heads' keys)
   const int kv = blockIdx.x % a.kv_heads;
-  const Found f = find_longest(a.s.count, blockIdx.x / a.kv_heads,
-                               [&](int b) { return (queries_of(a.s, b) * a.group + kColumns - 1) / kColumns; });
-  if (f.sequence < 0) return;
-  const Sequence s = sequence_at(a.s, f.sequence);
-  const int total = s.nq * a.group, c0 = f.nth * kColumns, w0 = c0 + wave * 32;
+  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads,
+                               [&](const Sequence &x) { return (x.nq * a.group + kColumns - 1) / kColumns; });
+  if (!s.there) return;
+  const int total = s.nq * a.group, c0 = s.nth * kColumns, w0 = c0 + wave * 32;
   const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
   const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i);
   const int most = w0 < total ? visible(a, s, std::min(w0 + 31, total - 1) / a.group) : 0;
@@ -157,29 +169,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   const float l = c.l + other_half(c.l);
   const bool there = column < total;
   store_column<T, DP>(o + ((s.q0 + i) * a.heads + head) * a.d, a.d, there, c.o, l == 0.f ? 0.f : 1.f / l);
-  if (a.stats && there && lane < 32) {
-    float *to = a.stats + head * a.s.rows + s.q0 + i;
-    const float base = c.m == -__builtin_inff() ? 0.f : c.m * a.scale2;
-    if constexpr (sizeof(T) == 2) {
-      *to = l == 0.f ? __builtin_inff() : base + __builtin_amdgcn_logf(l);
-    } else {
-      to[0] = base;
-      to[a.heads * a.s.rows] = l == 0.f ? 0.f : 1.f / l;
-    }
-  }
+  if (a.stats && there && lane < 32) put_statistics<T>(a, head, s.q0 + i, c.m, l);
 }
 
 // ---------------------------------------------------------------------------
 // few tokens
 // ---------------------------------------------------------------------------
-template <class T, int DP> constexpr int kTokenWaves = Rows<T, DP>::PITCH >= 512 ? 2 : 4;
+template <class T, int DP> constexpr int kTokenWaves = Rows<T, DP>::PITCH >= 256 ? 2 : 4;
 
 // DIRECT: no sequence has more than one part; the outputs themselves
 template <class T, int DP, bool DIRECT, bool DMA>
 __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)) void token_kernel(const Args a) {
   using R = Rows<T, DP>;
   constexpr int KT = 32, TILE = KT * R::PITCH, NW = kTokenWaves<T, DP>, NT = 64 * NW;
-  constexpr int LOADS = 2 * KT * R::CPR / 64, OPITCH = DP + 4;  // (of the sums in LDS)
+  constexpr int LOADS = 2 * KT * R::CPR / 64, OPITCH = kSumPitch<DP>;
   static_assert(32 * OPITCH * 4 <= 4 * TILE, "a wave's sums take its stages' place");
   __shared__ __align__(1024) char lds[NW][4 * TILE];
   __shared__ float wm[NW][32], wl[NW][32], top[32], total_l[32];
@@ -191,22 +194,23 @@ __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)
                     blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x,
                     static_cast<int64_t>(gridDim.x) * gridDim.y);
   const int kv = blockIdx.x % a.kv_heads;
-  // (a sequence without keys has a part of none where its outputs are written here)
-  const Found f = find_piece(a.s.count, blockIdx.x / a.kv_heads, [&](int b) {
-    const int n = (keys_of(a.s, b) + a.part_keys - 1) / a.part_keys;
-    return queries_of(a.s, b) == 0 ? 0 : DIRECT ? 1 : n;
-  });
-  if (f.sequence < 0) return;
-  const Sequence s = sequence_at(a.s, f.sequence);
-  const int first = f.nth * a.part_keys, total = s.nq * a.group;
+  // DIRECT: a piece is 32 columns (whose outputs are written without keys too); else a
+  // part of the keys, for columns from blockIdx.y on
+  const Found s = DIRECT ? find_longest(a.s, blockIdx.x / a.kv_heads,
+                                        [&](const Sequence &x) { return (x.nq * a.group + 31) / 32; })
+                         : find_piece(a.s, blockIdx.x / a.kv_heads, [&](const Sequence &x) {
+                             return x.nq == 0 ? 0 : (x.nk + a.part_keys - 1) / a.part_keys;
+                           });
+  if (!s.there) return;
+  const int first = DIRECT ? 0 : s.nth * a.part_keys, total = s.nq * a.group;
   const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
   const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + (s.k0 + first) * a.k_row + kv * a.k_head);
   const char *values =
       reinterpret_cast<const char *>(static_cast<const T *>(a.v) + (s.k0 + first) * a.v_row + kv * a.v_head);
-  const int part = std::min(s.nk - first, a.part_keys);
+  const int part = DIRECT ? s.nk : std::min(s.nk - first, a.part_keys);
   const Fetch<T, DP, KT, 64, DMA> fetch_keys(kstride, a.d, lane), fetch_values(vstride, a.d, lane);
   const Reader<T, DP> read;
-  for (int w0 = blockIdx.y * 32; w0 < total; w0 += gridDim.y * 32) {
+  for (int w0 = (DIRECT ? s.nth : blockIdx.y) * 32; w0 < total; w0 += gridDim.y * 32) {
     const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
     const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i) - first;
     const int least = visible(a, s, w0 / a.group) - first;
@@ -245,13 +249,7 @@ __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)
     wait_loads();
     asm volatile("" ::: "memory");
     // the waves' columns to LDS, and their sum from there
-    float *sums = reinterpret_cast<float *>(lds[wave]) + (lane & 31) * OPITCH + 4 * (lane >> 5);
-#pragma unroll
-    for (int n = 0; n < DP / 32; ++n)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<floatx4_t *>(sums + 32 * n + 8 * g) =
-            floatx4_t{c.o[n][4 * g], c.o[n][4 * g + 1], c.o[n][4 * g + 2], c.o[n][4 * g + 3]};
+    put_sums<DP>(reinterpret_cast<float *>(lds[wave]), c.o);
     const float l = c.l + other_half(c.l);
     if (lane < 32) {
       wm[wave][lane] = c.m;
@@ -282,15 +280,18 @@ __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)
       const int64_t at = (s.q0 + q_at) * a.heads + h_at;
       const float sum = total_l[col];
       if constexpr (DIRECT) o[at * a.d + d] = from_float<T>(sum == 0.f ? 0.f : v / sum);
-      else a.partial[(f.nth * a.s.rows * a.heads + at) * a.d + d] = v;
+      else a.partial[(s.nth * a.s.rows * a.heads + at) * a.d + d] = v;
     }
-    if constexpr (!DIRECT)
-      if (static_cast<int>(threadIdx.x) < columns) {
+    if constexpr (DIRECT) {
+      if (a.stats && static_cast<int>(threadIdx.x) < columns)
+        put_statistics<T>(a, head, s.q0 + i, top[lane], total_l[lane]);
+      return;
+    } else if (static_cast<int>(threadIdx.x) < columns) {
         const int q_at = (w0 + lane) / a.group, h_at = kv * a.group + (w0 + lane - q_at * a.group);
-        float *to = a.partial_stats + (f.nth * a.s.rows * a.heads + (s.q0 + q_at) * a.heads + h_at) * 2;
+        float *to = a.partial_stats + (s.nth * a.s.rows * a.heads + (s.q0 + q_at) * a.heads + h_at) * 2;
         to[0] = top[lane] == -__builtin_inff() ? top[lane] : top[lane] * a.scale2;
         to[1] = total_l[lane];
-      }
+    }
     __syncthreads();  // (the next columns' tiles take the sums' place)
   }
 }
@@ -307,7 +308,7 @@ template <class T> __global__ __launch_bounds__(256) void join_kernel(const Args
     const bool mine = b < a.s.count && row >= a.s.offsets[b] && row < a.s.offsets[b + 1];
     const uint64_t found = ballot(mine);
     if (found) {
-      parts = (keys_of(a.s, first + __builtin_ctzll(found)) + a.part_keys - 1) / a.part_keys;
+      parts = (sequence_at(a.s, first + __builtin_ctzll(found)).nk + a.part_keys - 1) / a.part_keys;
       break;
     }
   }
@@ -387,16 +388,21 @@ struct Plan {
   int part_keys;
   int64_t parts;  // most of a sequence
 };
-static Plan plan(const spira_hip_attention_t &x) {
+static Plan plan(const spira_hip_attention_t &x, bool stats) {
   const int64_t group = x.heads / x.kv_heads, columns = div_up(x.rows * group, x.sequences);
-  if (columns > 64) return {false, 0, 0};
+  const Plan prompts{false, 0, 0}, direct{true, 1, 1};
+  const int64_t blocks = (x.rows * group / kColumns + x.sequences) * x.kv_heads;
+  // (a gradient's statistics come from one block per column)
+  if (columns > 64 || stats) return blocks < kFewBlocks ? direct : prompts;
   const int64_t tiles = div_up(columns, 32);
-  const int64_t size = round_up(std::max<int64_t>(div_up(x.keys * x.kv_heads * tiles, 1024), 256), 128);
+  const int64_t size = round_up(std::max<int64_t>(div_up(x.keys * x.kv_heads * tiles, 2048), 256), 64);
   // (partial sums of at most 256 MB)
   int64_t part = size;
   while (x.rows * x.heads * div_up(x.keys, part) * (x.head_dim + 2) * 4 > (int64_t(1) << 28) && part < x.keys)
     part *= 2;
-  return {true, static_cast<int>(std::min<int64_t>(part, int64_t(1) << 30)), div_up(x.keys, part)};
+  // (no sequence has keys for more than four parts: a join would cost more)
+  if (x.keys <= 4 * part) return direct;
+  return {true, static_cast<int>(part), div_up(x.keys, part)};
 }
 
 static size_t partial_bytes(const spira_hip_attention_t &x, const Plan &p) {
@@ -415,8 +421,8 @@ template <class T, int DP, bool DMA> static int launch_form(const Args &base, co
   a.part_keys = p.part_keys;
   constexpr int threads = 64 * kTokenWaves<T, DP>;
   const bool direct = p.parts <= 1;
-  const int64_t blocks = (direct ? a.s.count : a.s.keys / p.part_keys + a.s.count) * a.kv_heads;
-  const uint32_t y = static_cast<uint32_t>(div_up(div_up(a.s.rows * a.group, a.s.count), 32));
+  const int64_t blocks = ((direct ? a.s.rows * a.group / 32 : a.s.keys / p.part_keys) + a.s.count) * a.kv_heads;
+  const uint32_t y = direct ? 1 : static_cast<uint32_t>(div_up(div_up(a.s.rows * a.group, a.s.count), 32));
   SPIRA_HIP_REQUIRE(launchable(blocks * y, threads), "attention: too many tiles for a launch");
   if (direct)
     hipLaunchKernelGGL((token_kernel<T, DP, true, DMA>), dim3(blocks, y), dim3(threads), 0, stream, a);
@@ -446,7 +452,7 @@ extern "C" {
 int spira_hip_attention_workspace(const spira_hip_attention_t *x, int gradient, size_t *bytes) {
   SPIRA_HIP_REQUIRE(x && bytes, "attention: null arguments");
   if (int rc = attention::check(*x)) return rc;
-  *bytes = gradient ? attention::delta_bytes(*x) + attention::key_sums_bytes(*x) : attention::partial_bytes(*x, attention::plan(*x));
+  *bytes = gradient ? attention::delta_bytes(*x) + attention::key_sums_bytes(*x) : attention::partial_bytes(*x, attention::plan(*x, false));
   return kOk;
 }
 
@@ -457,8 +463,7 @@ int spira_hip_attention(const spira_hip_attention_t *x, void *out, float *stats,
   if (int rc = attention::arguments(*x, a, x->dtype == SPIRA_F32 ? 4 : 2)) return rc;
   if (x->rows == 0) return kOk;
   SPIRA_HIP_REQUIRE(out, "attention: null output");
-  // (a gradient's statistics come from the prompts' form)
-  const attention::Plan p = stats ? attention::Plan{false, 0, 0} : attention::plan(*x);
+  const attention::Plan p = attention::plan(*x, stats != nullptr);
   const size_t need = attention::partial_bytes(*x, p);
   SPIRA_HIP_REQUIRE(workspace_bytes >= need && (workspace || need == 0), "attention: workspace too small");
   a.o = out;

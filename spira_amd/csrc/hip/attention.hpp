@@ -46,35 +46,41 @@ struct Sequence {
 
 // (whatever the numbers are, no row outside the tensors)
 __device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t most) { return v < 0 ? 0 : v > most ? most : v; }
-__device__ __forceinline__ int queries_of(const Sequences &s, int b) {
-  const int64_t lo = clamp_row(s.offsets[b], s.rows), hi = clamp_row(s.offsets[b + 1], s.rows);
-  return hi > lo ? static_cast<int>(hi - lo) : 0;
-}
-__device__ __forceinline__ int room_of(const Sequences &s, int b) {
-  const int64_t lo = clamp_row(s.key_offsets[b], s.keys), hi = clamp_row(s.key_offsets[b + 1], s.keys);
-  return hi > lo ? static_cast<int>(hi - lo) : 0;
-}
-__device__ __forceinline__ int keys_of(const Sequences &s, int b) {
-  const int room = room_of(s, b);
-  if (!s.key_counts) return room;
-  const int n = s.key_counts[b];
-  return n < 0 ? 0 : n < room ? n : room;
-}
 __device__ __forceinline__ Sequence sequence_at(const Sequences &s, int b) {
-  return {uniform(clamp_row(s.offsets[b], s.rows)), uniform(clamp_row(s.key_offsets[b], s.keys)),
-          uniform(queries_of(s, b)), uniform(keys_of(s, b)), uniform(room_of(s, b))};
+  const int64_t q0 = clamp_row(s.offsets[b], s.rows), q1 = clamp_row(s.offsets[b + 1], s.rows);
+  const int64_t k0 = clamp_row(s.key_offsets[b], s.keys), k1 = clamp_row(s.key_offsets[b + 1], s.keys);
+  const int counted = s.key_counts ? s.key_counts[b] : INT32_MAX;
+  Sequence r{q0, k0, q1 > q0 ? static_cast<int>(q1 - q0) : 0, 0, k1 > k0 ? static_cast<int>(k1 - k0) : 0};
+  r.nk = counted < 0 ? 0 : counted < r.room ? counted : r.room;
+  return r;
 }
 
-struct Found {
-  int sequence;  // -1: past the last
-  int nth, of;   // the piece within its sequence, and their number
+// Which sequence, and which piece of it.  A lane holds a sequence's numbers while the
+// wave looks; the one found goes to all from there.
+struct Found : Sequence {
+  bool there;
+  int nth, of;  // the piece within its sequence, and their number
 };
-// Piece `index` of the sequences cut into pieces(b) each, the same on every lane.
-template <class Pieces> __device__ __forceinline__ Found find_piece(int count, int64_t index, Pieces &&pieces) {
+__device__ __forceinline__ Found found_at(const Sequence &held, int lane, int nth, int of) {
+  Found f;
+  f.q0 = uniform(static_cast<int64_t>(__shfl(held.q0, lane, 64)));
+  f.k0 = uniform(static_cast<int64_t>(__shfl(held.k0, lane, 64)));
+  f.nq = uniform(__shfl(held.nq, lane, 64));
+  f.nk = uniform(__shfl(held.nk, lane, 64));
+  f.room = uniform(__shfl(held.room, lane, 64));
+  f.there = true;
+  f.nth = uniform(nth);
+  f.of = uniform(of);
+  return f;
+}
+// Piece `index` of the sequences cut into pieces(sequence) each, the same on every lane.
+template <class Pieces> __device__ __forceinline__ Found find_piece(const Sequences &s, int64_t index, Pieces &&pieces) {
   const int lane = lane_id();
   int64_t before = 0;
-  for (int first = 0; first < count; first += 64) {
-    const int b = first + lane, n = b < count ? pieces(b) : 0;
+  for (int first = 0; first < s.count; first += 64) {
+    const int b = first + lane;
+    const Sequence held = sequence_at(s, b < s.count ? b : s.count - 1);
+    const int n = b < s.count ? pieces(held) : 0;
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
@@ -83,27 +89,28 @@ template <class Pieces> __device__ __forceinline__ Found find_piece(int count, i
     }
     const uint64_t past = ballot(before + upto > index);
     if (past) {
-      const int at = __builtin_ctzll(past);
-      const int of = __shfl(n, at, 64);
-      return {uniform(first + at), uniform(static_cast<int>(index - before - (__shfl(upto, at, 64) - of))), uniform(of)};
+      const int at = __builtin_ctzll(past), of = __shfl(n, at, 64);
+      return found_at(held, at, static_cast<int>(index - before - (__shfl(upto, at, 64) - of)), of);
     }
     before += __shfl(upto, 63, 64);
   }
-  return {-1, 0, 0};
+  return Found{};
 }
 
 // Piece `index` in the order of what is left of its sequence from it on, the most
 // first: with a causal mask that is a piece's work, and the longest begin first.  nth
 // is what is left behind it (0: the sequence's last).  Lanes hold the sequences; of more
 // than 64, sequence by sequence.
-template <class Pieces> __device__ __forceinline__ Found find_longest(int count, int64_t index, Pieces &&pieces) {
-  if (count > 64) {
-    Found f = find_piece(count, index, pieces);
+template <class Pieces> __device__ __forceinline__ Found find_longest(const Sequences &s, int64_t index, Pieces &&pieces) {
+  if (s.count > 64) {
+    Found f = find_piece(s, index, pieces);
     f.nth = f.of - 1 - f.nth;
     return f;
   }
-  const int lane = lane_id(), n = lane < count ? pieces(lane) : 0;
-  // pieces with more than r left behind them and themselves: the sum of max(0, n - r)
+  const int lane = lane_id();
+  const Sequence held = sequence_at(s, lane < s.count ? lane : s.count - 1);
+  const int n = lane < s.count ? pieces(held) : 0;
+  // pieces with more than r left, themselves among it: the sum of max(0, n - r)
   const auto longer = [&](int r) {
     int64_t sum = n > r ? n - r : 0;
 #pragma unroll
@@ -114,16 +121,16 @@ template <class Pieces> __device__ __forceinline__ Found find_longest(int count,
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) most = std::max(most, __shfl_xor(most, o, 64));
   int lo = 0, hi = uniform(most);  // longer(lo) > index >= longer(hi)
-  if (longer(0) <= index) return {-1, 0, 0};
+  if (longer(0) <= index) return Found{};
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (longer(mid) > index) lo = mid;
     else hi = mid;
   }
   const int64_t rank = index - longer(hi);
-  const uint64_t held = ballot(n >= hi);
-  const int b = __builtin_ctzll(ballot((held >> lane & 1) && lane_prefix(held) == rank));
-  return {uniform(b), hi - 1, uniform(__shfl(n, b, 64))};
+  const uint64_t level = ballot(n >= hi);
+  const int b = __builtin_ctzll(ballot((level >> lane & 1) && lane_prefix(level) == rank));
+  return found_at(held, b, hi - 1, __shfl(n, b, 64));
 }
 
 // zeros in the rows (of `width` values) that no sequence covers, by the launch's
@@ -437,6 +444,19 @@ template <class F> int with_width(int d, F &&f) {
   return f(integral_constant<int, 128>{});
 }
 
+// The sums of a wave's 32 columns to LDS, [32][DP + 4], where the waves of a block share
+// the columns.
+template <int DP> constexpr int kSumPitch = DP + 4;
+template <int DP> __device__ __forceinline__ void put_sums(float *to, const floatx16 (&acc)[DP / 32]) {
+  float *at = to + (lane_id() & 31) * kSumPitch<DP> + 4 * (lane_id() >> 5);
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<floatx4_t *>(at + 32 * n + 8 * g) =
+          floatx4_t{acc[n][4 * g], acc[n][4 * g + 1], acc[n][4 * g + 2], acc[n][4 * g + 3]};
+}
+
 constexpr int kKeysByDma = 1, kQueriesByDma = 2;
 
 // Strides in values.
@@ -463,6 +483,8 @@ struct Args {
 // columns of queries
 // ---------------------------------------------------------------------------
 constexpr int kColumns = 128;  // of a block: a key head's query heads and their queries, heads fastest
+// Below so many blocks of 128 columns a block owns 32, and its waves share out the keys.
+constexpr int kFewBlocks = 256;
 // keys of a tile
 template <class T> constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
 

@@ -19,23 +19,83 @@ namespace attention {
 // ---------------------------------------------------------------------------
 // queries: delta and dq; columns as in the forward pass
 // ---------------------------------------------------------------------------
+// a lane's column on its way: its query, its output's gradient, and dq (this half's
+// share, without the scale)
+template <class T, int DP> struct QueryColumn {
+  using R = Rows<T, DP>;
+  Frag<T> q[DP / 16], g[DP / 16];
+  float delta;
+  Stat<T> stat;
+  floatx16 acc[DP / 32];
+
+  // query i of sequence s, of this head; `there`: delta is to be written
+  __device__ __forceinline__ void load(const Args &a, const Sequence &s, int i, int head, bool there) {
+    const int64_t at = (s.q0 + i) * a.heads + head;
+    const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
+    const T *grow = static_cast<const T *>(a.dout) + at * a.d, *orow = static_cast<const T *>(a.out) + at * a.d;
+    delta = 0;
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) {
+      q[st] = load_frag(row, a.d, st);
+      g[st] = load_frag(grow, a.d, st);
+      const Frag<T> of = load_frag(orow, a.d, st);
+      T x[8], y[8];
+      __builtin_memcpy(x, &g[st], sizeof(x));
+      __builtin_memcpy(y, &of, sizeof(y));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta += to_float(x[e]) * to_float(y[e]);
+    }
+    delta += other_half(delta);
+    const int64_t to = head * a.s.rows + s.q0 + i;
+    if (there && lane_id() < 32) a.delta[to] = delta;
+    stat = {a.stats[to], 1.f};
+    if constexpr (sizeof(T) == 4) stat.by = a.stats[a.heads * a.s.rows + to];
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) acc[n] = floatx16{};
+  }
+  // ds of 32 keys (MASKED: of which this lane's column sees the first `seen`)
+  template <bool MASKED>
+  __device__ __forceinline__ void gradients(const Args &a, const Reader<T, DP> &read, lds_char *kt, lds_char *vt, int seen,
+                                            floatx16 &ds) const {
+    floatx16 p{}, dp{};
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) mma(p, read.rows(kt, 0, st), q[st]);
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) mma(dp, read.rows(vt, 0, st), g[st]);
+    const int mine = seen - 4 * (lane_id() >> 5);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const float w = weight(p[x], a.scale2, stat) * (dp[x] - delta);
+      ds[x] = !MASKED || 8 * (x / 4) + x % 4 < mine ? w : 0.f;
+    }
+  }
+  __device__ __forceinline__ void accumulate(const Reader<T, DP> &read, lds_char *kt, const floatx16 &ds) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const Frag<T> f = as_operand<T>(ds, st);
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n) mma(acc[n], read.cols(kt, 16 * st, n), f);
+    }
+  }
+};
+
 template <class T, int DP, bool DMA>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(const Args a) {
   using R = Rows<T, DP>;
   constexpr int KT = kKeys<T>, TILE = KT * R::PITCH;
   __shared__ __align__(1024) char lds[4 * TILE];
-  const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id(), h = lane >> 5;
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id();
   T *dq = static_cast<T *>(a.dq);
   if (dq)
     clear_uncovered(a.s.offsets, a.s.count, a.s.rows, dq, static_cast<int64_t>(a.heads) * a.d, blockIdx.x, gridDim.x);
   const int kv = blockIdx.x % a.kv_heads;
-  const Found f = find_longest(a.s.count, blockIdx.x / a.kv_heads,
-                               [&](int b) { return (queries_of(a.s, b) * a.group + kColumns - 1) / kColumns; });
-  if (f.sequence < 0) return;
-  const Sequence s = sequence_at(a.s, f.sequence);
-  const int total = s.nq * a.group, c0 = f.nth * kColumns, w0 = c0 + wave * 32;
+  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads,
+                               [&](const Sequence &x) { return (x.nq * a.group + kColumns - 1) / kColumns; });
+  if (!s.there) return;
+  const int total = s.nq * a.group, c0 = s.nth * kColumns, w0 = c0 + wave * 32;
   const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
   const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i);
+  // (without dq, delta alone)
   const int fewest = visible(a, s, c0 / a.group), end = dq ? visible(a, s, std::min(c0 + kColumns - 1, total - 1) / a.group) : 0;
   const int steps = (end + KT - 1) / KT;
   const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
@@ -48,52 +108,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
     fetch_values(values + t * (KT * vstride), s.nk - t * KT, to + TILE);
   };
   if (steps > 0) issue(0, 0);
-  const int64_t at = (s.q0 + i) * a.heads + head;
-  Frag<T> q[DP / 16], g[DP / 16];
-  const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
-  const T *grow = static_cast<const T *>(a.dout) + at * a.d, *orow = static_cast<const T *>(a.out) + at * a.d;
-  float delta = 0;
-#pragma unroll
-  for (int st = 0; st < DP / 16; ++st) {
-    q[st] = load_frag(row, a.d, st);
-    g[st] = load_frag(grow, a.d, st);
-    const Frag<T> of = load_frag(orow, a.d, st);
-    T x[8], y[8];
-    __builtin_memcpy(x, &g[st], sizeof(x));
-    __builtin_memcpy(y, &of, sizeof(y));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) delta += to_float(x[e]) * to_float(y[e]);
-  }
-  delta += other_half(delta);
   const bool there = column < total;
-  const int64_t stat = head * a.s.rows + s.q0 + i;
-  if (there && lane < 32) a.delta[stat] = delta;
-  Stat<T> r{a.stats[stat], 1.f};
-  if constexpr (sizeof(T) == 4) r.by = a.stats[a.heads * a.s.rows + stat];
-  floatx16 acc[DP / 32] = {};
+  QueryColumn<T, DP> c;
+  c.load(a, s, i, head, there);
   const Reader<T, DP> read;
-  // ds of 32 keys (MASKED: of which this lane's column sees the first `seen`), in place of their scores
-  const auto gradients = [&](auto MASKED, lds_char *kt, lds_char *vt, int seen, floatx16 &ds) {
-    floatx16 p{}, dp{};
-#pragma unroll
-    for (int st = 0; st < DP / 16; ++st) {
-      mma(p, read.rows(kt, 0, st), q[st]);
-      mma(dp, read.rows(vt, 0, st), g[st]);
-    }
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      const float w = weight(p[x], a.scale2, r) * (dp[x] - delta);
-      ds[x] = !decltype(MASKED)::value || 8 * (x / 4) + x % 4 < seen - 4 * h ? w : 0.f;
-    }
-  };
-  const auto accumulate = [&](lds_char *kt, const floatx16 &ds) {
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const Frag<T> f = as_operand<T>(ds, st);
-#pragma unroll
-      for (int n = 0; n < DP / 32; ++n) mma(acc[n], read.cols(kt, 16 * st, n), f);
-    }
-  };
   const int whole = std::min(fewest / KT, steps);  // tiles that every column sees whole
   ring(whole, 0, [&](int t, auto STAGE) {
     constexpr int stage = decltype(STAGE)::value;
@@ -103,8 +121,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u) {
       floatx16 ds;
-      gradients(std::false_type{}, kt + 32 * u * R::PITCH, kt + TILE + 32 * u * R::PITCH, 0, ds);
-      accumulate(kt + 32 * u * R::PITCH, ds);
+      c.template gradients<false>(a, read, kt + 32 * u * R::PITCH, kt + TILE + 32 * u * R::PITCH, 0, ds);
+      c.accumulate(read, kt + 32 * u * R::PITCH, ds);
     }
   });
   // the others; the block stays together
@@ -116,29 +134,100 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
       lds_char *kt = (lds_char *)lds + (t & 1) * 2 * TILE + 32 * u * R::PITCH;
       const int first = t * KT + 32 * u, seen = limit - first;
       floatx16 ds;
-      gradients(std::true_type{}, kt, kt + TILE, seen, ds);
+      c.template gradients<true>(a, read, kt, kt + TILE, seen, ds);
       bool found = false;
       if (a.causal) {
         __syncthreads();  // (every wave has the scores)
         found = __syncthreads_or(clear_not_finite<T, DP, 32, 256>(kt, threadIdx.x));
       }
-      accumulate(kt, ds);
+      c.accumulate(read, kt, ds);
       if (found)
-        add_not_finite<T, DP>(acc, keys + first * kstride, kstride, std::min(s.nk - first, 32), a.d,
+        add_not_finite<T, DP>(c.acc, keys + first * kstride, kstride, std::min(s.nk - first, 32), a.d,
                               [&](int x) { return x < seen; });
     }
   }
-  if (dq) store_column<T, DP>(dq + at * a.d, a.d, there, acc, a.scale);
+  if (dq) store_column<T, DP>(dq + ((s.q0 + i) * a.heads + head) * a.d, a.d, there, c.acc, a.scale);
+}
+
+// Few columns: a block's waves share 32 of them and take the keys' tiles in turn, each
+// on its own, and add up their dq in order.
+template <class T, int DP, bool DMA>
+__global__ __launch_bounds__(64 * 2, 1) void few_queries_kernel(const Args a) {
+  using R = Rows<T, DP>;
+  constexpr int KT = 32, TILE = KT * R::PITCH, NW = 2, LOADS = 2 * KT * R::CPR / 64;
+  static_assert(32 * kSumPitch<DP> * 4 <= 4 * TILE, "a wave's sums take its stages' place");
+  __shared__ __align__(1024) char lds[NW][4 * TILE];
+  const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = lane_id();
+  lds_char *own = (lds_char *)lds[wave];
+  T *dq = static_cast<T *>(a.dq);
+  if (dq)
+    clear_uncovered(a.s.offsets, a.s.count, a.s.rows, dq, static_cast<int64_t>(a.heads) * a.d, blockIdx.x, gridDim.x);
+  const int kv = blockIdx.x % a.kv_heads;
+  const Found s =
+      find_longest(a.s, blockIdx.x / a.kv_heads, [&](const Sequence &x) { return (x.nq * a.group + 31) / 32; });
+  if (!s.there) return;
+  const int total = s.nq * a.group, w0 = s.nth * 32, column = w0 + (lane & 31), j = column < total ? column : total - 1;
+  const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i);
+  const int fewest = visible(a, s, w0 / a.group), end = dq ? visible(a, s, std::min(w0 + 31, total - 1) / a.group) : 0;
+  const int steps = (end + KT - 1) / KT;
+  const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
+  const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + s.k0 * a.k_row + kv * a.k_head);
+  const char *values = reinterpret_cast<const char *>(static_cast<const T *>(a.v) + s.k0 * a.v_row + kv * a.v_head);
+  const Fetch<T, DP, KT, 64, DMA> fetch_keys(kstride, a.d, lane), fetch_values(vstride, a.d, lane);
+  const auto issue = [&](int t, int stage) {
+    lds_char *to = own + stage * 2 * TILE;
+    const int64_t n = t < steps ? s.nk - t * KT : 0;
+    fetch_keys(keys + t * (KT * kstride), n, to);
+    fetch_values(values + t * (KT * vstride), n, to + TILE);
+  };
+  issue(wave, 0);
+  QueryColumn<T, DP> c;
+  c.load(a, s, i, head, column < total && wave == 0);
+  const Reader<T, DP> read;
+  for (int t = wave, stage = 0; t < steps; t += NW, stage ^= 1) {
+    issue(t + NW, stage ^ 1);
+    // until this tile's loads have landed (the next one's are on their way)
+    __builtin_amdgcn_s_waitcnt((LOADS & 15) | (7 << 4) | ((LOADS >> 4) << 14));
+    asm volatile("" ::: "memory");
+    lds_char *kt = own + stage * 2 * TILE;
+    floatx16 ds;
+    if (fewest >= (t + 1) * KT) {
+      c.template gradients<false>(a, read, kt, kt + TILE, 0, ds);
+      c.accumulate(read, kt, ds);
+      continue;
+    }
+    const int seen = limit - t * KT;
+    c.template gradients<true>(a, read, kt, kt + TILE, seen, ds);
+    const bool found = a.causal && ballot(clear_not_finite<T, DP, KT, 64>(kt, lane)) != 0;
+    c.accumulate(read, kt, ds);
+    if (found)
+      add_not_finite<T, DP>(c.acc, keys + t * (KT * kstride), kstride, std::min(s.nk - t * KT, KT), a.d,
+                            [&](int x) { return x < seen; });
+  }
+  wait_loads();
+  asm volatile("" ::: "memory");
+  if (!dq) return;
+  put_sums<DP>(reinterpret_cast<float *>(lds[wave]), c.acc);
+  __syncthreads();
+  const int columns = std::min(32, total - w0);
+  for (int k = threadIdx.x; k < columns * a.d; k += 64 * NW) {
+    const int col = k / a.d, d = k - col * a.d, at_q = (w0 + col) / a.group, at_h = kv * a.group + (w0 + col - at_q * a.group);
+    float v = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += reinterpret_cast<const float *>(lds[w])[col * kSumPitch<DP> + d];
+    dq[((s.q0 + at_q) * a.heads + at_h) * a.d + d] = from_float<T>(v * a.scale);
+  }
 }
 
 template <class T, int DP> static int launch(const Args &a, hipStream_t stream) {
   if (a.s.rows > 0) {
-    const int64_t blocks = (a.s.rows * a.group / kColumns + a.s.count) * a.kv_heads;
+    int64_t blocks = (a.s.rows * a.group / kColumns + a.s.count) * a.kv_heads;
+    const bool few = blocks < kFewBlocks;
+    if (few) blocks = (a.s.rows * a.group / 32 + a.s.count) * a.kv_heads;
     SPIRA_HIP_REQUIRE(launchable(blocks, 256), "attention: too many tiles for a launch");
-    if (a.dma & kKeysByDma)
-      hipLaunchKernelGGL((queries_kernel<T, DP, true>), dim3(blocks), dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL((queries_kernel<T, DP, false>), dim3(blocks), dim3(256), 0, stream, a);
+    const auto kernel = few ? (a.dma & kKeysByDma ? few_queries_kernel<T, DP, true> : few_queries_kernel<T, DP, false>)
+                            : (a.dma & kKeysByDma ? queries_kernel<T, DP, true> : queries_kernel<T, DP, false>);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(few ? 128 : 256), 0, stream, a);
     SPIRA_HIP_LAUNCH_CHECK();
   }
   return kOk;

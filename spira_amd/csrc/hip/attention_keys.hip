@@ -33,11 +33,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   if (!SPLIT && dk) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dk, width, blockIdx.x, gridDim.x);
   if (!SPLIT && dv) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dv, width, blockIdx.x, gridDim.x);
   const int kv = blockIdx.x % a.kv_heads;
-  const Found f = find_longest(a.s.count, blockIdx.x / a.kv_heads,
-                               [&](int b) { return static_cast<int>((room_of(a.s, b) + int64_t(kOwnKeys) - 1) / kOwnKeys); });
-  if (f.sequence < 0) return;
-  const Sequence s = sequence_at(a.s, f.sequence);
-  const int c0 = (f.of - 1 - f.nth) * kOwnKeys, w0 = c0 + wave * 32, key = w0 + (lane & 31);
+  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads, [&](const Sequence &x) {
+    return static_cast<int>((x.room + int64_t(kOwnKeys) - 1) / kOwnKeys);
+  });
+  if (!s.there) return;
+  const int c0 = (s.of - 1 - s.nth) * kOwnKeys, w0 = c0 + wave * 32, key = w0 + (lane & 31);
   const bool there = key < s.nk;
   // the first query that sees a key
   const auto first_of = [&](int k) { return a.causal ? std::max(0, k - (s.nk - s.nq)) : 0; };
@@ -216,7 +216,7 @@ template <class T> __global__ __launch_bounds__(256) void sums_kernel(const Args
     else hi = mid;
   }
   const int64_t first = clamp_row(a.s.key_offsets[lo], a.s.keys);
-  there = row >= first && row < first + keys_of(a.s, lo);
+  there = row >= first && row < first + sequence_at(a.s, lo).nk;
   Chunk<T> sum{};
   if (there) {
     const float *from = a.partial + blockIdx.y * a.s.keys * width + row * width + at;
