@@ -175,13 +175,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
 // ---------------------------------------------------------------------------
 // few tokens
 // ---------------------------------------------------------------------------
-template <class T, int DP> constexpr int kTokenWaves = Rows<T, DP>::PITCH >= 256 ? 2 : 4;
+// Waves of a block, with two stages of two tiles of 32 keys each.  Parts of a long
+// cache: blocks of 64 KB, two to a CU, so that one streams while the other begins.
+// (32 caches of 4096 keys on average, 8 heads of 128: 125 us.  One wave a block with four
+// stages, as many loads under way, 156; two with three stages, one block to a CU, 176:
+// four waves a CU are what it takes to work off what arrives.)
+template <class T, int DP, bool DIRECT> struct TokenShape {
+  static constexpr int PITCH = Rows<T, DP>::PITCH;
+  static constexpr int NW = DIRECT ? (PITCH >= 512 ? 2 : 4) : (PITCH >= 512 ? 1 : PITCH >= 256 ? 2 : 4);
+};
 
 // DIRECT: no sequence has more than one part; the outputs themselves
 template <class T, int DP, bool DIRECT, bool DMA>
-__global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)) void token_kernel(const Args a) {
+__global__ __launch_bounds__((64 * TokenShape<T, DP, DIRECT>::NW), 1) void token_kernel(const Args a) {
   using R = Rows<T, DP>;
-  constexpr int KT = 32, TILE = KT * R::PITCH, NW = kTokenWaves<T, DP>, NT = 64 * NW;
+  constexpr int KT = 32, TILE = KT * R::PITCH, NT = 64 * TokenShape<T, DP, DIRECT>::NW;
+  constexpr int NW = TokenShape<T, DP, DIRECT>::NW;
   constexpr int LOADS = 2 * KT * R::CPR / 64, OPITCH = kSumPitch<DP>;
   static_assert(32 * OPITCH * 4 <= 4 * TILE, "a wave's sums take its stages' place");
   __shared__ __align__(1024) char lds[NW][4 * TILE];
@@ -227,11 +236,17 @@ __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)
     const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
 #pragma unroll
     for (int st = 0; st < DP / 16; ++st) q[st] = load_frag(row, a.d, st);
+    // (waited for here, with the first tile: a later wait would be for the next one too)
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st)
+#pragma unroll
+      for (auto &v : q[st].v) asm volatile("" : "+v"(v));
     Columns<DP> c{};
     c.m = -__builtin_inff();
     for (int t = wave, stage = 0; t < steps; t += NW, stage ^= 1) {
       issue(t + NW, stage ^ 1);
       // until this tile's loads have landed (the next one's are on their way)
+      static_assert(LOADS < 64, "vmcnt range");
       __builtin_amdgcn_s_waitcnt((LOADS & 15) | (7 << 4) | ((LOADS >> 4) << 14));
       asm volatile("" ::: "memory");
       lds_char *kt = mine + stage * 2 * TILE;
@@ -296,52 +311,84 @@ __global__ __launch_bounds__((64 * kTokenWaves<T, DP>), (sizeof(T) == 2 ? 2 : 1)
   }
 }
 
-// The parts of a row joined: a wave to a row of one head.
+// The parts of a row of one head joined, by a block: its four waves take the parts in
+// turn, half a wave each, four values a lane, so that many parts' sums are under way
+// at once (and before their weights are known).
+constexpr int kJoinParts = 8;  // at a time
 template <class T> __global__ __launch_bounds__(256) void join_kernel(const Args a) {
-  const int lane = lane_id();
-  const int64_t at = blockIdx.x * static_cast<int64_t>(4) + (threadIdx.x >> 6), all = a.s.rows * a.heads;
-  if (at >= all) return;
-  const int64_t row = at / a.heads;
+  __shared__ float sums[kJoinParts][kMostHeadDim], stats[2];
+  const int lane = lane_id(), slot = threadIdx.x / 32, d = (threadIdx.x & 31) * 4;
+  const int64_t at = blockIdx.x, all = a.s.rows * a.heads, row = at / a.heads;
   int parts = 0;
   for (int first = 0; first < a.s.count; first += 64) {
     const int b = first + lane;
-    const bool mine = b < a.s.count && row >= a.s.offsets[b] && row < a.s.offsets[b + 1];
-    const uint64_t found = ballot(mine);
+    const Sequence s = sequence_at(a.s, b < a.s.count ? b : a.s.count - 1);
+    const uint64_t found = ballot(b < a.s.count && row >= s.q0 && row < s.q0 + s.nq);
     if (found) {
-      parts = (sequence_at(a.s, first + __builtin_ctzll(found)).nk + a.part_keys - 1) / a.part_keys;
+      parts = (__shfl(s.nk, __builtin_ctzll(found), 64) + a.part_keys - 1) / a.part_keys;
       break;
     }
   }
-  float m = -__builtin_inff(), l = 0;
-  for (int p = lane; p < parts; p += 64) {
-    const float *from = a.partial_stats + (p * all + at) * 2;
-    const float pm = from[0], higher = __builtin_fmaxf(m, pm);
-    l = (m == higher ? l : l * __builtin_amdgcn_exp2f(m - higher)) +
-        (pm == higher ? from[1] : from[1] * __builtin_amdgcn_exp2f(pm - higher));
+  parts = uniform(parts);
+  const auto stat = [&](int p, int i) { return a.partial_stats[(p * all + at) * 2 + i]; };
+  constexpr int BATCH = 4;
+  float v[4] = {}, m = -__builtin_inff();
+  for (int p0 = 0; p0 < parts; p0 += kJoinParts * BATCH) {
+    Chunk<float> part[BATCH];
+    float pm[BATCH];
+#pragma unroll
+    for (int n = 0; n < BATCH; ++n) {
+      const int p = p0 + n * kJoinParts + slot;
+      const bool there = p < parts;
+      part[n] = load_chunk(a.partial + ((there ? p : 0) * all + at) * a.d + d, there ? a.d - d : 0);
+      pm[n] = there ? stat(p, 0) : -__builtin_inff();
+    }
+    float higher = m;
+#pragma unroll
+    for (int n = 0; n < BATCH; ++n) higher = __builtin_fmaxf(higher, pm[n]);
+    const float by = m == higher ? 1.f : __builtin_amdgcn_exp2f(m - higher);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= by;
+#pragma unroll
+    for (int n = 0; n < BATCH; ++n) {
+      const float w = pm[n] == higher ? 1.f : __builtin_amdgcn_exp2f(pm[n] - higher);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += w * part[n].v[i];
+    }
     m = higher;
   }
+  // the row's reference and sum, by the first wave
+  if (threadIdx.x < 64) {
+    float top = -__builtin_inff(), l = 0;
+    for (int p = lane; p < parts; p += 64) {
+      const float x = stat(p, 0), higher = __builtin_fmaxf(top, x);
+      l = (top == higher ? l : l * __builtin_amdgcn_exp2f(top - higher)) +
+          (x == higher ? stat(p, 1) : stat(p, 1) * __builtin_amdgcn_exp2f(x - higher));
+      top = higher;
+    }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float om = __shfl_xor(m, o, 64), ol = __shfl_xor(l, o, 64), higher = __builtin_fmaxf(m, om);
-    l = (m == higher ? l : l * __builtin_amdgcn_exp2f(m - higher)) +
-        (om == higher ? ol : ol * __builtin_amdgcn_exp2f(om - higher));
-    m = higher;
-  }
-  float v[kMostHeadDim / 64] = {};
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float pm = a.partial_stats[(p * all + at) * 2];
-    const float by = pm == m ? 1.f : __builtin_amdgcn_exp2f(pm - m);
-#pragma unroll
-    for (int i = 0; i < kMostHeadDim / 64; ++i) {
-      const int d = i * 64 + lane;
-      if (d < a.d) v[i] += by * a.partial[(p * all + at) * a.d + d];
+    for (int o = 32; o > 0; o >>= 1) {
+      const float om = __shfl_xor(top, o, 64), ol = __shfl_xor(l, o, 64), higher = __builtin_fmaxf(top, om);
+      l = (top == higher ? l : l * __builtin_amdgcn_exp2f(top - higher)) +
+          (om == higher ? ol : ol * __builtin_amdgcn_exp2f(om - higher));
+      top = higher;
+    }
+    if (threadIdx.x == 0) {
+      stats[0] = top;
+      stats[1] = l;
     }
   }
+  __syncthreads();
+  const float top = stats[0], l = stats[1];
+  const float w = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
-  for (int i = 0; i < kMostHeadDim / 64; ++i) {
-    const int d = i * 64 + lane;
-    if (d < a.d) static_cast<T *>(a.o)[at * a.d + d] = from_float<T>(l == 0.f ? 0.f : v[i] / l);
+  for (int i = 0; i < 4; ++i) sums[slot][d + i] = w * v[i];
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < a.d) {
+    float o = 0;
+#pragma unroll
+    for (int n = 0; n < kJoinParts; ++n) o += sums[n][threadIdx.x];
+    static_cast<T *>(a.o)[at * a.d + threadIdx.x] = from_float<T>(l == 0.f ? 0.f : o / l);
   }
 }
 
@@ -419,8 +466,8 @@ template <class T, int DP, bool DMA> static int launch_form(const Args &base, co
     return kOk;
   }
   a.part_keys = p.part_keys;
-  constexpr int threads = 64 * kTokenWaves<T, DP>;
   const bool direct = p.parts <= 1;
+  const int threads = 64 * (direct ? TokenShape<T, DP, true>::NW : TokenShape<T, DP, false>::NW);
   const int64_t blocks = ((direct ? a.s.rows * a.group / 32 : a.s.keys / p.part_keys) + a.s.count) * a.kv_heads;
   const uint32_t y = direct ? 1 : static_cast<uint32_t>(div_up(div_up(a.s.rows * a.group, a.s.count), 32));
   SPIRA_HIP_REQUIRE(launchable(blocks * y, threads), "attention: too many tiles for a launch");
@@ -430,7 +477,7 @@ template <class T, int DP, bool DMA> static int launch_form(const Args &base, co
     hipLaunchKernelGGL((token_kernel<T, DP, false, DMA>), dim3(blocks, y), dim3(threads), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();
   if (direct) return kOk;
-  const int64_t joins = div_up(a.s.rows * a.heads, 4);
+  const int64_t joins = a.s.rows * a.heads;
   SPIRA_HIP_REQUIRE(launchable(joins, 256), "attention: too many rows for a launch");
   hipLaunchKernelGGL(join_kernel<T>, dim3(joins), dim3(256), 0, stream, a);
   SPIRA_HIP_LAUNCH_CHECK();

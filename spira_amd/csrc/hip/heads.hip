@@ -36,12 +36,12 @@ struct Side {  // queries or keys
 struct Args {
   Side side[2];
   int64_t n;
-  int d, axes, interleaved, rows;  // rows of a block at a time
+  int d, axes, rows;  // rows of a block at a time
   float eps;
   const int32_t *positions;  // [n, axes] or null
   float *partial;            // [blocks, 2, d]
   uint64_t speed[kMostDim / 2];  // 2^64 turns of a pair by a position
-  int32_t axis[kMostDim / 2];
+  uint8_t axis[kMostDim / 2];
 };
 
 // cos and sin of `turn` / 2^64 of a whole turn
@@ -60,15 +60,6 @@ struct Pairs {
   float a[kPairs], b[kPairs];
 };
 
-// values [at, at + 8) of a vector of n
-template <class T> __device__ __forceinline__ void load8(const T *p, int at, int n, float (&v)[kPairs]) {
-#pragma unroll
-  for (int i = 0; i < kPairs / kVec<T>; ++i) {
-    const Chunk<T> c = load_chunk(p + at + i * kVec<T>, p ? n - at - i * kVec<T> : 0);
-#pragma unroll
-    for (int j = 0; j < kVec<T>; ++j) v[i * kVec<T> + j] = c.v[j];
-  }
-}
 template <class T> __device__ __forceinline__ void store8(T *p, int at, int n, const float (&v)[kPairs]) {
 #pragma unroll
   for (int i = 0; i < kPairs / kVec<T>; ++i) {
@@ -77,26 +68,6 @@ template <class T> __device__ __forceinline__ void store8(T *p, int at, int n, c
     for (int j = 0; j < kVec<T>; ++j) c.v[j] = v[i * kVec<T> + j];
     store_chunk(p + at + i * kVec<T>, n - at - i * kVec<T>, c);
   }
-}
-// lane `lane` of a vector's pairs; `half` pairs (of an odd d the last has no second)
-template <class T> __device__ __forceinline__ Pairs load_pairs(const T *p, int lane, int d, int half, bool interleaved) {
-  Pairs r;
-  if (interleaved) {
-    float lo[kPairs], hi[kPairs];
-    load8(p, lane * 2 * kPairs, d, lo);
-    load8(p, lane * 2 * kPairs + kPairs, d, hi);
-#pragma unroll
-    for (int i = 0; i < kPairs / 2; ++i) {
-      r.a[i] = lo[2 * i];
-      r.b[i] = lo[2 * i + 1];
-      r.a[kPairs / 2 + i] = hi[2 * i];
-      r.b[kPairs / 2 + i] = hi[2 * i + 1];
-    }
-  } else {
-    load8(p, lane * kPairs, half, r.a);
-    load8(p ? p + half : p, lane * kPairs, d - half, r.b);
-  }
-  return r;
 }
 template <class T>
 __device__ __forceinline__ void store_pairs(T *p, int lane, int d, int half, bool interleaved, const Pairs &r) {
@@ -117,6 +88,44 @@ __device__ __forceinline__ void store_pairs(T *p, int lane, int d, int half, boo
   }
 }
 
+// a lane's pairs as they lie in memory
+template <class T> struct RawPairs {
+  uintx4_t a[kPairs / kVec<T>], b[kPairs / kVec<T>];
+};
+template <class T>
+__device__ __forceinline__ RawPairs<T> load_raw_pairs(const T *p, int lane, int d, int half, bool interleaved) {
+  RawPairs<T> r;
+  const int first = interleaved ? lane * 2 * kPairs : lane * kPairs, second = interleaved ? first + kPairs : half + first;
+  const int upto = interleaved ? d : half;
+#pragma unroll
+  for (int i = 0; i < kPairs / kVec<T>; ++i) {
+    r.a[i] = load_raw(p + first + i * kVec<T>, p ? upto - first - i * kVec<T> : 0);
+    r.b[i] = load_raw(p + second + i * kVec<T>, p ? d - second - i * kVec<T> : 0);
+  }
+  return r;
+}
+template <class T> __device__ __forceinline__ Pairs unpack_pairs(const RawPairs<T> &raw, bool interleaved) {
+  float lo[kPairs], hi[kPairs];
+#pragma unroll
+  for (int i = 0; i < kPairs / kVec<T>; ++i) {
+    const Chunk<T> x = unpack<T>(raw.a[i]), y = unpack<T>(raw.b[i]);
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) {
+      lo[i * kVec<T> + j] = x.v[j];
+      hi[i * kVec<T> + j] = y.v[j];
+    }
+  }
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < kPairs / 2; ++i) {
+    r.a[i] = interleaved ? lo[2 * i] : lo[i];
+    r.b[i] = interleaved ? lo[2 * i + 1] : hi[i];
+    r.a[kPairs / 2 + i] = interleaved ? hi[2 * i] : lo[kPairs / 2 + i];
+    r.b[kPairs / 2 + i] = interleaved ? hi[2 * i + 1] : hi[kPairs / 2 + i];
+  }
+  return r;
+}
+
 constexpr int kMostTurns = 2048;  // of the rows that a block holds
 
 // cos and sin of the rows' pairs
@@ -129,37 +138,52 @@ __device__ __forceinline__ void make_turns(const Args &a, int64_t first, int cou
   }
 }
 
-template <class T, int G> __global__ __launch_bounds__(256) void forward_kernel(const Args a) {
+// A lane's vectors come one turn ahead: the next one's loads are under way while it
+// works on this one, and the first's while the sines are made.
+template <class T, int G, bool INTERLEAVED> __global__ __launch_bounds__(256) void forward_kernel(const Args a) {
   __shared__ float2 turns[kMostTurns];
   constexpr int GROUPS = 256 / G;
   const int lane = threadIdx.x % G, group = threadIdx.x / G, half = (a.d + 1) / 2;
   const float inv_d = 1.f / static_cast<float>(a.d);
   const int all = a.side[0].heads + a.side[1].heads;
-  Pairs w[2];
+  RawPairs<T> w[2];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) w[s] = load_pairs(static_cast<const T *>(a.side[s].w), lane, a.d, half, a.interleaved);
+  for (int s = 0; s < 2; ++s) w[s] = load_raw_pairs(static_cast<const T *>(a.side[s].w), lane, a.d, half, INTERLEAVED);
   for (int64_t first = blockIdx.x * static_cast<int64_t>(a.rows); first < a.n; first += gridDim.x * static_cast<int64_t>(a.rows)) {
-    const int count = static_cast<int>(std::min<int64_t>(a.rows, a.n - first));
+    const int count = static_cast<int>(std::min<int64_t>(a.rows, a.n - first)) * all;
+    const auto fetch = [&](int i) {
+      const int r = i / all, h = i - r * all, k = h >= a.side[0].heads;
+      const T *x = static_cast<const T *>(k ? a.side[1].x : a.side[0].x);
+      const int64_t row = k ? a.side[1].row : a.side[0].row, head = k ? a.side[1].head : a.side[0].head;
+      return load_raw_pairs(i < count ? x + (first + r) * row + (k ? h - a.side[0].heads : h) * head : nullptr, lane, a.d,
+                            half, INTERLEAVED);
+    };
+    RawPairs<T> next = fetch(group);
     if (a.positions) {
       __syncthreads();
-      make_turns(a, first, count, turns);
+      make_turns(a, first, count / all, turns);
       __syncthreads();
     }
-    for (int i = group; i < count * all; i += GROUPS) {
+    for (int i = group; i < count; i += GROUPS) {
       const int r = i / all, h = i - r * all, k = h >= a.side[0].heads;
-      const Side &side = k ? a.side[1] : a.side[0];
-      const int head = k ? h - a.side[0].heads : h;
-      Pairs v = load_pairs(static_cast<const T *>(side.x) + (first + r) * side.row + head * side.head, lane, a.d, half,
-                           a.interleaved);
-      if (side.w) {
+      Pairs v = unpack_pairs<T>(next, INTERLEAVED);
+      next = fetch(i + GROUPS);
+      if (k ? a.side[1].w : a.side[0].w) {
         float ss = 0;
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) ss += v.a[j] * v.a[j] + v.b[j] * v.b[j];
         const float inv = rsqrtf(group_sum<G>(ss) * inv_d + a.eps);
+        RawPairs<T> raw;
+#pragma unroll
+        for (int j = 0; j < kPairs / kVec<T>; ++j) {
+          raw.a[j] = k ? w[1].a[j] : w[0].a[j];
+          raw.b[j] = k ? w[1].b[j] : w[0].b[j];
+        }
+        const Pairs by = unpack_pairs<T>(raw, INTERLEAVED);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
-          v.a[j] *= inv * (k ? w[1].a[j] : w[0].a[j]);
-          v.b[j] *= inv * (k ? w[1].b[j] : w[0].b[j]);
+          v.a[j] *= inv * by.a[j];
+          v.b[j] *= inv * by.b[j];
         }
       }
       if (a.positions) {
@@ -172,12 +196,13 @@ template <class T, int G> __global__ __launch_bounds__(256) void forward_kernel(
           v.b[j] = x * t.y + y * t.x;
         }
       }
-      store_pairs(static_cast<T *>(side.y) + ((first + r) * side.heads + head) * a.d, lane, a.d, half, a.interleaved, v);
+      const int64_t to = k ? (first + r) * a.side[1].heads + h - a.side[0].heads : (first + r) * a.side[0].heads + h;
+      store_pairs(static_cast<T *>(k ? a.side[1].y : a.side[0].y) + to * a.d, lane, a.d, half, INTERLEAVED, v);
     }
   }
 }
 
-template <class T, int G> __global__ __launch_bounds__(256) void backward_kernel(const Args a) {
+template <class T, int G, bool INTERLEAVED> __global__ __launch_bounds__(256) void backward_kernel(const Args a) {
   __shared__ float2 turns[kMostTurns];
   constexpr int GROUPS = 256 / G;
   const int lane = threadIdx.x % G, group = threadIdx.x / G, half = (a.d + 1) / 2;
@@ -194,14 +219,22 @@ template <class T, int G> __global__ __launch_bounds__(256) void backward_kernel
     for (int k = 0; k < 2; ++k) {
       const Side &side = a.side[k];
       if (!side.dy) continue;
-      const Pairs w = load_pairs(static_cast<const T *>(side.w), lane, a.d, half, a.interleaved);
+      const RawPairs<T> w_raw = load_raw_pairs(static_cast<const T *>(side.w), lane, a.d, half, INTERLEAVED);
+      RawPairs<T> next_g, next_x;
+      const auto fetch = [&](int i) {
+        const int r = i / side.heads, head = i - r * side.heads;
+        const bool there = i < count * side.heads;
+        const int64_t at = ((first + r) * side.heads + head) * a.d;
+        next_g = load_raw_pairs(there ? static_cast<const T *>(side.dy) + at : nullptr, lane, a.d, half, INTERLEAVED);
+        next_x = load_raw_pairs(there && side.w ? static_cast<const T *>(side.x) + (first + r) * side.row + head * side.head : nullptr,
+                                lane, a.d, half, INTERLEAVED);
+      };
+      fetch(group);
       for (int i = group; i < count * side.heads; i += GROUPS) {
         const int r = i / side.heads, head = i - r * side.heads;
         const int64_t at = ((first + r) * side.heads + head) * a.d;
-        Pairs g = load_pairs(static_cast<const T *>(side.dy) + at, lane, a.d, half, a.interleaved), v{};
-        if (side.w)
-          v = load_pairs(static_cast<const T *>(side.x) + (first + r) * side.row + head * side.head, lane, a.d, half,
-                         a.interleaved);
+        Pairs g = unpack_pairs<T>(next_g, INTERLEAVED), v = unpack_pairs<T>(next_x, INTERLEAVED);
+        fetch(i + GROUPS);
         if (a.positions) {
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) {
@@ -217,6 +250,7 @@ template <class T, int G> __global__ __launch_bounds__(256) void backward_kernel
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) ss += v.a[j] * v.a[j] + v.b[j] * v.b[j];
           const float inv = rsqrtf(group_sum<G>(ss) * inv_d + a.eps);
+          const Pairs w = unpack_pairs<T>(w_raw, INTERLEAVED);
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) {
             v.a[j] *= inv;
@@ -234,7 +268,7 @@ template <class T, int G> __global__ __launch_bounds__(256) void backward_kernel
             g.b[j] = inv * (g.b[j] - v.b[j] * along);
           }
         }
-        if (side.y) store_pairs(static_cast<T *>(side.y) + at, lane, a.d, half, a.interleaved, g);
+        if (side.y) store_pairs(static_cast<T *>(side.y) + at, lane, a.d, half, INTERLEAVED, g);
       }
     }
   }
@@ -256,7 +290,7 @@ template <class T, int G> __global__ __launch_bounds__(256) void backward_kernel
       float *to = sums + (threadIdx.x >> 6) * kMostDim;
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
-        const int p = lane * kPairs + j, x = a.interleaved ? 2 * p : p, y = a.interleaved ? 2 * p + 1 : half + p;
+        const int p = lane * kPairs + j, x = INTERLEAVED ? 2 * p : p, y = INTERLEAVED ? 2 * p + 1 : half + p;
         if (p < half) to[x] = dw[k].a[j];
         if (p < half && y < a.d) to[y] = dw[k].b[j];
       }
@@ -331,6 +365,34 @@ static int64_t blocks_of(const spira_hip_heads_t &x, int lanes, int most) {
 }
 constexpr int kForwardBlocks = 2048, kBackwardBlocks = 512;
 
+// Turns of the pairs by a position, and their axes.  (64 powers in long double take as
+// long as a launch: a thread keeps the last ones.)
+struct Speeds {
+  double base = 0;
+  int pairs = 0, axes = 0;
+  uint64_t speed[kMostDim / 2] = {};
+  uint8_t axis[kMostDim / 2] = {};
+};
+static const Speeds &speeds(double base, int pairs, int axes) {
+  static thread_local Speeds t;
+  if (t.base == base && t.pairs == pairs && t.axes == axes) return t;
+  for (int axis = 0; axis < axes; ++axis) {
+    const int lo = axis * pairs / axes, hi = (axis + 1) * pairs / axes;
+    for (int p = lo; p < hi; ++p) {
+      // (in long double: 64 bits of the turn's fraction)
+      const long double turns = powl(static_cast<long double>(base), -static_cast<long double>(p - lo) / (hi - lo)) /
+                                6.283185307179586476925286766559L;
+      const long double scaled = (turns - floorl(turns)) * 18446744073709551616.0L;
+      t.speed[p] = scaled >= 18446744073709551615.0L ? ~uint64_t(0) : static_cast<uint64_t>(scaled);
+      t.axis[p] = static_cast<uint8_t>(axis);
+    }
+  }
+  t.base = base;
+  t.pairs = pairs;
+  t.axes = axes;
+  return t;
+}
+
 static Args arguments(const spira_hip_heads_t &x, int lanes) {
   Args a{};
   a.side[0] = {x.queries, x.query_weight, nullptr, x.query_row, x.query_head, x.heads, nullptr};
@@ -338,25 +400,13 @@ static Args arguments(const spira_hip_heads_t &x, int lanes) {
   a.n = x.rows;
   a.d = x.head_dim;
   a.axes = x.axes;
-  a.interleaved = x.interleaved;
   a.rows = block_rows(x, lanes);
   a.eps = x.eps;
   if (x.axes > 0) {
     a.positions = x.positions;
-    const int pairs = x.head_dim / 2;
-    for (int axis = 0; axis < x.axes; ++axis) {
-      const int lo = axis * pairs / x.axes, hi = (axis + 1) * pairs / x.axes;
-      for (int p = lo; p < hi; ++p) {
-        // (in long double: 64 bits of the turn's fraction)
-        const long double turns =
-            powl(static_cast<long double>(x.base), -static_cast<long double>(p - lo) / (hi - lo)) /
-            6.283185307179586476925286766559L;
-        const long double fraction = turns - floorl(turns);
-        const long double scaled = fraction * 18446744073709551616.0L;
-        a.speed[p] = scaled >= 18446744073709551615.0L ? ~uint64_t(0) : static_cast<uint64_t>(scaled);
-        a.axis[p] = axis;
-      }
-    }
+    const Speeds &t = speeds(x.base, x.head_dim / 2, x.axes);
+    std::copy(t.speed, t.speed + kMostDim / 2, a.speed);
+    std::copy(t.axis, t.axis + kMostDim / 2, a.axis);
   }
   return a;
 }
@@ -380,8 +430,9 @@ int spira_hip_norm_rotate_heads(const spira_hip_heads_t *x, void *queries, void 
       heads::Args a = heads::arguments(*x, g);
       a.side[0].y = queries;
       a.side[1].y = key;
-      hipLaunchKernelGGL((heads::forward_kernel<decltype(t), g>), dim3(heads::blocks_of(*x, g, heads::kForwardBlocks)),
-                         dim3(256), 0, stream, a);
+      using T = decltype(t);
+      const auto kernel = x->interleaved ? heads::forward_kernel<T, g, true> : heads::forward_kernel<T, g, false>;
+      hipLaunchKernelGGL(kernel, dim3(heads::blocks_of(*x, g, heads::kForwardBlocks)), dim3(256), 0, stream, a);
       SPIRA_HIP_LAUNCH_CHECK();
       return kOk;
     });
@@ -425,7 +476,8 @@ int spira_hip_norm_rotate_heads_backward(const spira_hip_heads_t *x, const void 
         a.partial = static_cast<float *>(workspace);
       }
       if (blocks > 0) {
-        hipLaunchKernelGGL((heads::backward_kernel<T, g>), dim3(blocks), dim3(256), 0, stream, a);
+        const auto kernel = x->interleaved ? heads::backward_kernel<T, g, true> : heads::backward_kernel<T, g, false>;
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, a);
         SPIRA_HIP_LAUNCH_CHECK();
       }
       if (dquery_weight || dkey_weight) {
