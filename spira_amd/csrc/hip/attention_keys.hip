@@ -19,10 +19,10 @@ namespace attention {
 constexpr int kOwnKeys = 128;
 template <class T> constexpr int kQueries = sizeof(T) == 2 ? 64 : 32;
 
-// SPLIT: a block takes every `splits`th step of its keys', from blockIdx.y on, and writes its
-// sums in fp32 to be joined.
+// SPLIT: a block takes every `splits`th step of its keys', the parts of a tile's keys behind
+// each other in the launch, and writes its sums in fp32 to be joined.
 template <class T, int DP, bool DMA, bool SPLIT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_kernel(const Args a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_kernel(const Args a, int parts) {
   using R = Rows<T, DP>;
   constexpr int QT = kQueries<T>, TILE = QT * R::PITCH;
   __shared__ __align__(1024) char lds[4 * TILE];
@@ -33,7 +33,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   if (!SPLIT && dk) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dk, width, blockIdx.x, gridDim.x);
   if (!SPLIT && dv) clear_uncovered(a.s.key_offsets, a.s.count, a.s.keys, dv, width, blockIdx.x, gridDim.x);
   const int kv = blockIdx.x % a.kv_heads;
-  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads, [&](const Sequence &x) {
+  const int splits = SPLIT ? parts : 1;
+  const int64_t piece = blockIdx.x / a.kv_heads;
+  const int part = SPLIT ? static_cast<int>(piece % splits) : 0;
+  const Found s = find_longest(a.s, piece / splits, [&](const Sequence &x) {
     return static_cast<int>((x.room + int64_t(kOwnKeys) - 1) / kOwnKeys);
   });
   if (!s.there) return;
@@ -46,7 +49,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   const int end = c0 < s.nk ? (s.nq + QT - 1) / QT : 0, middle = std::max(begin, std::min((latest + QT - 1) / QT, end));
   // The tiles of all heads that some key hides from (or the block's last), then those of
   // all heads that see every key: `splits`th by splits`th of them.
-  const int splits = SPLIT ? static_cast<int>(gridDim.y) : 1, part = SPLIT ? static_cast<int>(blockIdx.y) : 0;
   const auto mine_of = [&](int64_t n) { return static_cast<int>(n > part ? (n - part + splits - 1) / splits : 0); };
   const int64_t masked = static_cast<int64_t>(middle - begin) * a.group;
   const int hidden = mine_of(masked), steps = mine_of(masked + static_cast<int64_t>(std::max(0, end - middle)) * a.group);
@@ -251,11 +253,11 @@ template <class T, int DP, bool DMA> static int launch_keys(const Args &a, int s
   const int64_t blocks = (a.s.keys / kOwnKeys + a.s.count) * a.kv_heads;
   SPIRA_HIP_REQUIRE(launchable(blocks * splits, 256), "attention: too many tiles for a launch");
   if (splits == 1) {
-    hipLaunchKernelGGL((keys_kernel<T, DP, DMA, false>), dim3(blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((keys_kernel<T, DP, DMA, false>), dim3(blocks), dim3(256), 0, stream, a, 1);
     SPIRA_HIP_LAUNCH_CHECK();
     return kOk;
   }
-  hipLaunchKernelGGL((keys_kernel<T, DP, DMA, true>), dim3(blocks, splits), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((keys_kernel<T, DP, DMA, true>), dim3(blocks * splits), dim3(256), 0, stream, a, splits);
   SPIRA_HIP_LAUNCH_CHECK();
   const int64_t sums = div_up(a.s.keys * div_up(static_cast<int64_t>(a.kv_heads) * a.d, kVec<T>), 256);
   SPIRA_HIP_REQUIRE(launchable(sums * 2, 256), "attention: too many rows for a launch");

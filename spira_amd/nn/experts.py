@@ -2,7 +2,7 @@
 gate, dropout and residual.  No reference counterpart."""
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 from torch import nn
@@ -21,6 +21,10 @@ class ExpertBlock(nn.Module):
     softmax weights.  ``gate`` is learned per channel.  Takes and returns a
     ``SparseTensor`` of the same coordinates, behind any ``SparseConv`` block;
     parameters have the features' type (``.half()``, ``.bfloat16()``).
+
+    With ``balance`` a call returns (output, ``BalanceLoss``): the loss that keeps
+    the experts in use, for the training program to weigh and add to its own, and
+    how often each was chosen.
 
     Dropout acts in training mode.  Without a ``seed`` each call's mask is drawn
     from torch's CPU generator: another in every call, block and, where their
@@ -84,14 +88,16 @@ class ExpertBlock(nn.Module):
                                "(checkpointing has to preserve the state of torch's generator)")
         return draw if self.seed is None else (self.seed, self._numbers[draw])
 
-    def forward(self, input: SparseTensor) -> SparseTensor:
+    def forward(self, input: SparseTensor, balance: bool = False) -> Union[SparseTensor, Tuple[SparseTensor, F.BalanceLoss]]:
         x = input.features
         n = F.rms_norm(x, self.entry, self.eps)
-        routes = F.route_experts(n @ self.router, self.choices)
+        logits = n @ self.router
+        routes = F.route_experts(logits, self.choices)
         h = F.grouped_linear(n, self.up, routes, bias=self.up_bias, relu=True)
         h = F.grouped_linear(h, self.down, routes.offsets, bias=self.down_bias)
         h = F.combine_experts(h, routes)
         if self.training and self.dropout > 0:
             h = F.dropout(h, self.dropout, *self._mask())
         y, _ = F.gated_residual_norm(x, h, weight=self.exit, gate=self.gate, scale=self.scale, eps=self.eps)
-        return SparseTensor(coordinates=input.coordinates, features=y, stride=input.stride)
+        output = SparseTensor(coordinates=input.coordinates, features=y, stride=input.stride)
+        return (output, F.balance_loss(logits, routes)) if balance else output
