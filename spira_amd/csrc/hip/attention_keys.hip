@@ -235,13 +235,13 @@ template <class T> __global__ __launch_bounds__(256) void sums_kernel(const Args
 
 // Parts of the keys' steps.  A block of 128 keys has as many steps as its sequence has
 // queries (times the group's heads, over 64): a long sequence's blocks run on alone when
-// the others are done.  With parts for 8 blocks a CU, however long the sequences, at
+// the others are done.  With parts for 5 blocks a CU, however long the sequences, at
 // most 8 of them (their sums in fp32 are written and read again).
 int key_splits(const spira_hip_attention_t &x) {
   const int64_t blocks = (x.keys / kOwnKeys + x.sequences) * x.kv_heads;
   const int64_t steps = div_up(x.rows, 64) * (x.heads / x.kv_heads);
   const int64_t bytes = 2 * x.keys * x.kv_heads * x.head_dim * 4;
-  int64_t splits = std::min<int64_t>({2048 / std::max<int64_t>(blocks, 1), steps, 8});
+  int64_t splits = std::min<int64_t>({1280 / std::max<int64_t>(blocks, 1), steps, 8});
   if (bytes > 0) splits = std::min<int64_t>(splits, (int64_t(1) << 30) / bytes);
   return static_cast<int>(std::max<int64_t>(splits, 1));
 }
