@@ -664,15 +664,17 @@ typedef struct {
 int spira_hip_attention_workspace(const spira_hip_attention_t *x, int gradient, size_t *bytes);
 
 /* out [rows, heads, head_dim]; stats (null without a gradient): fp32 [heads, rows],
- * of fp32 features [2, heads, rows].  A call with stats needs no workspace. */
-int spira_hip_attention(const spira_hip_attention_t *x, void *out, float *stats, void *workspace,
+ * of fp32 features [2, heads, rows]; rest (null, and not written of fp32 features):
+ * like out, what its rounding left.  A call with stats needs no workspace. */
+int spira_hip_attention(const spira_hip_attention_t *x, void *out, float *stats, void *rest, void *workspace,
                         size_t workspace_bytes, hipStream_t stream);
 
-/* The gradients (any may be null) from dout, with out and stats of the forward pass:
+/* The gradients (any may be null) from dout, with out, stats and rest (or null: a
+ * little less exact) of the forward pass:
  * dqueries [rows, heads, head_dim], dkey and dvalue [keys, kv_heads, head_dim], zeros
  * in rows of no sequence and behind a sequence's keys. */
-int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out, const float *stats, const void *dout,
-                                 void *dqueries, void *dkey, void *dvalue, void *workspace, size_t workspace_bytes,
+int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out, const float *stats, const void *rest,
+                                 const void *dout, void *dqueries, void *dkey, void *dvalue, void *workspace, size_t workspace_bytes,
                                  hipStream_t stream);
 
 /* For each head of each row, n = x / sqrt(mean(x^2) + eps) * weight (weight

@@ -168,7 +168,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   }
   const float l = c.l + other_half(c.l);
   const bool there = column < total;
-  store_column<T, DP>(o + ((s.q0 + i) * a.heads + head) * a.d, a.d, there, c.o, l == 0.f ? 0.f : 1.f / l);
+  const int64_t at = ((s.q0 + i) * a.heads + head) * a.d;
+  store_column<T, DP>(o + at, a.d, there, c.o, l == 0.f ? 0.f : 1.f / l, a.rest ? static_cast<T *>(a.rest) + at : nullptr);
   if (a.stats && there && lane < 32) put_statistics<T>(a, head, s.q0 + i, c.m, l);
 }
 
@@ -294,8 +295,12 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP, DIRECT>::NW), 1) void token
       const int q_at = (w0 + col) / a.group, h_at = kv * a.group + (w0 + col - q_at * a.group);
       const int64_t at = (s.q0 + q_at) * a.heads + h_at;
       const float sum = total_l[col];
-      if constexpr (DIRECT) o[at * a.d + d] = from_float<T>(sum == 0.f ? 0.f : v / sum);
-      else a.partial[(s.nth * a.s.rows * a.heads + at) * a.d + d] = v;
+      if constexpr (DIRECT) {
+        const float value = sum == 0.f ? 0.f : v / sum;
+        const T rounded = from_float<T>(value);
+        o[at * a.d + d] = rounded;
+        if (a.rest) static_cast<T *>(a.rest)[at * a.d + d] = from_float<T>(value - to_float(rounded));
+      } else a.partial[(s.nth * a.s.rows * a.heads + at) * a.d + d] = v;
     }
     if constexpr (DIRECT) {
       if (a.stats && static_cast<int>(threadIdx.x) < columns)
@@ -503,7 +508,7 @@ int spira_hip_attention_workspace(const spira_hip_attention_t *x, int gradient, 
   return kOk;
 }
 
-int spira_hip_attention(const spira_hip_attention_t *x, void *out, float *stats, void *workspace,
+int spira_hip_attention(const spira_hip_attention_t *x, void *out, float *stats, void *rest, void *workspace,
                         size_t workspace_bytes, hipStream_t stream) {
   SPIRA_HIP_REQUIRE(x, "attention: null arguments");
   attention::Args a;
@@ -515,6 +520,8 @@ int spira_hip_attention(const spira_hip_attention_t *x, void *out, float *stats,
   SPIRA_HIP_REQUIRE(workspace_bytes >= need && (workspace || need == 0), "attention: workspace too small");
   a.o = out;
   a.stats = stats;
+  // (in fp32 nothing that counts is left)
+  a.rest = x->dtype == SPIRA_F32 ? nullptr : rest;
   a.partial = static_cast<float *>(workspace);
   a.partial_stats = a.partial ? a.partial + p.parts * x->rows * x->heads * x->head_dim : nullptr;
   return with_type(x->dtype, [&](auto t) -> int {

@@ -212,6 +212,17 @@ template <class T> __device__ __forceinline__ Frag<T> as_operand(const floatx16 
   return f;
 }
 
+// What as_operand's rounding left of them, as another operand: with both, the sums that
+// follow are as good as in fp32.
+template <class T> __device__ __forceinline__ Frag<T> rest_operand(const floatx16 &p, int s, const Frag<T> &rounded) {
+  T t[8];
+  __builtin_memcpy(t, &rounded, sizeof(t));
+  floatx16 rest{};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest[i] = p[8 * s + i] - to_float(t[i]);
+  return as_operand<T>(rest, 0);
+}
+
 // Where a lane reads of a tile.  What a fragment's number changes of an address is
 // bits that the swizzle has not moved together: an exclusive or of a constant, and
 // a constant offset.
@@ -398,11 +409,13 @@ __device__ __forceinline__ void add_not_finite(floatx16 (&acc)[DP / 32], const c
 // ---------------------------------------------------------------------------
 // columns to memory
 // ---------------------------------------------------------------------------
-// A column's sums times `by` to its row of d values.  The halves exchange groups of
-// four values, so that each lane writes eight consecutive ones.  Every lane takes
-// part; `there`: its column is to be written.
+// A column's sums times `by` to its row of d values, and what their rounding left of them
+// to another (or null).  The halves exchange groups of four values, so that each lane
+// writes eight consecutive ones.  Every lane takes part; `there`: its column is to be
+// written.
 template <class T, int DP>
-__device__ __forceinline__ void store_column(T *row, int d, bool there, const floatx16 (&acc)[DP / 32], float by) {
+__device__ __forceinline__ void store_column(T *row, int d, bool there, const floatx16 (&acc)[DP / 32], float by,
+                                             T *rest = nullptr) {
   const int h = lane_id() >> 5;
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n)
@@ -424,6 +437,11 @@ __device__ __forceinline__ void store_column(T *row, int d, bool there, const fl
 #pragma unroll
         for (int i = 0; i < kVec<T>; ++i) k.v[i] = v[c * kVec<T> + i];
         if (there) store_chunk(row + at + c * kVec<T>, d - at - c * kVec<T>, k);
+        if (there && rest) {
+#pragma unroll
+          for (int i = 0; i < kVec<T>; ++i) k.v[i] -= to_float(from_float<T>(k.v[i]));
+          store_chunk(rest + at + c * kVec<T>, d - at - c * kVec<T>, k);
+        }
       }
     }
 }
@@ -470,6 +488,7 @@ struct Args {
   void *o;       // [rows, heads, d]
   float *stats;  // [heads, rows] log2 of the sum of exp2 of a row's scaled scores; fp32: [2, heads, rows], their
                  // largest and the inverse of the sum beside it
+  void *rest;    // [rows, heads, d], 16 bits: what the outputs' rounding left of them, for delta
   // few tokens
   float *partial, *partial_stats;
   int part_keys;  // keys a part

@@ -33,17 +33,21 @@ template <class T, int DP> struct QueryColumn {
     const int64_t at = (s.q0 + i) * a.heads + head;
     const T *row = static_cast<const T *>(a.q) + (s.q0 + i) * a.q_row + head * a.q_head;
     const T *grow = static_cast<const T *>(a.dout) + at * a.d, *orow = static_cast<const T *>(a.out) + at * a.d;
+    // (the outputs with what their rounding left: without, delta's error doubles that of dq
+    // and dk in sequences of some ten tokens, and adds a twentieth in long ones)
+    const T *rest = a.rest ? static_cast<const T *>(a.rest) + at * a.d : nullptr;
     delta = 0;
 #pragma unroll
     for (int st = 0; st < DP / 16; ++st) {
       q[st] = load_frag(row, a.d, st);
       g[st] = load_frag(grow, a.d, st);
-      const Frag<T> of = load_frag(orow, a.d, st);
-      T x[8], y[8];
+      const Frag<T> of = load_frag(orow, a.d, st), rf = load_frag(rest, a.d, st);
+      T x[8], y[8], z[8];
       __builtin_memcpy(x, &g[st], sizeof(x));
       __builtin_memcpy(y, &of, sizeof(y));
+      __builtin_memcpy(z, &rf, sizeof(z));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta += to_float(x[e]) * to_float(y[e]);
+      for (int e = 0; e < 8; ++e) delta += to_float(x[e]) * (to_float(y[e]) + to_float(z[e]));
     }
     delta += other_half(delta);
     const int64_t to = head * a.s.rows + s.q0 + i;
@@ -69,12 +73,20 @@ template <class T, int DP> struct QueryColumn {
       ds[x] = !MASKED || 8 * (x / 4) + x % 4 < mine ? w : 0.f;
     }
   }
-  __device__ __forceinline__ void accumulate(const Reader<T, DP> &read, lds_char *kt, const floatx16 &ds) {
+  // FINE (16 bits): with what the rounding of ds leaves.  Tiles on the mask's edge take it:
+  // the rows that see few keys have their weights there, whose roundings do not average out.
+  template <bool FINE> __device__ __forceinline__ void accumulate(const Reader<T, DP> &read, lds_char *kt, const floatx16 &ds) {
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const Frag<T> f = as_operand<T>(ds, st);
+      Frag<T> g;
+      if constexpr (FINE && sizeof(T) == 2) g = rest_operand<T>(ds, st, f);
 #pragma unroll
-      for (int n = 0; n < DP / 32; ++n) mma(acc[n], read.cols(kt, 16 * st, n), f);
+      for (int n = 0; n < DP / 32; ++n) {
+        const Frag<T> k = read.cols(kt, 16 * st, n);
+        mma(acc[n], k, f);
+        if constexpr (FINE && sizeof(T) == 2) mma(acc[n], k, g);
+      }
     }
   }
 };
@@ -122,7 +134,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
     for (int u = 0; u < KT / 32; ++u) {
       floatx16 ds;
       c.template gradients<false>(a, read, kt + 32 * u * R::PITCH, kt + TILE + 32 * u * R::PITCH, 0, ds);
-      c.accumulate(read, kt + 32 * u * R::PITCH, ds);
+      c.template accumulate<false>(read, kt + 32 * u * R::PITCH, ds);
     }
   });
   // the others; the block stays together
@@ -140,7 +152,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
         __syncthreads();  // (every wave has the scores)
         found = __syncthreads_or(clear_not_finite<T, DP, 32, 256>(kt, threadIdx.x));
       }
-      c.accumulate(read, kt, ds);
+      c.template accumulate<true>(read, kt, ds);
       if (found)
         add_not_finite<T, DP>(c.acc, keys + first * kstride, kstride, std::min(s.nk - first, 32), a.d,
                               [&](int x) { return x < seen; });
@@ -193,13 +205,13 @@ __global__ __launch_bounds__(64 * 2, 1) void few_queries_kernel(const Args a) {
     floatx16 ds;
     if (fewest >= (t + 1) * KT) {
       c.template gradients<false>(a, read, kt, kt + TILE, 0, ds);
-      c.accumulate(read, kt, ds);
+      c.template accumulate<false>(read, kt, ds);
       continue;
     }
     const int seen = limit - t * KT;
     c.template gradients<true>(a, read, kt, kt + TILE, seen, ds);
     const bool found = a.causal && ballot(clear_not_finite<T, DP, KT, 64>(kt, lane)) != 0;
-    c.accumulate(read, kt, ds);
+    c.template accumulate<true>(read, kt, ds);
     if (found)
       add_not_finite<T, DP>(c.acc, keys + t * (KT * kstride), kstride, std::min(s.nk - t * KT, KT), a.d,
                             [&](int x) { return x < seen; });
@@ -241,8 +253,8 @@ using namespace spira_hip;
 
 extern "C" {
 
-int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out, const float *stats, const void *dout,
-                                 void *dqueries, void *dkey, void *dvalue, void *workspace, size_t workspace_bytes,
+int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out, const float *stats, const void *rest,
+                                 const void *dout,                                 void *dqueries, void *dkey, void *dvalue, void *workspace, size_t workspace_bytes,
                                  hipStream_t stream) {
   SPIRA_HIP_REQUIRE(x, "attention: null arguments");
   const int size = x->dtype == SPIRA_F32 ? 4 : 2;
@@ -254,6 +266,7 @@ int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out
   a.out = out;
   a.dout = dout;
   a.stats = const_cast<float *>(stats);
+  a.rest = x->dtype == SPIRA_F32 ? nullptr : const_cast<void *>(rest);
   a.delta = static_cast<float *>(workspace);
   a.partial = a.delta ? a.delta + attention::delta_bytes(*x) / sizeof(float) : nullptr;
   a.dq = dqueries;

@@ -134,12 +134,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       }
     }
   };
-  const auto accumulate = [&](floatx16 (&acc)[DP / 32], lds_char *tile, const floatx16 &p) {
+  // FINE (16 bits): with what the rounding leaves, as for dq
+  const auto accumulate = [&](auto FINE, floatx16 (&acc)[DP / 32], lds_char *tile, const floatx16 &p) {
+    constexpr bool fine = decltype(FINE)::value && sizeof(T) == 2;
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const Frag<T> f = as_operand<T>(p, st);
+      Frag<T> g;
+      if constexpr (fine) g = rest_operand<T>(p, st, f);
 #pragma unroll
-      for (int n = 0; n < DP / 32; ++n) mma(acc[n], read.cols(tile, 16 * st, n), f);
+      for (int n = 0; n < DP / 32; ++n) {
+        const Frag<T> x = read.cols(tile, 16 * st, n);
+        mma(acc[n], x, f);
+        if constexpr (fine) mma(acc[n], x, g);
+      }
     }
   };
   for (int index = 0; index < hidden; ++index) {
@@ -159,8 +167,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       __syncthreads();  // (every wave has the scores)
       const bool x = clear_not_finite<T, DP, 32, 256>(qu, threadIdx.x), y = clear_not_finite<T, DP, 32, 256>(gu, threadIdx.x);
       const bool found = __syncthreads_or(x || y);
-      accumulate(av, gu, p);
-      accumulate(ak, qu, ds);
+      accumulate(std::true_type{}, av, gu, p);
+      accumulate(std::true_type{}, ak, qu, ds);
       if (found) {
         const int64_t r0 = s.q0 + q0 + 32 * u;
         const int n = std::min(s.nq - q0 - 32 * u, 32);
@@ -183,8 +191,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
     for (int u = 0; u < QT / 32; ++u) {
       floatx16 p, ds;
       weights(std::false_type{}, stage, 32 * u, 0, p, ds);
-      accumulate(av, gt + 32 * u * R::PITCH, p);
-      accumulate(ak, qt + 32 * u * R::PITCH, ds);
+      accumulate(std::false_type{}, av, gt + 32 * u * R::PITCH, p);
+      accumulate(std::false_type{}, ak, qt + 32 * u * R::PITCH, ds);
     }
   });
   // (keys that are none, in the room behind the others, get zeros)

@@ -66,34 +66,37 @@ static spira_hip_attention_t attention_arguments(const Tensor &q, const Tensor &
   return x;
 }
 
-// (output, statistics of its rows or None unless `train`)
-static std::tuple<Tensor, OptTensor> attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets,
+// (output, statistics of its rows and what rounding left of it, or None unless `train`)
+static std::tuple<Tensor, OptTensor, OptTensor> attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets,
                                                const Tensor &key_offsets, const OptTensor &key_counts, bool causal,
                                                double scale, bool train) {
   const spira_hip_attention_t x = attention_arguments(q, k, v, offsets, key_offsets, key_counts, causal, scale);
   const c10::DeviceGuard guard(q.device());
   Tensor out = like(q, q.sizes());
-  OptTensor stats;
+  OptTensor stats, rest;
   size_t bytes = 0;
-  if (train) stats = floats(q, {q.scalar_type() == torch::kFloat ? 2 : 1, q.size(1), q.size(0)});
-  else check_rc(spira_hip_attention_workspace(&x, 0, &bytes), "attention");
+  const bool full = q.scalar_type() == torch::kFloat;
+  if (train) stats = floats(q, {full ? 2 : 1, q.size(1), q.size(0)});
+  if (train && !full) rest = like(q, q.sizes());
+  if (!train) check_rc(spira_hip_attention_workspace(&x, 0, &bytes), "attention");
   Tensor ws = bytes > 0 ? workspace(bytes, q.device()) : Tensor();
   check_rc(spira_hip_attention(&x, out.data_ptr(), stats ? stats->data_ptr<float>() : nullptr,
-                               bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()),
+                               rest ? rest->data_ptr() : nullptr, bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()),
            "attention");
-  return {out, stats};
+  return {out, stats, rest};
 }
 
 // (dq, dk, dv), each None unless it is in `need`
 static std::array<OptTensor, 3> attention_backward(const Tensor &q, const Tensor &k, const Tensor &v,
                                                    const Tensor &offsets, const Tensor &key_offsets,
                                                    const OptTensor &key_counts, bool causal, double scale,
-                                                   const Tensor &out, const Tensor &stats, const Tensor &dout,
+                                                   const Tensor &out, const Tensor &stats, const OptTensor &rest, const Tensor &dout,
                                                    int64_t need) {
   const spira_hip_attention_t x = attention_arguments(q, k, v, offsets, key_offsets, key_counts, causal, scale);
   require(dout, "gradient", q, q.scalar_type(), {q.size(0), q.size(1), q.size(2)});
   require(out, "output", q, q.scalar_type(), {q.size(0), q.size(1), q.size(2)});
   require(stats, "statistics", q, torch::kFloat, {q.scalar_type() == torch::kFloat ? 2 : 1, q.size(1), q.size(0)});
+  require(rest, "rest", q, q.scalar_type(), {q.size(0), q.size(1), q.size(2)});
   const c10::DeviceGuard guard(q.device());
   std::array<OptTensor, 3> d;
   if (need & 1) d[0] = like(q, q.sizes());
@@ -103,8 +106,8 @@ static std::array<OptTensor, 3> attention_backward(const Tensor &q, const Tensor
   check_rc(spira_hip_attention_workspace(&x, 1, &bytes), "attention");
   Tensor ws = workspace(bytes, q.device());
   const auto at = [&](int i) { return d[i] ? d[i]->data_ptr() : nullptr; };
-  check_rc(spira_hip_attention_backward(&x, out.data_ptr(), stats.data_ptr<float>(), dout.data_ptr(), at(0), at(1),
-                                        at(2), ws.data_ptr(), bytes, current_stream()),
+  check_rc(spira_hip_attention_backward(&x, out.data_ptr(), stats.data_ptr<float>(), ptr(rest), dout.data_ptr(), at(0),
+                                        at(1), at(2), ws.data_ptr(), bytes, current_stream()),
            "attention");
   return d;
 }
@@ -112,8 +115,8 @@ static std::array<OptTensor, 3> attention_backward(const Tensor &q, const Tensor
 struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
   static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets,
                         const Tensor &key_offsets, const OptTensor &key_counts, bool causal, double scale) {
-    auto [out, stats] = attention(q, k, v, offsets, key_offsets, key_counts, causal, scale, true);
-    ctx->save_for_backward({q, k, v, offsets, key_offsets, given(key_counts), out, *stats});
+    auto [out, stats, rest] = attention(q, k, v, offsets, key_offsets, key_counts, causal, scale, true);
+    ctx->save_for_backward({q, k, v, offsets, key_offsets, given(key_counts), out, *stats, given(rest)});
     ctx->saved_data["need"] = int64_t(q.requires_grad()) | int64_t(k.requires_grad()) << 1 | int64_t(v.requires_grad()) << 2;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
@@ -122,7 +125,7 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
   static variable_list backward(AutogradContext *ctx, variable_list d) {
     const variable_list v = ctx->get_saved_variables();
     auto g = attention_backward(v[0], v[1], v[2], v[3], v[4], maybe(v[5]), ctx->saved_data["causal"].toBool(),
-                                ctx->saved_data["scale"].toDouble(), v[6], v[7], dense(d[0]),
+                                ctx->saved_data["scale"].toDouble(), v[6], v[7], maybe(v[8]), dense(d[0]),
                                 ctx->saved_data["need"].toInt());
     return once({given(g[0]), given(g[1]), given(g[2]), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, "attention");
   }

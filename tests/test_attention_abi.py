@@ -54,33 +54,33 @@ BAD = [(dict(rows=-1), "rows"), (dict(rows=1 << 31), "rows"), (dict(keys=1 << 31
 @pytest.mark.parametrize("bad,text", BAD)
 def test_attention(bad, text):
     x, size = attention(**bad), SIZE()
-    refused(LIB.spira_hip_attention(ctypes.byref(x), P(SOME), None, None, SIZE(0), None), text)
+    refused(LIB.spira_hip_attention(ctypes.byref(x), P(SOME), None, None, None, SIZE(0), None), text)
     refused(LIB.spira_hip_attention_workspace(ctypes.byref(x), 0, ctypes.byref(size)), text)
-    refused(LIB.spira_hip_attention_backward(ctypes.byref(x), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME),
+    refused(LIB.spira_hip_attention_backward(ctypes.byref(x), P(SOME), P(SOME), None, P(SOME), P(SOME), P(SOME), P(SOME), P(SOME),
                                              SIZE(1 << 40), None), text)
 
 
 def test_attention_outputs_and_workspaces():
     x, size = attention(), SIZE()
-    refused(LIB.spira_hip_attention(None, P(SOME), None, None, SIZE(0), None), "null")
-    refused(LIB.spira_hip_attention(ctypes.byref(x), None, None, None, SIZE(0), None), "null")
-    refused(LIB.spira_hip_attention(ctypes.byref(attention(dtype=7)), P(SOME), None, None, SIZE(0), None), "dtype")
-    refused(LIB.spira_hip_attention_backward(ctypes.byref(x), P(SOME), None, P(SOME), P(SOME), P(SOME), P(SOME), P(SOME),
+    refused(LIB.spira_hip_attention(None, P(SOME), None, None, None, SIZE(0), None), "null")
+    refused(LIB.spira_hip_attention(ctypes.byref(x), None, None, None, None, SIZE(0), None), "null")
+    refused(LIB.spira_hip_attention(ctypes.byref(attention(dtype=7)), P(SOME), None, None, None, SIZE(0), None), "dtype")
+    refused(LIB.spira_hip_attention_backward(ctypes.byref(x), P(SOME), None, None, P(SOME), P(SOME), P(SOME), P(SOME), P(SOME),
                                              SIZE(1 << 40), None), "null")
     assert LIB.spira_hip_attention_workspace(ctypes.byref(x), 1, ctypes.byref(size)) == 0 and size.value >= 100 * 4 * 4
-    refused(LIB.spira_hip_attention_backward(ctypes.byref(x), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME), P(SOME),
+    refused(LIB.spira_hip_attention_backward(ctypes.byref(x), P(SOME), P(SOME), None, P(SOME), P(SOME), P(SOME), P(SOME), P(SOME),
                                              SIZE(size.value - 1), None), "workspace")
     # few tokens against a long cache: the parts' sums
     x = attention(rows=2, keys=100_000)
     assert LIB.spira_hip_attention_workspace(ctypes.byref(x), 0, ctypes.byref(size)) == 0 and size.value > 0
     assert size.value % (2 * 4 * 66 * 4) == 0
-    refused(LIB.spira_hip_attention(ctypes.byref(x), P(SOME), None, P(SOME), SIZE(size.value - 1), None), "workspace")
-    refused(LIB.spira_hip_attention(ctypes.byref(x), P(SOME), None, None, SIZE(1 << 40), None), "workspace")
+    refused(LIB.spira_hip_attention(ctypes.byref(x), P(SOME), None, None, P(SOME), SIZE(size.value - 1), None), "workspace")
+    refused(LIB.spira_hip_attention(ctypes.byref(x), P(SOME), None, None, None, SIZE(1 << 40), None), "workspace")
     # whatever the sizes, they stay within some hundred MB
     for rows, keys, heads, kv in ((1, (1 << 31) - 1, 64, 1), (4000, 1 << 30, 64, 64), (64, 1 << 20, 128, 2), (1, 0, 1, 1)):
         x = attention(rows=rows, keys=keys, heads=heads, kv_heads=kv, sequences=max(1, rows // 2), head_dim=128)
         assert LIB.spira_hip_attention_workspace(ctypes.byref(x), 0, ctypes.byref(size)) == 0 and size.value < 1 << 29
-    assert LIB.spira_hip_attention(ctypes.byref(attention(rows=0, queries=None)), None, None, None, SIZE(0), None) == 0
+    assert LIB.spira_hip_attention(ctypes.byref(attention(rows=0, queries=None)), None, None, None, None, SIZE(0), None) == 0
 
 
 def test_norm_rotate_heads():
