@@ -93,7 +93,7 @@ __device__ __forceinline__ void put_statistics(const Args &a, int head, int64_t 
   float *to = a.stats + head * a.s.rows + row;
   const float base = m == -__builtin_inff() ? 0.f : m * a.scale2;
   if constexpr (sizeof(T) == 2) {
-    *to = l == 0.f ? __builtin_inff() : base + __builtin_amdgcn_logf(l);
+    *to = l == 0.f ? __builtin_inff() : base + __builtin_amdgcn_logf(l) - kLift<T>;
   } else {
     to[0] = base;
     to[a.heads * a.s.rows] = l == 0.f ? 0.f : 1.f / l;
@@ -209,7 +209,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP, DIRECT>::NW), 1) void token
   const Found s = DIRECT ? find_longest(a.s, blockIdx.x / a.kv_heads,
                                         [&](const Sequence &x) { return (x.nq * a.group + 31) / 32; })
                          : find_piece(a.s, blockIdx.x / a.kv_heads, [&](const Sequence &x) {
-                             return x.nq == 0 ? 0 : (x.nk + a.part_keys - 1) / a.part_keys;
+                             return x.nq == 0 || x.nk == 0 ? 0 : (x.nk - 1) / a.part_keys + 1;
                            });
   if (!s.there) return;
   const int first = DIRECT ? 0 : s.nth * a.part_keys, total = s.nq * a.group;
@@ -330,7 +330,8 @@ template <class T> __global__ __launch_bounds__(256) void join_kernel(const Args
     const Sequence s = sequence_at(a.s, b < a.s.count ? b : a.s.count - 1);
     const uint64_t found = ballot(b < a.s.count && row >= s.q0 && row < s.q0 + s.nq);
     if (found) {
-      parts = (__shfl(s.nk, __builtin_ctzll(found), 64) + a.part_keys - 1) / a.part_keys;
+      const int n = __shfl(s.nk, __builtin_ctzll(found), 64);
+      parts = n > 0 ? (n - 1) / a.part_keys + 1 : 0;
       break;
     }
   }
@@ -401,14 +402,14 @@ template <class T> __global__ __launch_bounds__(256) void join_kernel(const Args
 // launches
 // ---------------------------------------------------------------------------
 static int check(const spira_hip_attention_t &x) {
-  SPIRA_HIP_REQUIRE(x.rows >= 0 && x.rows < (int64_t(1) << 31) && x.keys >= 0 && x.keys < (int64_t(1) << 31),
-                    "attention: bad number of rows");
+  constexpr int64_t most = (int64_t(1) << 31) - 256;  // (whole tiles are counted in 32 bits)
+  SPIRA_HIP_REQUIRE(x.rows >= 0 && x.rows <= most && x.keys >= 0 && x.keys <= most, "attention: bad number of rows");
   SPIRA_HIP_REQUIRE(x.sequences > 0 && x.sequences <= (1 << 24), "attention: needs 1 to 2^24 sequences");
   SPIRA_HIP_REQUIRE(x.heads > 0 && x.kv_heads > 0 && x.heads <= 65536 && x.heads % x.kv_heads == 0,
                     "attention: the number of query heads must be a multiple of the key heads'");
   SPIRA_HIP_REQUIRE(x.head_dim > 0 && x.head_dim <= kMostHeadDim, "attention: needs heads of 1 to 128 values");
-  SPIRA_HIP_REQUIRE(x.rows * (x.heads / x.kv_heads) < (int64_t(1) << 31) - kColumns, "attention: too many queries");
-  SPIRA_HIP_REQUIRE(x.scale > 0 && x.scale < __builtin_inff(), "attention: the scale must be positive and finite");
+  SPIRA_HIP_REQUIRE(x.rows * (x.heads / x.kv_heads) <= most, "attention: too many queries");
+  SPIRA_HIP_REQUIRE(x.scale > 0 && x.scale <= 1e38f, "attention: the scale must be positive and finite");
   SPIRA_HIP_REQUIRE(x.offsets && x.key_offsets, "attention: null offsets");
   SPIRA_HIP_REQUIRE((x.rows == 0 || x.queries) && (x.keys == 0 || (x.key && x.value)), "attention: null features");
   return kOk;

@@ -486,15 +486,15 @@ struct Args {
   const void *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   void *o;       // [rows, heads, d]
-  float *stats;  // [heads, rows] log2 of the sum of exp2 of a row's scaled scores; fp32: [2, heads, rows], their
-                 // largest and the inverse of the sum beside it
+  float *stats;  // [heads, rows] log2 of the sum of exp2 of a row's scaled scores, less kLift; fp32: [2, heads,
+                 // rows], their largest and the inverse of the sum beside it
   void *rest;    // [rows, heads, d], 16 bits: what the outputs' rounding left of them, for delta
   // few tokens
   float *partial, *partial_stats;
   int part_keys;  // keys a part
   // backward
   const void *dout, *out;
-  float *delta;  // [heads, rows]
+  float *delta;  // [heads, rows], times kLower
   void *dq, *dk, *dv;
 };
 
@@ -510,9 +510,15 @@ template <class T> constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
 // keys that query i of a sequence sees
 __device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) {
   if (!a.causal) return s.nk;
-  const int n = i + 1 + s.nk - s.nq;
+  const int n = s.nk - (s.nq - 1 - i);
   return n < 0 ? 0 : n < s.nk ? n : s.nk;
 }
+
+// fp16: weights take part in sums lifted by 2^14, and their statistics are kept so:
+// those of long sequences, some 1 / n each, would be below 2^-14, where the type has
+// fewer bits.
+template <class T> constexpr int kLift = std::is_same_v<T, _Float16> ? 14 : 0;
+template <class T> constexpr float kLower = 1.f / static_cast<float>(1 << kLift<T>);
 
 // a row's statistics, and p from a raw score
 template <class T> struct Stat {

@@ -129,7 +129,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       for (int y = 0; y < 4; ++y) {
         const float w = weight(p[4 * x + y], a.scale2, Stat<T>{base[y], by[y]});
         const bool seen = !decltype(MASKED)::value || 8 * x + y >= mine - 4 * h;
-        ds[4 * x + y] = seen ? w * (ds[4 * x + y] - delta[y]) : 0.f;
+        // (w is lifted, delta lowered)
+        ds[4 * x + y] = seen ? w * __builtin_fmaf(ds[4 * x + y], kLower<T>, -delta[y]) : 0.f;
         p[4 * x + y] = seen ? w : 0.f;
       }
     }
@@ -204,11 +205,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   if constexpr (SPLIT) {
     float *sums = a.partial + part * 2 * a.s.keys * width + to;
     store_column<float, DP>(sums, a.d, there, ak, a.scale);
-    store_column<float, DP>(sums + a.s.keys * width, a.d, there, av, 1.f);
+    store_column<float, DP>(sums + a.s.keys * width, a.d, there, av, kLower<T>);
     return;
   }
   if (dk) store_column<T, DP>(dk + to, a.d, key < s.room, ak, a.scale);
-  if (dv) store_column<T, DP>(dv + to, a.d, key < s.room, av, 1.f);
+  if (dv) store_column<T, DP>(dv + to, a.d, key < s.room, av, kLower<T>);
 }
 
 // dk (blockIdx.y 0) and dv from the splits' sums, in their order; zeros in rows that are no keys

@@ -38,7 +38,7 @@ static spira_hip_attention_t attention_arguments(const Tensor &q, const Tensor &
   require(offsets, "offsets", q, torch::kInt, {-1});
   require(key_offsets, "key_offsets", q, torch::kInt, {offsets.size(0)});
   require(key_counts, "key_counts", q, torch::kInt, {offsets.size(0) - 1});
-  SPIRA_CHECK_ARG(scale > 0 && scale <= 3e38, "attention: the scale must be positive and finite, got ", scale);
+  SPIRA_CHECK_ARG(scale > 1e-38 && scale <= 1e38, "attention: the scale must be positive and finite, got ", scale);
   spira_hip_attention_t x{};
   x.rows = q.size(0);
   x.keys = k.size(0);
@@ -136,7 +136,7 @@ static Tensor attention_call(const Tensor &q, const Tensor &k, const Tensor &v, 
                              std::optional<double> scale) {
   SPIRA_CHECK_ARG(q.dim() == 3, "queries must have the shape [rows, heads, values], got ", q.sizes());
   const double by = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(q.size(2), 1)));
-  SPIRA_CHECK_ARG(key_offsets || key_counts || k.size(0) == q.size(0),
+  SPIRA_CHECK_ARG(key_offsets || (k.dim() == 3 && k.size(0) == q.size(0)),
                   "attention: without offsets of their own the keys are as many as the queries, got ", k.sizes(), " and ",
                   q.sizes());
   const Tensor off = dense(offsets), key_off = key_offsets ? dense(*key_offsets) : off;

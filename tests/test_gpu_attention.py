@@ -142,6 +142,13 @@ def test_sequences(dev, lengths, heads, kv, d, causal, dtype):
     check(dev, randn((n, heads, d), dt, 1), randn((n, kv, d), dt, 2), randn((n, kv, d), dt, 3), lengths, causal=causal)
 
 
+@pytest.mark.parametrize("dtype,causal", [("f16", False), ("bf16", True)])
+def test_a_long_sequence(dev, dtype, causal):
+    """Weights of some 1e-4 each, many tiles, and parts of the keys' steps."""
+    dt, n = DTYPES[dtype], 9001
+    check(dev, randn((n, 2, 24), dt, 1), randn((n, 1, 24), dt, 2), randn((n, 1, 24), dt, 3), [n], causal=causal)
+
+
 CROSS = [
     # queries, keys (room), keys in use, heads, key heads, values
     ([1, 1], [40, 700], None, 8, 2, 64), ([1] * 5, [300, 64, 128, 1024, 70], [299, 0, 128, 1000, 1], 4, 1, 128),
@@ -371,6 +378,7 @@ def test_refusals(dev):
     refused("key_offsets must have the shape", q, k, k, off, key_offsets=torch.zeros(3, dtype=torch.int32, device=dev))
     refused("key_counts must have the shape", q, k, k, off, key_counts=off)
     refused("as many as the queries", q, k[:4], k[:4], off)
+    refused("as many as the queries", q, k[:4], k[:4], off, key_counts=off[1:])
     refused("must be a GPU tensor", q, k.cpu(), k, off)
     refused("must be a GPU tensor", q, k, k, off.cpu())
     for scale in (0.0, -1.0, math.inf, math.nan):
