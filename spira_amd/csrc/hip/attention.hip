@@ -444,9 +444,8 @@ struct Plan {
 static Plan plan(const spira_hip_attention_t &x, bool stats) {
   const int64_t group = x.heads / x.kv_heads, columns = div_up(x.rows * group, x.sequences);
   const Plan prompts{false, 0, 0}, direct{true, 1, 1};
-  const int64_t blocks = (x.rows * group / kColumns + x.sequences) * x.kv_heads;
   // (a gradient's statistics come from one block per column)
-  if (columns > 64 || stats) return blocks < kFewBlocks ? direct : prompts;
+  if (columns > 64 || stats) return few_columns(x) ? direct : prompts;
   const int64_t tiles = div_up(columns, 32);
   const int64_t size = round_up(std::max<int64_t>(div_up(x.keys * x.kv_heads * tiles, 2048), 256), 64);
   // (partial sums of at most 256 MB)

@@ -231,10 +231,9 @@ __global__ __launch_bounds__(64 * 2, 1) void few_queries_kernel(const Args a) {
   }
 }
 
-template <class T, int DP> static int launch(const Args &a, hipStream_t stream) {
+template <class T, int DP> static int launch(const Args &a, bool few, hipStream_t stream) {
   if (a.s.rows > 0) {
     int64_t blocks = (a.s.rows * a.group / kColumns + a.s.count) * a.kv_heads;
-    const bool few = blocks < kFewBlocks;
     if (few) blocks = (a.s.rows * a.group / 32 + a.s.count) * a.kv_heads;
     SPIRA_HIP_REQUIRE(launchable(blocks, 256), "attention: too many tiles for a launch");
     const auto kernel = few ? (a.dma & kKeysByDma ? few_queries_kernel<T, DP, true> : few_queries_kernel<T, DP, false>)
@@ -276,7 +275,7 @@ int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out
     a.dma &= ~attention::kQueriesByDma;
   const int rc = with_type(x->dtype, [&](auto t) -> int {
     return attention::with_width(x->head_dim, [&](auto W) -> int {
-      return attention::launch<decltype(t), decltype(W)::value>(a, stream);
+      return attention::launch<decltype(t), decltype(W)::value>(a, attention::few_columns(*x), stream);
     });
   });
   // (delta is the first launch's)
