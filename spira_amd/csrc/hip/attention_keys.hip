@@ -5,6 +5,10 @@
 // (attention_backward.hip has the formulas of ds).  A block owns 128 keys, a wave 32 of
 // them as its columns, and walks its group's query heads and their queries in tiles;
 // p and ds go from the scores' registers to the products as they are.
+//
+// 16384 uneven packed tokens, 16 heads of 64 on 4, causal, bf16: 303 us (four products a
+// pair, 700 TFLOP/s) and 15 to join two parts.  A block's steps in one part 797; three parts,
+// each in a launch order of its own behind the one before, 382.
 #include "attention.hpp"
 
 #include <algorithm>

@@ -15,7 +15,9 @@
 //
 // A block takes a few rows at a time, G lanes a head's vector of a row, eight pairs
 // each.  Everything in fp32, outputs rounded once; sums over rows (the gradients of
-// w) go over the blocks in a fixed order.  Bound by memory.
+// w) go over the blocks in a fixed order.  Bound by memory: 200k rows of 6 heads of 32,
+// fp16, 52 us where their bytes take 29 (rows lie 576 bytes apart, 384 of them read); 16384
+// rows of 20 heads of 64, bf16, 26 us and 37 for the gradients.
 #include "numeric.hpp"
 
 #include <algorithm>
