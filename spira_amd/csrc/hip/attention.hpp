@@ -25,7 +25,6 @@ using namespace tiles;
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
-constexpr float kLog2e = 1.44269504f;
 constexpr int kMostHeadDim = 128;
 
 // ---------------------------------------------------------------------------

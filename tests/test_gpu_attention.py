@@ -154,7 +154,8 @@ CROSS = [
     ([1, 1], [40, 700], None, 8, 2, 64), ([1] * 5, [300, 64, 128, 1024, 70], [299, 0, 128, 1000, 1], 4, 1, 128),
     ([3, 2, 0, 9], [20, 1, 5, 9], [20, 1, 5, 4], 4, 2, 32),          # (more queries than keys: some see none)
     ([40, 100], [2, 1300], None, 2, 2, 36), ([1], [5000], [4993], 16, 2, 96), ([2] * 40, [100] * 40, [97] * 40, 2, 1, 64),
-    ([1, 1, 1], [3000, 0, 50], [2990, 0, 50], 3, 3, 63), ([150], [400], None, 4, 2, 64), ([7], [0], None, 2, 1, 32)]
+    ([1, 1, 1], [3000, 0, 50], [2990, 0, 50], 3, 3, 63), ([150], [400], None, 4, 2, 64), ([7], [0], None, 2, 1, 32),
+    ([70], [9000], [8999], 8, 1, 64), ([40, 33], [4100, 5000], None, 4, 2, 24)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
