@@ -449,10 +449,13 @@ struct Plan {
 static Plan plan(const spira_hip_attention_t &x, bool stats) {
   const int64_t group = x.heads / x.kv_heads, columns = div_up(x.rows * group, x.sequences);
   const Plan prompts{false, 0, 0}, direct{true, 1, 1};
-  // Parts where a sequence has few columns, or where there are few in all against long
-  // caches (100 queries of 8 heads on 2 against 100k keys: 121 us, by whole columns 844).
+  // Parts where a sequence has few columns, or where whole columns' blocks leave CUs idle
+  // and walk long caches: 100 queries of 8 heads on 2 against 100k keys 844 us by whole
+  // columns, 121 in parts, 2048 keys 25.5 and 15.0; where there are blocks enough the parts'
+  // sums cost more (2 sequences of 1024, themselves: 19.2 and 71.9).
   // (A gradient's statistics come from one block per column.)
-  const bool few = few_columns(x), parted = columns <= 64 || (few && x.keys / x.sequences >= 4096);
+  const bool few = few_columns(x), idle = (x.rows * group / 32 + x.sequences) * x.kv_heads < 256;
+  const bool parted = columns <= 64 || (idle && x.keys / x.sequences >= 1024);
   if (stats || !parted) return few ? direct : prompts;
   const int64_t tiles = div_up(columns, 32);
   const int64_t size = round_up(std::max<int64_t>(div_up(x.keys * x.kv_heads * tiles, 2048), 256), 64);
