@@ -155,7 +155,7 @@ CROSS = [
     ([3, 2, 0, 9], [20, 1, 5, 9], [20, 1, 5, 4], 4, 2, 32),          # (more queries than keys: some see none)
     ([40, 100], [2, 1300], None, 2, 2, 36), ([1], [5000], [4993], 16, 2, 96), ([2] * 40, [100] * 40, [97] * 40, 2, 1, 64),
     ([1, 1, 1], [3000, 0, 50], [2990, 0, 50], 3, 3, 63), ([150], [400], None, 4, 2, 64), ([7], [0], None, 2, 1, 32),
-    ([70], [9000], [8999], 8, 1, 64), ([40, 33], [4100, 5000], None, 4, 2, 24)]
+    ([1] * 70, [100] * 70, [99] * 70, 2, 1, 40), ([70], [9000], [8999], 8, 1, 64), ([40, 33], [4100, 5000], None, 4, 2, 24)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -275,6 +275,41 @@ def test_offsets_that_are_no_rows(dev):
         with torch.no_grad():
             F.attention(q, k, k, offsets, key_offsets=keys, key_counts=counts)
     torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits(dev):
+    """Sequences at the end of a cache of more than 2^32 bytes, and rows 32 MB apart: what the same rows
+    give close together."""
+    d, lengths = 64, [300, 200]
+    n = sum(lengths)
+    q, k, v = (randn((n, h, d), torch.float16, i).to(dev) for i, h in ((1, 2), (2, 1), (3, 1)))
+    at, dout = offsets_of(lengths), randn((n, 2, d), torch.float16, 4).to(dev)
+    far = 34_000_000
+    big = [torch.empty(far, 1, d, dtype=torch.float16, device=dev) for _ in range(2)]
+    wide = [torch.empty(n, 1 << 24, dtype=torch.float16, device=dev)[:, None, :d] for _ in range(2)]
+    for t, x in zip((*big, *wide), (k, v, k, v)):
+        t[-n:] = x
+    offsets = at.to(dev)
+    for causal in (False, True):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        ref = F.attention(*leaves, offsets, causal=causal)
+        grads = torch.autograd.grad(ref, leaves, dout)
+        for keys, first in ((big, far - n), (wide, 0)):
+            moved = [q.detach().requires_grad_(True), *(t.detach().requires_grad_(True) for t in keys)]
+            kw = dict(key_offsets=(at + first).to(dev), causal=causal)
+            y = F.attention(*moved, offsets, **kw)
+            got = torch.autograd.grad(y, moved, dout)
+            assert torch.equal(y, ref) and torch.equal(got[0], grads[0])
+            for a, b in zip(got[1:], grads[1:]):
+                # (in how many parts a tile's steps are summed goes by the number of keys: 16 bits apart by a step)
+                assert torch.allclose(a[-n:].float(), b.float(), rtol=2.0 ** -10, atol=1e-4)
+                assert torch.count_nonzero(a[:-n]) == 0
+            del y, got, moved
+            last = torch.tensor([n - 1, n], dtype=torch.int32, device=dev)  # one token, in parts
+            ends = torch.tensor([first + 300, first + n], dtype=torch.int32, device=dev)
+            with torch.no_grad():
+                one = F.attention(q[-1:], *keys, last - (n - 1), key_offsets=ends, causal=causal)
+            assert torch.allclose(one.float(), ref[-1:].float(), rtol=2.0 ** -9, atol=2e-3)
 
 
 def test_gradients_by_differences(dev):

@@ -131,6 +131,24 @@ def test_norm_rotate_heads(dev, n, heads, kv, d, axes, far, interleaved, weighte
             close(got[2 + i], *dw, f"dw {i}")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_heads_strides(dev, dtype):
+    """Views at any stride give what their copies give, forward and in the gradients."""
+    dt, n, d = DTYPES[dtype], 77, 48
+    x = randn((n, 6, d), dt, 1).to(dev)
+    flat = torch.cat([torch.zeros(3, dtype=dt, device=dev), x.reshape(-1)])[3:].view(x.shape)
+    w = randn((d,), dt, 2).to(dev)
+    pos = torch.arange(n, dtype=torch.int32, device=dev)
+    g = [randn((n, h, d), dt, 5 + h).to(dev) for h in (4, 2)]
+    for v in (x, flat, x.transpose(0, 1).contiguous().transpose(0, 1), x.transpose(1, 2).contiguous().transpose(1, 2)):
+        out = []
+        for q, k in ((v[:, :4], v[:, 4:]), (v[:, :4].contiguous(), v[:, 4:].contiguous())):
+            leaves = [q.detach().requires_grad_(True), k.detach().requires_grad_(True)]
+            y = F.norm_rotate_heads(*leaves, query_weight=w, key_weight=w, positions=pos)
+            out.append((*y, *torch.autograd.grad(y, leaves, [t.transpose(0, 1).contiguous().transpose(0, 1) for t in g])))
+        assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
 def test_one_output_without_a_gradient(dev):
     q, k = (randn((20, h, 32), torch.float32, h).to(dev).requires_grad_(True) for h in (2, 1))
     wq, wk = (torch.ones(32, device=dev, requires_grad=True) for _ in range(2))
