@@ -647,7 +647,7 @@ int spira_hip_dropout(const void *x, const void *residual, int64_t n, int dtype,
 /* Attention over packed sequences with grouped heads.  Sequence b has the queries
  * offsets[b] to offsets[b + 1] and the first key_counts[b] (null: all) of the keys
  * key_offsets[b] to key_offsets[b + 1], int32 on the device, ascending; what lies
- * behind a sequence's keys is not read.  Query head h reads key head h kv_heads /
+ * behind a sequence's keys is not read.  1 to 65536 sequences.  Query head h reads key head h kv_heads /
  * heads.  causal: query i of n sees key j of m if j <= i + m - n.  head_dim: 1 to
  * 128 values, consecutive; rows and heads at any stride (in values).  A query
  * without visible keys, or in no sequence, gets zeros. */

@@ -329,15 +329,22 @@ template <class T> __global__ __launch_bounds__(256) void join_kernel(const Args
   __shared__ float sums[kJoinParts][kMostHeadDim], stats[2];
   const int lane = lane_id(), slot = threadIdx.x / 32, d = (threadIdx.x & 31) * 4;
   const int64_t at = blockIdx.x, all = a.s.rows * a.heads, row = at / a.heads;
-  int parts = 0;
-  for (int first = 0; first < a.s.count; first += 64) {
-    const int b = first + lane;
+  // the row's sequence: of at most 64 by looking at all at once, of more the last that
+  // begins at or before the row
+  int parts = 0, lo = 0;
+  if (a.s.count > 64)
+    for (int hi = a.s.count; hi - lo > 1;) {
+      const int mid = (lo + hi) / 2;
+      if (a.s.offsets[mid] <= row) lo = mid;
+      else hi = mid;
+    }
+  {
+    const int b = a.s.count > 64 ? lo : lane;
     const Sequence s = sequence_at(a.s, b < a.s.count ? b : a.s.count - 1);
     const uint64_t found = ballot(b < a.s.count && row >= s.q0 && row < s.q0 + s.nq);
     if (found) {
       const int n = __shfl(s.nk, __builtin_ctzll(found), 64);
       parts = n > 0 ? (n - 1) / a.part_keys + 1 : 0;
-      break;
     }
   }
   parts = uniform(parts);
@@ -409,7 +416,7 @@ template <class T> __global__ __launch_bounds__(256) void join_kernel(const Args
 static int check(const spira_hip_attention_t &x) {
   constexpr int64_t most = (int64_t(1) << 31) - 256;  // (whole tiles are counted in 32 bits)
   SPIRA_HIP_REQUIRE(x.rows >= 0 && x.rows <= most && x.keys >= 0 && x.keys <= most, "attention: bad number of rows");
-  SPIRA_HIP_REQUIRE(x.sequences > 0 && x.sequences <= (1 << 24), "attention: needs 1 to 2^24 sequences");
+  SPIRA_HIP_REQUIRE(x.sequences > 0 && x.sequences <= 65536, "attention: needs 1 to 65536 sequences");
   SPIRA_HIP_REQUIRE(x.heads > 0 && x.kv_heads > 0 && x.heads <= 65536 && x.heads % x.kv_heads == 0,
                     "attention: the number of query heads must be a multiple of the key heads'");
   SPIRA_HIP_REQUIRE(x.head_dim > 0 && x.head_dim <= kMostHeadDim, "attention: needs heads of 1 to 128 values");

@@ -73,14 +73,23 @@ __device__ __forceinline__ Found found_at(const Sequence &held, int lane, int nt
   return f;
 }
 // Piece `index` of the sequences cut into pieces(sequence) each, the same on every lane.
+// A lane holds four sequences at a time, so that few waits for memory come before a block
+// of the last ones (3000 windows: 12).
 template <class Pieces> __device__ __forceinline__ Found find_piece(const Sequences &s, int64_t index, Pieces &&pieces) {
+  constexpr int HELD = 4;
   const int lane = lane_id();
   int64_t before = 0;
-  for (int first = 0; first < s.count; first += 64) {
-    const int b = first + lane;
-    const Sequence held = sequence_at(s, b < s.count ? b : s.count - 1);
-    const int n = b < s.count ? pieces(held) : 0;
-    int upto = n;
+  for (int first = 0; first < s.count; first += 64 * HELD) {
+    Sequence held[HELD];
+    int n[HELD], upto = 0;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      const int b = first + lane * HELD + k;
+      held[k] = sequence_at(s, b < s.count ? b : s.count - 1);
+      n[k] = b < s.count ? pieces(held[k]) : 0;
+      upto += n[k];
+    }
+    const int own = upto;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
       const int u = __shfl_up(upto, o, 64);
@@ -88,8 +97,21 @@ template <class Pieces> __device__ __forceinline__ Found find_piece(const Sequen
     }
     const uint64_t past = ballot(before + upto > index);
     if (past) {
-      const int at = __builtin_ctzll(past), of = __shfl(n, at, 64);
-      return found_at(held, at, static_cast<int>(index - before - (__shfl(upto, at, 64) - of)), of);
+      // (what each lane takes for its own, of which the found one's is right)
+      int64_t nth = index - before - (upto - own);
+      Sequence mine = held[0];
+      int of = n[0];
+      bool open = nth >= n[0];
+#pragma unroll
+      for (int k = 1; k < HELD; ++k)
+        if (open) {
+          nth -= n[k - 1];
+          mine = held[k];
+          of = n[k];
+          open = nth >= n[k];
+        }
+      const int at = __builtin_ctzll(past);
+      return found_at(mine, at, __shfl(static_cast<int>(nth), at, 64), __shfl(of, at, 64));
     }
     before += __shfl(upto, 63, 64);
   }

@@ -42,7 +42,7 @@ static spira_hip_attention_t attention_arguments(const Tensor &q, const Tensor &
   spira_hip_attention_t x{};
   x.rows = q.size(0);
   x.keys = k.size(0);
-  SPIRA_CHECK_ARG(offsets.size(0) - 1 <= (1 << 24), "attention: needs 1 to 2^24 sequences, got ", offsets.size(0) - 1);
+  SPIRA_CHECK_ARG(offsets.size(0) - 1 <= 65536, "attention: needs 1 to 65536 sequences, got ", offsets.size(0) - 1);
   SPIRA_CHECK_ARG(q.size(1) <= 65536, "attention: needs 1 to 65536 heads, got ", q.size(1));
   x.sequences = static_cast<int>(offsets.size(0) - 1);
   x.heads = static_cast<int>(q.size(1));

@@ -33,7 +33,7 @@ def attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, o
     gets no gradient.  ``causal``: query i of n sees key j of m if j <= i + m - n,
     the last query all of them.  ``scale`` (positive) is D ** -0.5 unless given.
 
-    Sequences may have any lengths, none included.  A query that sees no key, or
+    Up to 65536 sequences of any lengths, none included.  A query that sees no key, or
     is in no sequence, gets zeros.  Values that are not finite reach the queries
     that see them only.  In 16 bits the softmax's weights are rounded to the
     features' type before their product with the values, in fp32 nothing is.

@@ -44,7 +44,7 @@ def attention(**kw):
     return Attention(**x)
 
 
-BAD = [(dict(rows=-1), "rows"), (dict(rows=1 << 31), "rows"), (dict(keys=1 << 31), "rows"), (dict(sequences=0), "sequences"),
+BAD = [(dict(rows=-1), "rows"), (dict(rows=1 << 31), "rows"), (dict(keys=(1 << 31) - 255), "rows"), (dict(sequences=0), "sequences"), (dict(sequences=65537), "sequences"),
        (dict(heads=0), "multiple"), (dict(heads=5), "multiple"), (dict(kv_heads=0), "multiple"), (dict(head_dim=0), "128"),
        (dict(head_dim=129), "128"), (dict(rows=(1 << 31) - 1000, heads=4, kv_heads=1), "queries"), (dict(scale=0), "scale"),
        (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(offsets=None), "offsets"),
@@ -77,7 +77,7 @@ def test_attention_outputs_and_workspaces():
     refused(LIB.spira_hip_attention(ctypes.byref(x), P(SOME), None, None, P(SOME), SIZE(size.value - 1), None), "workspace")
     refused(LIB.spira_hip_attention(ctypes.byref(x), P(SOME), None, None, None, SIZE(1 << 40), None), "workspace")
     # whatever the sizes, they stay within some hundred MB
-    for rows, keys, heads, kv in ((1, (1 << 31) - 1, 64, 1), (4000, 1 << 30, 64, 64), (64, 1 << 20, 128, 2), (1, 0, 1, 1)):
+    for rows, keys, heads, kv in ((1, (1 << 31) - 256, 64, 1), (4000, 1 << 30, 64, 64), (64, 1 << 20, 128, 2), (1, 0, 1, 1)):
         x = attention(rows=rows, keys=keys, heads=heads, kv_heads=kv, sequences=max(1, rows // 2), head_dim=128)
         assert LIB.spira_hip_attention_workspace(ctypes.byref(x), 0, ctypes.byref(size)) == 0 and size.value < 1 << 29
     assert LIB.spira_hip_attention(ctypes.byref(attention(rows=0, queries=None)), None, None, None, None, SIZE(0), None) == 0

@@ -142,6 +142,20 @@ def test_sequences(dev, lengths, heads, kv, d, causal, dtype):
     check(dev, randn((n, heads, d), dt, 1), randn((n, kv, d), dt, 2), randn((n, kv, d), dt, 3), lengths, causal=causal)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_sequences(dev, causal):
+    """More than a wave looks at at once, of uneven lengths and none: themselves, and a token each
+    against caches in parts."""
+    lengths = [(i * 7) % 11 for i in range(700)]
+    n = sum(lengths)
+    check(dev, randn((n, 2, 16), torch.float16, 1), randn((n, 1, 16), torch.float16, 2), randn((n, 1, 16), torch.float16, 3),
+          lengths, causal=causal)
+    room = [(i * 37) % 300 for i in range(300)]
+    m = sum(room)
+    check(dev, randn((300, 2, 16), torch.float16, 1), randn((m, 1, 16), torch.float16, 2), randn((m, 1, 16), torch.float16, 3),
+          [1] * 300, k_lengths=room, causal=causal)
+
+
 @pytest.mark.parametrize("dtype,causal", [("f16", False), ("bf16", True)])
 def test_a_long_sequence(dev, dtype, causal):
     """Weights of some 1e-4 each, many tiles, and parts of the keys' steps."""
