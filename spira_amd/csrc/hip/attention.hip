@@ -120,8 +120,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   // (key heads fastest: where their number divides 8 or 8 it, an XCD's blocks share
   // few heads' keys)
   const int kv = blockIdx.x % a.kv_heads;
-  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads,
-                               [&](const Sequence &x) { return (x.nq * a.group + kColumns - 1) / kColumns; });
+  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads, Cut{false, a.group, kColumns});
   if (!s.there) return;
   const int total = s.nq * a.group, c0 = s.nth * kColumns, w0 = c0 + wave * 32;
   const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
@@ -212,13 +211,11 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP, DIRECT>::NW), 1) void token
   const int kv = blockIdx.x % a.kv_heads;
   // DIRECT: a piece is 32 columns (whose outputs are written without keys too); else a
   // part of the keys, for columns from blockIdx.y on
-  const Found s = DIRECT ? find_longest(a.s, blockIdx.x / a.kv_heads,
-                                        [&](const Sequence &x) { return (x.nq * a.group + 31) / 32; })
-                         : find_piece(a.s, blockIdx.x / a.kv_heads, [&](const Sequence &x) {
-                             return x.nq == 0 || x.nk == 0 ? 0 : (x.nk - 1) / a.part_keys + 1;
-                           });
+  const Found s = DIRECT ? find_longest(a.s, blockIdx.x / a.kv_heads, Cut{false, a.group, 32})
+                         : find_piece(a.s, blockIdx.x / a.kv_heads, Cut{true, 1, a.part_keys});
   if (!s.there) return;
   const int first = DIRECT ? 0 : s.nth * a.part_keys, total = s.nq * a.group;
+  if (!DIRECT && first >= s.nk) return;  // (room)
   const int64_t kstride = a.k_row * R::SIZE, vstride = a.v_row * R::SIZE;
   const char *keys = reinterpret_cast<const char *>(static_cast<const T *>(a.k) + (s.k0 + first) * a.k_row + kv * a.k_head);
   const char *values =
@@ -456,13 +453,16 @@ struct Plan {
 static Plan plan(const spira_hip_attention_t &x, bool stats) {
   const int64_t group = x.heads / x.kv_heads, columns = div_up(x.rows * group, x.sequences);
   const Plan prompts{false, 0, 0}, direct{true, 1, 1};
-  // Parts where a sequence has few columns, or where whole columns' blocks leave CUs idle
-  // and walk long caches: 100 queries of 8 heads on 2 against 100k keys 844 us by whole
-  // columns, 121 in parts, 2048 keys 25.5 and 15.0; where there are blocks enough the parts'
-  // sums cost more (2 sequences of 1024, themselves: 19.2 and 71.9).
-  // (A gradient's statistics come from one block per column.)
-  const bool few = few_columns(x), idle = (x.rows * group / 32 + x.sequences) * x.kv_heads < 256;
-  const bool parted = columns <= 64 || (idle && x.keys / x.sequences >= 1024);
+  // Parts of the keys: where a sequence has few columns against many keys (or few rows in all,
+  // whose join costs little however uneven the keys), and where whole columns' blocks leave
+  // CUs idle and walk long caches.  100 queries of 8 heads on 2 against 100k keys 844 us by
+  // whole columns, 121 in parts, 2048 keys 25.5 and 15.0; where there are blocks enough the
+  // parts' sums cost more (2 sequences of 1024, themselves: 19.2 and 71.9; 65k voxels of 3
+  // heads of 32 in windows of 64: 23 and 449, of 8: 127 and 601).  (A gradient's statistics
+  // come from one block per column.)
+  const bool few = few_columns(x), many_keys = x.keys / x.sequences >= 1024;
+  const bool idle = (x.rows * group / 32 + x.sequences) * x.kv_heads < 256;
+  const bool parted = columns <= 64 ? many_keys || x.rows * x.heads <= 8192 : many_keys && idle;
   if (stats || !parted) return few ? direct : prompts;
   const int64_t tiles = div_up(columns, 32);
   const int64_t size = round_up(std::max<int64_t>(div_up(x.keys * x.kv_heads * tiles, 2048), 256), 64);
@@ -471,7 +471,7 @@ static Plan plan(const spira_hip_attention_t &x, bool stats) {
   while (x.rows * x.heads * div_up(x.keys, part) * (x.head_dim + 2) * 4 > (int64_t(1) << 28) && part < x.keys)
     part *= 2;
   // (no sequence has keys for more than four parts: a join would cost more)
-  if (x.keys <= 4 * part) return direct;
+  if (x.keys <= 4 * part) return few ? direct : prompts;
   return {true, static_cast<int>(part), div_up(x.keys, part)};
 }
 

@@ -104,8 +104,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
   if (dq)
     clear_uncovered(a.s.offsets, a.s.count, a.s.rows, dq, static_cast<int64_t>(a.heads) * a.d, blockIdx.x, gridDim.x);
   const int kv = blockIdx.x % a.kv_heads;
-  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads,
-                               [&](const Sequence &x) { return (x.nq * a.group + kColumns - 1) / kColumns; });
+  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads, Cut{false, a.group, kColumns});
   if (!s.there) return;
   const int total = s.nq * a.group, c0 = s.nth * kColumns, w0 = c0 + wave * 32;
   const int column = w0 + (lane & 31), j = column < total ? column : total - 1;
@@ -178,8 +177,7 @@ __global__ __launch_bounds__(64 * 2, 1) void few_queries_kernel(const Args a) {
   if (dq)
     clear_uncovered(a.s.offsets, a.s.count, a.s.rows, dq, static_cast<int64_t>(a.heads) * a.d, blockIdx.x, gridDim.x);
   const int kv = blockIdx.x % a.kv_heads;
-  const Found s =
-      find_longest(a.s, blockIdx.x / a.kv_heads, [&](const Sequence &x) { return (x.nq * a.group + 31) / 32; });
+  const Found s = find_longest(a.s, blockIdx.x / a.kv_heads, Cut{false, a.group, 32});
   if (!s.there) return;
   const int total = s.nq * a.group, w0 = s.nth * 32, column = w0 + (lane & 31), j = column < total ? column : total - 1;
   const int i = j / a.group, head = kv * a.group + (j - i * a.group), limit = visible(a, s, i);

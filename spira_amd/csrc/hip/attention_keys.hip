@@ -40,9 +40,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
   const int splits = SPLIT ? parts : 1;
   const int64_t piece = blockIdx.x / a.kv_heads;
   const int part = SPLIT ? static_cast<int>(piece % splits) : 0;
-  const Found s = find_longest(a.s, piece / splits, [&](const Sequence &x) {
-    return static_cast<int>((x.room + int64_t(kOwnKeys) - 1) / kOwnKeys);
-  });
+  const Found s = find_longest(a.s, piece / splits, Cut{true, 1, kOwnKeys});
   if (!s.there) return;
   const int c0 = (s.of - 1 - s.nth) * kOwnKeys, w0 = c0 + wave * 32, key = w0 + (lane & 31);
   const bool there = key < s.nk;

@@ -156,6 +156,19 @@ def test_many_sequences(dev, causal):
           [1] * 300, k_lengths=room, causal=causal)
 
 
+def test_thousands_of_sequences(dev):
+    """More than 64 times 64 of them, each found in three steps, some with nothing; in windows, and a
+    token each against caches of few keys and of more room."""
+    lengths = [(i * 5) % 8 if i % 9 else 0 for i in range(4500)]
+    n = sum(lengths)
+    check(dev, randn((n, 1, 8), torch.float16, 1), randn((n, 1, 8), torch.float16, 2), randn((n, 1, 8), torch.float16, 3),
+          lengths, causal=True)
+    room = [(i * 37) % 20 for i in range(4500)]
+    m = sum(room)
+    check(dev, randn((4500, 1, 8), torch.float16, 1), randn((m, 1, 8), torch.float16, 2), randn((m, 1, 8), torch.float16, 3),
+          [1] * 4500, k_lengths=room, counts=[r // 2 for r in room], causal=False)
+
+
 @pytest.mark.parametrize("dtype,causal", [("f16", False), ("bf16", True)])
 def test_a_long_sequence(dev, dtype, causal):
     """Weights of some 1e-4 each, many tiles, and parts of the keys' steps."""
