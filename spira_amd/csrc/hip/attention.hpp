@@ -373,9 +373,12 @@ __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 
 // found any.
 template <class T, int DP, int R, int NT> __device__ __forceinline__ bool clear_not_finite(lds_char *tile, int thread) {
   constexpr uint32_t E = sizeof(T) == 4 ? 0x7F800000u : std::is_same_v<T, _Float16> ? 0x7C00u : 0x7F80u;
+  // (heads of up to 32 values in 16 bits: 32 rows have fewer chunks than a block has threads)
+  constexpr int CHUNKS = R * Rows<T, DP>::CPR;
   bool found = false;
 #pragma unroll
-  for (int i = 0; i < R * Rows<T, DP>::CPR / NT; ++i) {
+  for (int i = 0; i < (CHUNKS + NT - 1) / NT; ++i) {
+    if (CHUNKS % NT != 0 && i * NT + thread >= CHUNKS) break;
     lds_chunk *at = (lds_chunk *)(tile + (i * NT + thread) * 16);
     uintx4_t v = *at;
     bool here = false;
