@@ -461,10 +461,11 @@ __device__ __forceinline__ void store_column(T *row, int d, bool there, const fl
     }
 }
 
-// whether tiles (of at most 64 rows) can be fetched by DMA
+// whether tiles (of at most 64 rows) can be fetched by DMA: their rows' zeros behind the last
+// one come from the buffer's end, so no row may begin before the end of the one before it
 inline bool dma_rows(const void *p, int64_t row, int64_t head, int d, int size) {
   const auto whole = [&](int64_t values) { return values * size % 16 == 0; };
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && whole(row) && whole(head) && whole(d) &&
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row >= d && whole(row) && whole(head) && whole(d) &&
          row * size * 64 < kBufferLimit / 2;
 }
 

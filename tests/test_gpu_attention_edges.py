@@ -1,12 +1,14 @@
 """Attention where its kernels' shortcuts end: values that are not finite behind the mask,
-for narrow heads among others.  Units are those of test_gpu_attention.py."""
+for narrow heads among others, rows
+that overlap.  Units and the
+reference are those of test_gpu_attention.py."""
 import math
 
 import pytest
 import torch
 
 from spira_amd.nn import functional as F
-from test_gpu_attention import DTYPES, randn
+from test_gpu_attention import DTYPES, check, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +51,37 @@ def test_not_finite_where_hidden(dev, many, d, what, dtype):
         last = at + 8
         assert torch.equal(got[2][last:], ref[2][last:]) and torch.equal(got[3][last:], ref[3][last:])
         assert not torch.isfinite(got[3][:at]).all(2).any()
+
+
+# ---------------------------------------------------------------------------
+# rows that overlap
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths", [[1] * 5, [70], [3, 0, 129, 33]])
+def test_a_query_expanded_over_rows(dev, lengths, causal, dtype):
+    """One query for all rows (a row stride of 0), with scores far above those that exp2 takes in 16 bits."""
+    n, room = sum(lengths), [m * 3 + 60 for m in lengths]
+    m = sum(room)
+    q = (randn((1, 4, 64), DTYPES[dtype], 1) * 3).to(dev).expand(n, -1, -1)
+    assert q.stride(0) == 0
+    k, v = randn((m, 2, 64), DTYPES[dtype], 2) * 3, randn((m, 2, 64), DTYPES[dtype], 3)
+    check(dev, q, k, v, lengths, k_lengths=room, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("step", [0, 8, 32])
+def test_rows_closer_than_their_width(dev, step, dtype):
+    """Queries, keys and values whose rows lie `step` values apart, less than a head has; infinities in the
+    room behind a cache's keys."""
+    dt, n, d = DTYPES[dtype], 150, 64
+
+    def rows(seed, size):
+        flat = (randn(((n - 1) * step + d,), dt, seed) * size).to(dev)
+        return flat.as_strided((n, 1, d), (step, d, 1))
+    q, k, v = rows(1, 3.0), rows(2, 3.0), rows(3, 1.0)
+    check(dev, q, k, v, [60, 90], causal=True)
+    used = n - 20
+    if step:
+        v.as_strided(((n - 1) * step + d,), (1,))[(used - 1) * step + d:] = math.inf
+    check(dev, q[:4], k, v, [4], k_lengths=[n], counts=[used], causal=False)
