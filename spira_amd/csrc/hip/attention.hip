@@ -19,8 +19,8 @@
 // memory: 32 caches of 4096 keys on average, 8 heads of 128: 120 us, 4.5 TB/s.
 //
 // The softmax is taken in one pass with a running maximum and sum in fp32.  The
-// maximum moves only when a score passes it by 2^8 (in exp2): the sums are exact
-// under any reference, and columns are seldom scaled anew.
+// maximum moves only when a score passes it by 2^8 (in exp2; fp16 2^4): the sums are
+// exact under any reference, and columns are seldom scaled anew.
 #include "attention.hpp"
 
 #include <algorithm>
@@ -29,7 +29,10 @@ namespace spira_hip {
 
 namespace attention {
 
-constexpr float kSlack = 8.f;
+// fp16: weights are lifted by 2^11 over that reference (2^15 at most, the type ends at 2^16): the
+// many of some e^-17 beside one that takes nearly all would be a step or none of the type's 2^-24.
+template <class T> constexpr float kRaise = std::is_same_v<T, _Float16> ? 11.f : 0.f;
+template <class T> constexpr float kSlack = std::is_same_v<T, _Float16> ? 4.f : 8.f;
 
 // a wave's 32 columns on their way: output, reference maximum of the raw scores
 // (-inf: nothing seen) and this half's share of the sum
@@ -64,7 +67,7 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
     for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[u][r]);
   top = __builtin_fmaxf(top, other_half(top));
   // (each column by its own scores: a result does not depend on the wave's others)
-  const bool moves = (top - c.m) * scale2 > kSlack;
+  const bool moves = (top - c.m) * scale2 > kSlack<T>;
   if (ballot(moves)) {
     const float m = moves ? top : c.m, by = moves ? __builtin_amdgcn_exp2f((c.m - m) * scale2) : 1.f;
     c.l *= by;
@@ -74,7 +77,8 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
       for (int r = 0; r < 16; ++r) c.o[n][r] *= by;
     c.m = m;
   }
-  const float base = c.m == -__builtin_inff() ? 0.f : -c.m * scale2;
+  float base = c.m == -__builtin_inff() ? 0.f : -c.m * scale2;
+  if constexpr (kRaise<T> > 0) base += kRaise<T>;
 #pragma unroll
   for (int u = 0; u < KT / 32; ++u) {
     float sum = 0;
@@ -99,7 +103,7 @@ __device__ __forceinline__ void put_statistics(const Args &a, int head, int64_t 
   float *to = a.stats + head * a.s.rows + row;
   const float base = m == -__builtin_inff() ? 0.f : m * a.scale2;
   if constexpr (sizeof(T) == 2) {
-    *to = l == 0.f ? __builtin_inff() : base + __builtin_amdgcn_logf(l) - kLift<T>;
+    *to = l == 0.f ? __builtin_inff() : base + __builtin_amdgcn_logf(l) - (kRaise<T> + kLift<T>);
   } else {
     to[0] = base;
     to[a.heads * a.s.rows] = l == 0.f ? 0.f : 1.f / l;

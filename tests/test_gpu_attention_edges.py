@@ -1,14 +1,13 @@
-"""Attention where its kernels' shortcuts end: values that are not finite behind the mask,
-for narrow heads among others, rows
-that overlap.  Units and the
-reference are those of test_gpu_attention.py."""
+"""Attention where its kernels' shortcuts end: values that are not finite behind the mask
+(in narrow heads among others), rows that overlap, small weights.  Units and
+the reference are those of test_gpu_attention.py."""
 import math
 
 import pytest
 import torch
 
 from spira_amd.nn import functional as F
-from test_gpu_attention import DTYPES, check, randn
+from test_gpu_attention import DTYPES, E, check, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +84,27 @@ def test_rows_closer_than_their_width(dev, step, dtype):
     if step:
         v.as_strided(((n - 1) * step + d,), (1,))[(used - 1) * step + d:] = math.inf
     check(dev, q[:4], k, v, [4], k_lengths=[n], counts=[used], causal=False)
+
+
+# ---------------------------------------------------------------------------
+# small weights in fp16
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("queries,kv,train", [(3, 1, False), (3, 1, True), (200, 96, False)])
+def test_many_small_weights(dev, queries, kv, train):
+    """fp16, few keys that take nearly all with values of 0, and 8000 others with e^-17 each, whose part is the
+    output: by a token's waves and by blocks of 128 columns.  In the product a weight is off by 2^-11 of itself or, lifted
+    by 2^11, by 2^-25 under that; sums and scores as in the reference's docstring."""
+    n, gap, d, large = 8000, 17.0, 16, [0, 32, 64, 96]
+    q = torch.zeros(queries, kv, d, dtype=torch.float16)
+    q[..., 0] = 1.0
+    k, v = torch.zeros(n, kv, d, dtype=torch.float16), 1 + randn((n, kv, d), torch.float16, 5).abs() / 4
+    k[large, :, 0], v[large] = gap, 0.0
+    y = F.attention(q.to(dev).requires_grad_(train), k.to(dev), v.to(dev),
+                    torch.tensor([0, queries], dtype=torch.int32, device=dev),
+                    key_offsets=torch.tensor([0, n], dtype=torch.int32, device=dev), scale=1.0).detach().cpu().double()
+    each = math.exp(-gap) / (len(large) + (n - len(large)) * math.exp(-gap))
+    small = v.double().sum(0)
+    ref = each * small
+    w = 2 * 4 * E * gap + 2 * (n + 16) * E
+    tol = 2.0 ** -11 * ref + ((w + 2.0 ** -11) * each + 2.0 ** -36) * small
+    assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / ref).max()
