@@ -29,6 +29,7 @@ template <class T, int DP> struct QueryColumn {
   Frag<T> q[DP / 16], g[DP / 16];
   float delta;
   Stat<T> stat;
+  Lift<T> lift;  // of ds, and so of dq
   floatx16 acc[DP / 32];
 
   // query i of sequence s, of this head; `there`: delta is to be written
@@ -78,7 +79,8 @@ template <class T, int DP> struct QueryColumn {
   }
   // FINE (16 bits): with what the rounding of ds leaves.  Tiles on the mask's edge take it:
   // the rows that see few keys have their weights there, whose roundings do not average out.
-  template <bool FINE> __device__ __forceinline__ void accumulate(const Reader<T, DP> &read, lds_char *kt, const floatx16 &ds) {
+  template <bool FINE> __device__ __forceinline__ void accumulate(const Reader<T, DP> &read, lds_char *kt, floatx16 &ds) {
+    lift.fit(ds, acc);
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const Frag<T> f = as_operand<T>(ds, st);
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void queries_kernel(co
                               [&](int x) { return x < seen; });
     }
   }
-  if (dq) store_column<T, DP>(dq + ((s.q0 + i) * a.heads + head) * a.d, a.d, there, c.acc, a.scale);
+  if (dq) store_column<T, DP>(dq + ((s.q0 + i) * a.heads + head) * a.d, a.d, there, c.acc, a.scale * c.lift.lower());
 }
 
 // Few columns: a block's waves share 32 of them and take the keys' tiles in turn, each
@@ -220,6 +222,13 @@ __global__ __launch_bounds__(64 * 2, 1) void few_queries_kernel(const Args a) {
   wait_loads();
   asm volatile("" ::: "memory");
   if (!dq) return;
+  // (the waves' lifts are their own)
+  if constexpr (std::is_same_v<T, _Float16>) {
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) c.acc[n][r] *= c.lift.lower();
+  }
   put_sums<DP>(reinterpret_cast<float *>(lds[wave]), c.acc);
   __syncthreads();
   const int columns = std::min(32, total - w0);

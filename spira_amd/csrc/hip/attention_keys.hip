@@ -110,6 +110,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
     }
   }
   floatx16 ak[DP / 32] = {}, av[DP / 32] = {};
+  Lift<T> lift;  // of ds, and so of ak
   const Reader<T, DP> read;
   // p and ds of 32 queries from row `row` of the tile on; MASKED: this lane's key is seen from the `mine`th on
   const auto weights = [&](auto MASKED, int stage, int row, int mine, floatx16 &p, floatx16 &ds) {
@@ -171,6 +172,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       const bool x = clear_not_finite<T, DP, 32, 256>(qu, threadIdx.x), y = clear_not_finite<T, DP, 32, 256>(gu, threadIdx.x);
       const bool found = __syncthreads_or(x || y);
       accumulate(std::true_type{}, av, gu, p);
+      lift.fit(ds, ak);
       accumulate(std::true_type{}, ak, qu, ds);
       if (found) {
         const int64_t r0 = s.q0 + q0 + 32 * u;
@@ -195,6 +197,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       floatx16 p, ds;
       weights(std::false_type{}, stage, 32 * u, 0, p, ds);
       accumulate(std::false_type{}, av, gt + 32 * u * R::PITCH, p);
+      lift.fit(ds, ak);
       accumulate(std::false_type{}, ak, qt + 32 * u * R::PITCH, ds);
     }
   });
@@ -203,14 +206,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) ak[n] = av[n] = floatx16{};
   }
+  const float scale = a.scale * lift.lower();
   const int64_t to = ((s.k0 + key) * a.kv_heads + kv) * a.d;
   if constexpr (SPLIT) {
     float *sums = a.partial + part * 2 * a.s.keys * width + to;
-    store_column<float, DP>(sums, a.d, there, ak, a.scale);
+    store_column<float, DP>(sums, a.d, there, ak, scale);
     store_column<float, DP>(sums + a.s.keys * width, a.d, there, av, kLower<T>);
     return;
   }
-  if (dk) store_column<T, DP>(dk + to, a.d, key < s.room, ak, a.scale);
+  if (dk) store_column<T, DP>(dk + to, a.d, key < s.room, ak, scale);
   if (dv) store_column<T, DP>(dv + to, a.d, key < s.room, av, kLower<T>);
 }
 

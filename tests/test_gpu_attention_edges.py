@@ -1,5 +1,5 @@
 """Attention where its kernels' shortcuts end: values that are not finite behind the mask
-(in narrow heads among others), rows that overlap, small weights.  Units and
+(in narrow heads among others), rows that overlap, small weights and gradients in fp16.  Units and
 the reference are those of test_gpu_attention.py."""
 import math
 
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from spira_amd.nn import functional as F
-from test_gpu_attention import DTYPES, E, check, randn
+from test_gpu_attention import DTYPES, E, UNIT, check, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,49 @@ def test_many_small_weights(dev, queries, kv, train):
     w = 2 * 4 * E * gap + 2 * (n + 16) * E
     tol = 2.0 ** -11 * ref + ((w + 2.0 ** -11) * each + 2.0 ** -36) * small
     assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / ref).max()
+
+
+# ---------------------------------------------------------------------------
+# small gradients in fp16
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -7, 2.0 ** -13])
+@pytest.mark.parametrize("kv,causal", [(1, False), (1, True), (24, True)])
+def test_small_gradients(dev, kv, causal, size):
+    """fp16, even weights of 4000 keys, and gradients of the outputs down to what fp16 holds few bits of: ds is
+    some sqrt(n) below dq and dk.  Each ds is off by half a step, 2^-11 of itself (but 2^-34 of the largest of its
+    column, in what the kernels lift by it), dp and delta by their sums' 2 (d + 16) e, and the outputs round once."""
+    n, d = 4000, 64
+    u = UNIT[torch.float16]
+    v, dout = randn((n, kv, d), torch.float16, 3), (randn((n, kv, d), torch.float32, 4) * size).half()
+    small, large = randn((n, kv, d), torch.float32, 1) * 2.0 ** -6, randn((n, kv, d), torch.float32, 2) * 16
+    offsets = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    heads = slice(0, min(kv, 2))
+    for which in ("dq", "dk"):
+        q, k = (t.half() for t in ((small, large) if which == "dq" else (large, small)))
+        got = gradients([t.to(dev) for t in (q, k, v)], offsets, dout.to(dev), causal=causal)[1 if which == "dq" else 2]
+        for h in range(heads.start, heads.stop):
+            x, y, z, g = (t[:, h].to(dev).double() for t in (q, k, v, dout))
+            seen = torch.ones(n, n, dtype=torch.bool, device=dev)
+            seen = seen.tril() if causal else seen
+            s = torch.where(seen, d ** -0.5 * (x @ y.t()), -math.inf)
+            p = torch.softmax(s, 1)
+            dp = g @ z.t()
+            delta = (p * dp).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            es = d ** -0.5 * (d + 16) * E * (x.abs() @ y.abs().t()) + 4 * E * torch.where(seen, s, 0).abs()
+            w = 2 * es.amax(1, keepdim=True) + 2 * (n + 16) * E
+            # (delta by way of the outputs in two pieces, whose weights round by u each, at random: 6 of their deviation)
+            to = 6 * u * (p.square() @ z.square()).sqrt() + 2.0 ** -36 * (seen.double() @ z.abs())
+            edp = (d + 16) * E * (g.abs() @ z.abs().t() + (p * dp.abs()).sum(1, keepdim=True)) + (g.abs() * to).sum(1, keepdim=True)
+            eds = w * ds.abs() + p * edp
+            if which == "dq":
+                low = 2.0 ** -34 * ds.abs().amax(1, keepdim=True)
+                eds = torch.where(seen, eds + u * ds.abs() + low, 0)
+                ref, tol = d ** -0.5 * ds @ y, d ** -0.5 * eds @ y.abs()
+            else:
+                low = 2.0 ** -34 * ds.abs().amax(0, keepdim=True)
+                eds = torch.where(seen, eds + u * ds.abs() + low, 0)
+                ref, tol = d ** -0.5 * ds.t() @ x, d ** -0.5 * eds.t() @ x.abs()
+            tol = tol + u * ref.abs() + 2.0 ** -25 + 2 * n * E * tol
+            bad = (got[:, h].double() - ref).abs() > tol
+            assert not bad.any(), (which, h, int(bad.sum()), (got[:, h].double() - ref).abs().max().item(), tol.max().item())
