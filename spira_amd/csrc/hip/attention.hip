@@ -42,8 +42,9 @@ template <int DP> struct Columns {
 };
 
 // One tile of KT keys.  MASKED: this lane's column sees the first `limit` of them (any
-// number); else every column of the wave sees all.
-template <bool MASKED, class T, int DP, int KT>
+// number); else every column of the wave sees all.  FINE (16 bits): the weights with what
+// their rounding leaves.
+template <bool MASKED, bool FINE, class T, int DP, int KT>
 __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[DP / 16], const Reader<T, DP> &read,
                                             lds_char *kt, lds_char *vt, float scale2, int limit) {
   floatx16 s[KT / 32];
@@ -91,8 +92,14 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const Frag<T> p = as_operand<T>(s[u], st);
+      Frag<T> rest;
+      if constexpr (FINE && sizeof(T) == 2) rest = rest_operand<T>(s[u], st, p);
 #pragma unroll
-      for (int n = 0; n < DP / 32; ++n) mma(c.o[n], read.cols(vt, 32 * u + 16 * st, n), p);
+      for (int n = 0; n < DP / 32; ++n) {
+        const Frag<T> v = read.cols(vt, 32 * u + 16 * st, n);
+        mma(c.o[n], v, p);
+        if constexpr (FINE && sizeof(T) == 2) mma(c.o[n], v, rest);
+      }
     }
   }
 }
@@ -158,7 +165,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
     wait_loads_and_meet<0>();
     if (t + 1 < steps) issue(t + 1, stage ^ 1);
     lds_char *kt = (lds_char *)lds + stage * 2 * TILE;
-    attend_tile<false, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, 0);
+    attend_tile<false, false, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, 0);
   });
   // the others
   for (int t = whole; t < steps; ++t) {
@@ -169,7 +176,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
     const bool found = a.causal && __syncthreads_or(clear_not_finite<T, DP, KT, 256>(kt + TILE, threadIdx.x));
     if (t < own) {
       const int mine = limit - t * KT;
-      attend_tile<true, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, mine);
+      attend_tile<true, true, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, mine);
       if (found)
         add_not_finite<T, DP>(c.o, values + t * (KT * vstride), vstride, std::min(s.nk - t * KT, KT), a.d,
                               [&](int x) { return x < mine; });
@@ -259,12 +266,12 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP, DIRECT>::NW), 1) void token
       asm volatile("" ::: "memory");
       lds_char *kt = mine + stage * 2 * TILE;
       if (std::min(least, part) >= (t + 1) * KT) {
-        attend_tile<false, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, 0);
+        attend_tile<false, true, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, 0);
         continue;
       }
       const bool found = a.causal && ballot(clear_not_finite<T, DP, KT, 64>(kt + TILE, lane)) != 0;
       const int seen = std::min(limit, part) - t * KT;
-      attend_tile<true, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, seen);
+      attend_tile<true, true, T, DP, KT>(c, q, read, kt, kt + TILE, a.scale2, seen);
       if (found)
         add_not_finite<T, DP>(c.o, values + t * (KT * vstride), vstride, std::min(part - t * KT, KT), a.d,
                               [&](int x) { return x < seen; });

@@ -1,5 +1,6 @@
 """Attention where its kernels' shortcuts end: values that are not finite behind the mask
-(in narrow heads among others), rows that overlap, small weights and gradients in fp16.  Units and
+(in narrow heads among others), rows that overlap, small weights and gradients in fp16, common
+parts that cancel.  Units and
 the reference are those of test_gpu_attention.py."""
 import math
 
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 from spira_amd.nn import functional as F
-from test_gpu_attention import DTYPES, E, UNIT, check, randn
+from test_gpu_attention import DTYPES, E, UNIT, check, offsets_of, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -154,3 +155,44 @@ def test_small_gradients(dev, kv, causal, size):
             tol = tol + u * ref.abs() + 2.0 ** -25 + 2 * n * E * tol
             bad = (got[:, h].double() - ref).abs() > tol
             assert not bad.any(), (which, h, int(bad.sum()), (got[:, h].double() - ref).abs().max().item(), tol.max().item())
+
+
+# ---------------------------------------------------------------------------
+# common parts that cancel
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,part", [("f16", 32.0), ("bf16", 16.0)])
+@pytest.mark.parametrize("what", ["values", "keys", "queries"])
+def test_common_parts_cancel(dev, what, dtype, part):
+    """Few keys a row (all of them on the mask's edge), and values, keys or a pair of heads' queries that have
+    a common part of `part` times what tells them apart: it cancels in dq or dk, what the roundings of the outputs, of
+    the weights and of ds leave of it does not.  With those kept as second operands each is held to u^2 / 2, so a
+    gradient's norm is off by u (its own rounding) and by the cancelled part's 4 roundings of u^2 / 2 each, on sums of
+    12 terms at most, times `part`: below u / 4.  Rounded without, one of them alone is some part u / sqrt(12)."""
+    dt, lengths = DTYPES[dtype], [9, 12, 7, 11] * 6
+    u, n, d = UNIT[DTYPES[dtype]], sum([9, 12, 7, 11] * 6), 64
+    q, k, v, g = (randn((n, h, d), torch.float32, i) for i, h in ((1, 2), (2, 1), (3, 1), (4, 2)))
+    if what == "values":
+        v = 1 + v / part
+    elif what == "keys":
+        k = 1 + k / part
+    else:  # the second head's query is the first's and a little, its gradient the other way
+        q[:, 1], g[:, 1] = q[:, 0] + q[:, 1] / part, -g[:, 0]
+    q, k, v, g = (t.to(dt).to(dev) for t in (q, k, v, g))
+    offsets = offsets_of(lengths)
+    got = gradients((q, k, v), offsets.to(dev), g, causal=True)
+    refs = [torch.zeros_like(t, dtype=torch.float64) for t in (q, k, v)]
+    for a, b in zip(offsets.tolist(), offsets.tolist()[1:]):
+        seen = torch.ones(b - a, b - a, dtype=torch.bool, device=dev).tril()
+        for h in range(2):
+            x, y, z, w = (t.double() for t in (q[a:b, h], k[a:b, 0], v[a:b, 0], g[a:b, h]))
+            p = torch.softmax(torch.where(seen, d ** -0.5 * (x @ y.t()), -math.inf), 1)
+            dp = w @ z.t()
+            ds = p * (dp - (p * dp).sum(1, keepdim=True))
+            refs[0][a:b, h] = d ** -0.5 * ds @ y
+            refs[1][a:b, 0] += d ** -0.5 * ds.t() @ x
+            refs[2][a:b, 0] += p.t() @ w
+    for i, name in ((1, "dq"), (2, "dk"), (3, "dv")):
+        if (what, name) in (("queries", "dq"), ("values", "dv"), ("keys", "dv")):
+            continue  # (nothing cancels)
+        off = (got[i].double() - refs[i - 1]).norm() / refs[i - 1].norm()
+        assert off <= 1.25 * u, (name, off.item() / u)
