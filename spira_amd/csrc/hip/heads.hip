@@ -386,32 +386,21 @@ static int64_t blocks_of(const spira_hip_heads_t &x, int lanes, int most) {
 }
 constexpr int kForwardBlocks = 1 << 23, kBackwardBlocks = 512;
 
-// Turns of the pairs by a position, and their axes.  (64 powers in long double take as
-// long as a launch: a thread keeps the last ones.)
-struct Speeds {
-  double base = 0;
-  int pairs = 0, axes = 0;
-  uint64_t speed[kMostDim / 2] = {};
-  uint8_t axis[kMostDim / 2] = {};
-};
-static const Speeds &speeds(double base, int pairs, int axes) {
-  static thread_local Speeds t;
-  if (t.base == base && t.pairs == pairs && t.axes == axes) return t;
-  for (int axis = 0; axis < axes; ++axis) {
-    const int lo = axis * pairs / axes, hi = (axis + 1) * pairs / axes;
-    for (int p = lo; p < hi; ++p) {
-      // (in long double: 64 bits of the turn's fraction)
-      const long double turns = powl(static_cast<long double>(base), -static_cast<long double>(p - lo) / (hi - lo)) /
-                                6.283185307179586476925286766559L;
-      const long double scaled = (turns - floorl(turns)) * 18446744073709551616.0L;
-      t.speed[p] = scaled >= 18446744073709551615.0L ? ~uint64_t(0) : static_cast<uint64_t>(scaled);
-      t.axis[p] = static_cast<uint8_t>(axis);
+// Turns of the pairs by a position, and their axes, in long double: 64 bits of the turn's
+// fraction.  A band's speeds are a geometric row: one power, then products, whose roundings
+// leave 2^-58 of a speed (2^-26 radians at position 2^31, below fp32's own).  A power each
+// takes as long as the launch: 32 of them 12 us.
+static void speeds(double base, int pairs, int axes, uint64_t *speed, uint8_t *axis) {
+  for (int a = 0; a < axes; ++a) {
+    const int lo = a * pairs / axes, hi = (a + 1) * pairs / axes;
+    const long double by = hi - lo > 1 ? powl(static_cast<long double>(base), -1.0L / (hi - lo)) : 1.0L;
+    long double turns = 1 / 6.283185307179586476925286766559L;
+    for (int p = lo; p < hi; ++p, turns *= by) {
+      // (a fraction of 64 bits is below 2^64 times it)
+      speed[p] = static_cast<uint64_t>((turns < 1 ? turns : turns - floorl(turns)) * 18446744073709551616.0L);
+      axis[p] = static_cast<uint8_t>(a);
     }
   }
-  t.base = base;
-  t.pairs = pairs;
-  t.axes = axes;
-  return t;
 }
 
 static Args arguments(const spira_hip_heads_t &x, int lanes) {
@@ -425,9 +414,7 @@ static Args arguments(const spira_hip_heads_t &x, int lanes) {
   a.eps = x.eps;
   if (x.axes > 0) {
     a.positions = x.positions;
-    const Speeds &t = speeds(x.base, x.head_dim / 2, x.axes);
-    std::copy(t.speed, t.speed + kMostDim / 2, a.speed);
-    std::copy(t.axis, t.axis + kMostDim / 2, a.axis);
+    speeds(x.base, x.head_dim / 2, x.axes, a.speed, a.axis);
   }
   return a;
 }
