@@ -91,9 +91,13 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
     c.l += sum;
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      const Frag<T> p = as_operand<T>(s[u], st);
-      Frag<T> rest;
-      if constexpr (FINE && sizeof(T) == 2) rest = rest_operand<T>(s[u], st, p);
+      Frag<T> p, rest;
+      if constexpr (FINE && sizeof(T) == 2) {
+        p = below_operand<T>(s[u], st);
+        rest = rest_operand<T>(s[u], st, p);
+      } else {
+        p = as_operand<T>(s[u], st);
+      }
 #pragma unroll
       for (int n = 0; n < DP / 32; ++n) {
         const Frag<T> v = read.cols(vt, 32 * u + 16 * st, n);

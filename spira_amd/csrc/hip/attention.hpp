@@ -224,6 +224,20 @@ template <class T> __device__ __forceinline__ Frag<T> as_operand(const floatx16 
   return f;
 }
 
+// The same of 16 bits and of numbers that are not negative, rounded to below them by 2^-12 of
+// themselves or more: what is left is positive wherever they are, and an infinity that
+// both parts are multiplied with stays one.
+template <class T> __device__ __forceinline__ Frag<T> below_operand(const floatx16 &p, int s) {
+  Frag<T> f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = p[8 * s + 2 * i] * (1 - 0x1p-12f), b = p[8 * s + 2 * i + 1] * (1 - 0x1p-12f);
+    if constexpr (std::is_same_v<T, _Float16>) f.v[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    else f.v[0][i] = __builtin_bit_cast(uint32_t, a) >> 16 | (__builtin_bit_cast(uint32_t, b) & 0xFFFF0000u);
+  }
+  return f;
+}
+
 // What as_operand's rounding left of them, as another operand: with both, the sums that
 // follow are as good as in fp32.
 template <class T> __device__ __forceinline__ Frag<T> rest_operand(const floatx16 &p, int s, const Frag<T> &rounded) {

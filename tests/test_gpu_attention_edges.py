@@ -53,6 +53,35 @@ def test_not_finite_where_hidden(dev, many, d, what, dtype):
         assert not torch.isfinite(got[3][:at]).all(2).any()
 
 
+INFINITE = [
+    # queries, keys (None: as many), heads, key heads, causal
+    (1, 700, 8, 2, False), (1, 6000, 2, 1, True), (3, 45, 4, 1, False), (100, None, 2, 1, True), (100, None, 2, 2, False),
+    (1000, None, 24, 24, True), (1000, None, 24, 24, False), (90, 5000, 4, 4, False)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,m,heads,kv,causal", INFINITE)
+def test_infinite_values_are_the_output(dev, n, m, heads, kv, causal, dtype):
+    """Of the rows that see them, under weights that are all positive, in whole tiles, the last and those on the
+    mask's edge; of both signs NaN."""
+    dt, d, m, own = DTYPES[dtype], 32, m or n, m is None
+    q, k, v = (randn((r, h, d), dt, i, 0.1).to(dev) for i, (r, h) in enumerate(((n, heads), (m, kv), (m, kv))))
+    at = [m // 2, m - 1]
+    for a in at:
+        v[a, :, 5], v[a, :, 6] = math.inf, -math.inf
+    v[at[0], :, 7], v[at[1], :, 7] = math.inf, -math.inf
+    offsets, keys = (torch.tensor([0, r], dtype=torch.int32, device=dev) for r in (n, m))
+    kw = {} if own else dict(key_offsets=keys)
+    with torch.no_grad():
+        y = F.attention(q, k, v, offsets, causal=causal, **kw)
+    for y in (y, F.attention(q.requires_grad_(True), k, v, offsets, causal=causal, **kw).detach()):
+        sees = torch.arange(n, device=dev) >= n - m + at[0] if causal else torch.ones(n, dtype=torch.bool, device=dev)
+        both = torch.arange(n, device=dev) >= n - m + at[1] if causal else sees
+        assert torch.isfinite(y[~sees]).all() and torch.isfinite(y[..., :5]).all() and torch.isfinite(y[..., 8:]).all()
+        assert (y[sees][..., 5] == math.inf).all() and (y[sees][..., 6] == -math.inf).all()
+        assert torch.isnan(y[both][..., 7]).all() and (y[sees & ~both][..., 7] == math.inf).all()
+
+
 # ---------------------------------------------------------------------------
 # rows that overlap
 # ---------------------------------------------------------------------------
@@ -165,9 +194,10 @@ def test_small_gradients(dev, kv, causal, size):
 def test_common_parts_cancel(dev, what, dtype, part):
     """Few keys a row (all of them on the mask's edge), and values, keys or a pair of heads' queries that have
     a common part of `part` times what tells them apart: it cancels in dq or dk, what the roundings of the outputs, of
-    the weights and of ds leave of it does not.  With those kept as second operands each is held to u^2 / 2, so a
-    gradient's norm is off by u (its own rounding) and by the cancelled part's 4 roundings of u^2 / 2 each, on sums of
-    12 terms at most, times `part`: below u / 4.  Rounded without, one of them alone is some part u / sqrt(12)."""
+    the weights and of ds leave of it does not.  With those kept as second operands an output, a weight of the
+    gradients and ds are held to u^2 / 2 and a weight of the outputs to 2 u^2, so a gradient's norm is off by u (its own
+    rounding) and by `part` times some of these: below u / 4.  Rounded without, one of them alone is some
+    part u / sqrt(12)."""
     dt, lengths = DTYPES[dtype], [9, 12, 7, 11] * 6
     u, n, d = UNIT[DTYPES[dtype]], sum([9, 12, 7, 11] * 6), 64
     q, k, v, g = (randn((n, h, d), torch.float32, i) for i, h in ((1, 2), (2, 1), (3, 1), (4, 2)))
