@@ -191,15 +191,17 @@ def test_small_gradients(dev, kv, causal, size):
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,part", [("f16", 32.0), ("bf16", 16.0)])
 @pytest.mark.parametrize("what", ["values", "keys", "queries"])
-def test_common_parts_cancel(dev, what, dtype, part):
+@pytest.mark.parametrize("times", [6, 48])
+def test_common_parts_cancel(dev, times, what, dtype, part):
     """Few keys a row (all of them on the mask's edge), and values, keys or a pair of heads' queries that have
     a common part of `part` times what tells them apart: it cancels in dq or dk, what the roundings of the outputs, of
     the weights and of ds leave of it does not.  With those kept as second operands an output, a weight of the
     gradients and ds are held to u^2 / 2 and a weight of the outputs to 2 u^2, so a gradient's norm is off by u (its own
     rounding) and by `part` times some of these: below u / 4.  Rounded without, one of them alone is some
     part u / sqrt(12)."""
-    dt, lengths = DTYPES[dtype], [9, 12, 7, 11] * 6
-    u, n, d = UNIT[DTYPES[dtype]], sum([9, 12, 7, 11] * 6), 64
+    dt, lengths = DTYPES[dtype], [9, 12, 7, 11] * times
+    u, n, d = UNIT[dt], sum(lengths), 64
+    assert columns_fill_blocks(n, 2, 1, len(lengths), dt) == (times > 6)
     q, k, v, g = (randn((n, h, d), torch.float32, i) for i, h in ((1, 2), (2, 1), (3, 1), (4, 2)))
     if what == "values":
         v = 1 + v / part
