@@ -8,15 +8,23 @@
 // Two forms.  Prompts: a block owns 128 columns (a key head's query heads and
 // their queries, heads fastest), four waves of 32, and walks the keys in tiles
 // that it holds in LDS, the next one under way while it multiplies.  Few tokens:
-// the keys of a sequence are cut into parts, a block's four waves walk a part's
-// tiles each on their own (without barriers) for the same 32 columns, and the
-// parts are joined by a second launch.
+// the keys of a sequence are cut into parts, a block's one to four waves (by a row's
+// bytes) walk a part's tiles each on their own (without barriers) for the same 32
+// columns, and the parts are joined by a second launch.
 //
 // Prompts are bound by the matrix and the vector units in turn, and by power: 16 heads of
-// 128 on 4 over 16384 tokens, causal, bf16: 1220 us = 901 TFLOP/s (8192^3 product of the
-// library 1126), matrix cores busy 36 % at 2.05 GHz; heads of 32 over windows of 1024 voxels
-// 82 us, of which the exponentials and their like issue for 59.  Few tokens are bound by
-// memory: 32 caches of 4096 keys on average, 8 heads of 128: 120 us, 4.5 TB/s.
+// 128 on 4 over 16384 tokens, causal, bf16: 1180 us = 931 TFLOP/s (8192^3 product of the
+// library 1126), matrix cores busy 38 % at 2.05 GHz; heads of 32 over windows of 1024 voxels
+// 85 us, vector instructions issuing for 56 % of it and the matrix cores busy for 19 %.  Few
+// tokens are bound by memory: 32 caches of 4096 keys on average, 8 heads of 128: 121 us, 4.5
+// TB/s in the kernel.
+//
+// In 16 bits weights are rounded to the features' type before their product, half a step of
+// each term.  For few tokens and on the mask's edge a second operand holds what that leaves (one
+// token against 700 keys 11.6 us without, 12.3 with; 32 caches 116 and 118; 100 queries against
+// 100k keys 115 and 117), and outputs are as good as fp32 arithmetic's, rounded once.  Whole tiles
+// of prompts go without: outputs are off by 1.2 to 1.4 times as much, and with it that prompt took
+// 1623 us and the voxels 109.
 //
 // The softmax is taken in one pass with a running maximum and sum in fp32.  The
 // maximum moves only when a score passes it by 2^8 (in exp2; fp16 2^4): the sums are

@@ -534,7 +534,7 @@ struct Args {
 constexpr int kColumns = 128;  // of a block: a key head's query heads and their queries, heads fastest
 // Whether blocks of 128 columns are too few to fill the CUs: then a block owns 32, and its
 // waves share out the keys.  Forward, four sequences, heads of 64 (causal, 8 on 2): bf16 136
-// blocks of 128 columns 16.1 us, of 32 14.7; 264 blocks 25.1 and 32.5.  fp32 72 blocks 28.1
+// blocks of 128 columns 16.1 us, of 32 15.3; 264 blocks 25.1 and 32.5.  fp32 72 blocks 28.1
 // and 15.9, 258 (one sequence) 334 and 230, its dq, dk and dv 801 and 617.
 inline bool few_columns(const spira_hip_attention_t &x) {
   const int64_t blocks = (x.rows * (x.heads / x.kv_heads) / kColumns + x.sequences) * x.kv_heads;

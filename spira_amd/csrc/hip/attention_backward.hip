@@ -263,8 +263,8 @@ using namespace spira_hip;
 extern "C" {
 
 int spira_hip_attention_backward(const spira_hip_attention_t *x, const void *out, const float *stats, const void *rest,
-                                 const void *dout,                                 void *dqueries, void *dkey, void *dvalue, void *workspace, size_t workspace_bytes,
-                                 hipStream_t stream) {
+                                 const void *dout, void *dqueries, void *dkey, void *dvalue, void *workspace,
+                                 size_t workspace_bytes, hipStream_t stream) {
   SPIRA_HIP_REQUIRE(x, "attention: null arguments");
   const int size = x->dtype == SPIRA_F32 ? 4 : 2;
   attention::Args a;

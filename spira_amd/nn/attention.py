@@ -26,7 +26,7 @@ class AttentionBlock(nn.Module):
     rows are one sequence, or with ``window`` sequences of so many consecutive rows
     each: of an ordered tensor, windows along the order of its keys.  A batch of
     scenes behind each other passes their ``offsets`` [scenes + 1] (int32, on the GPU)
-    instead.  ``causal``: a voxel sees those before it and itself.  Parameters have
+    instead of the window.  ``causal``: a voxel sees those before it and itself.  Parameters have
     the features' type (``.half()``, ``.bfloat16()``).
     """
 
