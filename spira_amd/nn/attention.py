@@ -74,4 +74,4 @@ class AttentionBlock(nn.Module):
         y = F.attention(q, keys, p[:, h + k:], offsets, causal=self.causal)
         y, _ = F.gated_residual_norm(x, y.flatten(1) @ self.out, weight=self.exit, gate=self.gate, scale=self.scale,
                                      eps=self.eps)
-        return SparseTensor(coordinates=input.coordinates, features=y, stride=input.stride)
+        return SparseTensor(coordinates=input.coordinates, features=y, stride=input.stride, double=input._double)

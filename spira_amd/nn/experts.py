@@ -99,5 +99,5 @@ class ExpertBlock(nn.Module):
         if self.training and self.dropout > 0:
             h = F.dropout(h, self.dropout, *self._mask())
         y, _ = F.gated_residual_norm(x, h, weight=self.exit, gate=self.gate, scale=self.scale, eps=self.eps)
-        output = SparseTensor(coordinates=input.coordinates, features=y, stride=input.stride)
+        output = SparseTensor(coordinates=input.coordinates, features=y, stride=input.stride, double=input._double)
         return (output, F.balance_loss(logits, routes)) if balance else output
