@@ -524,7 +524,7 @@ struct Args {
   int part_keys;  // keys a part
   // backward
   const void *dout, *out;
-  float *delta;  // [heads, rows], times kLower
+  float *delta;  // [heads, rows]
   void *dq, *dk, *dv;
 };
 
@@ -556,36 +556,42 @@ __device__ __forceinline__ int visible(const Args &a, const Sequence &s, int i) 
 template <class T> constexpr int kLift = std::is_same_v<T, _Float16> ? 14 : 0;
 template <class T> constexpr float kLower = 1.f / static_cast<float>(1 << kLift<T>);
 
-// fp16: ds takes part in its products lifted, since n of them are some sqrt(n) below the
-// sum that they make and would lose their bits long before it does.  The power of two is a
-// column's own: its largest ds so far lies from 2^10 to 2^15, the sums follow where it moves
-// (seldom: a value has to pass it by 2^4).  Small ones keep 2^-35 of the largest.
-// Gradients of 100k voxels, 3 heads of 32, windows of 1024: 252 us without, 282 with; 16k
-// tokens of 16 heads of 64 on 4 347 and 352, of 128 1579 and 1645.
+// ds is lifted with the weight that it is made of: n of them are some sqrt(n) below the sum
+// that they make, and would lose their bits long before it does.  Where a column's largest
+// passes 2^15 so, its lift is lowered by a power of two that takes it to 2^10, and the sums
+// follow (until it passes 2^15 again): what is held is good to 2^-39, or 2^-35 of the
+// column's largest.  Gradients of 100k voxels, 3 heads of 32, windows of 1024: 231
+// us without, 245 with, 256 where every column is lowered; 16k tokens, 16 heads of 64 on 4, 291,
+// 292 and 299.
 template <class T> struct Lift {
-  float by = 0x1p100f;  // (before the first value)
+  float by = 1;
+  uint64_t lowered = 0;  // (lanes that have been, of the wave)
   template <int N> __device__ __forceinline__ void fit(floatx16 &ds, floatx16 (&acc)[N]) {
-    if constexpr (std::is_same_v<T, _Float16>) {
+    if constexpr (kLift<T> > 0) {
       constexpr float most = 0x1p15f;
       float top = 0;
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, __builtin_fabsf(ds[r]));
-      if (ballot(top * by > most)) {
-        // (both halves of a column as one)
-        top = __builtin_fmaxf(top, other_half(top));
-        const float next = top * by > most ? __builtin_ldexpf(1.f, 11 - __builtin_amdgcn_frexp_expf(top)) : by;
-        const float ratio = next * (1.f / by);
+      const uint64_t over = ballot(top * by > most);
+      if (over | lowered) {
+        if (over) {
+          // (both halves of a column as one)
+          top = __builtin_fmaxf(top, other_half(top));
+          const float next = top * by > most ? __builtin_ldexpf(1.f, 11 - __builtin_amdgcn_frexp_expf(top)) : by;
+          const float ratio = next * (1.f / by);
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[n][r] *= ratio;
-        by = next;
+            for (int r = 0; r < 16; ++r) acc[n][r] *= ratio;
+          by = next;
+          lowered |= over;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] *= by;
       }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] *= by;
     }
   }
-  __device__ __forceinline__ float lower() const { return std::is_same_v<T, _Float16> ? 1.f / by : 1.f; }
+  __device__ __forceinline__ float lower() const { return kLift<T> > 0 ? kLower<T> / by : 1.f; }
 };
 
 // a row's statistics, and p from a raw score

@@ -55,13 +55,13 @@ template <class T, int DP> struct QueryColumn {
     }
     delta += other_half(delta);
     const int64_t to = head * a.s.rows + s.q0 + i;
-    if (there && lane_id() < 32) a.delta[to] = delta * kLower<T>;
-    stat = {a.stats[to] + kLift<T>, 1.f};
+    if (there && lane_id() < 32) a.delta[to] = delta;
+    stat = {a.stats[to], 1.f};
     if constexpr (sizeof(T) == 4) stat.by = a.stats[a.heads * a.s.rows + to];
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) acc[n] = floatx16{};
   }
-  // ds of 32 keys (MASKED: of which this lane's column sees the first `seen`)
+  // ds, lifted, of 32 keys (MASKED: of which this lane's column sees the first `seen`)
   template <bool MASKED>
   __device__ __forceinline__ void gradients(const Args &a, const Reader<T, DP> &read, lds_char *kt, lds_char *vt, int seen,
                                             floatx16 &ds) const {

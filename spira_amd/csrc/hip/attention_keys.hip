@@ -132,8 +132,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       for (int y = 0; y < 4; ++y) {
         const float w = weight(p[4 * x + y], a.scale2, Stat<T>{base[y], by[y]});
         const bool seen = !decltype(MASKED)::value || 8 * x + y >= mine - 4 * h;
-        // (w is lifted, delta lowered)
-        ds[4 * x + y] = seen ? w * __builtin_fmaf(ds[4 * x + y], kLower<T>, -delta[y]) : 0.f;
+        // (w is lifted, and ds with it)
+        ds[4 * x + y] = seen ? w * (ds[4 * x + y] - delta[y]) : 0.f;
         p[4 * x + y] = seen ? w : 0.f;
       }
     }
@@ -171,8 +171,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
       __syncthreads();  // (every wave has the scores)
       const bool x = clear_not_finite<T, DP, 32, 256>(qu, threadIdx.x), y = clear_not_finite<T, DP, 32, 256>(gu, threadIdx.x);
       const bool found = __syncthreads_or(x || y);
-      accumulate(std::true_type{}, av, gu, p);
       lift.fit(ds, ak);
+      accumulate(std::true_type{}, av, gu, p);
       accumulate(std::true_type{}, ak, qu, ds);
       if (found) {
         const int64_t r0 = s.q0 + q0 + 32 * u;
@@ -196,8 +196,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void keys_
     for (int u = 0; u < QT / 32; ++u) {
       floatx16 p, ds;
       weights(std::false_type{}, stage, 32 * u, 0, p, ds);
-      accumulate(std::false_type{}, av, gt + 32 * u * R::PITCH, p);
       lift.fit(ds, ak);
+      accumulate(std::false_type{}, av, gt + 32 * u * R::PITCH, p);
       accumulate(std::false_type{}, ak, qt + 32 * u * R::PITCH, ds);
     }
   });

@@ -143,12 +143,13 @@ def test_many_small_weights(dev, queries, kv, train):
 # ---------------------------------------------------------------------------
 # small gradients in fp16
 # ---------------------------------------------------------------------------
-@pytest.mark.parametrize("size", [1.0, 2.0 ** -7, 2.0 ** -13])
+@pytest.mark.parametrize("size", [64.0, 1.0, 2.0 ** -7, 2.0 ** -13])
 @pytest.mark.parametrize("kv,causal", [(1, False), (1, True), (24, True)])
 def test_small_gradients(dev, kv, causal, size):
     """fp16, even weights of 4000 keys, and gradients of the outputs down to what fp16 holds few bits of: ds is
-    some sqrt(n) below dq and dk.  Each ds is off by half a step, 2^-11 of itself (but 2^-34 of the largest of its
-    column, in what the kernels lift by it), dp and delta by their sums' 2 (d + 16) e, and the outputs round once."""
+    some sqrt(n) below dq and dk.  Each ds is off by half a step, 2^-11 of itself (but 2^-39, half a step under the
+    lift of 2^14, or 2^-34 of the largest of its column, which that is lowered by), dp and delta by their sums'
+    2 (d + 16) e, and the outputs round once."""
     n, d = 4000, 64
     u = UNIT[torch.float16]
     v, dout = randn((n, kv, d), torch.float16, 3), (randn((n, kv, d), torch.float32, 4) * size).half()
@@ -174,11 +175,11 @@ def test_small_gradients(dev, kv, causal, size):
             edp = (d + 16) * E * (g.abs() @ z.abs().t() + (p * dp.abs()).sum(1, keepdim=True)) + (g.abs() * to).sum(1, keepdim=True)
             eds = w * ds.abs() + p * edp
             if which == "dq":
-                low = 2.0 ** -34 * ds.abs().amax(1, keepdim=True)
+                low = 2.0 ** -39 + 2.0 ** -34 * ds.abs().amax(1, keepdim=True)
                 eds = torch.where(seen, eds + u * ds.abs() + low, 0)
                 ref, tol = d ** -0.5 * ds @ y, d ** -0.5 * eds @ y.abs()
             else:
-                low = 2.0 ** -34 * ds.abs().amax(0, keepdim=True)
+                low = 2.0 ** -39 + 2.0 ** -34 * ds.abs().amax(0, keepdim=True)
                 eds = torch.where(seen, eds + u * ds.abs() + low, 0)
                 ref, tol = d ** -0.5 * ds.t() @ x, d ** -0.5 * eds.t() @ x.abs()
             tol = tol + u * ref.abs() + 2.0 ** -25 + 2 * n * E * tol
