@@ -389,7 +389,7 @@ constexpr int kForwardBlocks = 1 << 23, kBackwardBlocks = 512;
 // Turns of the pairs by a position, and their axes, in long double: 64 bits of the turn's
 // fraction.  A band's speeds are a geometric row: one power, then products, whose roundings
 // leave 2^-58 of a speed (2^-26 radians at position 2^31, below fp32's own).  A power each
-// takes as long as the launch: 32 of them 12 us.
+// takes longer than a launch: 32 of them 14 us.
 static void speeds(double base, int pairs, int axes, uint64_t *speed, uint8_t *axis) {
   for (int a = 0; a < axes; ++a) {
     const int lo = a * pairs / axes, hi = (a + 1) * pairs / axes;

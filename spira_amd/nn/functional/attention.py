@@ -35,10 +35,10 @@ def attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, o
 
     Up to 65536 sequences of any lengths, none included.  A query that sees no key, or
     is in no sequence, gets zeros.  Values that are not finite reach the queries
-    that see them only.  In 16 bits the softmax's weights, and in the gradients they
-    and the scores' gradients, are rounded to the features' type before their products,
-    with what that leaves as a second term for few tokens (not in the gradients) and where
-    the mask or a sequence ends inside a tile; in fp32 nothing is.
+    that see them only.  In 16 bits the softmax's weights, and in the gradients the
+    scores' too, are rounded to the features' type before their products; the outputs of
+    few tokens, and the rows of tiles in which a causal mask ends, take what that leaves as
+    a second term.  In fp32 nothing is rounded.
     """
     _gpu(queries)
     return _C.attention(queries, keys, values, offsets, key_offsets, key_counts, causal, scale)
