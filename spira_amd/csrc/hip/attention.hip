@@ -42,6 +42,13 @@ namespace attention {
 template <class T> constexpr float kRaise = std::is_same_v<T, _Float16> ? 11.f : 0.f;
 template <class T> constexpr float kSlack = std::is_same_v<T, _Float16> ? 4.f : 8.f;
 
+// The reference in exp2: rounded once, and so wherever sums of another reference are joined (as
+// part of a longer expression it would not be).
+__device__ __forceinline__ float reference(float m, float scale2) {
+#pragma clang fp contract(off)
+  return m * scale2;
+}
+
 // a wave's 32 columns on their way: output, reference maximum of the raw scores
 // (-inf: nothing seen) and this half's share of the sum
 template <int DP> struct Columns {
@@ -78,7 +85,7 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
   // (each column by its own scores: a result does not depend on the wave's others)
   const bool moves = (top - c.m) * scale2 > kSlack<T>;
   if (ballot(moves)) {
-    const float m = moves ? top : c.m, by = moves ? __builtin_amdgcn_exp2f((c.m - m) * scale2) : 1.f;
+    const float m = moves ? top : c.m, by = moves ? __builtin_amdgcn_exp2f(reference(c.m, scale2) - reference(m, scale2)) : 1.f;
     c.l *= by;
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n)
@@ -86,7 +93,7 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
       for (int r = 0; r < 16; ++r) c.o[n][r] *= by;
     c.m = m;
   }
-  float base = c.m == -__builtin_inff() ? 0.f : -c.m * scale2;
+  float base = c.m == -__builtin_inff() ? 0.f : -reference(c.m, scale2);
   if constexpr (kRaise<T> > 0) base += kRaise<T>;
 #pragma unroll
   for (int u = 0; u < KT / 32; ++u) {
@@ -116,11 +123,11 @@ __device__ __forceinline__ void attend_tile(Columns<DP> &c, const Frag<T> (&q)[D
   }
 }
 
-// a row's statistics for the gradients, from its reference and sum
+// a row's statistics for the gradients, from its reference (in exp2) and sum
 template <class T>
 __device__ __forceinline__ void put_statistics(const Args &a, int head, int64_t row, float m, float l) {
   float *to = a.stats + head * a.s.rows + row;
-  const float base = m == -__builtin_inff() ? 0.f : m * a.scale2;
+  const float base = m == -__builtin_inff() ? 0.f : m;
   if constexpr (sizeof(T) == 2) {
     *to = l == 0.f ? __builtin_inff() : base + __builtin_amdgcn_logf(l) - (kRaise<T> + kLift<T>);
   } else {
@@ -198,7 +205,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void prompt_kernel(con
   const bool there = column < total;
   const int64_t at = ((s.q0 + i) * a.heads + head) * a.d;
   store_column<T, DP>(o + at, a.d, there, c.o, l == 0.f ? 0.f : 1.f / l, a.rest ? static_cast<T *>(a.rest) + at : nullptr);
-  if (a.stats && there && lane < 32) put_statistics<T>(a, head, s.q0 + i, c.m, l);
+  if (a.stats && there && lane < 32) put_statistics<T>(a, head, s.q0 + i, reference(c.m, a.scale2), l);
 }
 
 // ---------------------------------------------------------------------------
@@ -294,7 +301,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP, DIRECT>::NW), 1) void token
     put_sums<DP>(reinterpret_cast<float *>(lds[wave]), c.o);
     const float l = c.l + other_half(c.l);
     if (lane < 32) {
-      wm[wave][lane] = c.m;
+      wm[wave][lane] = reference(c.m, a.scale2);
       wl[wave][lane] = l;
     }
     __syncthreads();
@@ -304,7 +311,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP, DIRECT>::NW), 1) void token
       for (int w = 1; w < NW; ++w) m = __builtin_fmaxf(m, wm[w][lane]);
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float by = wm[w][lane] == m ? 1.f : __builtin_amdgcn_exp2f((wm[w][lane] - m) * a.scale2);
+        const float by = wm[w][lane] == m ? 1.f : __builtin_amdgcn_exp2f(wm[w][lane] - m);
         sum += wl[w][lane] * by;
         wm[w][lane] = by;
       }
@@ -334,7 +341,7 @@ __global__ __launch_bounds__((64 * TokenShape<T, DP, DIRECT>::NW), 1) void token
       return;
     } else if (static_cast<int>(threadIdx.x) < columns) {
       float *to = a.partial_stats + (s.nth * a.s.rows * a.heads + (s.q0 + i) * a.heads + head) * 2;
-      to[0] = top[lane] == -__builtin_inff() ? top[lane] : top[lane] * a.scale2;
+      to[0] = top[lane];
       to[1] = total_l[lane];
     }
     __syncthreads();  // (the next columns' tiles take the sums' place)

@@ -1,6 +1,6 @@
 """Attention where its kernels' shortcuts end: values that are not finite behind the mask
 (in narrow heads among others), rows that overlap, small weights and gradients in fp16, common
-parts that cancel.  Units and
+parts that cancel, large scores.  Units and
 the reference are those of test_gpu_attention.py."""
 import math
 
@@ -229,3 +229,37 @@ def test_common_parts_cancel(dev, times, what, dtype, part):
             continue  # (nothing cancels)
         off = (got[i].double() - refs[i - 1]).norm() / refs[i - 1].norm()
         assert off <= 1.25 * u, (name, off.item() / u)
+
+
+# ---------------------------------------------------------------------------
+# large scores in fp32
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("queries,keys,kv,rising", [(1, 300, 1, False), (3, 300, 2, True), (1, 5000, 1, False),
+                                                    (600, 300, 110, False), (600, 300, 110, True)])
+def test_large_scores_in_parts(dev, queries, keys, kv, rising):
+    """fp32, scores of 15000 and little more, exact in the type: what waves, parts and the maximum's steps put
+    together is of one reference each, rounded once.  A weight is off by its exponential's 2^-23 and its argument's
+    2^-24 of the distance from the largest (in exp2, once for the scale, once for the product), sums of n terms by n e, all
+    twice (over the weights' sum); joins by 2^-22 each.  By way of a rounded reference of 21640 they are off by some 2^-11."""
+    d, g = 16, torch.Generator().manual_seed(3)
+    s = 15000 + torch.randint(0, 256, (keys,), generator=g) / 256 + (torch.arange(keys) // 32 * 0.5 if rising else 0)
+    q, k = torch.zeros(queries, kv, d), torch.zeros(keys, kv, d)
+    q[..., 0], k[..., 0] = 1, s[:, None]
+    v = (1 - torch.arange(keys) // 32 % 2 * 2.0)[:, None, None].expand(-1, kv, d).contiguous()
+    q, k, v = (t.to(dev).requires_grad_(True) for t in (q, k, v))
+    offsets, at = (torch.tensor([0, n], dtype=torch.int32, device=dev) for n in (queries, keys))
+    assert columns_fill_blocks(queries, kv, kv, 1, torch.float32) == (queries > 3)
+    with torch.no_grad():
+        y = F.attention(q, k, v, offsets, key_offsets=at, scale=1.0)
+    z = F.attention(q, k, v, offsets, key_offsets=at, scale=1.0)
+    dv = torch.autograd.grad(z, v, torch.ones_like(z))[0]
+    s = s.to(dev).double()
+    p = torch.softmax(s, 0)
+    each = 2 ** -23 + 2 * E * (s.max() - s) * 1.45
+    off = 2 * ((p * each).sum() + min(keys, 640) * E + 4 * 2.0 ** -22)
+    ref = torch.einsum("n,nhd->hd", p, v.detach().double())
+    for out in (y, z):
+        assert ((out.double() - ref).abs() <= off).all(), ((out.double() - ref).abs().max() / off).item()
+    tol = (queries * p * (each + off + queries * E))[:, None, None]
+    bad = (dv.double() - queries * p[:, None, None]).abs() / tol
+    assert (bad <= 1).all(), bad.max().item()
